@@ -37,6 +37,7 @@ enum { RWKV_W_RAW_LOGIT = 0, RWKV_W_DECAY = 1 };
 enum { RWKV_IO_F16 = 0, RWKV_IO_F32 = 1 };
 enum { RWKV_ACT_NONE = 0, RWKV_ACT_TANH = 1, RWKV_ACT_SIGMOID = 2 };
 enum { RWKV_EPI_NONE = 0, RWKV_EPI_RELU_SQUARE = 1 };
+enum { RWKV_NORM_LAYER = 0, RWKV_NORM_RMS = 1 };
 
 const char* rwkv_hip_last_error(void);
 
@@ -242,6 +243,13 @@ int rwkv_hip_layer_norm(rwkv_stream_t s, int rows, int C, const void* x, const v
 /* rwkv7_v3a_add_layer_norm_f16_launch (:122-125) */
 int rwkv_hip_add_layer_norm(rwkv_stream_t s, int rows, int C, const void* x, const void* res, const void* w,
                             const void* b, void* x_out, void* y, float eps);
+/* Residual addition, norm and 8-bit output of rows of fp16 values, for a product with int8 weights (rwkv_hip_linear_logprobs); no
+ * counterpart in the reference.  s = x + res in fp32 (res may be NULL: s = x); x_out = f16(s) (may be NULL; may be x or res itself);
+ * y = (s - mean) / sqrt(variance + eps) * w + b (RWKV_NORM_LAYER) or s / sqrt(mean(s^2) + eps) * w + b (RWKV_NORM_RMS), b may be NULL;
+ * scale f32 [rows] = max|y| / 127;  q int8 [rows,C] = y / scale to the nearest, ties to even (both 0 where y is).  A row whose y is
+ * not finite somewhere gets the scale NaN and codes 0.  C % 8 == 0, C <= 8192; fp16 tensors aligned to 16 bytes, q to 8. */
+int rwkv_hip_add_norm_q8(rwkv_stream_t s, int rows, int C, int norm, const void* x, const void* res, const void* w, const void* b,
+                         float eps, void* x_out, void* q, void* scale);
 /* rwkv7_v3a_add_last_layer_norm_f16_launch (:127-130): y [B,C] from the last token of each row */
 int rwkv_hip_add_last_layer_norm(rwkv_stream_t s, int B, int T, int C, const void* x, const void* res,
                                  const void* w, const void* b, void* y, float eps);
@@ -282,6 +290,33 @@ int rwkv_hip_sample(rwkv_stream_t s, int B, int V, const void* logits, void* pen
                     double top_p, uint64_t seed, uint64_t step);
 /* lm_head -> argmax without the sampler: out i32 [B] = lowest index of the row maximum */
 int rwkv_hip_argmax(rwkv_stream_t s, int B, int V, const void* logits, void* out);
+
+/* Log probabilities of given tokens (no counterpart in the reference; what `logprobs` and `echo` of a server and the scoring of a text
+ * ask for).  logits [rows,V] of type io (RWKV_IO_F32 / RWKV_IO_F16), rows ld >= V entries apart, any alignment of their type;
+ * tokens i32 [rows].  Outputs, each may be NULL (not all):
+ *   logprob f32 [rows]       ln of the softmax at tokens[row]: 0 for a token < 0 (none, as in padding), NaN for one >= V
+ *   entropy f32 [rows]       of the softmax, in nats
+ *   rank i32 [rows]          entries ahead of the token in the order "larger first, equal ones by index": 0 = most probable; -1 where
+ *                            the token is < 0 or >= V or its logit is NaN
+ *   top_ids i32, top_logprobs f32 [rows,top_n]  the first top_n (0 .. 64) entries in that order
+ * Logits of -infinity have probability 0 and are no alternatives; places without one hold -1 and -infinity.  A row of nothing but
+ * -infinity gives log probability -infinity, entropy 0.  A row with a NaN or +infinity gives NaN for every log probability and the
+ * entropy (NaN entries are no alternatives).  V <= 1048576.  Sums are held in fp32 in a fixed order: a call repeats bitwise, and a
+ * row's results do not depend on the other rows' values (how a row is shared out goes by rows, V and top_n).  The workspace
+ * (rwkv_hip_token_logprobs_workspace bytes, aligned to 16; NULL where 0) need not be cleared; calls that share one must not overlap. */
+int rwkv_hip_token_logprobs_workspace(int rows, int V, int top_n, size_t* bytes);
+int rwkv_hip_token_logprobs(rwkv_stream_t s, int rows, int V, int io, const void* logits, int64_t ld, const void* tokens, int top_n,
+                            void* logprob, void* entropy, void* rank, void* top_ids, void* top_logprobs, void* workspace,
+                            size_t workspace_bytes);
+/* The same (without the rank) for logits z = x[M,K] . W[N,K]^T, which are kept in fp32 and never leave: the head product of a scored
+ * text.  packed: rwkv_hip_pack_weights of fp16 weights (RWKV_FMT_F16) or int8 codes (RWKV_FMT_W8, scale f16 [N]).  x: f16 [M,K] with
+ * x_scale NULL, or int8 [M,K] (RWKV_FMT_W8 only) with x_scale f32 [M] >= 0 as rwkv_hip_add_norm_q8 gives them, z = (whole-number
+ * product) * scale * x_scale.  N % 32 == 0, K % 256 == 0, N <= 1048576, K <= 16384; x and packed aligned to 16 bytes, scale to 8.
+ * Repeats bitwise.  Workspace as above (aligned to 16). */
+int rwkv_hip_linear_logprobs_workspace(int fmt, int x_int8, int M, int N, int K, int top_n, size_t* bytes);
+int rwkv_hip_linear_logprobs(rwkv_stream_t s, int fmt, int M, int N, int K, const void* x, const void* x_scale, const void* packed,
+                             const void* scale, const void* tokens, int top_n, void* logprob, void* entropy, void* top_ids,
+                             void* top_logprobs, void* workspace, size_t workspace_bytes);
 
 /* ---- model graph.  Replaces CudaWeights + run_backend_forward (src/rwkv7_fast_v4.cu:1046-1345) and
  * ModelBackend::{create_state,forward_prefill,forward_decode} (:1373-1419) below IModelBackend. ---- */

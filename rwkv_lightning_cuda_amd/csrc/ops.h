@@ -227,6 +227,36 @@ int ffn_sparse_launch(hipStream_t st, int fmt, int rows, int C, int F, int activ
 // out[b] = index of the largest logit of row b (the lowest one among equals); next / history (may be null) get the same id
 int argmax_launch(hipStream_t st, int B, int V, const float* logits, int* out, int64_t* next = nullptr, int* history = nullptr);
 
+// ---- logprobs.hip, linear_logprobs.hip: log probabilities of given tokens -------------------------------------
+constexpr int kMaxAlternatives = 64;
+constexpr int kMaxLogprobVocab = 1048576;  // as the sampler's
+struct TokenLogprobs {
+  const int* tokens;    // [rows]: < 0 none, log probability 0 and rank -1; >= V NaN and -1.  NULL where neither is asked for
+  int top_n;
+  float* logprob;       // [rows], may be NULL, as the others
+  float* entropy;       // [rows]
+  int* rank;            // [rows]
+  int* top_ids;         // [rows,top_n]
+  float* top_logprobs;  // [rows,top_n]
+  TokenLogprobs from_row(int64_t r) const {
+    TokenLogprobs t = *this;
+    if (tokens) t.tokens += r;
+    if (logprob) t.logprob += r;
+    if (entropy) t.entropy += r;
+    if (rank) t.rank += r;
+    if (top_ids) t.top_ids += r * top_n;
+    if (top_logprobs) t.top_logprobs += r * top_n;
+    return t;
+  }
+};
+int check_token_logprobs(const char* who, const TokenLogprobs& out);
+size_t token_logprobs_workspace_bytes(int rows, int V, int top_n);
+int token_logprobs_launch(hipStream_t st, int rows, int V, int io, const void* logits, int64_t ld, const TokenLogprobs& out, void* workspace);
+size_t linear_logprobs_workspace_bytes(int fmt, bool x_int8, int M, int N, int K, int top_n);
+// x_scale: x holds int8 codes
+int linear_logprobs_launch(hipStream_t st, int fmt, int M, int N, int K, const void* x, const float* x_scale, const void* packed,
+                           const half_t* scale, const TokenLogprobs& out, void* workspace);
+
 // ---- wkv7.hip -----------------------------------------------------------------------------------
 // T tokens of the recurrence, all tensors [B,T,C]; d is the decay itself in fp32.
 // The model's row-tiled time-mix pass in one launch: kk normalise / a-gate / decay while staging, the WKV recurrence,

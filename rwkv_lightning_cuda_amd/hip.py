@@ -17,6 +17,7 @@ W_RAW_LOGIT, W_DECAY = 0, 1
 IO_F16, IO_F32 = 0, 1
 ACT_NONE, ACT_TANH, ACT_SIGMOID = 0, 1, 2
 EPI_NONE, EPI_RELU_SQUARE = 0, 1
+NORM_LAYER, NORM_RMS = 0, 1
 
 # tensor / matrix ids (rwkv_hip.h)
 T_EMB_LN0, T_LN_OUT_W, T_LN_OUT_B = 0, 1, 2
@@ -46,7 +47,9 @@ EXPORTS = [
     "rwkv_hip_layer_norm", "rwkv_hip_add_layer_norm", "rwkv_hip_add_last_layer_norm", "rwkv_hip_token_shift_mix",
     "rwkv_hip_add_layer_norm_cmix_mix", "rwkv_hip_add_layer_norm_tmix_mix6", "rwkv_hip_kk_a_gate",
     "rwkv_hip_lnx_rkvres_xg", "rwkv_hip_relu_square", "rwkv_hip_add_vec", "rwkv_hip_f16_to_f32",
-    "rwkv_hip_advance_i32", "rwkv_hip_sample", "rwkv_hip_argmax", "rwkv_hip_model_create", "rwkv_hip_model_destroy",
+    "rwkv_hip_advance_i32", "rwkv_hip_sample", "rwkv_hip_argmax", "rwkv_hip_add_norm_q8",
+    "rwkv_hip_token_logprobs_workspace", "rwkv_hip_token_logprobs", "rwkv_hip_linear_logprobs_workspace", "rwkv_hip_linear_logprobs",
+    "rwkv_hip_model_create", "rwkv_hip_model_destroy",
     "rwkv_hip_model_set_tensor", "rwkv_hip_model_set_matrix", "rwkv_hip_model_weight_bytes",
     "rwkv_hip_session_debug_buffer",
     "rwkv_hip_session_create", "rwkv_hip_session_destroy", "rwkv_hip_session_stream", "rwkv_hip_session_set_graph",
@@ -396,6 +399,40 @@ def sample(B, V, logits, penalties, probs, out, presence=0.0, frequency=0.0, dec
 
 def argmax(B, V, logits, out, stream=None):
     check(load().rwkv_hip_argmax(_p(stream), _i(B), _i(V), _p(logits), _p(out)))
+
+
+def add_norm_q8(rows, C, x, res, w, b, q, scale, x_out=None, norm=NORM_LAYER, eps=1e-5, stream=None):
+    """Residual addition (res None: none), norm and int8 codes with a scale per row; x_out receives the sum."""
+    check(load().rwkv_hip_add_norm_q8(_p(stream), _i(rows), _i(C), _i(norm), _p(x), _p(res), _p(w), _p(b), ctypes.c_float(eps), _p(x_out),
+                                      _p(q), _p(scale)))
+
+
+def token_logprobs_workspace(rows, V, top_n=0):
+    n = ctypes.c_size_t(0)
+    check(load().rwkv_hip_token_logprobs_workspace(_i(rows), _i(V), _i(top_n), ctypes.byref(n)))
+    return n.value
+
+
+def token_logprobs(rows, V, logits, tokens, workspace=None, logprob=None, entropy=None, rank=None, top_n=0, top_ids=None,
+                   top_logprobs=None, io=IO_F32, ld=None, stream=None):
+    """ln softmax(logits)[token], entropy, rank of the token and the top_n first entries of every row; ld: entries between rows."""
+    check(load().rwkv_hip_token_logprobs(_p(stream), _i(rows), _i(V), _i(io), _p(logits), ctypes.c_int64(V if ld is None else ld),
+                                         _p(tokens), _i(top_n), _p(logprob), _p(entropy), _p(rank), _p(top_ids), _p(top_logprobs),
+                                         _p(workspace), ctypes.c_size_t(workspace.nbytes if workspace is not None else 0)))
+
+
+def linear_logprobs_workspace(fmt, M, N, K, top_n=0, x_int8=False):
+    n = ctypes.c_size_t(0)
+    check(load().rwkv_hip_linear_logprobs_workspace(_i(fmt), _i(1 if x_int8 else 0), _i(M), _i(N), _i(K), _i(top_n), ctypes.byref(n)))
+    return n.value
+
+
+def linear_logprobs(fmt, M, N, K, x, packed, scale, tokens, workspace, x_scale=None, logprob=None, entropy=None, top_n=0, top_ids=None,
+                    top_logprobs=None, stream=None):
+    """token_logprobs (without the rank) of the logits x . W^T; x_scale: x holds int8 codes."""
+    check(load().rwkv_hip_linear_logprobs(_p(stream), _i(fmt), _i(M), _i(N), _i(K), _p(x), _p(x_scale), _p(packed), _p(scale), _p(tokens),
+                                          _i(top_n), _p(logprob), _p(entropy), _p(top_ids), _p(top_logprobs), _p(workspace),
+                                          ctypes.c_size_t(workspace.nbytes if workspace is not None else 0)))
 
 
 class Event:
