@@ -13,7 +13,11 @@ namespace rwkv {
 
 namespace {
 
-constexpr int kLpThreads = 256;
+constexpr int kCandidates = 1024;  // places for entries that may be among the first top_n
+constexpr int kRefine = 4;         // batches between looks at whether the candidates can be thinned out
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLowest = -3.402823466e38f;
+constexpr float kGone = -200.0f;   // e^-200 is 0 in fp32; a difference that is multiplied by it must not be infinite
 
 struct LogprobArgs {
   const void* logits;
@@ -27,77 +31,289 @@ struct LogprobArgs {
   int V, top_n;
 };
 
-template <typename T>
-__global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(LogprobArgs a) {
-  __shared__ float red[4][kLpThreads / 64];
-  __shared__ int idx[kLpThreads / 64];
+// m, S and U of the entries seen so far.  m starts at the lowest finite value, not at -infinity: differences with it are no NaN,
+// and S stays 0 as long as every entry is -infinity.  A NaN or +infinity among the entries makes S a NaN that stays.
+struct SoftSum {
+  float m = kLowest, s = 0.0f, u = 0.0f;
+  __device__ __forceinline__ void raise(float to) {
+    const float t = fmaxf(m - to, kGone);
+    const float f = __builtin_amdgcn_exp2f(t * kLog2e);
+    u = f * fmaf(t, s, u);
+    s *= f;
+    m = to;
+  }
+};
+
+__device__ __forceinline__ float next_above(float v) {  // the smallest float above v; NaN above +infinity
+  const uint32_t b = __builtin_bit_cast(uint32_t, v);
+  return v == 0.0f ? __builtin_bit_cast(float, 1u) : __builtin_bit_cast(float, v > 0.0f ? b + 1 : b - 1);
+}
+
+__device__ __forceinline__ bool ahead_of(float v, int i, float w, int k) { return v > w || (v == w && i < k); }
+
+// One block per row, which it reads once: 64 bytes per thread at a time, the next 64 requested before they are looked at.  A thread
+// keeps m, S and U of its entries and raises m when a batch exceeds it.  The rank is a count against the token's logit, which is
+// read first.  Alternatives: of the first batch the largest entry of each of 64 or 256 groups of threads is known; top_n of these are
+// at least as large as the top_n-th of them, so that nothing below it can be an alternative.  What is not below goes to a list in LDS (its
+// order is that of an atomic counter, its use is not), which is sorted by counting at the end, and thinned out to the first top_n - with
+// the last one as the new bound - whenever it has grown to four times as many.  A list that overflows (a row that rises, or is of one
+// value) is given up: the alternatives are then found one after the other in top_n walks over the row.
+template <typename T, int NT>
+__global__ __launch_bounds__(NT) void token_logprobs_kernel(LogprobArgs a) {
+  constexpr int VE = 16 / sizeof(T);  // entries of a 16-byte vector
+  constexpr int VB = 4;               // vectors of a batch
+  typedef T vec_t __attribute__((ext_vector_type(VE)));
+  __shared__ float cand_z[2][kCandidates];
+  __shared__ int cand_i[2][kCandidates];
+  __shared__ __align__(16) float group_max[256];
+  __shared__ float red[4][NT / 64];
+  __shared__ int n_cand;
+  __shared__ float bound_s;
+  const int tid = threadIdx.x;
   const T* z = static_cast<const T*>(a.logits) + blockIdx.x * a.ld;
   const int V = a.V;
-  auto at = [&](int i) { return static_cast<float>(z[i]); };
-  auto block_max = [&](float v, int slot) {
-    v = wave_reduce_dpp(v, [](float x, float y) { return fmaxf(x, y); });
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[slot][threadIdx.x >> 6] = v;
-    __syncthreads();
-    float r = red[slot][0];
+  const int misaligned = static_cast<int>((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
+  const int head = misaligned ? min(VE - misaligned, V) : 0;  // entries in front of the first 16-byte boundary
+  const int vecs = (V - head) / VE;
+  const int tail = head + vecs * VE;                          // first entry behind the last vector
+  const vec_t* body = reinterpret_cast<const vec_t*>(z + head);
+  const int batches = (vecs + NT * VB - 1) / (NT * VB);
+
+  vec_t next[VB];
+  auto request = [&](int b) {
 #pragma unroll
-    for (int i = 1; i < kLpThreads / 64; ++i) r = fmaxf(r, red[slot][i]);
-    return r;
+    for (int q = 0; q < VB; ++q) {
+      const int v = (b * VB + q) * NT + tid;
+      if (v < vecs) {
+        next[q] = body[v];
+      } else {
+#pragma unroll
+        for (int e = 0; e < VE; ++e) next[q][e] = static_cast<T>(-INFINITY);
+      }
+    }
   };
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < V; i += kLpThreads) m = fmaxf(m, at(i));
-  m = block_max(m, 0);
+  request(0);
+  // the entries of the two ends, at most one per thread
+  const int stray = tid < head ? tid : tail + tid - head;
+  const float stray_z = stray < V ? static_cast<float>(z[stray]) : -INFINITY;
   const int t = a.tokens ? a.tokens[blockIdx.x] : -1;
-  const float zt = t >= 0 && t < V ? at(t) : 0.0f;
-  float s = 0.0f, u = 0.0f, ahead = 0.0f;
-  for (int i = threadIdx.x; i < V; i += kLpThreads) {
-    const float x = at(i);
-    float d = x - m;
-    if (d < -200.0f) d = -200.0f;  // e^-200 is 0 in fp32, and 0 times an infinity is none
-    if (x == -INFINITY) d = -200.0f;
-    const float e = __expf(d);
-    s += e;
-    u = fmaf(d, e, u);
-    if (x > zt || (x == zt && i < t)) ahead += 1.0f;
+  const bool has_token = t >= 0 && t < V;
+  const float zt = has_token ? static_cast<float>(z[t]) : 0.0f;
+  const bool count = a.rank && has_token;
+  const float zt_above = next_above(zt);
+  if (a.top_n > 0 && tid == 0) n_cand = 0;
+
+  SoftSum sum;
+  int ahead = 0;
+  float bound = INFINITY;
+  int list = 0;
+  auto offer = [&](float v, int i) {
+    if (v >= bound && v > -INFINITY) {
+      const int at = atomicAdd(&n_cand, 1);
+      if (at < kCandidates) {
+        cand_z[list][at] = v;
+        cand_i[list][at] = i;
+      }
+    }
+  };
+  // the top_n-th largest of the groups' maxima (equal ones by group): every thread of the block comes here
+  auto first_bound = [&](float mine) {
+    const int groups = a.top_n <= 24 ? 64 : 256;
+    if (mine != mine) mine = -INFINITY;
+    const int width = NT / groups;
+    if (width > 1) mine = fmaxf(mine, __builtin_bit_cast(float, lane_xor_dpp<1>(__builtin_bit_cast(int, mine))));
+    if (width > 2) mine = fmaxf(mine, __builtin_bit_cast(float, lane_xor_dpp<2>(__builtin_bit_cast(int, mine))));
+    if (width > 4) mine = fmaxf(mine, __builtin_bit_cast(float, lane_xor_dpp<4>(__builtin_bit_cast(int, mine))));
+    if (width > 8) mine = fmaxf(mine, __builtin_bit_cast(float, lane_xor_dpp<8>(__builtin_bit_cast(int, mine))));
+    if (tid % width == 0) group_max[tid / width] = mine;
+    __syncthreads();
+    if (tid < groups) {
+      const float v = group_max[tid];
+      int before = 0;
+      for (int i = 0; i < groups; i += 4) {
+        const float4_t w = *reinterpret_cast<const float4_t*>(group_max + i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) before += ahead_of(w[e], i + e, v, tid);
+      }
+      if (before == a.top_n - 1) bound_s = v;
+    }
+    __syncthreads();
+    bound = bound_s;
+  };
+  // the first top_n of the list, in order, to the other list; returns how many there were
+  auto thin_out = [&](int n) {
+    for (int c = tid; c < n; c += NT) {
+      const float v = cand_z[list][c];
+      const int i = cand_i[list][c];
+      int before = 0;
+      for (int k = 0; k < n; ++k) before += ahead_of(cand_z[list][k], cand_i[list][k], v, i);
+      if (before < a.top_n) {
+        cand_z[list ^ 1][before] = v;
+        cand_i[list ^ 1][before] = i;
+      }
+    }
+    list ^= 1;
+  };
+
+  // (fmaxf of a NaN and a number is the number)
+  for (int b = 0; b < batches || b == 0; ++b) {
+    float x[VB * VE];
+#pragma unroll
+    for (int q = 0; q < VB; ++q)
+#pragma unroll
+      for (int e = 0; e < VE; ++e) x[q * VE + e] = static_cast<float>(next[q][e]);
+    if (b + 1 < batches) request(b + 1);
+    float most = fmaxf(x[0], x[1]);
+#pragma unroll
+    for (int e = 2; e < VB * VE; ++e) most = fmaxf(most, x[e]);
+    if (a.top_n > 0) {
+      if (b == 0) {
+        first_bound(fmaxf(most, stray_z));
+        offer(stray_z, stray);
+      }
+      if (most >= bound) {
+        uint32_t mask = 0;
+#pragma unroll
+        for (int e = VB * VE - 1; e >= 0; --e) mask = mask * 2 + (x[e] >= bound);
+        while (mask) {
+          const int e = __builtin_ctz(mask);
+          mask &= mask - 1;
+          const int i = head + ((b * VB + e / VE) * NT + tid) * VE + e % VE;
+          if (i < tail) offer(static_cast<float>(z[i]), i);  // (again from memory: a register cannot be chosen by a number)
+        }
+      }
+      if (b % kRefine == kRefine - 1) {
+        __syncthreads();
+        const int n = n_cand;
+        if (n > 4 * a.top_n && n <= kCandidates) {
+          thin_out(n);
+          __syncthreads();
+          bound = cand_z[list][a.top_n - 1];
+          if (tid == 0) n_cand = a.top_n;
+        }
+        __syncthreads();
+      }
+    }
+    if (count) {
+      // entries ahead of the token: as large in front of it, larger behind it (the vector it lies in: larger, made good at the end)
+#pragma unroll
+      for (int q = 0; q < VB; ++q) {
+        const float least = head + ((b * VB + q) * NT + tid) * VE + VE <= t ? zt : zt_above;
+#pragma unroll
+        for (int e = 0; e < VE; ++e) ahead += x[q * VE + e] >= least;
+      }
+    }
+    if (most > sum.m) sum.raise(most);
+#pragma unroll
+    for (int e = 0; e < VB * VE; ++e) {
+      const float d = x[e] - sum.m;
+      const float p = __builtin_amdgcn_exp2f(d * kLog2e);
+      sum.s += p;
+      sum.u = fmaf(fmaxf(d, kGone), p, sum.u);
+    }
   }
-  s = block_sum<kLpThreads / 64>(s, red[1]);
-  u = block_sum<kLpThreads / 64>(u, red[2]);
-  ahead = block_sum<kLpThreads / 64>(ahead, red[3]);
-  const bool nothing = m == -INFINITY && s == 0.0f;
-  const float log_s = logf(s);
-  if (threadIdx.x == 0) {
-    if (a.logprob) a.logprob[blockIdx.x] = t < 0 ? 0.0f : t >= V ? __builtin_nanf("") : nothing ? -INFINITY : zt - m - log_s;
-    if (a.entropy) a.entropy[blockIdx.x] = nothing ? 0.0f : log_s - u / s;
-    if (a.rank) a.rank[blockIdx.x] = t < 0 || t >= V || zt != zt ? -1 : static_cast<int>(ahead);
+  {
+    if (stray_z > sum.m) sum.raise(stray_z);
+    const float d = stray_z - sum.m;
+    const float p = __builtin_amdgcn_exp2f(d * kLog2e);
+    sum.s += p;
+    sum.u = fmaf(fmaxf(d, kGone), p, sum.u);
+    if (count) ahead += stray < V && ahead_of(stray_z, stray, zt, t);
+    // equal entries of the token's own vector in front of it
+    if (count && tid == 0 && t >= head && t < tail)
+      for (int i = t - (t - head) % VE; i < t; ++i) ahead += static_cast<float>(z[i]) == zt;
   }
-  // the alternatives one after the other: the first entry behind the one before
+
+  // the block's sums
+  {
+    const float m = wave_reduce_dpp(sum.m, [](float x, float y) { return fmaxf(x, y); });
+    if ((tid & 63) == 0) red[0][tid >> 6] = m;
+    __syncthreads();
+    float all = red[0][0];
+#pragma unroll
+    for (int i = 1; i < NT / 64; ++i) all = fmaxf(all, red[0][i]);
+    sum.raise(all);
+    const float s = wave_sum_dpp(sum.s), u = wave_sum_dpp(sum.u);
+    const int c = wave_reduce_dpp(ahead, [](int x, int y) { return x + y; });
+    if ((tid & 63) == 0) {
+      red[1][tid >> 6] = s;
+      red[2][tid >> 6] = u;
+      red[3][tid >> 6] = __builtin_bit_cast(float, c);
+    }
+    __syncthreads();
+    sum.s = sum.u = 0.0f;
+    ahead = 0;
+#pragma unroll
+    for (int i = 0; i < NT / 64; ++i) {
+      sum.s += red[1][i];
+      sum.u += red[2][i];
+      ahead += __builtin_bit_cast(int, red[3][i]);
+    }
+  }
+  const bool nothing = sum.s == 0.0f;
+  const float log_s = logf(sum.s);
+  if (tid == 0) {
+    if (a.logprob) a.logprob[blockIdx.x] = t < 0 ? 0.0f : t >= V ? __builtin_nanf("") : nothing ? -INFINITY : zt - sum.m - log_s;
+    if (a.entropy) a.entropy[blockIdx.x] = nothing ? 0.0f : log_s - sum.u / sum.s;
+    if (a.rank) a.rank[blockIdx.x] = !has_token || zt != zt ? -1 : ahead;
+  }
+  if (a.top_n == 0) return;
+
+  int* ids = a.top_ids + static_cast<int64_t>(blockIdx.x) * a.top_n;
+  float* tops = a.top_logprobs + static_cast<int64_t>(blockIdx.x) * a.top_n;
+  const int n = n_cand;
+  if (n <= kCandidates) {
+    thin_out(n);
+    __syncthreads();
+    if (tid < a.top_n) {
+      const bool there = tid < n;
+      ids[tid] = there ? cand_i[list][tid] : -1;
+      tops[tid] = there ? cand_z[list][tid] - sum.m - log_s : -INFINITY;
+    }
+    return;
+  }
+  // one after the other: the first entry behind the one before
   float last = INFINITY;
   int last_i = -1;
   for (int k = 0; k < a.top_n; ++k) {
     float best = -INFINITY;
     int bi = V;
-    for (int i = threadIdx.x; i < V; i += kLpThreads) {
-      const float x = at(i);
-      if ((x < last || (x == last && i > last_i)) && x > best) {
-        best = x;
+    for (int i = tid; i < V; i += NT) {
+      const float v = static_cast<float>(z[i]);
+      if (ahead_of(last, last_i, v, i) && v > best) {
+        best = v;
         bi = i;
       }
     }
-    const float top = block_max(best, 0);
-    bi = best == top ? bi : V;
-    bi = wave_reduce_dpp(bi, [](int x, int y) { return min(x, y); });
+    const float wave_best = wave_reduce_dpp(best, [](float x, float y) { return fmaxf(x, y); });
+    bi = wave_reduce_dpp(best == wave_best ? bi : V, [](int x, int y) { return min(x, y); });
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) idx[threadIdx.x >> 6] = bi;
-    __syncthreads();
-    for (int i = 0; i < kLpThreads / 64; ++i) bi = min(bi, idx[i]);
-    if (threadIdx.x == 0) {
-      const int64_t o = static_cast<int64_t>(blockIdx.x) * a.top_n + k;
-      a.top_ids[o] = bi < V ? bi : -1;
-      a.top_logprobs[o] = bi < V ? top - m - log_s : -INFINITY;
+    if ((tid & 63) == 0) {
+      cand_z[0][tid >> 6] = wave_best;
+      cand_i[0][tid >> 6] = bi;
     }
-    last = top;
+    __syncthreads();
+    best = -INFINITY;
+    bi = V;
+    for (int i = 0; i < NT / 64; ++i) {
+      if (cand_i[0][i] < V && ahead_of(cand_z[0][i], cand_i[0][i], best, bi)) {
+        best = cand_z[0][i];
+        bi = cand_i[0][i];
+      }
+    }
+    if (tid == 0) {
+      ids[k] = bi < V ? bi : -1;
+      tops[k] = bi < V ? best - sum.m - log_s : -INFINITY;
+    }
+    last = best;
     last_i = bi;
   }
+}
+
+template <typename T>
+void launch_rows(hipStream_t st, int rows, const LogprobArgs& a) {
+  if (rows <= 2 * device_cu_count()) hipLaunchKernelGGL((token_logprobs_kernel<T, 1024>), dim3(rows), dim3(1024), 0, st, a);
+  else hipLaunchKernelGGL((token_logprobs_kernel<T, 256>), dim3(rows), dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -106,8 +322,8 @@ size_t token_logprobs_workspace_bytes(int rows, int V, int top_n) { return 0; }
 
 int token_logprobs_launch(hipStream_t st, int rows, int V, int io, const void* logits, int64_t ld, const TokenLogprobs& out, void* workspace) {
   LogprobArgs a = {logits, ld, out.tokens, out.logprob, out.entropy, out.rank, out.top_ids, out.top_logprobs, V, out.top_n};
-  if (io == RWKV_IO_F16) hipLaunchKernelGGL(token_logprobs_kernel<half_t>, dim3(rows), dim3(kLpThreads), 0, st, a);
-  else hipLaunchKernelGGL(token_logprobs_kernel<float>, dim3(rows), dim3(kLpThreads), 0, st, a);
+  if (io == RWKV_IO_F16) launch_rows<half_t>(st, rows, a);
+  else launch_rows<float>(st, rows, a);
   RWKV_LAUNCH_CHECK();
   return RWKV_OK;
 }
