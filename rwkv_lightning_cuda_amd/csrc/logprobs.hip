@@ -7,7 +7,7 @@
 //
 // Entries of -infinity have probability 0 and are no alternatives; a row of nothing else gives log probability -infinity, entropy 0
 // and no alternative.
-#include "ops.h"
+#include "softsum.h"
 
 namespace rwkv {
 
@@ -15,41 +15,18 @@ namespace {
 
 constexpr int kCandidates = 1024;  // places for entries that may be among the first top_n
 constexpr int kRefine = 4;         // batches between looks at whether the candidates can be thinned out
-constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kLowest = -3.402823466e38f;
-constexpr float kGone = -200.0f;   // e^-200 is 0 in fp32; a difference that is multiplied by it must not be infinite
 
 struct LogprobArgs {
   const void* logits;
   int64_t ld;
-  const int* tokens;
-  float* logprob;
-  float* entropy;
-  int* rank;
-  int* top_ids;
-  float* top_logprobs;
-  int V, top_n;
-};
-
-// m, S and U of the entries seen so far.  m starts at the lowest finite value, not at -infinity: differences with it are no NaN,
-// and S stays 0 as long as every entry is -infinity.  A NaN or +infinity among the entries makes S a NaN that stays.
-struct SoftSum {
-  float m = kLowest, s = 0.0f, u = 0.0f;
-  __device__ __forceinline__ void raise(float to) {
-    const float t = fmaxf(m - to, kGone);
-    const float f = __builtin_amdgcn_exp2f(t * kLog2e);
-    u = f * fmaf(t, s, u);
-    s *= f;
-    m = to;
-  }
+  int V;
+  TokenLogprobs out;
 };
 
 __device__ __forceinline__ float next_above(float v) {  // the smallest float above v; NaN above +infinity
   const uint32_t b = __builtin_bit_cast(uint32_t, v);
   return v == 0.0f ? __builtin_bit_cast(float, 1u) : __builtin_bit_cast(float, v > 0.0f ? b + 1 : b - 1);
 }
-
-__device__ __forceinline__ bool ahead_of(float v, int i, float w, int k) { return v > w || (v == w && i < k); }
 
 // One block per row, which it reads once: 64 bytes per thread at a time, the next 64 requested before they are looked at.  A thread
 // keeps m, S and U of its entries and raises m when a batch exceeds it.  The rank is a count against the token's logit, which is
@@ -71,7 +48,7 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(LogprobArgs a) {
   __shared__ float bound_s;
   const int tid = threadIdx.x;
   const T* z = static_cast<const T*>(a.logits) + blockIdx.x * a.ld;
-  const int V = a.V;
+  const int V = a.V, top_n = a.out.top_n;
   const int misaligned = static_cast<int>((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
   const int head = misaligned ? min(VE - misaligned, V) : 0;  // entries in front of the first 16-byte boundary
   const int vecs = (V - head) / VE;
@@ -96,12 +73,12 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(LogprobArgs a) {
   // the entries of the two ends, at most one per thread
   const int stray = tid < head ? tid : tail + tid - head;
   const float stray_z = stray < V ? static_cast<float>(z[stray]) : -INFINITY;
-  const int t = a.tokens ? a.tokens[blockIdx.x] : -1;
+  const int t = a.out.tokens ? a.out.tokens[blockIdx.x] : -1;
   const bool has_token = t >= 0 && t < V;
   const float zt = has_token ? static_cast<float>(z[t]) : 0.0f;
-  const bool count = a.rank && has_token;
+  const bool count = a.out.rank && has_token;
   const float zt_above = next_above(zt);
-  if (a.top_n > 0 && tid == 0) n_cand = 0;
+  if (top_n > 0 && tid == 0) n_cand = 0;
 
   SoftSum sum;
   int ahead = 0;
@@ -118,7 +95,7 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(LogprobArgs a) {
   };
   // the top_n-th largest of the groups' maxima (equal ones by group): every thread of the block comes here
   auto first_bound = [&](float mine) {
-    const int groups = a.top_n <= 24 ? 64 : 256;
+    const int groups = top_n <= 24 ? 64 : 256;
     if (mine != mine) mine = -INFINITY;
     const int width = NT / groups;
     if (width > 1) mine = fmaxf(mine, __builtin_bit_cast(float, lane_xor_dpp<1>(__builtin_bit_cast(int, mine))));
@@ -135,7 +112,7 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(LogprobArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) before += ahead_of(w[e], i + e, v, tid);
       }
-      if (before == a.top_n - 1) bound_s = v;
+      if (before == top_n - 1) bound_s = v;
     }
     __syncthreads();
     bound = bound_s;
@@ -147,7 +124,7 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(LogprobArgs a) {
       const int i = cand_i[list][c];
       int before = 0;
       for (int k = 0; k < n; ++k) before += ahead_of(cand_z[list][k], cand_i[list][k], v, i);
-      if (before < a.top_n) {
+      if (before < top_n) {
         cand_z[list ^ 1][before] = v;
         cand_i[list ^ 1][before] = i;
       }
@@ -166,7 +143,7 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(LogprobArgs a) {
     float most = fmaxf(x[0], x[1]);
 #pragma unroll
     for (int e = 2; e < VB * VE; ++e) most = fmaxf(most, x[e]);
-    if (a.top_n > 0) {
+    if (top_n > 0) {
       if (b == 0) {
         first_bound(fmaxf(most, stray_z));
         offer(stray_z, stray);
@@ -185,11 +162,11 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(LogprobArgs a) {
       if (b % kRefine == kRefine - 1) {
         __syncthreads();
         const int n = n_cand;
-        if (n > 4 * a.top_n && n <= kCandidates) {
+        if (n > 4 * top_n && n <= kCandidates) {
           thin_out(n);
           __syncthreads();
-          bound = cand_z[list][a.top_n - 1];
-          if (tid == 0) n_cand = a.top_n;
+          bound = cand_z[list][top_n - 1];
+          if (tid == 0) n_cand = top_n;
         }
         __syncthreads();
       }
@@ -250,22 +227,20 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(LogprobArgs a) {
       ahead += __builtin_bit_cast(int, red[3][i]);
     }
   }
-  const bool nothing = sum.s == 0.0f;
   const float log_s = logf(sum.s);
   if (tid == 0) {
-    if (a.logprob) a.logprob[blockIdx.x] = t < 0 ? 0.0f : t >= V ? __builtin_nanf("") : nothing ? -INFINITY : zt - sum.m - log_s;
-    if (a.entropy) a.entropy[blockIdx.x] = nothing ? 0.0f : log_s - sum.u / sum.s;
-    if (a.rank) a.rank[blockIdx.x] = !has_token || zt != zt ? -1 : ahead;
+    write_logprobs(sum, a.out, blockIdx.x, V, &zt);
+    if (a.out.rank) a.out.rank[blockIdx.x] = !has_token || zt != zt ? -1 : ahead;
   }
-  if (a.top_n == 0) return;
+  if (top_n == 0) return;
 
-  int* ids = a.top_ids + static_cast<int64_t>(blockIdx.x) * a.top_n;
-  float* tops = a.top_logprobs + static_cast<int64_t>(blockIdx.x) * a.top_n;
+  int* ids = a.out.top_ids + static_cast<int64_t>(blockIdx.x) * top_n;
+  float* tops = a.out.top_logprobs + static_cast<int64_t>(blockIdx.x) * top_n;
   const int n = n_cand;
   if (n <= kCandidates) {
     thin_out(n);
     __syncthreads();
-    if (tid < a.top_n) {
+    if (tid < top_n) {
       const bool there = tid < n;
       ids[tid] = there ? cand_i[list][tid] : -1;
       tops[tid] = there ? cand_z[list][tid] - sum.m - log_s : -INFINITY;
@@ -275,7 +250,7 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(LogprobArgs a) {
   // one after the other: the first entry behind the one before
   float last = INFINITY;
   int last_i = -1;
-  for (int k = 0; k < a.top_n; ++k) {
+  for (int k = 0; k < top_n; ++k) {
     float best = -INFINITY;
     int bi = V;
     for (int i = tid; i < V; i += NT) {
@@ -321,7 +296,7 @@ void launch_rows(hipStream_t st, int rows, const LogprobArgs& a) {
 size_t token_logprobs_workspace_bytes(int rows, int V, int top_n) { return 0; }
 
 int token_logprobs_launch(hipStream_t st, int rows, int V, int io, const void* logits, int64_t ld, const TokenLogprobs& out, void* workspace) {
-  LogprobArgs a = {logits, ld, out.tokens, out.logprob, out.entropy, out.rank, out.top_ids, out.top_logprobs, V, out.top_n};
+  LogprobArgs a = {logits, ld, V, out};
   if (io == RWKV_IO_F16) launch_rows<half_t>(st, rows, a);
   else launch_rows<float>(st, rows, a);
   RWKV_LAUNCH_CHECK();
