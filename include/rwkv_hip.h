@@ -369,6 +369,18 @@ int rwkv_hip_session_set_graph(rwkv_hip_session* s, int use_graph);
  * src/rwkv7_fast_v4.cu:1343) unless sync == 0. */
 int rwkv_hip_forward(rwkv_hip_session* s, const int64_t* tokens_host, int B, int T, void* shift, void* wkv,
                      void* elapsed, void* logits, int sync);
+/* Scores texts (no counterpart in the reference, whose forward pass gives the last position's logits only): runs tokens_host [B,T] as
+ * rwkv_hip_forward does, state and all, and gives the log probability of targets_host [B,T] (host, int64; -1: none, 0 is its log
+ * probability; NULL with logprob NULL) at EVERY position, as rwkv_hip_token_logprobs defines it: device tensors logprob, entropy f32
+ * [B,T], top_ids i32 and top_logprobs f32 [B,T,top_n], each may be NULL, not all.  logits f32 [B,V] of the last position, or NULL
+ * (which saves its head product).  A text is scored in one call or in several, the state between them, with the target of a
+ * call's last position being the next call's first token.  Heads in fp16 and int8 with a packed copy (rwkv_hip_linear_logprobs) keep
+ * their logits in fp32; other heads' are rounded to fp16 as rwkv_hip_forward gives them.  act_int8 != 0 (int8 heads): the final norm's output
+ * in 8 bits with a scale per position (rwkv_hip_add_norm_q8), whole-number products: up to twice as fast, log probabilities about a
+ * hundredth off.  Not captured into graphs; not while a profiling mode is on.  The session keeps a workspace of its largest call. */
+int rwkv_hip_score(rwkv_hip_session* s, const int64_t* tokens_host, const int64_t* targets_host, int B, int T, void* shift, void* wkv,
+                   void* elapsed, void* logits, int act_int8, int top_n, void* logprob, void* entropy, void* top_ids, void* top_logprobs,
+                   int sync);
 /* Greedy decode loop kept on the device: runs `steps` decode steps at batch B, feeding each row's
  * argmax back as its next token without a host round trip; out_tokens_host [steps,B] int32.
  * first_tokens_host [B] are the tokens of step 0. */

@@ -48,6 +48,16 @@ class InferenceEngine {
                                               const StreamCallback& emit,
                                               const ControlCallback& should_stop = {}) const;
 
+  // How probable a text is, token by token (no counterpart in the reference).  Row i of `at` belongs to tokens[i] given the tokens in
+  // front of it; row 0 has none: log probability and entropy 0, no alternatives.  Texts of any lengths in one call; each starts from
+  // an empty state.
+  struct TextScore {
+    std::vector<int64_t> tokens;
+    TokenLogprobs at;
+    double total() const;  // sum of the log probabilities
+  };
+  std::vector<TextScore> score(const std::vector<std::string>& texts, const ScoreOptions& options = {}) const;
+
   std::string format_openai_prompt(const std::string& system,
                                    const std::vector<std::pair<std::string, std::string>>& messages,
                                    ThinkType think_type) const;

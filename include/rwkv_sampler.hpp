@@ -37,4 +37,9 @@ std::vector<int> sample_batch_repetition_temperature_topk_topp(const DeviceLogit
                                                                SamplerPenaltyState& penalties,
                                                                const GenerateOptions& options);
 
+// Log probability, entropy and rank of tokens[row] (-1: none) under each row of logits, with the top_n (0 .. 64) most probable entries:
+// what a server returns as `logprobs` beside a sampled token.  Of the logits as they are, before penalties and temperature.  Streams as
+// above.  No counterpart in the reference.
+TokenLogprobs token_logprobs(const DeviceLogits& logits, const std::vector<int>& tokens, int top_n = 0);
+
 }  // namespace rwkv7_server

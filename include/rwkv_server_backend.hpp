@@ -64,6 +64,22 @@ struct DeviceLogits {
   DeviceLogits& operator=(DeviceLogits&&) noexcept = default;
 };
 
+// Log probabilities of given tokens, on the host, `rows` of them one after the other (no counterpart in the reference).
+struct TokenLogprobs {
+  int rows = 0;
+  int top_n = 0;
+  std::vector<float> logprob;        // ln of the softmax at the row's token; 0 where it has none (-1)
+  std::vector<float> entropy;        // nats
+  std::vector<int> rank;             // entries ahead of the token, 0 = most probable; empty where it is not known (score)
+  std::vector<int> top_ids;          // [rows, top_n] most probable first, -1 past the last with any probability
+  std::vector<float> top_logprobs;   // [rows, top_n]
+};
+
+struct ScoreOptions {
+  int top_n = 0;           // most probable entries per position, up to 64
+  bool int8_head = false;  // int8 heads: the head's input in 8 bits too (faster, log probabilities about a hundredth off)
+};
+
 class IModelBackend {
  public:
   virtual ~IModelBackend() = default;
@@ -78,6 +94,11 @@ class IModelBackend {
   virtual void copy_logits_slice(const DeviceLogits& src, int src_offset, DeviceLogits& dst, int dst_offset,
                                  int count) const = 0;
   virtual PrefillCapacity query_prefill_capacity(int prefill_chunk_size) const = 0;
+
+  // forward_prefill without logits, with the log probability of target_batches (same shape; -1: none) at every position, rows of a
+  // batch one after the other.  Backends that do not score refuse.
+  virtual TokenLogprobs score(const std::vector<std::vector<int64_t>>& token_batches, const std::vector<std::vector<int64_t>>& target_batches,
+                              GenerationState& state, const ScoreOptions& options) const;
 
   virtual int vocab_size() const = 0;
   virtual const std::string& model_path() const = 0;
@@ -109,6 +130,8 @@ class ModelBackend final : public IModelBackend {
   void copy_logits_slice(const DeviceLogits& src, int src_offset, DeviceLogits& dst, int dst_offset,
                          int count) const override;
   PrefillCapacity query_prefill_capacity(int prefill_chunk_size) const override;
+  TokenLogprobs score(const std::vector<std::vector<int64_t>>& token_batches, const std::vector<std::vector<int64_t>>& target_batches,
+                      GenerationState& state, const ScoreOptions& options) const override;
 
   int vocab_size() const override;
   const std::string& model_path() const override;

@@ -394,7 +394,7 @@ int check_shape(const char* who, int fmt, bool x_int8, int M, int N, int K) {
   RWKV_REQUIRE(!x_int8 || fmt == RWKV_FMT_W8, "%s: int8 x needs int8 weights", who);
   RWKV_REQUIRE(M > 0, "%s: M must be positive, got %d", who, M);
   RWKV_REQUIRE(linear_packed_supported(fmt, M, N, K), "%s: unsupported shape N=%d K=%d (multiples of 32 and 256)", who, N, K);
-  RWKV_REQUIRE(N <= kMaxLogprobVocab && K <= 16384, "%s: N up to %d and K up to 16384, got %d and %d", who, kMaxLogprobVocab, N, K);
+  RWKV_REQUIRE(N <= kMaxLogprobVocab && K <= kMaxHeadWidth, "%s: N up to %d and K up to %d, got %d and %d", who, kMaxLogprobVocab, kMaxHeadWidth, N, K);
   return RWKV_OK;
 }
 

@@ -158,6 +158,10 @@ struct rwkv_hip_session {
   std::vector<std::pair<hipEvent_t, hipEvent_t>> prof_events;
   void* gemm_ws = nullptr;  // split-K partials of the packed GEMM
   size_t gemm_ws_bytes = 0;
+  void* score_ws = nullptr;   // rwkv_hip_score: targets, scales of int8 values, what the head leaves between its launches
+  size_t score_ws_bytes = 0;
+  int* targets_pinned = nullptr;
+  int targets_cap = 0;
   void* sparse_ws = nullptr;  // partial rows of the row-skipping ffn.value product
   size_t sparse_ws_bytes = 0;
   float* widened[4] = {};     // rwkv_hip_session_debug_buffer: fp32 copies of r, k2, nkk, kka, made when they are asked for
@@ -434,8 +438,67 @@ bool walks_ffn_value(const rwkv_hip_session* s, const Matrix& mv, int rows) {
     if (s->profile != 2) TRY(expr);  \
   } while (0)
 
-// Enqueues the whole forward pass on the session stream.  tokens are already in s->tokens_dev.
-int enqueue_forward(rwkv_hip_session* s, int B, int T, half_t* shift, void* wkv_any, int* elapsed, float* logits) {
+// What rwkv_hip_score asks of a forward pass: log probabilities at every position.
+struct ScoreArgs {
+  bool act_int8;
+  TokenLogprobs out;   // tokens: in the session's workspace
+  float* x_scale;      // [rows], int8 values only
+  unsigned char* rest;
+};
+
+// Heads whose logits become log probabilities inside the product; the others' (int4, no packed copy) go through blocks of rows of
+// logits, rounded to fp16 as a forward pass gives them.
+bool head_scores_itself(const rwkv_hip_model* m) { return m->head.packed && m->head.fmt != RWKV_FMT_W4; }
+constexpr int kScoreLogitRows = 64;
+
+size_t score_rest_bytes(const rwkv_hip_model* m, bool act_int8, int rows, int top_n) {
+  if (head_scores_itself(m)) return linear_logprobs_workspace_bytes(m->head.fmt, act_int8, rows, m->V, m->C, top_n);
+  const int block = std::min(rows, kScoreLogitRows);
+  size_t gemm = 0;
+  if (m->head.packed) {
+    const PackedProblem p = m->head.packed_problem(m->V, nullptr, nullptr);
+    gemm = linear_packed_multi_workspace_bytes(block, m->C, 1, &p, RWKV_EPI_NONE, 1);
+    if (rows % block) gemm = std::max(gemm, linear_packed_multi_workspace_bytes(rows % block, m->C, 1, &p, RWKV_EPI_NONE, 1));
+  }
+  return align_up(static_cast<size_t>(block) * m->V * sizeof(float), 256) + align_up(token_logprobs_workspace_bytes(block, m->V, top_n), 256) + gemm;
+}
+
+// The final norm of every row and the head's log probabilities; x1 + cm is the residual stream behind the last layer.
+int enqueue_score(rwkv_hip_session* s, int rows, const ScoreArgs& a) {
+  const rwkv_hip_model* m = s->model;
+  Buffers& b = s->buf;
+  const int C = m->C, V = m->V;
+  if (a.act_int8) {
+    TRY(rwkv_hip_add_norm_q8(s->stream, rows, C, RWKV_NORM_LAYER, b.x1, b.cm, m->ln_out_w, m->ln_out_b, kLnEps, nullptr, b.scratch, a.x_scale));
+  } else {
+    LnArgs n = {};
+    n.x = b.x1; n.res = b.cm; n.w = m->ln_out_w; n.b = m->ln_out_b; n.x_out = b.x; n.y = b.scratch; n.C = C; n.T = 1; n.eps = kLnEps;
+    TRY(ln_launch(s->stream, kAddLn, rows, n));
+  }
+  if (head_scores_itself(m))
+    return linear_logprobs_launch(s->stream, m->head.fmt, rows, V, C, b.scratch, a.act_int8 ? a.x_scale : nullptr, m->head.packed, m->head.scale, a.out, a.rest);
+  const int block = std::min(rows, kScoreLogitRows);
+  float* logits = reinterpret_cast<float*>(a.rest);
+  unsigned char* lp_ws = a.rest + align_up(static_cast<size_t>(block) * V * sizeof(float), 256);
+  unsigned char* gemm_ws = lp_ws + align_up(token_logprobs_workspace_bytes(block, V, a.out.top_n), 256);
+  for (int r = 0; r < rows; r += block) {
+    const int n = std::min(block, rows - r);
+    const half_t* x = b.scratch + static_cast<int64_t>(r) * C;
+    if (m->head.packed) {
+      const PackedProblem p = m->head.packed_problem(V, x, logits);
+      const size_t bytes = linear_packed_multi_workspace_bytes(n, C, 1, &p, RWKV_EPI_NONE, 1);
+      TRY(linear_packed_multi(s->stream, n, C, 1, &p, RWKV_EPI_NONE, 1, gemm_ws, bytes));
+    } else {
+      TRY(linear_any_m(s->stream, m->head.fmt, n, V, C, x, m->head.data, m->head.scale, m->head.zp, RWKV_EPI_NONE, 1, logits));
+    }
+    TRY(token_logprobs_launch(s->stream, n, V, RWKV_IO_F32, logits, V, a.out.from_row(r), lp_ws));
+  }
+  return RWKV_OK;
+}
+
+// Enqueues the whole forward pass on the session stream.  tokens are already in s->tokens_dev.  With `score` logits may be NULL.
+int enqueue_forward(rwkv_hip_session* s, int B, int T, half_t* shift, void* wkv_any, int* elapsed, float* logits,
+                    const ScoreArgs* score = nullptr) {
   float* wkv = static_cast<float*>(wkv_any);            // fp32 state (the default)
   half_t* wkv16 = static_cast<half_t*>(wkv_any);        // fp16 state (session option)
   const rwkv_hip_model* m = s->model;
@@ -736,6 +799,7 @@ int enqueue_forward(rwkv_hip_session* s, int B, int T, half_t* shift, void* wkv_
     // On the packed path the LayerNorm kernels that consume the output projection and
     // ffn.value sum the split-K partials themselves instead of a reduce launch; att / cm then stay unwritten.
     const bool defer_ok = !s->trace && !ln_in_linear;
+    const bool defer_cm = defer_ok && !(score && l + 1 == L);  // (two norms read the last one)
     DeferredReduce att_partial;
     if (gate_split) {
       const Matrix& mo = w.m[RWKV_M_ATT_O];
@@ -796,7 +860,7 @@ int enqueue_forward(rwkv_hip_session* s, int B, int T, half_t* shift, void* wkv_
                                   &cp, true));
       } else if (rows > 8 || (mv.packed && rows >= kPackedMinRows)) {
         // (rows too long for the few-row launches: the packed product, whose first block moves the row too)
-        TRY_PROF(apply_matrix(s, mv, rows, C, F, b.act, RWKV_EPI_NONE, 0, b.cm, defer_ok ? &cm_partial : nullptr, &cp));
+        TRY_PROF(apply_matrix(s, mv, rows, C, F, b.act, RWKV_EPI_NONE, 0, b.cm, defer_cm ? &cm_partial : nullptr, &cp));
       } else {
         LinearProblem pv = {mv.data, mv.scale, mv.zp, b.act, b.cm, C, mv.fmt, nullptr};
         TRY_PROF(linear_small_m(st, rows, F, 1, &pv, RWKV_EPI_NONE, 0, nullptr, &cp));
@@ -810,7 +874,7 @@ int enqueue_forward(rwkv_hip_session* s, int B, int T, half_t* shift, void* wkv_
         TRY_AUX(ffn_sparse_launch(st, mv.fmt, rows, C, F, 1, b.act, mv.sparse_t, mv.scale, s->sparse_ws, s->sparse_ws_bytes, b.cm,
                                   nullptr, true));
       } else {
-        TRY_PROF(apply_matrix(s, mv, rows, C, F, b.act, RWKV_EPI_NONE, 0, b.cm, defer_ok ? &cm_partial : nullptr));
+        TRY_PROF(apply_matrix(s, mv, rows, C, F, b.act, RWKV_EPI_NONE, 0, b.cm, defer_cm ? &cm_partial : nullptr));
       }
     }
 
@@ -843,7 +907,7 @@ int enqueue_forward(rwkv_hip_session* s, int B, int T, half_t* shift, void* wkv_
       LnArgs a = {};
       a.x = b.x1; a.res = b.cm; a.w = m->ln_out_w; a.b = m->ln_out_b; a.y = b.xf; a.C = C; a.T = T; a.eps = kLnEps;
       take_deferred(a, cm_partial);
-      TRY_AUX(ln_launch(st, kAddLastLn, B, a));
+      if (logits) TRY_AUX(ln_launch(st, kAddLastLn, B, a));
       if (s->trace) {
         LnArgs t = {};
         t.x = b.x1; t.res = b.cm; t.w = m->ln_out_w; t.b = m->ln_out_b; t.x_out = b.x; t.y = b.scratch;
@@ -859,7 +923,8 @@ int enqueue_forward(rwkv_hip_session* s, int B, int T, half_t* shift, void* wkv_
 
   TRY(flush_pending());
   TRY_AUX(advance_launch(st, B, T, elapsed));
-  TRY_PROF(apply_matrix(s, m->head, B, V, C, b.xf, RWKV_EPI_NONE, 1, logits));
+  if (logits) TRY_PROF(apply_matrix(s, m->head, B, V, C, b.xf, RWKV_EPI_NONE, 1, logits));
+  if (score) TRY(enqueue_score(s, rows, *score));
   if (pass_begin) {
     hipEvent_t pass_end = nullptr;
     RWKV_HIP_TRY(hipEventCreate(&pass_end));
@@ -1116,6 +1181,8 @@ int rwkv_hip_session_destroy(rwkv_hip_session* s) {
   }
   if (s->arena.base) (void)hipFree(s->arena.base);
   if (s->gemm_ws) (void)hipFree(s->gemm_ws);
+  if (s->score_ws) (void)hipFree(s->score_ws);
+  if (s->targets_pinned) (void)hipHostFree(s->targets_pinned);
   if (s->sparse_ws) (void)hipFree(s->sparse_ws);
   for (float* p : s->widened)
     if (p) (void)hipFree(p);
@@ -1300,6 +1367,63 @@ int rwkv_hip_forward(rwkv_hip_session* s, const int64_t* tokens_host, int B, int
   } else {
     TRY(enqueue_forward(s, B, T, static_cast<half_t*>(shift), wkv, static_cast<int*>(elapsed), static_cast<float*>(logits)));
   }
+  if (sync) RWKV_HIP_TRY(hipStreamSynchronize(s->stream));
+  return RWKV_OK;
+}
+
+int rwkv_hip_score(rwkv_hip_session* s, const int64_t* tokens_host, const int64_t* targets_host, int B, int T, void* shift, void* wkv,
+                   void* elapsed, void* logits, int act_int8, int top_n, void* logprob, void* entropy, void* top_ids, void* top_logprobs,
+                   int sync) {
+  RWKV_REQUIRE(s != nullptr, "session is NULL");
+  RWKV_REQUIRE(B > 0, "token_batches must not be empty");
+  RWKV_REQUIRE(T > 0, "token batch length must be positive");
+  RWKV_REQUIRE(static_cast<int64_t>(B) * T <= (1 << 24), "score: %d x %d tokens in one call", B, T);
+  RWKV_REQUIRE(shift && wkv && elapsed, "score: NULL state tensor");
+  TRY(model_ready(s->model));
+  const rwkv_hip_model* m = s->model;
+  RWKV_REQUIRE(tokens_host, "score: tokens is NULL");
+  RWKV_REQUIRE(!s->profile, "score: not while a profiling mode is on");
+  const int rows = B * T;
+  for (int i = 0; i < rows; ++i) {
+    RWKV_REQUIRE(tokens_host[i] >= 0 && tokens_host[i] < m->V, "token id out of range");
+    RWKV_REQUIRE(!targets_host || (targets_host[i] >= -1 && targets_host[i] < m->V), "target id out of range");
+  }
+  RWKV_REQUIRE(!act_int8 || (head_scores_itself(m) && m->head.fmt == RWKV_FMT_W8), "score: int8 values need an int8 head (with a packed copy)");
+  RWKV_REQUIRE(m->V <= kMaxLogprobVocab && m->C <= kMaxHeadWidth, "score: V up to %d and C up to %d", kMaxLogprobVocab, kMaxHeadWidth);
+  ScoreArgs a = {act_int8 != 0, {}, nullptr, nullptr};
+  a.out = {targets_host ? reinterpret_cast<const int*>(s) : nullptr,  // (whether there are any; the device copy is made below)
+           top_n, static_cast<float*>(logprob), static_cast<float*>(entropy), nullptr, static_cast<int*>(top_ids), static_cast<float*>(top_logprobs)};
+  TRY(check_token_logprobs("score", a.out));
+  TRY(ensure_arena(s, B, T));
+  // the pinned staging buffers may still be in flight from the previous call
+  RWKV_HIP_TRY(hipStreamSynchronize(s->stream));
+  const size_t targets_bytes = align_up(static_cast<size_t>(rows) * sizeof(int), 256);
+  const size_t need = 2 * targets_bytes + score_rest_bytes(m, a.act_int8, rows, top_n);
+  if (need > s->score_ws_bytes) {
+    if (s->score_ws) RWKV_HIP_TRY(hipFree(s->score_ws));
+    s->score_ws = nullptr;
+    s->score_ws_bytes = 0;
+    RWKV_HIP_TRY(hipMalloc(&s->score_ws, need));
+    s->score_ws_bytes = need;
+  }
+  if (rows > s->targets_cap) {
+    if (s->targets_pinned) RWKV_HIP_TRY(hipHostFree(s->targets_pinned));
+    s->targets_pinned = nullptr;
+    s->targets_cap = 0;
+    RWKV_HIP_TRY(hipHostMalloc(reinterpret_cast<void**>(&s->targets_pinned), rows * sizeof(int), hipHostMallocDefault));
+    s->targets_cap = rows;
+  }
+  unsigned char* ws = static_cast<unsigned char*>(s->score_ws);
+  a.x_scale = reinterpret_cast<float*>(ws + targets_bytes);
+  a.rest = ws + 2 * targets_bytes;
+  std::copy(tokens_host, tokens_host + rows, s->tokens_pinned);
+  RWKV_HIP_TRY(hipMemcpyAsync(s->tokens_dev, s->tokens_pinned, sizeof(int64_t) * rows, hipMemcpyHostToDevice, s->stream));
+  if (targets_host) {
+    for (int i = 0; i < rows; ++i) s->targets_pinned[i] = static_cast<int>(targets_host[i]);
+    RWKV_HIP_TRY(hipMemcpyAsync(ws, s->targets_pinned, sizeof(int) * rows, hipMemcpyHostToDevice, s->stream));
+    a.out.tokens = reinterpret_cast<const int*>(ws);
+  }
+  TRY(enqueue_forward(s, B, T, static_cast<half_t*>(shift), wkv, static_cast<int*>(elapsed), static_cast<float*>(logits), &a));
   if (sync) RWKV_HIP_TRY(hipStreamSynchronize(s->stream));
   return RWKV_OK;
 }

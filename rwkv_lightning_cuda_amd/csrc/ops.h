@@ -230,6 +230,7 @@ int argmax_launch(hipStream_t st, int B, int V, const float* logits, int* out, i
 // ---- logprobs.hip, linear_logprobs.hip: log probabilities of given tokens -------------------------------------
 constexpr int kMaxAlternatives = 64;
 constexpr int kMaxLogprobVocab = 1048576;  // as the sampler's
+constexpr int kMaxHeadWidth = 16384;
 struct TokenLogprobs {
   const int* tokens;    // [rows]: < 0 none, log probability 0 and rank -1; >= V NaN and -1.  NULL where neither is asked for
   int top_n;

@@ -665,6 +665,61 @@ void ModelBackend::forward_decode(const std::vector<int64_t>& token_batch, Gener
   impl_->forward(token_batch, B, 1, state, logits);
 }
 
+TokenLogprobs IModelBackend::score(const std::vector<std::vector<int64_t>>&, const std::vector<std::vector<int64_t>>&, GenerationState&,
+                                   const ScoreOptions&) const {
+  throw std::runtime_error("this backend does not score");
+}
+
+TokenLogprobs ModelBackend::score(const std::vector<std::vector<int64_t>>& token_batches,
+                                  const std::vector<std::vector<int64_t>>& target_batches, GenerationState& state,
+                                  const ScoreOptions& options) const {
+  const int B = static_cast<int>(token_batches.size());
+  if (B <= 0) throw std::runtime_error("token_batches must not be empty");
+  if (state.batch_size != B) throw std::runtime_error("state batch size mismatch");
+  if (state.wkv32 != impl_->use_wkv32) throw std::runtime_error("state wkv precision mismatch");
+  const int T = static_cast<int>(token_batches.front().size());
+  if (T <= 0) throw std::runtime_error("token batch length must be positive");
+  if (target_batches.size() != token_batches.size()) throw std::runtime_error("target batches do not match token batches");
+  if (options.top_n < 0 || options.top_n > 64) throw std::runtime_error("top_n must lie in 0 .. 64");
+  std::vector<int64_t> tokens, targets;
+  for (int b = 0; b < B; ++b) {
+    if (static_cast<int>(token_batches[b].size()) != T) throw std::runtime_error("all token batches must share the same length");
+    if (static_cast<int>(target_batches[b].size()) != T) throw std::runtime_error("target batches do not match token batches");
+    tokens.insert(tokens.end(), token_batches[b].begin(), token_batches[b].end());
+    targets.insert(targets.end(), target_batches[b].begin(), target_batches[b].end());
+  }
+  TokenLogprobs out;
+  out.rows = B * T;
+  out.top_n = options.top_n;
+  const std::size_t rows = static_cast<std::size_t>(B) * T, top = rows * options.top_n;
+  // one buffer: log probabilities, entropies, the alternatives' and their ids
+  DeviceBuffer<float> dev;
+  dev.resize_recycled(2 * rows + 2 * top, "alloc scores");
+  float* top_logprobs = top ? dev.p + 2 * rows : nullptr;
+  float* top_ids = top ? dev.p + 2 * rows + top : nullptr;
+  rwkv_hip_session* s = impl_->acquire();
+  int rc = rwkv_hip_session_set_wkv_fp16(s, impl_->use_wkv32 ? 0 : 1);
+  if (rc == RWKV_OK) {
+    void* wkv = impl_->use_wkv32 ? static_cast<void*>(state.wkv_state32.p) : static_cast<void*>(state.wkv_state.p);
+    rc = rwkv_hip_score(s, tokens.data(), targets.data(), B, T, state.shift.p, wkv, state.elapsed.p, nullptr, options.int8_head ? 1 : 0,
+                        options.top_n, dev.p, dev.p + rows, top_ids, top_logprobs, 1);
+  }
+  const std::string msg = rc == RWKV_OK ? std::string() : std::string(rwkv_hip_last_error());
+  impl_->release(s);
+  if (rc != RWKV_OK) throw std::runtime_error(msg);
+  out.logprob.resize(rows);
+  out.entropy.resize(rows);
+  out.top_logprobs.resize(top);
+  out.top_ids.resize(top);
+  check_hip(rwkv_hip_memcpy_d2h(out.logprob.data(), dev.p, rows * sizeof(float)), "copy log probabilities");
+  check_hip(rwkv_hip_memcpy_d2h(out.entropy.data(), dev.p + rows, rows * sizeof(float)), "copy entropies");
+  if (top) {
+    check_hip(rwkv_hip_memcpy_d2h(out.top_logprobs.data(), top_logprobs, top * sizeof(float)), "copy alternatives");
+    check_hip(rwkv_hip_memcpy_d2h(out.top_ids.data(), top_ids, top * sizeof(int)), "copy alternatives");
+  }
+  return out;
+}
+
 void ModelBackend::copy_state_slice(const GenerationState& src, int src_offset, GenerationState& dst, int dst_offset,
                                     int count) const {
   if (src_offset < 0 || dst_offset < 0 || count <= 0) throw std::runtime_error("invalid backend state slice range");

@@ -6,6 +6,7 @@
 
 #include <algorithm>
 #include <chrono>
+#include <limits>
 #include <numeric>
 #include <stdexcept>
 
@@ -265,6 +266,56 @@ int InferenceEngine::prefill_prompt(const std::string& prompt, GenerationState& 
   std::vector<std::vector<int64_t>> one{encode_prompt(prompt)};
   prefill_batch_chunked(one, state, logits);
   return static_cast<int>(one.front().size());
+}
+
+double InferenceEngine::TextScore::total() const { return std::accumulate(at.logprob.begin(), at.logprob.end(), 0.0); }
+
+// Rectangular calls of at most prefill_chunk_size_ positions over the texts that are not finished (a prefix, longest first); a text that
+// ends inside a chunk is filled up with token 0 and no target, and drops out of the state behind it.
+std::vector<InferenceEngine::TextScore> InferenceEngine::score(const std::vector<std::string>& texts, const ScoreOptions& options) const {
+  if (texts.empty()) return {};
+  std::vector<size_t> original;
+  const std::vector<std::vector<int64_t>> sorted = encode_prompts_sorted(texts, original);
+  std::vector<TextScore> out(texts.size());
+  for (size_t i = 0; i < sorted.size(); ++i) {
+    TextScore& t = out[original[i]];
+    t.tokens = sorted[i];
+    t.at.rows = static_cast<int>(sorted[i].size());
+    t.at.top_n = options.top_n;
+    t.at.logprob.assign(1, 0.0f);
+    t.at.entropy.assign(1, 0.0f);
+    t.at.top_ids.assign(options.top_n, -1);
+    t.at.top_logprobs.assign(options.top_n, -std::numeric_limits<float>::infinity());
+  }
+  int width = 0;
+  GenerationState state;
+  for (size_t done = 0;; done += prefill_chunk_size_) {
+    int active = 0;
+    while (active < static_cast<int>(sorted.size()) && sorted[active].size() > done + 1) ++active;
+    if (active == 0) return out;
+    if (active != width) {
+      GenerationState next = model_->create_state(active);
+      if (done > 0) model_->copy_state_slice(state, 0, next, 0, active);
+      state = std::move(next);
+      width = active;
+    }
+    const size_t step = std::min(sorted[0].size() - 1 - done, static_cast<size_t>(prefill_chunk_size_));
+    std::vector<std::vector<int64_t>> tokens(active, std::vector<int64_t>(step, 0)), targets(active, std::vector<int64_t>(step, -1));
+    for (int b = 0; b < active; ++b)
+      for (size_t i = 0; i < step && done + i + 1 < sorted[b].size(); ++i) {
+        tokens[b][i] = sorted[b][done + i];
+        targets[b][i] = sorted[b][done + i + 1];
+      }
+    const TokenLogprobs part = model_->score(tokens, targets, state, options);
+    for (int b = 0; b < active; ++b) {
+      TokenLogprobs& at = out[original[b]].at;
+      const size_t n = std::min(step, sorted[b].size() - 1 - done), row = b * step, top = options.top_n;
+      at.logprob.insert(at.logprob.end(), part.logprob.begin() + row, part.logprob.begin() + row + n);
+      at.entropy.insert(at.entropy.end(), part.entropy.begin() + row, part.entropy.begin() + row + n);
+      at.top_ids.insert(at.top_ids.end(), part.top_ids.begin() + row * top, part.top_ids.begin() + (row + n) * top);
+      at.top_logprobs.insert(at.top_logprobs.end(), part.top_logprobs.begin() + row * top, part.top_logprobs.begin() + (row + n) * top);
+    }
+  }
 }
 
 // Single-row loop with an optional emitter.  The returned text is the concatenation of every generated

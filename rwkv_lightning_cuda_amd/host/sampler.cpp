@@ -62,4 +62,43 @@ int sample_repetition_temperature_topk_topp(const DeviceLogits& logits, SamplerP
   return sample_batch_repetition_temperature_topk_topp(logits, penalties, options).front();
 }
 
+TokenLogprobs token_logprobs(const DeviceLogits& logits, const std::vector<int>& tokens, int top_n) {
+  using rwkv7_fast_v4::DeviceBuffer;
+  using rwkv7_fast_v4::check_hip;
+  if (logits.rows <= 0) throw std::runtime_error("token_logprobs expects at least one logits row");
+  if (logits.vocab_size <= 0 || logits.values.p == nullptr) throw std::runtime_error("empty device logits");
+  if (static_cast<int>(tokens.size()) != logits.rows) throw std::runtime_error("token_logprobs expects a token per logits row");
+  for (const int t : tokens)
+    if (t < -1 || t >= logits.vocab_size) throw std::runtime_error("token id out of range");
+  std::size_t need = 0;
+  if (rwkv_hip_token_logprobs_workspace(logits.rows, logits.vocab_size, top_n, &need) != RWKV_OK) throw std::invalid_argument(rwkv_hip_last_error());
+  const std::size_t rows = tokens.size(), top = rows * top_n;
+  // one buffer of 32-bit values: tokens, log probabilities, entropies, ranks, the alternatives' log probabilities and ids
+  DeviceBuffer<float> dev;
+  DeviceBuffer<std::uint8_t> workspace;
+  dev.resize_recycled(4 * rows + 2 * top, "alloc log probabilities");
+  if (need) workspace.resize_recycled(need, "alloc log probability workspace");
+  check_hip(rwkv_hip_memcpy_h2d(dev.p, tokens.data(), rows * sizeof(int)), "copy tokens");
+  const int rc = rwkv_hip_token_logprobs(nullptr, logits.rows, logits.vocab_size, RWKV_IO_F32, logits.values.p, logits.vocab_size, dev.p, top_n,
+                                         dev.p + rows, dev.p + 2 * rows, dev.p + 3 * rows, top ? dev.p + 4 * rows + top : nullptr,
+                                         top ? dev.p + 4 * rows : nullptr, workspace.p, need);
+  if (rc != RWKV_OK) throw std::invalid_argument(rwkv_hip_last_error());
+  TokenLogprobs out;
+  out.rows = logits.rows;
+  out.top_n = top_n;
+  out.logprob.resize(rows);
+  out.entropy.resize(rows);
+  out.rank.resize(rows);
+  out.top_logprobs.resize(top);
+  out.top_ids.resize(top);
+  check_hip(rwkv_hip_memcpy_d2h(out.logprob.data(), dev.p + rows, rows * sizeof(float)), "copy log probabilities");
+  check_hip(rwkv_hip_memcpy_d2h(out.entropy.data(), dev.p + 2 * rows, rows * sizeof(float)), "copy entropies");
+  check_hip(rwkv_hip_memcpy_d2h(out.rank.data(), dev.p + 3 * rows, rows * sizeof(int)), "copy ranks");
+  if (top) {
+    check_hip(rwkv_hip_memcpy_d2h(out.top_logprobs.data(), dev.p + 4 * rows, top * sizeof(float)), "copy alternatives");
+    check_hip(rwkv_hip_memcpy_d2h(out.top_ids.data(), dev.p + 4 * rows + top, top * sizeof(int)), "copy alternatives");
+  }
+  return out;
+}
+
 }  // namespace rwkv7_server

@@ -315,6 +315,26 @@ class Session:
                                               ctypes.c_int(T), hip._p(state.shift), hip._p(state.wkv),
                                               hip._p(state.elapsed), hip._p(logits), ctypes.c_int(1 if sync else 0)))
 
+    def score(self, tokens, targets, state, logprob=None, entropy=None, top_n=0, top_ids=None, top_logprobs=None, logits=None,
+              act_int8=False, sync=True):
+        """forward() with the log probability of targets [B,T] (-1: none) at every position: device arrays logprob, entropy f32 [B,T],
+        top_ids i32, top_logprobs f32 [B,T,top_n]; logits f32 [B,V] of the last position if given.  act_int8: the head's input in 8 bits."""
+        tokens = np.ascontiguousarray(tokens, dtype=np.int64)
+        B, T = tokens.shape
+        if B != state.B:
+            raise ValueError("state batch size mismatch")
+        p_targets = ctypes.c_void_p(0)
+        if targets is not None:
+            targets = np.ascontiguousarray(targets, dtype=np.int64)
+            if targets.shape != tokens.shape:
+                raise ValueError("targets have another shape than tokens")
+            p_targets = targets.ctypes.data_as(ctypes.c_void_p)
+        self.set_wkv_fp16(state.wkv_fp16)
+        hip.check(hip.load().rwkv_hip_score(self.handle, tokens.ctypes.data_as(ctypes.c_void_p), p_targets, ctypes.c_int(B), ctypes.c_int(T),
+                                            hip._p(state.shift), hip._p(state.wkv), hip._p(state.elapsed), hip._p(logits),
+                                            ctypes.c_int(1 if act_int8 else 0), ctypes.c_int(top_n), hip._p(logprob), hip._p(entropy),
+                                            hip._p(top_ids), hip._p(top_logprobs), ctypes.c_int(1 if sync else 0)))
+
     def decode_greedy(self, first_tokens, steps, state, logits):
         first = np.ascontiguousarray(first_tokens, dtype=np.int64)
         B = first.shape[0]
