@@ -26,17 +26,18 @@ struct HeadArgs {
   const char* wp;        // packed
   const half_t* scale;   // int8 weights: [N]
   int M, N, K;
-  float* logits;         // [M,N]
-  // sums of the tiles instead of logits
   const int* tokens;     // may be NULL
-  float4_t* part;        // [blocks of 256 columns][M]: m, S, U and the first column of value m
+  float4_t* sums;        // [M][parts]: m, S, U of a part's columns (few rows: 32 columns, tiles: 256)
   float* token_logit;    // [M], written where the token is a column
-  bool want_first;
-  int row_tiles, col_blocks;
+  // alternatives only
+  float* logits;         // [M,N], written where it may hold one
+  float* strips;         // [M][4 parts]: largest of each 64 columns (tiles)
+  const float* bound;    // [M] or NULL: strips below it are not written
+  int parts, row_tiles;
+  // which blocks of 256 columns a launch takes: block i is c = i * every, or with `rest` what is left out by that
+  int col_blocks, every;
+  bool rest;
 };
-
-__device__ __forceinline__ int other_half(int v) { return lane_xor_dpp<32>(v); }
-__device__ __forceinline__ float other_half(float v) { return __builtin_bit_cast(float, lane_xor_dpp<32>(__builtin_bit_cast(int, v))); }
 
 // ---- few rows: the weights are streamed once, which is what bounds it ------------------------------------------------
 // A wavefront takes whole bands of 32 columns, one after the other in memory, 8 KiB of them requested ahead of the 8 KiB that it
@@ -91,6 +92,7 @@ __global__ __launch_bounds__(kFewThreads) void head_few_kernel(HeadArgs g, int l
   const uint32_t x_lane = ((h << log_rows) + (j & (R - 1))) * 16;
   const uint32_t x_step = 2u * 16u << log_rows;  // from one product's fragment to the next
   const float xs = TYPES == kI8W8 ? g.x_scale[min(j, g.M - 1)] : 1.0f;
+  const int token = g.tokens ? g.tokens[min(j, g.M - 1)] : -1;
   typedef typename WideTile<T::kTile, 2>::acc_t acc_t;
   int left = chunks;
   for (int band = band0; band < band1; ++band) {
@@ -119,41 +121,61 @@ __global__ __launch_bounds__(kFewThreads) void head_few_kernel(HeadArgs g, int l
         }
       }
     }
+    float z[16];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      half4_t sc = {1, 1, 1, 1};
+      if (TYPES != kF16F16) sc = *reinterpret_cast<const half4_t*>(g.scale + band * 32 + 8 * q + 4 * h);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        z[4 * q + i] = static_cast<float>(acc[4 * q + i]);
+        if (TYPES != kF16F16) z[4 * q + i] = mul_f32(z[4 * q + i], h2f(sc[i]));
+        if (TYPES == kI8W8) z[4 * q + i] = mul_f32(z[4 * q + i], xs);
+      }
+    }
+    SoftSum a;
+#pragma unroll
+    for (int v = 0; v < 16; ++v) a.m = fmaxf(a.m, z[v]);
+#pragma unroll
+    for (int v = 0; v < 16; ++v) {
+      const float d = z[v] - a.m;
+      const float p = __builtin_amdgcn_exp2f(d * kLog2e);
+      a.s += p;
+      a.u = fmaf(fmaxf(d, kGone), p, a.u);
+    }
+    a.merge_lanes<32>();
     if (j < g.M) {
+      if (h == 0) g.sums[static_cast<int64_t>(j) * g.parts + band] = float4_t{a.m, a.s, a.u, 0.0f};
+      const int t = token - band * 32 - 4 * h;
+      if (t >= 0 && t < 32) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int col = band * 32 + 8 * q + 4 * h;
-        float4_t out;
+        for (int v = 0; v < 16; ++v)
+          if (t == 8 * (v >> 2) + (v & 3)) g.token_logit[j] = z[v];
+      }
+      if (g.logits) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) out[i] = static_cast<float>(acc[4 * q + i]);
-        if constexpr (TYPES != kF16F16) {
-          const half4_t sc = *reinterpret_cast<const half4_t*>(g.scale + col);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) out[i] = mul_f32(out[i], h2f(sc[i]));
-        }
-        if constexpr (TYPES == kI8W8) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) out[i] = mul_f32(out[i], xs);
-        }
-        *reinterpret_cast<float4_t*>(g.logits + static_cast<int64_t>(j) * g.N + col) = out;
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<float4_t*>(g.logits + static_cast<int64_t>(j) * g.N + band * 32 + 8 * q + 4 * h) =
+              float4_t{z[4 * q], z[4 * q + 1], z[4 * q + 2], z[4 * q + 3]};
       }
     }
   }
 }
 
 // ---- many rows: the tiles of the packed product -----------------------------------------------------------------------
-// SUMS: a tile leaves m, S and U of its 256 columns for every row (16 bytes for 1 KiB of logits), otherwise the logits.
-// A lane has 32 columns of a row in registers: they are reduced there, with the other half's 32 by a swap of rows, with the other
-// three wavefronts' 64 each through LDS.
-template <int TYPES, int MT, bool SUMS>
+// A tile leaves m, S and U of its 256 columns for every row (16 bytes for 1 KiB of logits).  A lane has 32 columns of a row in
+// registers: they are reduced there, with the other half's 32 by a swap of rows, with the other three wavefronts' 64 each through LDS.
+// LOGITS: also the largest of each 64 columns, and the logits of those 64 where that is not below the row's bound.
+template <int TYPES, int MT, bool LOGITS>
 __global__ __launch_bounds__(64 * kTileWaves, 2) void head_tile_kernel(HeadArgs g) {
   typedef Types<TYPES> T;
   typedef WideTile<T::kTile, MT> W;
   __shared__ __align__(1024) unsigned char lds[W::kStages * W::kStageBytes];
   const int id = blockIdx.x;
   const int row_tile = (id >> 3) % g.row_tiles;
-  const int col_block = (id / (8 * g.row_tiles)) * 8 + (id & 7);
-  if (col_block >= g.col_blocks) return;
+  const int index = (id / (8 * g.row_tiles)) * 8 + (id & 7);
+  if (index >= g.col_blocks) return;
+  const int col_block = g.rest ? index + index / (g.every - 1) + 1 : index * g.every;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int lane = threadIdx.x & 63, j = lane & 31, h = lane >> 5;
   const int wm = wave & 1, wn = wave >> 1;
@@ -187,141 +209,232 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void head_tile_kernel(HeadArgs 
         z[nb][v] = static_cast<float>(acc[nb][mt][v]);
         if (TYPES != kF16F16) z[nb][v] = mul_f32(z[nb][v], h2f(sc[nb][v >> 2][v & 3]));
       }
-    if constexpr (!SUMS) {
-      if (!live) continue;
+    // m and U in units of x_scale, as everything up to the exponent
+    SoftSum a;
 #pragma unroll
-      for (int nb = 0; nb < 2; ++nb)
-        if (col0 + nb * 32 < g.N) {
+    for (int nb = 0; nb < 2; ++nb)
+      if (col0 + nb * 32 < g.N) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            float4_t out = {z[nb][4 * q], z[nb][4 * q + 1], z[nb][4 * q + 2], z[nb][4 * q + 3]};
-            if (TYPES == kI8W8) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) out[i] = mul_f32(out[i], xs);
-            }
-            *reinterpret_cast<float4_t*>(g.logits + static_cast<int64_t>(row) * g.N + col0 + nb * 32 + 8 * q + 4 * h) = out;
-          }
-        }
-    } else {
-      // the largest column, and the first of its value (in units of x_scale, as everything up to the exponent)
-      float m = kLowest;
-      int first = 0;
-#pragma unroll
-      for (int nb = 0; nb < 2; ++nb)
-        if (col0 + nb * 32 < g.N) {
-#pragma unroll
-          for (int v = 0; v < 16; ++v) m = fmaxf(m, z[nb][v]);
-        }
-      if (g.want_first) {
-#pragma unroll
-        for (int nb = 1; nb >= 0; --nb)
-          if (col0 + nb * 32 < g.N) {
-#pragma unroll
-            for (int v = 15; v >= 0; --v)
-              if (z[nb][v] == m) first = nb * 32 + 8 * (v >> 2) + (v & 3);
-          }
-        first += col0 + 4 * h;
+        for (int v = 0; v < 16; ++v) a.m = fmaxf(a.m, z[nb][v]);
       }
-      const float to_log2 = xs * kLog2e;
-      float s = 0.0f, u = 0.0f;
+    const float to_log2 = xs * kLog2e;
+#pragma unroll
+    for (int nb = 0; nb < 2; ++nb)
+      if (col0 + nb * 32 < g.N) {
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          const float d = z[nb][v] - a.m;
+          const float p = __builtin_amdgcn_exp2f(d * to_log2);
+          a.s += p;
+          a.u = fmaf(fmaxf(d, kLowest), p, a.u);
+        }
+      }
+    const int t = g.tokens && live ? g.tokens[row] - col0 : -1;
+    if (t >= 0 && t < 64 && ((t >> 2) & 1) == h && col0 + t < g.N) {
+      float zt = 0.0f;
 #pragma unroll
       for (int nb = 0; nb < 2; ++nb)
-        if (col0 + nb * 32 < g.N) {
 #pragma unroll
-          for (int v = 0; v < 16; ++v) {
-            const float d = z[nb][v] - m;
-            const float p = __builtin_amdgcn_exp2f(d * to_log2);
-            s += p;
-            u = fmaf(fmaxf(d, kLowest), p, u);
-          }
-        }
-      const int t = g.tokens && live ? g.tokens[row] - col0 : -1;
-      if (t >= 0 && t < 64 && ((t >> 2) & 1) == h && col0 + t < g.N) {
-        float zt = 0.0f;
+        for (int v = 0; v < 16; ++v)
+          if (t - 4 * h == nb * 32 + 8 * (v >> 2) + (v & 3)) zt = z[nb][v];
+      g.token_logit[row] = mul_f32(zt, xs);
+    }
+    if (TYPES == kI8W8 && a.m != kLowest) {  // (the lowest value stands for none)
+      a.m *= xs;
+      a.u *= xs;
+    }
+    a.merge_lanes<32>();
+    if (h == 0) merge[wn * W::BM + r] = float4_t{a.m, a.s, a.u, 0.0f};
+    if constexpr (LOGITS) {
+      if (live && !(g.bound && a.m < g.bound[row])) {
 #pragma unroll
         for (int nb = 0; nb < 2; ++nb)
+          if (col0 + nb * 32 < g.N) {
 #pragma unroll
-          for (int v = 0; v < 16; ++v)
-            if (t - 4 * h == nb * 32 + 8 * (v >> 2) + (v & 3)) zt = z[nb][v];
-        g.token_logit[row] = mul_f32(zt, xs);
+            for (int q = 0; q < 4; ++q) {
+              float4_t out = {z[nb][4 * q], z[nb][4 * q + 1], z[nb][4 * q + 2], z[nb][4 * q + 3]};
+              if (TYPES == kI8W8) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) out[i] = mul_f32(out[i], xs);
+              }
+              *reinterpret_cast<float4_t*>(g.logits + static_cast<int64_t>(row) * g.N + col0 + nb * 32 + 8 * q + 4 * h) = out;
+            }
+          }
       }
-      // both halves in one
-      SoftSum a = {m * xs, s, u * xs};
-      if (m == kLowest) a = {kLowest, s, 0.0f};
-      a.merge(SoftSum{other_half(a.m), other_half(a.s), other_half(a.u)}, first, other_half(first));
-      if (h == 0) merge[wn * W::BM + r] = float4_t{a.m, a.s, a.u, __builtin_bit_cast(float, first)};
     }
   }
-  if constexpr (SUMS) {
-    __syncthreads();
-    const int r = threadIdx.x;
-    if (r < W::BM && m0 + r < g.M) {
-      const float4_t p = merge[r];
-      SoftSum a = {p[0], p[1], p[2]};
-      int first = as_int(p[3]);
+  __syncthreads();
+  const int r = threadIdx.x;
+  if (r < W::BM && m0 + r < g.M) {
+    SoftSum a;
+    float4_t most;
 #pragma unroll
-      for (int i = 1; i < 4; ++i) {
-        const float4_t o = merge[i * W::BM + r];
-        a.merge(SoftSum{o[0], o[1], o[2]}, first, as_int(o[3]));
-      }
-      g.part[static_cast<int64_t>(col_block) * g.M + m0 + r] = float4_t{a.m, a.s, a.u, __builtin_bit_cast(float, first)};
+    for (int i = 0; i < 4; ++i) {
+      const float4_t o = merge[i * W::BM + r];
+      most[i] = o[0];
+      a.merge(SoftSum{o[0], o[1], o[2]});
     }
+    const int64_t at = static_cast<int64_t>(m0 + r) * g.parts + col_block;
+    g.sums[at] = float4_t{a.m, a.s, a.u, 0.0f};
+    if constexpr (LOGITS) *reinterpret_cast<float4_t*>(g.strips + at * 4) = most;
   }
 }
 
-// 16 rows per block, 16 threads per row over the blocks of columns
-__global__ __launch_bounds__(256) void head_join_kernel(HeadArgs g, TokenLogprobs out) {
-  __shared__ float4_t parts[16][17];
-  const int r = threadIdx.x & 15, i = threadIdx.x >> 4;
-  const int row = blockIdx.x * 16 + r;
-  SoftSum a;
-  int first = 0;
-  if (row < g.M) {
-    for (int c = i; c < g.col_blocks; c += 16) {
-      const float4_t p = g.part[static_cast<int64_t>(c) * g.M + row];
-      a.merge(SoftSum{p[0], p[1], p[2]}, first, as_int(p[3]));
-    }
+// The top_n-th largest of the strips that the first launch has left, of one row per block: no alternative lies below it.
+constexpr int kBoundStrips = 1024;
+__global__ __launch_bounds__(256) void head_bound_kernel(HeadArgs g, int top_n, float* bound) {
+  __shared__ __align__(16) float most[kBoundStrips];
+  const float4_t* strips = reinterpret_cast<const float4_t*>(g.strips) + static_cast<int64_t>(blockIdx.x) * g.parts;
+  const int n = 4 * g.col_blocks;
+  for (int i = threadIdx.x; i < g.col_blocks; i += 256) {
+    float4_t v = strips[i * g.every];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (v[e] != v[e]) v[e] = -INFINITY;
+    *reinterpret_cast<float4_t*>(most + 4 * i) = v;
   }
-  parts[r][i] = float4_t{a.m, a.s, a.u, __builtin_bit_cast(float, first)};
   __syncthreads();
-  if (threadIdx.x >= 16 || row >= g.M) return;
-  for (int k = 1; k < 16; ++k) {
-    const float4_t p = parts[r][k];
-    a.merge(SoftSum{p[0], p[1], p[2]}, first, as_int(p[3]));
+  for (int k = threadIdx.x; k < n; k += 256) {
+    const float mine = most[k];
+    int before = 0;
+    for (int i = 0; i < n; i += 4) {
+      const float4_t w = *reinterpret_cast<const float4_t*>(most + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) before += w[e] > mine || (w[e] == mine && i + e < k);
+    }
+    if (before == top_n - 1) bound[blockIdx.x] = mine;
   }
-  write_logprobs(a, out, row, g.N, g.token_logit + row);
-  if (out.top_n == 1) {
-    const bool there = a.m > kLowest;
-    out.top_ids[row] = there ? first : -1;
-    out.top_logprobs[row] = there ? -logf(a.s) : -INFINITY;
+}
+
+// Log probability and entropy from the parts' sums: a wavefront per row.
+__global__ __launch_bounds__(256) void head_sums_kernel(HeadArgs g, TokenLogprobs out) {
+  const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= g.M) return;
+  const float4_t* sums = g.sums + static_cast<int64_t>(row) * g.parts;
+  SoftSum a;
+  for (int i = threadIdx.x & 63; i < g.parts; i += 64) {
+    const float4_t p = sums[i];
+    a.merge(SoftSum{p[0], p[1], p[2]});
   }
+  a.merge_wave();
+  if ((threadIdx.x & 63) == 0) write_logprobs(a, out, row, g.N, g.token_logit + row);
+}
+
+// The same with the alternatives, a block per row: they lie in the strips whose largest reaches the top_n-th largest of 64 or 256 groups
+// of strips - few more than top_n of them - whose logits are there.  Four (or eight) strips at a time; the list never overflows, it is thinned out
+// first.  Strips of 64 columns with their largest in `strips` (tiles), or of 32 with it in `sums` (few rows).
+__global__ __launch_bounds__(256) void head_alternatives_kernel(HeadArgs g, TokenLogprobs out, int width) {
+  __shared__ __align__(16) Candidates<256> cand;
+  __shared__ float4_t waves[4];
+  __shared__ int chosen[256];
+  __shared__ int n_chosen;
+  const int tid = threadIdx.x, row = blockIdx.x, top_n = out.top_n;
+  const float4_t* sums = g.sums + static_cast<int64_t>(row) * g.parts;
+  const int n_strips = width == 64 ? 4 * g.parts : g.parts;
+  const float* strips = width == 64 ? g.strips + static_cast<int64_t>(row) * n_strips : reinterpret_cast<const float*>(sums);
+  const int apart = width == 64 ? 1 : 4;
+  const float* logits = g.logits + static_cast<int64_t>(row) * g.N;
+  SoftSum a;
+  for (int i = tid; i < g.parts; i += 256) {
+    const float4_t p = sums[i];
+    a.merge(SoftSum{p[0], p[1], p[2]});
+  }
+  a.merge_wave();
+  if ((tid & 63) == 0) waves[tid >> 6] = float4_t{a.m, a.s, a.u, 0.0f};
+  if (tid == 0) {
+    cand.n = 0;
+    n_chosen = 0;
+  }
+  float most = -INFINITY;
+  for (int i = tid; i < n_strips; i += 256) most = fmaxf(most, strips[i * apart]);
+  const float bound = first_bound(cand, top_n, most);
+  a = SoftSum{};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float4_t w = waves[i];
+    a.merge(SoftSum{w[0], w[1], w[2]});
+  }
+  key_t least = bound == -INFINITY ? 0 : key_of(bound, 0x7fffffff);  // what a candidate has to be ahead of
+  int list = 0;
+  const int at_once = 256 / width;
+  for (int base = 0; base < n_strips; base += 256) {
+    const int s = base + tid;
+    // (a strip whose largest ties with the last candidate and lies behind it has none)
+    if (s < n_strips) {
+      const float v = strips[s * apart];
+      if (v == v && key_of(v, s * width) > least) chosen[atomicAdd(&n_chosen, 1)] = s;
+    }
+    __syncthreads();
+    const int n = n_chosen;
+    for (int k = 0; k < n; k += at_once) {
+      const int which = k + tid / width;
+      if (which < n) {
+        const int col = chosen[which] * width + tid % width;
+        if (col < g.N) {
+          const float v = logits[col];
+          if (v > -INFINITY) {
+            const key_t key = key_of(v, col);
+            if (key > least) offer(cand, list, key);
+          }
+        }
+      }
+      __syncthreads();
+      const int have = cand.n;
+      __syncthreads();
+      if (have > kCandidates - 256) {
+        thin_out(cand, list, have, top_n);
+        list ^= 1;
+        __syncthreads();
+        least = cand.list[list][top_n - 1];
+        if (tid == 0) cand.n = top_n;
+        __syncthreads();
+      }
+    }
+    if (tid == 0) n_chosen = 0;
+    __syncthreads();
+  }
+  const int n = cand.n;
+  const float log_s = logf(a.s);
+  thin_out(cand, list, n, top_n);
+  __syncthreads();
+  if (tid < top_n) write_alternative(out, row, tid, tid < n ? cand.list[list ^ 1][tid] : 0, a.m, log_s);
+  if (tid == 0) write_logprobs(a, out, row, g.N, g.token_logit + row);
 }
 
 // ---- what a call takes ------------------------------------------------------------------------------------------------
-enum Way { kFew, kLogits, kSums };
 struct Plan {
-  Way way;
-  int rows;      // at a time
-  size_t logits, part, token_logit;  // bytes, of 256 each
-  size_t rest;
-  size_t bytes() const { return logits + part + token_logit + rest; }
+  bool few;
+  int rows;        // at a time
+  int tile;        // rows of a tile
+  int parts;       // of a row, with sums of their own
+  int every;       // > 1: a first launch takes every so many blocks of columns and bounds the alternatives of the others
+  size_t sums, token_logit, logits, strips, bound;  // bytes
+  size_t bytes() const { return sums + token_logit + logits + strips + bound; }
 };
 
-constexpr int kLogitRows = 256;  // rows whose logits exist at a time
-constexpr int kSumRows = 8192;   // rows whose tiles' sums do
+constexpr int kSumRows = 8192;    // rows at a time without alternatives: 32 MiB of sums at 65536 columns
+constexpr int kLogits = 1 << 27;  // and with them, rows times columns: 512 MiB of places for logits, few of which are written
+constexpr int kFewestTurns = 6;   // turns of blocks on the chip from which on two launches cost less than the logits they save
 
 Plan plan_of(bool x_int8, int M, int N, int K, int top_n) {
   Plan p = {};
-  p.way = takes_few(M, K, x_int8 ? 1 : 2) ? kFew : top_n > 1 ? kLogits : kSums;
-  p.rows = p.way == kFew ? M : std::min(M, p.way == kSums ? kSumRows : kLogitRows);
-  const auto align = [](size_t n) { return (n + 255) / 256 * 256; };
-  if (p.way == kSums) {
-    p.part = align(static_cast<size_t>(ceil_div(N, kTileCols)) * p.rows * sizeof(float4_t));
-    p.token_logit = align(static_cast<size_t>(p.rows) * 4);
-  } else {
-    p.logits = align(static_cast<size_t>(p.rows) * N * 4);
-    p.rest = token_logprobs_workspace_bytes(p.rows, N, top_n);
+  p.few = takes_few(M, K, x_int8 ? 1 : 2);
+  p.rows = p.few ? M : std::min(M, top_n > 0 ? std::max(kLogits / N / 256, 1) * 256 : kSumRows);
+  p.tile = p.rows <= 128 ? 128 : 256;
+  p.parts = ceil_div(N, p.few ? 32 : kTileCols);
+  p.every = 1;
+  if (!p.few && top_n > 0) {
+    const int64_t blocks = static_cast<int64_t>(ceil_div(p.rows, p.tile)) * p.parts, cus = device_cu_count();
+    // (as many strips as groups of them are wanted, and no more than the bound's launch holds)
+    if (blocks >= kFewestTurns * cus) p.every = std::min<int64_t>(ceil_div(blocks, cus), 4 * p.parts / std::max(2 * top_n, 128));
+    if (p.every < 2 || 4 * ceil_div(p.parts, p.every) > kBoundStrips) p.every = 1;
   }
+  const auto align = [](size_t n) { return (n + 255) / 256 * 256; };
+  p.sums = align(static_cast<size_t>(p.rows) * p.parts * sizeof(float4_t));
+  p.token_logit = align(static_cast<size_t>(p.rows) * 4);
+  if (top_n > 0) p.logits = align(static_cast<size_t>(p.rows) * N * 4);
+  if (top_n > 0 && !p.few) p.strips = p.sums;
+  if (p.every > 1) p.bound = p.token_logit;
   return p;
 }
 
@@ -338,31 +451,41 @@ int launch_few(hipStream_t st, const HeadArgs& g) {
   return RWKV_OK;
 }
 
-template <int TYPES, bool SUMS>
-int launch_tiles(hipStream_t st, HeadArgs g) {
-  const int rows = g.M <= 128 ? 128 : 256;
-  g.row_tiles = ceil_div(g.M, rows);
-  g.col_blocks = ceil_div(g.N, kTileCols);
+// `col_blocks` of g.parts blocks of columns: every `every`-th, or the rest
+template <int TYPES, bool LOGITS>
+int launch_tiles(hipStream_t st, HeadArgs& g, int tile, int every, bool rest) {
+  g.row_tiles = ceil_div(g.M, tile);
+  g.every = every;
+  g.rest = rest;
+  g.col_blocks = rest ? g.parts - ceil_div(g.parts, every) : ceil_div(g.parts, every);
   const dim3 grid(g.row_tiles * ceil_div(g.col_blocks, 8) * 8);
-  if (rows == 256) hipLaunchKernelGGL((head_tile_kernel<TYPES, 4, SUMS>), grid, dim3(64 * kTileWaves), 0, st, g);
-  else hipLaunchKernelGGL((head_tile_kernel<TYPES, 2, SUMS>), grid, dim3(64 * kTileWaves), 0, st, g);
+  if (tile == 256) hipLaunchKernelGGL((head_tile_kernel<TYPES, 4, LOGITS>), grid, dim3(64 * kTileWaves), 0, st, g);
+  else hipLaunchKernelGGL((head_tile_kernel<TYPES, 2, LOGITS>), grid, dim3(64 * kTileWaves), 0, st, g);
   RWKV_LAUNCH_CHECK();
   return RWKV_OK;
 }
 
 template <int TYPES>
-int launch_rows(hipStream_t st, const Plan& p, HeadArgs g, const TokenLogprobs& out, void* rest) {
-  if (p.way == kSums) {
-    const int rc = launch_tiles<TYPES, true>(st, g);
-    if (rc != RWKV_OK) return rc;
-    g.col_blocks = ceil_div(g.N, kTileCols);
-    hipLaunchKernelGGL(head_join_kernel, dim3(ceil_div(g.M, 16)), dim3(256), 0, st, g, out);
-    RWKV_LAUNCH_CHECK();
-    return RWKV_OK;
+int launch_rows(hipStream_t st, const Plan& p, HeadArgs g, const TokenLogprobs& out, float* bound) {
+  int rc = RWKV_OK;
+  if (p.few) {
+    rc = launch_few<TYPES>(st, g);
+  } else if (out.top_n == 0) {
+    rc = launch_tiles<TYPES, false>(st, g, p.tile, 1, false);
+  } else {
+    rc = launch_tiles<TYPES, true>(st, g, p.tile, p.every, false);
+    if (rc == RWKV_OK && p.every > 1) {
+      hipLaunchKernelGGL(head_bound_kernel, dim3(g.M), dim3(256), 0, st, g, out.top_n, bound);
+      RWKV_LAUNCH_CHECK();
+      g.bound = bound;
+      rc = launch_tiles<TYPES, true>(st, g, p.tile, p.every, true);
+    }
   }
-  const int rc = p.way == kFew ? launch_few<TYPES>(st, g) : launch_tiles<TYPES, false>(st, g);
   if (rc != RWKV_OK) return rc;
-  return token_logprobs_launch(st, g.M, g.N, RWKV_IO_F32, g.logits, g.N, out, rest);
+  if (out.top_n == 0) hipLaunchKernelGGL(head_sums_kernel, dim3(ceil_div(g.M, 4)), dim3(256), 0, st, g, out);
+  else hipLaunchKernelGGL(head_alternatives_kernel, dim3(g.M), dim3(256), 0, st, g, out, p.few ? 32 : 64);
+  RWKV_LAUNCH_CHECK();
+  return RWKV_OK;
 }
 
 }  // namespace
@@ -376,12 +499,23 @@ int linear_logprobs_launch(hipStream_t st, int fmt, int M, int N, int K, const v
   for (int m = 0; m < M; m += p.rows) {
     const int64_t off = static_cast<int64_t>(m) * K * (x_scale ? 1 : 2);
     const TokenLogprobs rows = out.from_row(m);
-    HeadArgs g = {static_cast<const char*>(x) + off, x_scale ? x_scale + m : nullptr, static_cast<const char*>(packed), scale,
-                  std::min(p.rows, M - m), N, K, reinterpret_cast<float*>(ws), rows.logprob ? rows.tokens : nullptr,
-                  reinterpret_cast<float4_t*>(ws + p.logits), reinterpret_cast<float*>(ws + p.logits + p.part), out.top_n == 1, 0, 0};
-    void* rest = ws + p.logits + p.part + p.token_logit;
-    const int rc = x_scale ? launch_rows<kI8W8>(st, p, g, rows, rest)
-                           : (fmt == RWKV_FMT_W8 ? launch_rows<kF16W8>(st, p, g, rows, rest) : launch_rows<kF16F16>(st, p, g, rows, rest));
+    HeadArgs g = {};
+    g.x = static_cast<const char*>(x) + off;
+    g.x_scale = x_scale ? x_scale + m : nullptr;
+    g.wp = static_cast<const char*>(packed);
+    g.scale = scale;
+    g.M = std::min(p.rows, M - m);
+    g.N = N;
+    g.K = K;
+    g.tokens = rows.logprob ? rows.tokens : nullptr;
+    g.parts = p.parts;
+    g.sums = reinterpret_cast<float4_t*>(ws);
+    g.token_logit = reinterpret_cast<float*>(ws + p.sums);
+    g.logits = p.logits ? reinterpret_cast<float*>(ws + p.sums + p.token_logit) : nullptr;
+    g.strips = reinterpret_cast<float*>(ws + p.sums + p.token_logit + p.logits);
+    float* bound = reinterpret_cast<float*>(ws + p.sums + p.token_logit + p.logits + p.strips);
+    const int rc = x_scale ? launch_rows<kI8W8>(st, p, g, rows, bound)
+                           : (fmt == RWKV_FMT_W8 ? launch_rows<kF16W8>(st, p, g, rows, bound) : launch_rows<kF16F16>(st, p, g, rows, bound));
     if (rc != RWKV_OK) return rc;
   }
   return RWKV_OK;

@@ -7,20 +7,26 @@
 //
 // Entries of -infinity have probability 0 and are no alternatives; a row of nothing else gives log probability -infinity, entropy 0
 // and no alternative.
+#include <algorithm>
+
 #include "softsum.h"
 
 namespace rwkv {
 
 namespace {
 
-constexpr int kCandidates = 1024;  // places for entries that may be among the first top_n
-constexpr int kRefine = 4;         // batches between looks at whether the candidates can be thinned out
+constexpr int kThreads = 256;
+constexpr int kRefine = 4;  // batches between looks at whether the candidates can be thinned out
 
 struct LogprobArgs {
   const void* logits;
   int64_t ld;
   int V;
   TokenLogprobs out;
+  // rows in several parts: what each leaves
+  int parts, part_len;
+  float4_t* sums;  // [rows][parts]: m, S, U and the entries ahead of the token
+  key_t* keys;     // [rows][parts][top_n] in order, 0 past the last
 };
 
 __device__ __forceinline__ float next_above(float v) {  // the smallest float above v; NaN above +infinity
@@ -28,27 +34,26 @@ __device__ __forceinline__ float next_above(float v) {  // the smallest float ab
   return v == 0.0f ? __builtin_bit_cast(float, 1u) : __builtin_bit_cast(float, v > 0.0f ? b + 1 : b - 1);
 }
 
-// One block per row, which it reads once: 64 bytes per thread at a time, the next 64 requested before they are looked at.  A thread
-// keeps m, S and U of its entries and raises m when a batch exceeds it.  The rank is a count against the token's logit, which is
-// read first.  Alternatives: of the first batch the largest entry of each of 64 or 256 groups of threads is known; top_n of these are
-// at least as large as the top_n-th of them, so that nothing below it can be an alternative.  What is not below goes to a list in LDS (its
-// order is that of an atomic counter, its use is not), which is sorted by counting at the end, and thinned out to the first top_n - with
-// the last one as the new bound - whenever it has grown to four times as many.  A list that overflows (a row that rises, or is of one
-// value) is given up: the alternatives are then found one after the other in top_n walks over the row.
-template <typename T, int NT>
-__global__ __launch_bounds__(NT) void token_logprobs_kernel(LogprobArgs a) {
+// One block per row, or per part of one, which it reads once: 64 bytes per thread at a time, the next 64 requested before they are
+// looked at.  A thread keeps m, S and U of its entries and raises m when a batch exceeds it.  The rank is a count against the token's
+// logit, which is read first.  Alternatives: what is not below the bound that the first batch gives goes to a list in LDS, which is
+// thinned out to the first top_n - with the last one as the new bound - whenever it has grown to four times as many.  A list that
+// overflows (a row that rises, or is of one value) is given up: the alternatives are then found one after the other in top_n walks.
+template <typename T, bool PART>
+__global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobArgs a) {
+  constexpr int NT = kThreads;
   constexpr int VE = 16 / sizeof(T);  // entries of a 16-byte vector
   constexpr int VB = 4;               // vectors of a batch
   typedef T vec_t __attribute__((ext_vector_type(VE)));
-  __shared__ float cand_z[2][kCandidates];
-  __shared__ int cand_i[2][kCandidates];
-  __shared__ __align__(16) float group_max[256];
-  __shared__ float red[4][NT / 64];
-  __shared__ int n_cand;
-  __shared__ float bound_s;
+  __shared__ __align__(16) Candidates<NT> cand;
+  __shared__ float4_t waves[NT / 64];
   const int tid = threadIdx.x;
-  const T* z = static_cast<const T*>(a.logits) + blockIdx.x * a.ld;
-  const int V = a.V, top_n = a.out.top_n;
+  const int top_n = a.out.top_n;
+  const T* row = static_cast<const T*>(a.logits) + blockIdx.x * a.ld;
+  // entries first .. first + V - 1 of the row; every index below counts from `first`
+  const int first = PART ? blockIdx.y * a.part_len : 0;
+  const int V = PART ? min(a.part_len, a.V - first) : a.V;
+  const T* z = row + first;
   const int misaligned = static_cast<int>((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
   const int head = misaligned ? min(VE - misaligned, V) : 0;  // entries in front of the first 16-byte boundary
   const int vecs = (V - head) / VE;
@@ -73,66 +78,18 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(LogprobArgs a) {
   // the entries of the two ends, at most one per thread
   const int stray = tid < head ? tid : tail + tid - head;
   const float stray_z = stray < V ? static_cast<float>(z[stray]) : -INFINITY;
-  const int t = a.out.tokens ? a.out.tokens[blockIdx.x] : -1;
-  const bool has_token = t >= 0 && t < V;
-  const float zt = has_token ? static_cast<float>(z[t]) : 0.0f;
+  const int token = a.out.tokens ? a.out.tokens[blockIdx.x] : -1;
+  const bool has_token = token >= 0 && token < a.V;
+  const float zt = has_token ? static_cast<float>(row[token]) : 0.0f;
+  const int t = token - first;  // (may lie in front of this part or behind it)
   const bool count = a.out.rank && has_token;
   const float zt_above = next_above(zt);
-  if (top_n > 0 && tid == 0) n_cand = 0;
+  if (top_n > 0 && tid == 0) cand.n = 0;
 
   SoftSum sum;
   int ahead = 0;
   float bound = INFINITY;
   int list = 0;
-  auto offer = [&](float v, int i) {
-    if (v >= bound && v > -INFINITY) {
-      const int at = atomicAdd(&n_cand, 1);
-      if (at < kCandidates) {
-        cand_z[list][at] = v;
-        cand_i[list][at] = i;
-      }
-    }
-  };
-  // the top_n-th largest of the groups' maxima (equal ones by group): every thread of the block comes here
-  auto first_bound = [&](float mine) {
-    const int groups = top_n <= 24 ? 64 : 256;
-    if (mine != mine) mine = -INFINITY;
-    const int width = NT / groups;
-    if (width > 1) mine = fmaxf(mine, __builtin_bit_cast(float, lane_xor_dpp<1>(__builtin_bit_cast(int, mine))));
-    if (width > 2) mine = fmaxf(mine, __builtin_bit_cast(float, lane_xor_dpp<2>(__builtin_bit_cast(int, mine))));
-    if (width > 4) mine = fmaxf(mine, __builtin_bit_cast(float, lane_xor_dpp<4>(__builtin_bit_cast(int, mine))));
-    if (width > 8) mine = fmaxf(mine, __builtin_bit_cast(float, lane_xor_dpp<8>(__builtin_bit_cast(int, mine))));
-    if (tid % width == 0) group_max[tid / width] = mine;
-    __syncthreads();
-    if (tid < groups) {
-      const float v = group_max[tid];
-      int before = 0;
-      for (int i = 0; i < groups; i += 4) {
-        const float4_t w = *reinterpret_cast<const float4_t*>(group_max + i);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) before += ahead_of(w[e], i + e, v, tid);
-      }
-      if (before == top_n - 1) bound_s = v;
-    }
-    __syncthreads();
-    bound = bound_s;
-  };
-  // the first top_n of the list, in order, to the other list; returns how many there were
-  auto thin_out = [&](int n) {
-    for (int c = tid; c < n; c += NT) {
-      const float v = cand_z[list][c];
-      const int i = cand_i[list][c];
-      int before = 0;
-      for (int k = 0; k < n; ++k) before += ahead_of(cand_z[list][k], cand_i[list][k], v, i);
-      if (before < top_n) {
-        cand_z[list ^ 1][before] = v;
-        cand_i[list ^ 1][before] = i;
-      }
-    }
-    list ^= 1;
-  };
-
-  // (fmaxf of a NaN and a number is the number)
   for (int b = 0; b < batches || b == 0; ++b) {
     float x[VB * VE];
 #pragma unroll
@@ -140,13 +97,13 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(LogprobArgs a) {
 #pragma unroll
       for (int e = 0; e < VE; ++e) x[q * VE + e] = static_cast<float>(next[q][e]);
     if (b + 1 < batches) request(b + 1);
-    float most = fmaxf(x[0], x[1]);
+    float most = fmaxf(x[0], x[1]);  // (fmaxf of a NaN and a number is the number)
 #pragma unroll
     for (int e = 2; e < VB * VE; ++e) most = fmaxf(most, x[e]);
     if (top_n > 0) {
       if (b == 0) {
-        first_bound(fmaxf(most, stray_z));
-        offer(stray_z, stray);
+        bound = first_bound(cand, top_n, fmaxf(most, stray_z));
+        if (stray_z >= bound && stray_z > -INFINITY) offer(cand, list, key_of(stray_z, first + stray));
       }
       if (most >= bound) {
         uint32_t mask = 0;
@@ -156,17 +113,20 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(LogprobArgs a) {
           const int e = __builtin_ctz(mask);
           mask &= mask - 1;
           const int i = head + ((b * VB + e / VE) * NT + tid) * VE + e % VE;
-          if (i < tail) offer(static_cast<float>(z[i]), i);  // (again from memory: a register cannot be chosen by a number)
+          if (i >= tail) continue;
+          const float v = static_cast<float>(z[i]);  // (again from memory: a register cannot be chosen by a number)
+          if (v > -INFINITY) offer(cand, list, key_of(v, first + i));
         }
       }
       if (b % kRefine == kRefine - 1) {
         __syncthreads();
-        const int n = n_cand;
+        const int n = cand.n;
         if (n > 4 * top_n && n <= kCandidates) {
-          thin_out(n);
+          thin_out(cand, list, n, top_n);
+          list ^= 1;
           __syncthreads();
-          bound = cand_z[list][top_n - 1];
-          if (tid == 0) n_cand = top_n;
+          bound = key_value(cand.list[list][top_n - 1]);
+          if (tid == 0) cand.n = top_n;
         }
         __syncthreads();
       }
@@ -175,7 +135,8 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(LogprobArgs a) {
       // entries ahead of the token: as large in front of it, larger behind it (the vector it lies in: larger, made good at the end)
 #pragma unroll
       for (int q = 0; q < VB; ++q) {
-        const float least = head + ((b * VB + q) * NT + tid) * VE + VE <= t ? zt : zt_above;
+        const int v = (b * VB + q) * NT + tid;
+        const float least = v < vecs && head + v * VE + VE <= t ? zt : zt_above;
 #pragma unroll
         for (int e = 0; e < VE; ++e) ahead += x[q * VE + e] >= least;
       }
@@ -195,110 +156,185 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(LogprobArgs a) {
     const float p = __builtin_amdgcn_exp2f(d * kLog2e);
     sum.s += p;
     sum.u = fmaf(fmaxf(d, kGone), p, sum.u);
-    if (count) ahead += stray < V && ahead_of(stray_z, stray, zt, t);
+    if (count) ahead += stray < V && (stray_z > zt || (stray_z == zt && stray < t));
     // equal entries of the token's own vector in front of it
     if (count && tid == 0 && t >= head && t < tail)
       for (int i = t - (t - head) % VE; i < t; ++i) ahead += static_cast<float>(z[i]) == zt;
   }
 
   // the block's sums
-  {
-    const float m = wave_reduce_dpp(sum.m, [](float x, float y) { return fmaxf(x, y); });
-    if ((tid & 63) == 0) red[0][tid >> 6] = m;
-    __syncthreads();
-    float all = red[0][0];
+  sum.merge_wave();
+  ahead = wave_reduce_dpp(ahead, [](int x, int y) { return x + y; });
+  if ((tid & 63) == 0) waves[tid >> 6] = float4_t{sum.m, sum.s, sum.u, as_float(ahead)};
+  __syncthreads();
+  sum = SoftSum{};
+  ahead = 0;
 #pragma unroll
-    for (int i = 1; i < NT / 64; ++i) all = fmaxf(all, red[0][i]);
-    sum.raise(all);
-    const float s = wave_sum_dpp(sum.s), u = wave_sum_dpp(sum.u);
-    const int c = wave_reduce_dpp(ahead, [](int x, int y) { return x + y; });
-    if ((tid & 63) == 0) {
-      red[1][tid >> 6] = s;
-      red[2][tid >> 6] = u;
-      red[3][tid >> 6] = __builtin_bit_cast(float, c);
-    }
-    __syncthreads();
-    sum.s = sum.u = 0.0f;
-    ahead = 0;
-#pragma unroll
-    for (int i = 0; i < NT / 64; ++i) {
-      sum.s += red[1][i];
-      sum.u += red[2][i];
-      ahead += __builtin_bit_cast(int, red[3][i]);
-    }
+  for (int i = 0; i < NT / 64; ++i) {
+    const float4_t w = waves[i];
+    sum.merge(SoftSum{w[0], w[1], w[2]});
+    ahead += as_int(w[3]);
   }
-  const float log_s = logf(sum.s);
-  if (tid == 0) {
-    write_logprobs(sum, a.out, blockIdx.x, V, &zt);
-    if (a.out.rank) a.out.rank[blockIdx.x] = !has_token || zt != zt ? -1 : ahead;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * a.parts + blockIdx.y;
+  float log_s = 0.0f;
+  if constexpr (PART) {
+    if (tid == 0) a.sums[at] = float4_t{sum.m, sum.s, sum.u, as_float(ahead)};
+  } else if (tid < 64) {
+    log_s = logf(sum.s);
+    if (tid == 0) {
+      write_logprobs(sum, a.out, blockIdx.x, V, &zt);
+      if (a.out.rank) a.out.rank[blockIdx.x] = !has_token || zt != zt ? -1 : ahead;
+    }
   }
   if (top_n == 0) return;
+  static_assert(kMaxAlternatives <= 64, "one wavefront writes them");
+  auto write = [&](int place, key_t key) {
+    if constexpr (PART) a.keys[at * top_n + place] = key;
+    else write_alternative(a.out, blockIdx.x, place, key, sum.m, log_s);
+  };
 
-  int* ids = a.out.top_ids + static_cast<int64_t>(blockIdx.x) * top_n;
-  float* tops = a.out.top_logprobs + static_cast<int64_t>(blockIdx.x) * top_n;
-  const int n = n_cand;
+  const int n = cand.n;
   if (n <= kCandidates) {
-    thin_out(n);
+    thin_out(cand, list, n, top_n);
     __syncthreads();
-    if (tid < top_n) {
-      const bool there = tid < n;
-      ids[tid] = there ? cand_i[list][tid] : -1;
-      tops[tid] = there ? cand_z[list][tid] - sum.m - log_s : -INFINITY;
-    }
+    if (tid < top_n) write(tid, tid < n ? cand.list[list ^ 1][tid] : 0);
     return;
   }
   // one after the other: the first entry behind the one before
-  float last = INFINITY;
-  int last_i = -1;
+  key_t last = ~static_cast<key_t>(0);
+  key_t* best_of = cand.list[0];
   for (int k = 0; k < top_n; ++k) {
-    float best = -INFINITY;
-    int bi = V;
+    key_t best = 0;
     for (int i = tid; i < V; i += NT) {
       const float v = static_cast<float>(z[i]);
-      if (ahead_of(last, last_i, v, i) && v > best) {
-        best = v;
-        bi = i;
-      }
-    }
-    const float wave_best = wave_reduce_dpp(best, [](float x, float y) { return fmaxf(x, y); });
-    bi = wave_reduce_dpp(best == wave_best ? bi : V, [](int x, int y) { return min(x, y); });
-    __syncthreads();
-    if ((tid & 63) == 0) {
-      cand_z[0][tid >> 6] = wave_best;
-      cand_i[0][tid >> 6] = bi;
+      if (!(v > -INFINITY)) continue;
+      const key_t key = key_of(v, first + i);
+      if (key < last && key > best) best = key;
     }
     __syncthreads();
-    best = -INFINITY;
-    bi = V;
-    for (int i = 0; i < NT / 64; ++i) {
-      if (cand_i[0][i] < V && ahead_of(cand_z[0][i], cand_i[0][i], best, bi)) {
-        best = cand_z[0][i];
-        bi = cand_i[0][i];
-      }
+    best_of[tid] = best;
+    __syncthreads();
+    for (int step = NT / 2; step > 0; step /= 2) {
+      if (tid < step && best_of[tid + step] > best_of[tid]) best_of[tid] = best_of[tid + step];
+      __syncthreads();
     }
-    if (tid == 0) {
-      ids[k] = bi < V ? bi : -1;
-      tops[k] = bi < V ? best - sum.m - log_s : -INFINITY;
-    }
-    last = best;
-    last_i = bi;
+    last = best_of[0];
+    if (tid == 0) write(k, last);
   }
 }
 
+// A block per row over what its parts have left.  Of many keys a bound is made first, as of the entries of a row: at most top_n groups of
+// four threads, or of one, reach it, with as many keys each as a thread holds.
+constexpr int kMaxParts = 256;
+__global__ __launch_bounds__(kThreads) void token_logprobs_join_kernel(LogprobArgs a, int io) {
+  __shared__ __align__(16) Candidates<kThreads> cand;
+  __shared__ float4_t waves[kThreads / 64];
+  const int tid = threadIdx.x;
+  const int64_t row = blockIdx.x;
+  const int top_n = a.out.top_n;
+  SoftSum sum;
+  int ahead = 0;
+  if (tid < a.parts) {
+    const float4_t p = a.sums[row * a.parts + tid];
+    sum = SoftSum{p[0], p[1], p[2]};
+    ahead = as_int(p[3]);
+  }
+  sum.merge_wave();
+  ahead = wave_reduce_dpp(ahead, [](int x, int y) { return x + y; });
+  if ((tid & 63) == 0) waves[tid >> 6] = float4_t{sum.m, sum.s, sum.u, as_float(ahead)};
+  if (tid == 0) cand.n = 0;
+  __syncthreads();
+  sum = SoftSum{};
+  ahead = 0;
+#pragma unroll
+  for (int i = 0; i < kThreads / 64; ++i) {
+    const float4_t w = waves[i];
+    sum.merge(SoftSum{w[0], w[1], w[2]});
+    ahead += as_int(w[3]);
+  }
+  const int token = a.out.tokens ? a.out.tokens[row] : -1;
+  const bool has_token = token >= 0 && token < a.V;
+  float zt = 0.0f;
+  if (has_token) {
+    const int64_t at = row * a.ld + token;
+    zt = io == RWKV_IO_F16 ? h2f(static_cast<const half_t*>(a.logits)[at]) : static_cast<const float*>(a.logits)[at];
+  }
+  if (tid == 0) {
+    write_logprobs(sum, a.out, row, a.V, &zt);
+    if (a.out.rank) a.out.rank[row] = !has_token || zt != zt ? -1 : ahead;
+  }
+  if (top_n == 0) return;
+  const int total = a.parts * top_n;
+  const key_t* keys = a.keys + row * total;
+  float bound = -INFINITY;
+  if (total > kThreads) {
+    float most = -INFINITY;
+    for (int k = tid; k < total; k += kThreads)
+      if (keys[k]) most = fmaxf(most, key_value(keys[k]));
+    bound = first_bound(cand, top_n, most);
+  }
+  for (int k = tid; k < total; k += kThreads)
+    if (keys[k] && key_value(keys[k]) >= bound) offer(cand, 0, keys[k]);
+  __syncthreads();
+  const int n = cand.n;
+  const float log_s = logf(sum.s);
+  if (n <= kCandidates) {
+    thin_out(cand, 0, n, top_n);
+    __syncthreads();
+    if (tid < top_n) write_alternative(a.out, row, tid, tid < n ? cand.list[1][tid] : 0, sum.m, log_s);
+    return;
+  }
+  // (equal values all over) one after the other, out of memory
+  key_t last = ~static_cast<key_t>(0);
+  key_t* best_of = cand.list[0];
+  for (int place = 0; place < top_n; ++place) {
+    key_t best = 0;
+    for (int k = tid; k < total; k += kThreads)
+      if (keys[k] < last && keys[k] > best) best = keys[k];
+    __syncthreads();
+    best_of[tid] = best;
+    __syncthreads();
+    for (int step = kThreads / 2; step > 0; step /= 2) {
+      if (tid < step && best_of[tid + step] > best_of[tid]) best_of[tid] = best_of[tid + step];
+      __syncthreads();
+    }
+    last = best_of[0];
+    if (tid == 0) write_alternative(a.out, row, place, last, sum.m, log_s);
+  }
+}
+
+// Parts of a row: as many as bring the call to four blocks of 256 threads for every CU, each at least one batch long.
+int parts_of(int rows, int V) {
+  const int batch = kThreads * 16;  // entries of fp32
+  return std::max(1, std::min({4 * device_cu_count() / rows, ceil_div(V, batch), kMaxParts}));
+}
+size_t sums_bytes(int rows, int parts) { return static_cast<size_t>(rows) * parts * sizeof(float4_t); }
+
 template <typename T>
-void launch_rows(hipStream_t st, int rows, const LogprobArgs& a) {
-  if (rows <= 2 * device_cu_count()) hipLaunchKernelGGL((token_logprobs_kernel<T, 1024>), dim3(rows), dim3(1024), 0, st, a);
-  else hipLaunchKernelGGL((token_logprobs_kernel<T, 256>), dim3(rows), dim3(256), 0, st, a);
+void launch_rows(hipStream_t st, int rows, int io, const LogprobArgs& a) {
+  if (a.parts == 1) {
+    hipLaunchKernelGGL((token_logprobs_kernel<T, false>), dim3(rows), dim3(kThreads), 0, st, a);
+  } else {
+    hipLaunchKernelGGL((token_logprobs_kernel<T, true>), dim3(rows, a.parts), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL(token_logprobs_join_kernel, dim3(rows), dim3(kThreads), 0, st, a, io);
+  }
 }
 
 }  // namespace
 
-size_t token_logprobs_workspace_bytes(int rows, int V, int top_n) { return 0; }
+size_t token_logprobs_workspace_bytes(int rows, int V, int top_n) {
+  const int parts = parts_of(rows, V);
+  return parts == 1 ? 0 : sums_bytes(rows, parts) + static_cast<size_t>(rows) * parts * top_n * sizeof(key_t);
+}
 
 int token_logprobs_launch(hipStream_t st, int rows, int V, int io, const void* logits, int64_t ld, const TokenLogprobs& out, void* workspace) {
-  LogprobArgs a = {logits, ld, V, out};
-  if (io == RWKV_IO_F16) launch_rows<half_t>(st, rows, a);
-  else launch_rows<float>(st, rows, a);
+  const int parts = parts_of(rows, V);
+  // (a multiple of a vector, so that the parts of an aligned row are aligned)
+  LogprobArgs a = {logits, ld, V, out, parts, ceil_div(ceil_div(V, parts), 64) * 64, static_cast<float4_t*>(workspace),
+                   reinterpret_cast<key_t*>(static_cast<char*>(workspace) + sums_bytes(rows, parts))};
+  a.parts = ceil_div(V, a.part_len);  // (rounding up may leave the last one without entries)
+  if (io == RWKV_IO_F16) launch_rows<half_t>(st, rows, io, a);
+  else launch_rows<float>(st, rows, io, a);
   RWKV_LAUNCH_CHECK();
   return RWKV_OK;
 }

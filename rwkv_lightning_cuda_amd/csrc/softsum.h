@@ -1,4 +1,5 @@
-// What the two files of the log probabilities share: the running sums of a softmax and its entropy, and the results they give.
+// What the two files of the log probabilities share: the running sums of a softmax and its entropy, the order of the alternatives, and
+// the results.
 #pragma once
 
 #include "ops.h"
@@ -8,6 +9,14 @@ namespace rwkv {
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kGone = -200.0f;  // e^-200 is 0 in fp32; a difference that is multiplied by it must not be infinite
+
+// by value, as as_half2: a bit cast of a vector's element reads element 0
+__device__ __forceinline__ int as_int(float v) { return __builtin_bit_cast(int, v); }
+__device__ __forceinline__ float as_float(int v) { return __builtin_bit_cast(float, v); }
+template <int D>
+__device__ __forceinline__ float lane_xor_f(float v) {
+  return as_float(lane_xor_dpp<D>(as_int(v)));
+}
 
 // m = max z, S = sum e^(z - m), U = sum (z - m) e^(z - m) of the entries seen so far.  m starts at the lowest finite value, not at
 // -infinity: differences with it are no NaN, and S stays 0 as long as every entry is -infinity.  A NaN or +infinity among the entries
@@ -21,26 +30,31 @@ struct SoftSum {
     s *= f;
     m = to;
   }
-  // first, o_first: where each has its largest entry; the lower one where they are equal
-  __device__ __forceinline__ void merge(SoftSum o, int& first, int o_first) {
-    first = o.m > m ? o_first : (o.m == m ? min(first, o_first) : first);
+  __device__ __forceinline__ void merge(SoftSum o) {
     const float to = fmaxf(m, o.m);
     raise(to);
     o.raise(to);
     s += o.s;
     u += o.u;
   }
+  // with what the lane of the other value of bit D has: both end with the same bits
+  template <int D>
+  __device__ __forceinline__ void merge_lanes() {
+    merge(SoftSum{lane_xor_f<D>(m), lane_xor_f<D>(s), lane_xor_f<D>(u)});
+  }
+  __device__ __forceinline__ void merge_wave() {
+    merge_lanes<32>();
+    merge_lanes<16>();
+    merge_lanes<8>();
+    merge_lanes<4>();
+    merge_lanes<2>();
+    merge_lanes<1>();
+  }
 };
 
-// by value, as as_half2: a bit cast of a vector's element reads element 0
-__device__ __forceinline__ int as_int(float v) { return __builtin_bit_cast(int, v); }
-
-// whether entry i of value v is ahead of entry k of value w
-__device__ __forceinline__ bool ahead_of(float v, int i, float w, int k) { return v > w || (v == w && i < k); }
-
 // log probability and entropy of a row: ln S - U / S is a sum of two terms that are not negative, nothing cancels.  token_logit is
-// that of the row's token, read only where it is an entry
-__device__ __forceinline__ void write_logprobs(const SoftSum& a, const TokenLogprobs& out, int64_t row, int V, const float* token_logit) {
+// that of the row's token, read only where it is an entry.  Returns ln S.
+__device__ __forceinline__ float write_logprobs(const SoftSum& a, const TokenLogprobs& out, int64_t row, int V, const float* token_logit) {
   const bool nothing = a.s == 0.0f;
   const float log_s = logf(a.s);
   if (out.logprob) {
@@ -48,6 +62,86 @@ __device__ __forceinline__ void write_logprobs(const SoftSum& a, const TokenLogp
     out.logprob[row] = t < 0 ? 0.0f : t >= V ? __builtin_nanf("") : nothing ? -INFINITY : *token_logit - a.m - log_s;
   }
   if (out.entropy) out.entropy[row] = nothing ? 0.0f : log_s - a.u / a.s;
+  return log_s;
+}
+
+// The order "larger first, equal ones by index" as that of whole numbers: the value's bits made to rise with it above the index's
+// complement.  No entry has the key 0.  (-0 is 0; NaN has no place and must not come here.)
+typedef unsigned long long key_t;
+__device__ __forceinline__ key_t key_of(float z, int i) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, z + 0.0f);
+  return static_cast<key_t>(b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u)) << 32 | ~static_cast<uint32_t>(i);
+}
+__device__ __forceinline__ float key_value(key_t k) {
+  const uint32_t b = static_cast<uint32_t>(k >> 32);
+  return __builtin_bit_cast(float, b & 0x80000000u ? b ^ 0x80000000u : ~b);
+}
+__device__ __forceinline__ int key_index(key_t k) { return static_cast<int>(~static_cast<uint32_t>(k)); }
+
+constexpr int kCandidates = 1024;
+
+// Entries that may be among the first top_n, in LDS.  They come in the order of an atomic counter, which no result depends on.
+template <int NT>
+struct Candidates {
+  key_t list[2][kCandidates];
+  float group_max[256];
+  int n;
+  float bound;
+};
+
+// The top_n-th largest of the maxima of 64 or 256 groups of threads: top_n entries are at least as large, so that none below it is among
+// the first top_n.  Every thread of the block comes here; -infinity where there are not as many.
+template <int NT>
+__device__ __forceinline__ float first_bound(Candidates<NT>& c, int top_n, float mine) {
+  const int tid = threadIdx.x;
+  const int groups = top_n <= 24 ? 64 : 256;
+  if (mine != mine) mine = -INFINITY;
+  if (groups == 64) {
+    static_assert(NT == 256, "four threads to one of 64 groups");
+    mine = fmaxf(mine, lane_xor_f<1>(mine));
+    mine = fmaxf(mine, lane_xor_f<2>(mine));
+    if ((tid & 3) == 0) c.group_max[tid >> 2] = mine;
+  } else {
+    c.group_max[tid] = mine;
+  }
+  __syncthreads();
+  if (tid < groups) {
+    const float v = c.group_max[tid];
+    int before = 0;
+    for (int i = 0; i < groups; i += 4) {
+      const float4_t w = *reinterpret_cast<const float4_t*>(c.group_max + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) before += w[e] > v || (w[e] == v && i + e < tid);
+    }
+    if (before == top_n - 1) c.bound = v;
+  }
+  __syncthreads();
+  return c.bound;
+}
+
+// The first top_n of the n in list `from`, in order, to the other list.  Behind a barrier; the caller waits for what it writes.
+template <int NT>
+__device__ __forceinline__ void thin_out(Candidates<NT>& c, int from, int n, int top_n) {
+  const key_t* list = c.list[from];
+  for (int k = threadIdx.x; k < n; k += NT) {
+    const key_t mine = list[k];
+    int before = 0;
+    for (int i = 0; i < n; ++i) before += list[i] > mine;
+    if (before < top_n) c.list[from ^ 1][before] = mine;
+  }
+}
+
+template <int NT>
+__device__ __forceinline__ void offer(Candidates<NT>& c, int to, key_t key) {
+  const int at = atomicAdd(&c.n, 1);
+  if (at < kCandidates) c.list[to][at] = key;
+}
+
+// key 0: none
+__device__ __forceinline__ void write_alternative(const TokenLogprobs& out, int64_t row, int place, key_t key, float m, float log_s) {
+  const int64_t o = row * out.top_n + place;
+  out.top_ids[o] = key ? key_index(key) : -1;
+  out.top_logprobs[o] = key ? key_value(key) - m - log_s : -INFINITY;
 }
 
 }  // namespace rwkv
