@@ -27,7 +27,7 @@ struct HeadArgs {
   const half_t* scale;   // int8 weights: [N]
   int M, N, K;
   const int* tokens;     // may be NULL
-  float4_t* sums;        // [M][parts]: m, S, U of a part's columns (few rows: 32 columns, tiles: 256)
+  float4_t* sums;        // [M][parts]: m, S, U of a part's columns (few rows: a block's, tiles: 256)
   float* token_logit;    // [M], written where the token is a column
   // alternatives only
   float* logits;         // [M,N], written where it may hold one
@@ -45,13 +45,16 @@ struct HeadArgs {
 // 32 g + 16 h (int8) or + 8 i (fp16) - R = the rows rounded up to a power of two.
 constexpr int kFewThreads = 512;
 constexpr int kFewLds = 128 * 1024;
-constexpr int kFewRows = 32;
+constexpr int kFewRows = 16;  // (24 rows: 64 us against 60 as tiles, 12 rows: 60 and 60, 5 rows: 59 and 62; fp16 rows and int8 weights: 12 rows 63 and 73)
+constexpr int kFewMergeBytes = kFewThreads / 64 * kFewRows * 16;
 
 int few_rows(int M) {
   int r = 1;
   while (r < M) r *= 2;
   return r;
 }
+// bands of 32 columns per wavefront: one round of blocks on the chip
+int few_bands(int N) { return ceil_div(N / 32, kFewThreads / 64 * device_cu_count()); }
 bool takes_few(int M, int K, int x_bytes) { return M <= kFewRows && static_cast<int64_t>(few_rows(M)) * K * x_bytes <= kFewLds; }
 
 template <int TYPES>
@@ -94,6 +97,7 @@ __global__ __launch_bounds__(kFewThreads) void head_few_kernel(HeadArgs g, int l
   const float xs = TYPES == kI8W8 ? g.x_scale[min(j, g.M - 1)] : 1.0f;
   const int token = g.tokens ? g.tokens[min(j, g.M - 1)] : -1;
   typedef typename WideTile<T::kTile, 2>::acc_t acc_t;
+  SoftSum total;
   int left = chunks;
   for (int band = band0; band < band1; ++band) {
     acc_t acc;
@@ -143,9 +147,8 @@ __global__ __launch_bounds__(kFewThreads) void head_few_kernel(HeadArgs g, int l
       a.s += p;
       a.u = fmaf(fmaxf(d, kGone), p, a.u);
     }
-    a.merge_lanes<32>();
+    total.merge(a);
     if (j < g.M) {
-      if (h == 0) g.sums[static_cast<int64_t>(j) * g.parts + band] = float4_t{a.m, a.s, a.u, 0.0f};
       const int t = token - band * 32 - 4 * h;
       if (t >= 0 && t < 32) {
 #pragma unroll
@@ -159,6 +162,22 @@ __global__ __launch_bounds__(kFewThreads) void head_few_kernel(HeadArgs g, int l
               float4_t{z[4 * q], z[4 * q + 1], z[4 * q + 2], z[4 * q + 3]};
       }
     }
+  }
+  // the block's columns
+  total.merge_lanes<32>();
+  __syncthreads();
+  float4_t* merge = reinterpret_cast<float4_t*>(x_lds);  // [kWaves][kFewRows]
+  if (h == 0 && j < g.M) merge[wave * kFewRows + j] = float4_t{total.m, total.s, total.u, 0.0f};
+  __syncthreads();
+  const int r = threadIdx.x;
+  if (r < g.M) {
+    SoftSum a;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+      const float4_t o = merge[i * kFewRows + r];
+      a.merge(SoftSum{o[0], o[1], o[2]});
+    }
+    g.sums[static_cast<int64_t>(r) * g.parts + blockIdx.x] = float4_t{a.m, a.s, a.u, 0.0f};
   }
 }
 
@@ -280,30 +299,21 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void head_tile_kernel(HeadArgs 
   }
 }
 
-// The top_n-th largest of the strips that the first launch has left, of one row per block: no alternative lies below it.
+// What the top_n-th largest of the strips that the first launch has left reaches, a wavefront per row: no alternative lies below it.
 constexpr int kBoundStrips = 1024;
+template <int N>
 __global__ __launch_bounds__(256) void head_bound_kernel(HeadArgs g, int top_n, float* bound) {
-  __shared__ __align__(16) float most[kBoundStrips];
-  const float4_t* strips = reinterpret_cast<const float4_t*>(g.strips) + static_cast<int64_t>(blockIdx.x) * g.parts;
-  const int n = 4 * g.col_blocks;
-  for (int i = threadIdx.x; i < g.col_blocks; i += 256) {
-    float4_t v = strips[i * g.every];
+  const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (row >= g.M) return;
+  const float* strips = g.strips + static_cast<int64_t>(row) * g.parts * 4;
+  float v[N];
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (v[e] != v[e]) v[e] = -INFINITY;
-    *reinterpret_cast<float4_t*>(most + 4 * i) = v;
+  for (int i = 0; i < N; ++i) {
+    const int k = i * 64 + lane;
+    v[i] = k < 4 * g.col_blocks ? strips[(k >> 2) * g.every * 4 + (k & 3)] : -INFINITY;
   }
-  __syncthreads();
-  for (int k = threadIdx.x; k < n; k += 256) {
-    const float mine = most[k];
-    int before = 0;
-    for (int i = 0; i < n; i += 4) {
-      const float4_t w = *reinterpret_cast<const float4_t*>(most + i);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) before += w[e] > mine || (w[e] == mine && i + e < k);
-    }
-    if (before == top_n - 1) bound[blockIdx.x] = mine;
-  }
+  const float found = wave_bound(v, top_n);
+  if (lane == 0) bound[row] = found;
 }
 
 // Log probability and entropy from the parts' sums: a wavefront per row.
@@ -312,17 +322,21 @@ __global__ __launch_bounds__(256) void head_sums_kernel(HeadArgs g, TokenLogprob
   if (row >= g.M) return;
   const float4_t* sums = g.sums + static_cast<int64_t>(row) * g.parts;
   SoftSum a;
-  for (int i = threadIdx.x & 63; i < g.parts; i += 64) {
-    const float4_t p = sums[i];
-    a.merge(SoftSum{p[0], p[1], p[2]});
+  for (int i = threadIdx.x & 63; i < g.parts; i += 4 * 64) {
+    float4_t p[4];  // requested together
+#pragma unroll
+    for (int q = 0; q < 4; ++q) p[q] = sums[min(i + q * 64, g.parts - 1)];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (i + q * 64 < g.parts) a.merge(SoftSum{p[q][0], p[q][1], p[q][2]});
   }
   a.merge_wave();
   if ((threadIdx.x & 63) == 0) write_logprobs(a, out, row, g.N, g.token_logit + row);
 }
 
 // The same with the alternatives, a block per row: they lie in the strips whose largest reaches the top_n-th largest of 64 or 256 groups
-// of strips - few more than top_n of them - whose logits are there.  Four (or eight) strips at a time; the list never overflows, it is thinned out
-// first.  Strips of 64 columns with their largest in `strips` (tiles), or of 32 with it in `sums` (few rows).
+// of strips - few more than top_n of them - whose logits are there.  768 columns at a time; the list never overflows, it is thinned out
+// first.  Strips of `width` columns: 64 with their largest in `strips` (tiles), or a part's with it in `sums` (few rows).
 __global__ __launch_bounds__(256) void head_alternatives_kernel(HeadArgs g, TokenLogprobs out, int width) {
   __shared__ __align__(16) Candidates<256> cand;
   __shared__ float4_t waves[4];
@@ -356,7 +370,10 @@ __global__ __launch_bounds__(256) void head_alternatives_kernel(HeadArgs g, Toke
   }
   key_t least = bound == -INFINITY ? 0 : key_of(bound, 0x7fffffff);  // what a candidate has to be ahead of
   int list = 0;
-  const int at_once = 256 / width;
+  const int at_once = width < 256 ? width : 256;  // columns of a strip
+  const int pieces = width / at_once;
+  constexpr int kAtOnce = 3;
+  static_assert(kMaxAlternatives <= kCandidates - kAtOnce * 256, "a list that has been thinned out takes the next entries");
   for (int base = 0; base < n_strips; base += 256) {
     const int s = base + tid;
     // (a strip whose largest ties with the last candidate and lies behind it has none)
@@ -365,23 +382,26 @@ __global__ __launch_bounds__(256) void head_alternatives_kernel(HeadArgs g, Toke
       if (v == v && key_of(v, s * width) > least) chosen[atomicAdd(&n_chosen, 1)] = s;
     }
     __syncthreads();
-    const int n = n_chosen;
-    for (int k = 0; k < n; k += at_once) {
-      const int which = k + tid / width;
-      if (which < n) {
-        const int col = chosen[which] * width + tid % width;
-        if (col < g.N) {
-          const float v = logits[col];
-          if (v > -INFINITY) {
-            const key_t key = key_of(v, col);
-            if (key > least) offer(cand, list, key);
-          }
-        }
+    const int n = n_chosen * pieces;
+    for (int k = 0; k < n; k += kAtOnce * (256 / at_once)) {
+      float v[kAtOnce];
+      int col[kAtOnce];
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q) {  // requested together
+        const int which = k + q * (256 / at_once) + tid / at_once;
+        col[q] = which < n ? chosen[which / pieces] * width + which % pieces * at_once + tid % at_once : g.N;
+        v[q] = col[q] < g.N ? logits[col[q]] : -INFINITY;
       }
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q)
+        if (v[q] > -INFINITY) {
+          const key_t key = key_of(v[q], col[q]);
+          if (key > least) offer(cand, list, key);
+        }
       __syncthreads();
       const int have = cand.n;
       __syncthreads();
-      if (have > kCandidates - 256) {
+      if (have > kCandidates - kAtOnce * 256) {
         thin_out(cand, list, have, top_n);
         list ^= 1;
         __syncthreads();
@@ -416,12 +436,16 @@ constexpr int kSumRows = 8192;    // rows at a time without alternatives: 32 MiB
 constexpr int kLogits = 1 << 27;  // and with them, rows times columns: 512 MiB of places for logits, few of which are written
 constexpr int kFewestTurns = 6;   // turns of blocks on the chip from which on two launches cost less than the logits they save
 
-Plan plan_of(bool x_int8, int M, int N, int K, int top_n) {
+Plan plan_of(int fmt, bool x_int8, int M, int N, int K, int top_n) {
   Plan p = {};
   p.few = takes_few(M, K, x_int8 ? 1 : 2);
   p.rows = p.few ? M : std::min(M, top_n > 0 ? std::max(kLogits / N / 256, 1) * 256 : kSumRows);
-  p.tile = p.rows <= 128 ? 128 : 256;
-  p.parts = ceil_div(N, p.few ? 32 : kTileCols);
+  // (us, 65536 x 4096 int8, 2048 rows: tiles of 128 rows 527, of 256 508, fp16 970 and 956, int8 weights under fp16 1033 and 890; 333 rows
+  // of 2048: 114 and 141, 116 and 141, 110 and 118 - a few rows of padding are worth more than the tile)
+  const int per_row = fmt == RWKV_FMT_W8 && !x_int8 ? 122 : 106;
+  p.tile = ceil_div(p.rows, 128) * 128 * per_row < ceil_div(p.rows, 256) * 256 * 100 ? 128 : 256;
+
+  p.parts = p.few ? ceil_div(N / 32, kFewThreads / 64 * few_bands(N)) : ceil_div(N, kTileCols);
   p.every = 1;
   if (!p.few && top_n > 0) {
     const int64_t blocks = static_cast<int64_t>(ceil_div(p.rows, p.tile)) * p.parts, cus = device_cu_count();
@@ -441,12 +465,9 @@ Plan plan_of(bool x_int8, int M, int N, int K, int top_n) {
 template <int TYPES>
 int launch_few(hipStream_t st, const HeadArgs& g) {
   const int R = few_rows(g.M);
-  const int lds = R * g.K * Types<TYPES>::kXBytes;
-  const int waves = kFewThreads / 64;
-  const int bands = g.N / 32;
-  const int per_wave = ceil_div(bands, waves * device_cu_count());
+  const int lds = std::max(R * g.K * Types<TYPES>::kXBytes, kFewMergeBytes);
   RWKV_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(head_few_kernel<TYPES>), hipFuncAttributeMaxDynamicSharedMemorySize, kFewLds));
-  hipLaunchKernelGGL(head_few_kernel<TYPES>, dim3(ceil_div(bands, waves * per_wave)), dim3(kFewThreads), lds, st, g, __builtin_ctz(R), per_wave);
+  hipLaunchKernelGGL(head_few_kernel<TYPES>, dim3(g.parts), dim3(kFewThreads), lds, st, g, __builtin_ctz(R), few_bands(g.N));
   RWKV_LAUNCH_CHECK();
   return RWKV_OK;
 }
@@ -475,7 +496,9 @@ int launch_rows(hipStream_t st, const Plan& p, HeadArgs g, const TokenLogprobs& 
   } else {
     rc = launch_tiles<TYPES, true>(st, g, p.tile, p.every, false);
     if (rc == RWKV_OK && p.every > 1) {
-      hipLaunchKernelGGL(head_bound_kernel, dim3(g.M), dim3(256), 0, st, g, out.top_n, bound);
+      const dim3 grid(ceil_div(g.M, 4));
+      if (4 * g.col_blocks <= 128) hipLaunchKernelGGL(head_bound_kernel<2>, grid, dim3(256), 0, st, g, out.top_n, bound);
+      else hipLaunchKernelGGL(head_bound_kernel<kBoundStrips / 64>, grid, dim3(256), 0, st, g, out.top_n, bound);
       RWKV_LAUNCH_CHECK();
       g.bound = bound;
       rc = launch_tiles<TYPES, true>(st, g, p.tile, p.every, true);
@@ -483,18 +506,18 @@ int launch_rows(hipStream_t st, const Plan& p, HeadArgs g, const TokenLogprobs& 
   }
   if (rc != RWKV_OK) return rc;
   if (out.top_n == 0) hipLaunchKernelGGL(head_sums_kernel, dim3(ceil_div(g.M, 4)), dim3(256), 0, st, g, out);
-  else hipLaunchKernelGGL(head_alternatives_kernel, dim3(g.M), dim3(256), 0, st, g, out, p.few ? 32 : 64);
+  else hipLaunchKernelGGL(head_alternatives_kernel, dim3(g.M), dim3(256), 0, st, g, out, p.few ? few_bands(g.N) * (kFewThreads / 64 * 32) : 64);
   RWKV_LAUNCH_CHECK();
   return RWKV_OK;
 }
 
 }  // namespace
 
-size_t linear_logprobs_workspace_bytes(int fmt, bool x_int8, int M, int N, int K, int top_n) { return plan_of(x_int8, M, N, K, top_n).bytes(); }
+size_t linear_logprobs_workspace_bytes(int fmt, bool x_int8, int M, int N, int K, int top_n) { return plan_of(fmt, x_int8, M, N, K, top_n).bytes(); }
 
 int linear_logprobs_launch(hipStream_t st, int fmt, int M, int N, int K, const void* x, const float* x_scale, const void* packed,
                            const half_t* scale, const TokenLogprobs& out, void* workspace) {
-  const Plan p = plan_of(x_scale != nullptr, M, N, K, out.top_n);
+  const Plan p = plan_of(fmt, x_scale != nullptr, M, N, K, out.top_n);
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   for (int m = 0; m < M; m += p.rows) {
     const int64_t off = static_cast<int64_t>(m) * K * (x_scale ? 1 : 2);

@@ -106,17 +106,13 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobArgs a)
         if (stray_z >= bound && stray_z > -INFINITY) offer(cand, list, key_of(stray_z, first + stray));
       }
       if (most >= bound) {
-        uint32_t mask = 0;
 #pragma unroll
-        for (int e = VB * VE - 1; e >= 0; --e) mask = mask * 2 + (x[e] >= bound);
-        while (mask) {
-          const int e = __builtin_ctz(mask);
-          mask &= mask - 1;
-          const int i = head + ((b * VB + e / VE) * NT + tid) * VE + e % VE;
-          if (i >= tail) continue;
-          const float v = static_cast<float>(z[i]);  // (again from memory: a register cannot be chosen by a number)
-          if (v > -INFINITY) offer(cand, list, key_of(v, first + i));
-        }
+        for (int q = 0; q < VB; ++q)
+#pragma unroll
+          for (int e = 0; e < VE; ++e) {
+            const float v = x[q * VE + e];
+            if (v >= bound && v > -INFINITY) offer(cand, list, key_of(v, first + head + ((b * VB + q) * NT + tid) * VE + e));
+          }
       }
       if (b % kRefine == kRefine - 1) {
         __syncthreads();
@@ -267,7 +263,7 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_join_kernel(LogprobAr
   const int total = a.parts * top_n;
   const key_t* keys = a.keys + row * total;
   float bound = -INFINITY;
-  if (total > kThreads) {
+  if (total > 32) {
     float most = -INFINITY;
     for (int k = tid; k < total; k += kThreads)
       if (keys[k]) most = fmaxf(most, key_value(keys[k]));
