@@ -299,10 +299,13 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_join_kernel(LogprobAr
   }
 }
 
-// Parts of a row: as many as bring the call to four blocks of 256 threads for every CU, each at least one batch long.
-int parts_of(int rows, int V) {
-  const int batch = kThreads * 16;  // entries of fp32
-  return std::max(1, std::min({4 * device_cu_count() / rows, ceil_div(V, batch), kMaxParts}));
+// Parts of a row: as many as bring the call to four blocks of 256 threads for every CU, each at least one batch long, and none where that
+// is fewer than three (us with the join, fp32, 65536 entries: 64 rows in 16 parts 12.6, in 4 18.3; 200 rows in 5 20.8, whole 24.9; 400
+// rows in 2 29.3, whole 27.9; 77 fp16 rows of 50277 in 7 12.3, in 13 13.6).
+int parts_of(int rows, int V, int io) {
+  const int batch = kThreads * (io == RWKV_IO_F16 ? 32 : 16);
+  const int parts = std::min({4 * device_cu_count() / rows, ceil_div(V, batch), kMaxParts});
+  return parts < 3 ? 1 : parts;
 }
 size_t sums_bytes(int rows, int parts) { return static_cast<size_t>(rows) * parts * sizeof(float4_t); }
 
@@ -319,12 +322,12 @@ void launch_rows(hipStream_t st, int rows, int io, const LogprobArgs& a) {
 }  // namespace
 
 size_t token_logprobs_workspace_bytes(int rows, int V, int top_n) {
-  const int parts = parts_of(rows, V);
+  const int parts = parts_of(rows, V, RWKV_IO_F32);  // (fp16 rows go in no more)
   return parts == 1 ? 0 : sums_bytes(rows, parts) + static_cast<size_t>(rows) * parts * top_n * sizeof(key_t);
 }
 
 int token_logprobs_launch(hipStream_t st, int rows, int V, int io, const void* logits, int64_t ld, const TokenLogprobs& out, void* workspace) {
-  const int parts = parts_of(rows, V);
+  const int parts = parts_of(rows, V, io);
   // (a multiple of a vector, so that the parts of an aligned row are aligned)
   LogprobArgs a = {logits, ld, V, out, parts, ceil_div(ceil_div(V, parts), 64) * 64, static_cast<float4_t*>(workspace),
                    reinterpret_cast<key_t*>(static_cast<char*>(workspace) + sums_bytes(rows, parts))};

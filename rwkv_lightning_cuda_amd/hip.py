@@ -57,6 +57,16 @@ EXPORTS = [
 ]
 
 
+# Argument types of the entry points that a serving loop calls after every token: ctypes then converts plain ints itself (a call with
+# 17 arguments 3 us instead of 9).
+_P, _N, _L, _S = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
+_ARGTYPES = {
+    "rwkv_hip_add_norm_q8": [_P, _N, _N, _N, _P, _P, _P, _P, ctypes.c_float, _P, _P, _P],
+    "rwkv_hip_token_logprobs": [_P, _N, _N, _N, _P, _L, _P, _N, _P, _P, _P, _P, _P, _P, _S],
+    "rwkv_hip_linear_logprobs": [_P, _N, _N, _N, _N, _P, _P, _P, _P, _P, _N, _P, _P, _P, _P, _P, _S],
+}
+
+
 class RwkvHipError(RuntimeError):
     pass
 
@@ -77,6 +87,8 @@ def load():
     if missing:
         raise RwkvHipError("librwkv_hip.so lacks symbols: %s" % ", ".join(missing))
     lib.rwkv_hip_last_error.restype = ctypes.c_char_p
+    for name, types in _ARGTYPES.items():
+        getattr(lib, name).argtypes = types
     _lib = lib
     return lib
 
@@ -88,6 +100,11 @@ def _p(x):
     if isinstance(x, DeviceArray):
         return ctypes.c_void_p(x.ptr)
     return ctypes.c_void_p(int(x))
+
+
+def _a(x):
+    """The same as a plain int or None, for the entry points whose argument types are declared."""
+    return x.ptr if isinstance(x, DeviceArray) else x if x is None else int(x)
 
 
 def check(rc):
@@ -403,8 +420,7 @@ def argmax(B, V, logits, out, stream=None):
 
 def add_norm_q8(rows, C, x, res, w, b, q, scale, x_out=None, norm=NORM_LAYER, eps=1e-5, stream=None):
     """Residual addition (res None: none), norm and int8 codes with a scale per row; x_out receives the sum."""
-    check(load().rwkv_hip_add_norm_q8(_p(stream), _i(rows), _i(C), _i(norm), _p(x), _p(res), _p(w), _p(b), ctypes.c_float(eps), _p(x_out),
-                                      _p(q), _p(scale)))
+    check(load().rwkv_hip_add_norm_q8(_a(stream), int(rows), int(C), int(norm), _a(x), _a(res), _a(w), _a(b), eps, _a(x_out), _a(q), _a(scale)))
 
 
 def token_logprobs_workspace(rows, V, top_n=0):
@@ -416,9 +432,9 @@ def token_logprobs_workspace(rows, V, top_n=0):
 def token_logprobs(rows, V, logits, tokens, workspace=None, logprob=None, entropy=None, rank=None, top_n=0, top_ids=None,
                    top_logprobs=None, io=IO_F32, ld=None, stream=None):
     """ln softmax(logits)[token], entropy, rank of the token and the top_n first entries of every row; ld: entries between rows."""
-    check(load().rwkv_hip_token_logprobs(_p(stream), _i(rows), _i(V), _i(io), _p(logits), ctypes.c_int64(V if ld is None else ld),
-                                         _p(tokens), _i(top_n), _p(logprob), _p(entropy), _p(rank), _p(top_ids), _p(top_logprobs),
-                                         _p(workspace), ctypes.c_size_t(workspace.nbytes if workspace is not None else 0)))
+    check(load().rwkv_hip_token_logprobs(_a(stream), int(rows), int(V), int(io), _a(logits), int(V if ld is None else ld), _a(tokens), int(top_n),
+                                         _a(logprob), _a(entropy), _a(rank), _a(top_ids), _a(top_logprobs), _a(workspace),
+                                         workspace.nbytes if workspace is not None else 0))
 
 
 def linear_logprobs_workspace(fmt, M, N, K, top_n=0, x_int8=False):
@@ -430,9 +446,9 @@ def linear_logprobs_workspace(fmt, M, N, K, top_n=0, x_int8=False):
 def linear_logprobs(fmt, M, N, K, x, packed, scale, tokens, workspace, x_scale=None, logprob=None, entropy=None, top_n=0, top_ids=None,
                     top_logprobs=None, stream=None):
     """token_logprobs (without the rank) of the logits x . W^T; x_scale: x holds int8 codes."""
-    check(load().rwkv_hip_linear_logprobs(_p(stream), _i(fmt), _i(M), _i(N), _i(K), _p(x), _p(x_scale), _p(packed), _p(scale), _p(tokens),
-                                          _i(top_n), _p(logprob), _p(entropy), _p(top_ids), _p(top_logprobs), _p(workspace),
-                                          ctypes.c_size_t(workspace.nbytes if workspace is not None else 0)))
+    check(load().rwkv_hip_linear_logprobs(_a(stream), int(fmt), int(M), int(N), int(K), _a(x), _a(x_scale), _a(packed), _a(scale), _a(tokens),
+                                          int(top_n), _a(logprob), _a(entropy), _a(top_ids), _a(top_logprobs), _a(workspace),
+                                          workspace.nbytes if workspace is not None else 0))
 
 
 class Event:
