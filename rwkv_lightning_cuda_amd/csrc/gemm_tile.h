@@ -32,8 +32,10 @@ struct WideTile {
 
 // 64 lanes x 16 bytes from base + off into LDS from `lds` on.  In asm, because the compiler would wait for every such load in flight
 // at the next read of LDS.
+template <bool ONCE = false>
 __device__ __forceinline__ void load_to_lds(uint32_t lds, uint32_t off, const void* base) {
-  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(lds), "v"(off), "s"(base) : "memory");
+  if constexpr (ONCE) asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"{m0}"(lds), "v"(off), "s"(base) : "memory");
+  else asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(lds), "v"(off), "s"(base) : "memory");
 }
 
 template <int N>
@@ -44,7 +46,8 @@ __device__ __forceinline__ void meet() {  // all but the N youngest loads of thi
 // acc[nb][mt] = the 32 columns nb of this wavefront's 64 x the 32 rows mt of its 32 MT: lane (j, h) holds, of row j, columns
 // 8 (v / 4) + 4 h + v % 4.  x_base: row 0 of the block's rows (`rows` of them exist; the others repeat the last one) at the first k;
 // w_base: the same k of band `wave` of the block's eight bands of 32 columns.  nstages: of T::kK k, at least one.
-template <int FMT, int MT>
+// ONCE: no other block reads these weights (they are not kept in the caches).
+template <int FMT, int MT, bool ONCE = false>
 __device__ __forceinline__ void tile_products(const char* x_base, uint32_t x_row_bytes, int rows, const char* w_base, int nstages,
                                               unsigned char* lds, typename WideTile<FMT, MT>::acc_t (&acc)[2][MT]) {
   using T = WideTile<FMT, MT>;
@@ -70,7 +73,7 @@ __device__ __forceinline__ void tile_products(const char* x_base, uint32_t x_row
       load_to_lds(dst + (i * kTileWaves + wave) * 1024, x_off[i < T::kXLoads ? i : 0], x_base + c * kTileRowBytes);
     } else {
       const int q = i - T::kXLoads;
-      load_to_lds(dst + T::kXBytes + (wave * T::kPieces + q) * 1024, lane * 16, w_base + (static_cast<int64_t>(c) * T::kPieces + q) * 1024);
+      load_to_lds<ONCE>(dst + T::kXBytes + (wave * T::kPieces + q) * 1024, lane * 16, w_base + (static_cast<int64_t>(c) * T::kPieces + q) * 1024);
     }
   };
 

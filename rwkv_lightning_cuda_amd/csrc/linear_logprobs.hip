@@ -74,7 +74,7 @@ __global__ __launch_bounds__(kFewThreads) void head_few_kernel(HeadArgs g, int l
   uint4_t ahead[kChunk];
   auto request = [&]() {
 #pragma unroll
-    for (int p = 0; p < kChunk; ++p) ahead[p] = w[p * 64];
+    for (int p = 0; p < kChunk; ++p) ahead[p] = __builtin_nontemporal_load(w + p * 64);
     w += kChunk * 64;
   };
   if (chunks > 0) request();
@@ -185,7 +185,7 @@ __global__ __launch_bounds__(kFewThreads) void head_few_kernel(HeadArgs g, int l
 // A tile leaves m, S and U of its 256 columns for every row (16 bytes for 1 KiB of logits).  A lane has 32 columns of a row in
 // registers: they are reduced there, with the other half's 32 by a swap of rows, with the other three wavefronts' 64 each through LDS.
 // LOGITS: also the largest of each 64 columns, and the logits of those 64 where that is not below the row's bound.
-template <int TYPES, int MT, bool LOGITS>
+template <int TYPES, int MT, bool LOGITS, bool ONE>
 __global__ __launch_bounds__(64 * kTileWaves, 2) void head_tile_kernel(HeadArgs g) {
   typedef Types<TYPES> T;
   typedef WideTile<T::kTile, MT> W;
@@ -201,7 +201,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void head_tile_kernel(HeadArgs 
   const int m0 = row_tile * W::BM;
   const int band = min(col_block * 8 + wave, g.N / 32 - 1);  // past the last band: repeat it
   typename W::acc_t acc[2][MT];
-  tile_products<T::kTile, MT>(g.x + static_cast<int64_t>(m0) * g.K * T::kXBytes, static_cast<uint32_t>(g.K) * T::kXBytes, g.M - m0,
+  tile_products<T::kTile, MT, ONE>(g.x + static_cast<int64_t>(m0) * g.K * T::kXBytes, static_cast<uint32_t>(g.K) * T::kXBytes, g.M - m0,
                               g.wp + static_cast<int64_t>(band) * g.K * T::kBandBytes, g.K / W::kK, lds, acc);
 
   const int col0 = col_block * kTileCols + wn * 64;
@@ -361,7 +361,8 @@ __global__ __launch_bounds__(256) void head_alternatives_kernel(HeadArgs g, Toke
   }
   float most = -INFINITY;
   for (int i = tid; i < n_strips; i += 256) most = fmaxf(most, strips[i * apart]);
-  const float bound = first_bound(cand, top_n, most);
+  // (not below the bound that the tiles went by: what lies below that has not been written)
+  const float bound = fmaxf(first_bound(cand, top_n, most), g.bound ? g.bound[row] : -INFINITY);
   a = SoftSum{};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -480,8 +481,9 @@ int launch_tiles(hipStream_t st, HeadArgs& g, int tile, int every, bool rest) {
   g.rest = rest;
   g.col_blocks = rest ? g.parts - ceil_div(g.parts, every) : ceil_div(g.parts, every);
   const dim3 grid(g.row_tiles * ceil_div(g.col_blocks, 8) * 8);
-  if (tile == 256) hipLaunchKernelGGL((head_tile_kernel<TYPES, 4, LOGITS>), grid, dim3(64 * kTileWaves), 0, st, g);
-  else hipLaunchKernelGGL((head_tile_kernel<TYPES, 2, LOGITS>), grid, dim3(64 * kTileWaves), 0, st, g);
+  const auto kernel = tile == 256 ? (g.row_tiles == 1 ? head_tile_kernel<TYPES, 4, LOGITS, true> : head_tile_kernel<TYPES, 4, LOGITS, false>)
+                                  : (g.row_tiles == 1 ? head_tile_kernel<TYPES, 2, LOGITS, true> : head_tile_kernel<TYPES, 2, LOGITS, false>);
+  hipLaunchKernelGGL(kernel, grid, dim3(64 * kTileWaves), 0, st, g);
   RWKV_LAUNCH_CHECK();
   return RWKV_OK;
 }

@@ -67,7 +67,7 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobArgs a)
     for (int q = 0; q < VB; ++q) {
       const int v = (b * VB + q) * NT + tid;
       if (v < vecs) {
-        next[q] = body[v];
+        next[q] = __builtin_nontemporal_load(body + v);
       } else {
 #pragma unroll
         for (int e = 0; e < VE; ++e) next[q][e] = static_cast<T>(-INFINITY);

@@ -191,6 +191,19 @@ def test_logprobs_match_the_formula(gpu, rows, V, dtype, top):
     check_logprobs(run_logprobs(gpu, z, tokens, top), ref_logprobs(z, tokens, top), V)
 
 
+@pytest.mark.parametrize("kind", ["plain", "ties", "equal", "rising", "falling", "masked"])
+@pytest.mark.parametrize("dtype,top", [(np.float32, 20), (np.float16, 3), (np.float32, 64)])
+def test_logprobs_of_many_long_rows(gpu, kind, dtype, top):
+    """Rows that a block reads alone, over many batches; a few of them are checked."""
+    rows, V = 1100, 20003
+    rng = np.random.default_rng(29)
+    z = np.tile(logits_of(kind, rng, 11, V, dtype), (100, 1))
+    tokens = rng.integers(0, V, rows)
+    got = run_logprobs(gpu, z, tokens, top)
+    some = np.r_[0:11, 545:550, 1098:1100]
+    check_logprobs({n: v[some] for n, v in got.items()}, ref_logprobs(z[some], tokens[some], top), V)
+
+
 @pytest.mark.parametrize("kind", ["ties", "equal", "rising", "falling", "sure", "masked", "lowest", "far"])
 @pytest.mark.parametrize("rows,V,dtype,top", [(2, 70, np.float32, 64), (3, 1000, np.float16, 20), (2, 5001, np.float32, 20), (3, 65536, np.float32, 5),
                                               (2, 65536, np.float16, 64), (260, 4096, np.float32, 3)])
@@ -260,7 +273,7 @@ def test_a_long_tensor_passes_32_bits(gpu):
 
 
 # ---- the head -------------------------------------------------------------------------------------------------------
-def head_case(hip, orc, types, M, N, K, seed):
+def head_case(hip, orc, types, M, N, K, seed, logits=True):
     """x, weights and logits in 64 bits with the bound of their error."""
     rng = np.random.default_rng(seed)
     w = (rng.standard_normal((N, K)) * 0.05).astype(np.float16)
@@ -285,12 +298,12 @@ def head_case(hip, orc, types, M, N, K, seed):
     else:
         x16 = x.astype(np.float16)
         xd, dx = x16.astype(np.float64), dev(x16)
-    z = xd @ wd.T
+    z = xd @ wd.T if logits else np.broadcast_to(0.0, (M, N))
     if types == "i8":
-        off = 3 * STEP * np.abs(z).max()              # the whole number's conversion and two products
+        off = 3 * STEP * (np.abs(xd).max(axis=0) @ np.abs(wd).T).max()  # the whole number's conversion and two products
     else:                                             # exact products, summed eight at a time
-        off = (K / 8 + 8) * STEP * (np.abs(xd) @ np.abs(wd).T).max()
-    return dict(fmt=fmt, x=dx, packed=packed, scale=scale, x_scale=x_scale, z=z, off=off)
+        off = (K / 8 + 8) * STEP * (np.abs(xd).max(axis=0) @ np.abs(wd).T).max()
+    return dict(xd=xd, wd=wd, fmt=fmt, x=dx, packed=packed, scale=scale, x_scale=x_scale, z=z, off=off)
 
 
 def run_head(hip, c, tokens, top, stream=None, workspace=None):
@@ -359,6 +372,69 @@ def test_head_tokens_that_are_none_and_rows_that_are_not_finite(gpu, orc, types,
     keep = [r for r in range(M) if r != 2]
     c["z"] = c["z"][keep]
     check_head({k: v[keep] for k, v in got.items()}, c, tokens[keep], 2)
+
+
+def crafted_head(hip, M, N, K, codes_of_column, top):
+    """int8 x and weights whose logits are whole numbers: every code of column c is codes_of_column[c], x is 1."""
+    src = hip.DeviceArray.from_numpy(np.repeat(codes_of_column.astype(np.int8)[:, None], K, axis=1))
+    packed = hip.DeviceArray((N * K,), np.uint8)
+    hip.pack_weights(hip.FMT_W8, N, K, src, packed)
+    hip.device_sync()
+    z = np.broadcast_to(codes_of_column.astype(np.float64) * K, (M, N))
+    return dict(fmt=hip.FMT_W8, x=hip.DeviceArray.from_numpy(np.ones((M, K), np.int8)), packed=packed,
+                scale=hip.DeviceArray.from_numpy(np.ones(N, np.float16)), x_scale=hip.DeviceArray.from_numpy(np.ones(M, np.float32)), z=z, off=0.0)
+
+
+def poisoned_workspace(hip, c, M, N, K, top):
+    """What a call has not written itself looks like the best logits."""
+    need = hip.linear_logprobs_workspace(c["fmt"], M, N, K, top, x_int8=True)
+    ws = hip.DeviceArray((need,), np.uint8)
+    piece = np.full(1 << 22, 1e30, np.float32)
+    for at in range(0, need, piece.nbytes):
+        n = min(piece.nbytes, need - at)
+        ws.view(at, (n,)).upload(piece.view(np.uint8)[:n])
+    return ws
+
+
+@pytest.mark.parametrize("top", [1, 5, 30, 64])
+@pytest.mark.parametrize("kind", ["one group", "first only", "last only", "equal"])
+def test_head_of_many_rows_finds_alternatives_wherever_they_lie(gpu, top, kind):
+    """Calls of many tiles write the logits of the strips that reach a bound only.  The best entries in strips that one group of threads looks
+    after, all among the columns that give the bound, none among them, or no entry better than another."""
+    hip = gpu
+    M, N, K = 2048, 65536, 256
+    rng = np.random.default_rng(3)
+    codes = rng.integers(-3, 4, N)
+    if kind == "one group":
+        for i, block in enumerate((0, 64, 128, 192)):
+            codes[block * 256:block * 256 + 256:64] = 40 + 4 * i + np.arange(4)
+    elif kind == "first only":
+        codes[(np.arange(N) // 256) % 8 == 0] += 20
+    elif kind == "last only":
+        codes[(np.arange(N) // 256) % 8 != 0] += 20
+    else:
+        codes[:] = 2
+    c = crafted_head(hip, M, N, K, codes, top)
+    got = run_head(hip, c, np.full(M, 777), top, workspace=poisoned_workspace(hip, c, M, N, K, top))
+    want = np.lexsort((np.arange(N), -codes))[:top]
+    assert np.array_equal(got["ids"], np.tile(want.astype(np.int32), (M, 1)))
+    ref = ref_logprobs(c["z"][:1], [777], top)
+    for name, value in (("logprob", "logprob"), ("entropy", "entropy"), ("tops", "tops")):
+        assert np.all(got[name] == got[name][0])
+    check_logprobs({n: got[n][:1] for n in ("logprob", "entropy", "tops")}, ref, N, slack=3 * STEP * np.abs(c["z"][0]).max())
+
+
+@pytest.mark.parametrize("types,M,top", [("i8", 2049, 5), ("f16", 1700, 2), ("w8", 2048, 20)])
+def test_head_of_many_rows_matches_the_formula(gpu, orc, types, M, top):
+    """Two launches of tiles with a bound between them (and a second block of rows), some rows checked."""
+    hip = gpu
+    N, K = 65536, 256
+    c = head_case(hip, orc, types, M, N, K, seed=12, logits=False)
+    tokens = np.random.default_rng(M).integers(0, N, M)
+    got = run_head(hip, c, tokens, top)
+    rows = np.unique(np.r_[0, 1, 127, 128, 255, 256, 1023, M - 2, M - 1])
+    c["z"] = c["xd"][rows] @ c["wd"].T
+    check_head({k: v[rows] for k, v in got.items()}, c, tokens[rows], top)
 
 
 def test_head_equal_logits_go_by_index(gpu, orc):
