@@ -494,3 +494,165 @@ def test_norm_codes_feed_the_head(gpu, orc):
     z = y @ (codes.astype(np.float64) * sc.astype(np.float64)[:, None]).T
     spread = np.sqrt(((codes.astype(np.float64) * sc.astype(np.float64)[:, None]) ** 2).sum(axis=1)).max() * xs.max() / np.sqrt(12)
     assert np.abs(c["z"] - z).max() <= 6 * spread
+
+
+# ---- streams and graphs ---------------------------------------------------------------------------------------------
+class Stream:
+    def __init__(self, hip):
+        import ctypes
+        self.hip, self.lib = hip, hip.load()
+        p = ctypes.c_void_p(0)
+        hip.check(self.lib.rwkv_hip_stream_create(ctypes.byref(p)))
+        self.ptr = p.value
+
+    def sync(self):
+        import ctypes
+        self.hip.check(self.lib.rwkv_hip_stream_sync(ctypes.c_void_p(self.ptr)))
+
+    def close(self):
+        import ctypes
+        self.hip.check(self.lib.rwkv_hip_stream_destroy(ctypes.c_void_p(self.ptr)))
+
+
+def scoring_chain(hip, orc, types, M, N, K, top, seed):
+    """Buffers of a norm, a head over its codes (or fp16 rows) and the log probabilities of some logits; launch(stream) enqueues all three."""
+    rng = np.random.default_rng(seed)
+    c = head_case(hip, orc, types, M, N, K, seed=seed)
+    new = lambda shape, t: hip.DeviceArray.zeros(shape, t)  # noqa: E731
+    x = hip.DeviceArray.from_numpy(rng.standard_normal((M, K)).astype(np.float16))
+    res = hip.DeviceArray.from_numpy(rng.standard_normal((M, K)).astype(np.float16))
+    w = hip.DeviceArray.from_numpy((1 + 0.1 * rng.standard_normal(K)).astype(np.float16))
+    z = hip.DeviceArray.from_numpy(rng.standard_normal((M, N)).astype(np.float32))
+    tokens = hip.DeviceArray.from_numpy(rng.integers(0, N, M).astype(np.int32))
+    out = dict(x_out=new((M, K), np.float16), q=new((M, K), np.int8), qs=new((M,), np.float32), hl=new((M,), np.float32), he=new((M,), np.float32),
+               hi=new((M, top), np.int32), ht=new((M, top), np.float32), ll=new((M,), np.float32), le=new((M,), np.float32),
+               lr=new((M,), np.int32), li=new((M, top), np.int32), lt=new((M, top), np.float32))
+    int8 = types == "i8"
+    ws = hip.DeviceArray((hip.linear_logprobs_workspace(c["fmt"], M, N, K, top, x_int8=int8),), np.uint8)
+    ws2 = hip.DeviceArray((max(16, hip.token_logprobs_workspace(M, N, top)),), np.uint8)
+
+    def launch(stream):
+        hip.add_norm_q8(M, K, x, res, w, None, out["q"], out["qs"], x_out=out["x_out"], norm=hip.NORM_RMS, stream=stream)
+        hip.linear_logprobs(c["fmt"], M, N, K, out["q"] if int8 else out["x_out"], c["packed"], c["scale"], tokens, ws,
+                            x_scale=out["qs"] if int8 else None, logprob=out["hl"], entropy=out["he"], top_n=top, top_ids=out["hi"] if top else None,
+                            top_logprobs=out["ht"] if top else None, stream=stream)
+        hip.token_logprobs(M, N, z, tokens, ws2, out["ll"], out["le"], out["lr"], top, out["li"] if top else None, out["lt"] if top else None,
+                           stream=stream)
+
+    return launch, out, (x, res, z, tokens, c)
+
+
+def bits(out):
+    return {n: v.numpy().view(np.uint8).copy() for n, v in out.items()}
+
+
+@pytest.mark.parametrize("types,M,N,K,top", [("i8", 3, 4096, 768, 5), ("f16", 200, 2048, 512, 3), ("i8", 300, 4096, 256, 0), ("i8", 1600, 65536, 256, 2)])
+def test_a_captured_call_replays(gpu, orc, types, M, N, K, top):
+    import ctypes
+    hip = gpu
+    launch, out, (x, res, z, tokens, keep) = scoring_chain(hip, orc, types, M, N, K, top, seed=31)
+    s = Stream(hip)
+    lib = s.lib                              # (the runtime that the library loads)
+    graph, run = ctypes.c_void_p(0), ctypes.c_void_p(0)
+    assert lib.hipStreamBeginCapture(ctypes.c_void_p(s.ptr), ctypes.c_int(1)) == 0
+    launch(s.ptr)
+    assert lib.hipStreamEndCapture(ctypes.c_void_p(s.ptr), ctypes.byref(graph)) == 0
+    assert lib.hipGraphInstantiate(ctypes.byref(run), graph, None, None, ctypes.c_size_t(0)) == 0
+    rng = np.random.default_rng(1)
+    for _ in range(3):
+        x.upload(rng.standard_normal((M, K)).astype(np.float16))
+        z.upload(rng.standard_normal((M, N)).astype(np.float32))
+        tokens.upload(rng.integers(0, N, M).astype(np.int32))
+        launch(None)
+        hip.device_sync()
+        want = bits(out)
+        for v in out.values():
+            v.fill0()
+        hip.device_sync()
+        assert lib.hipGraphLaunch(run, ctypes.c_void_p(s.ptr)) == 0
+        s.sync()
+        got = bits(out)
+        for name in want:
+            assert np.array_equal(got[name], want[name]), name
+    assert lib.hipGraphExecDestroy(run) == 0 and lib.hipGraphDestroy(graph) == 0
+    s.close()
+
+
+def test_calls_on_two_streams_at_once(gpu, orc):
+    hip = gpu
+    a, out_a, keep_a = scoring_chain(hip, orc, "i8", 40, 8192, 512, 4, seed=51)
+    b, out_b, keep_b = scoring_chain(hip, orc, "f16", 9, 16384, 256, 6, seed=52)
+    a(None)
+    b(None)
+    hip.device_sync()
+    want_a, want_b = bits(out_a), bits(out_b)
+    for v in list(out_a.values()) + list(out_b.values()):
+        v.fill0()
+    hip.device_sync()
+    s, t = Stream(hip), Stream(hip)
+    for _ in range(20):
+        a(s.ptr)
+        b(t.ptr)
+    s.sync()
+    t.sync()
+    for out, want in ((out_a, want_a), (out_b, want_b)):
+        got = bits(out)
+        for name in want:
+            assert np.array_equal(got[name], want[name]), name
+    s.close()
+    t.close()
+
+
+def test_calls_of_two_threads(gpu, orc):
+    import threading
+    hip = gpu
+    chains = [scoring_chain(hip, orc, "i8", 5, 4096, 512, 3, seed=61 + i) for i in range(3)]
+    want = []
+    for launch, out, _keep in chains:
+        launch(None)
+        hip.device_sync()
+        want.append(bits(out))
+    streams = [Stream(hip) for _ in chains]
+    errors = []
+
+    def work(i):
+        try:
+            for _ in range(50):
+                chains[i][0](streams[i].ptr)
+                streams[i].sync()
+        except Exception as e:  # noqa: BLE001 - reported below
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for (launch, out, _keep), w in zip(chains, want):
+        got = bits(out)
+        for name in w:
+            assert np.array_equal(got[name], w[name]), name
+    for s in streams:
+        s.close()
+
+
+def test_outputs_that_are_not_asked_for(gpu):
+    """Every output alone gives what all together give."""
+    hip = gpu
+    rng = np.random.default_rng(5)
+    for rows, V in ((2, 65536), (500, 700)):
+        z = logits_of("plain", rng, rows, V, np.float32)
+        tokens = rng.integers(0, V, rows)
+        whole = run_logprobs(hip, z, tokens, 6)
+        d, dt = hip.DeviceArray.from_numpy(z), hip.DeviceArray.from_numpy(tokens.astype(np.int32))
+        ws = hip.DeviceArray((max(16, hip.token_logprobs_workspace(rows, V, 6)),), np.uint8)
+        for name, kind in (("logprob", np.float32), ("entropy", np.float32), ("rank", np.int32)):
+            one = hip.DeviceArray.zeros((rows,), kind)
+            hip.token_logprobs(rows, V, d, None if name == "entropy" else dt, ws, **{name: one})
+            hip.device_sync()
+            assert np.array_equal(one.numpy().view(np.uint32), whole[name].view(np.uint32)), name
+        ids, tops = hip.DeviceArray.zeros((rows, 6), np.int32), hip.DeviceArray.zeros((rows, 6), np.float32)
+        hip.token_logprobs(rows, V, d, None, ws, top_n=6, top_ids=ids, top_logprobs=tops)
+        hip.device_sync()
+        assert np.array_equal(ids.numpy(), whole["ids"]) and np.array_equal(tops.numpy(), whole["tops"])
