@@ -141,12 +141,7 @@ __global__ __launch_bounds__(kFewThreads) void head_few_kernel(HeadArgs g, int l
 #pragma unroll
     for (int v = 0; v < 16; ++v) a.m = fmaxf(a.m, z[v]);
 #pragma unroll
-    for (int v = 0; v < 16; ++v) {
-      const float d = z[v] - a.m;
-      const float p = __builtin_amdgcn_exp2f(d * kLog2e);
-      a.s += p;
-      a.u = fmaf(fmaxf(d, kGone), p, a.u);
-    }
+    for (int v = 0; v < 16; ++v) a.add(z[v]);
     total.merge(a);
     if (j < g.M) {
       const int t = token - band * 32 - 4 * h;
@@ -167,17 +162,14 @@ __global__ __launch_bounds__(kFewThreads) void head_few_kernel(HeadArgs g, int l
   total.merge_lanes<32>();
   __syncthreads();
   float4_t* merge = reinterpret_cast<float4_t*>(x_lds);  // [kWaves][kFewRows]
-  if (h == 0 && j < g.M) merge[wave * kFewRows + j] = float4_t{total.m, total.s, total.u, 0.0f};
+  if (h == 0 && j < g.M) merge[wave * kFewRows + j] = total.stored();
   __syncthreads();
   const int r = threadIdx.x;
   if (r < g.M) {
     SoftSum a;
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-      const float4_t o = merge[i * kFewRows + r];
-      a.merge(SoftSum{o[0], o[1], o[2]});
-    }
-    g.sums[static_cast<int64_t>(r) * g.parts + blockIdx.x] = float4_t{a.m, a.s, a.u, 0.0f};
+    for (int i = 0; i < kWaves; ++i) a.merge(SoftSum(merge[i * kFewRows + r]));
+    g.sums[static_cast<int64_t>(r) * g.parts + blockIdx.x] = a.stored();
   }
 }
 
@@ -262,8 +254,12 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void head_tile_kernel(HeadArgs 
       a.m *= xs;
       a.u *= xs;
     }
+    if (a.s >= 1.0f) {  // (the largest's own 1)
+      a.s -= 1.0f;
+      a.n = 1.0f;
+    }
     a.merge_lanes<32>();
-    if (h == 0) merge[wn * W::BM + r] = float4_t{a.m, a.s, a.u, 0.0f};
+    if (h == 0) merge[wn * W::BM + r] = a.stored();
     if constexpr (LOGITS) {
       if (live && !(g.bound && a.m < g.bound[row])) {
 #pragma unroll
@@ -291,10 +287,10 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void head_tile_kernel(HeadArgs 
     for (int i = 0; i < 4; ++i) {
       const float4_t o = merge[i * W::BM + r];
       most[i] = o[0];
-      a.merge(SoftSum{o[0], o[1], o[2]});
+      a.merge(SoftSum(o));
     }
     const int64_t at = static_cast<int64_t>(m0 + r) * g.parts + col_block;
-    g.sums[at] = float4_t{a.m, a.s, a.u, 0.0f};
+    g.sums[at] = a.stored();
     if constexpr (LOGITS) *reinterpret_cast<float4_t*>(g.strips + at * 4) = most;
   }
 }
@@ -321,6 +317,8 @@ __global__ __launch_bounds__(256) void head_sums_kernel(HeadArgs g, TokenLogprob
   const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= g.M) return;
   const float4_t* sums = g.sums + static_cast<int64_t>(row) * g.parts;
+  const int token = g.tokens ? g.tokens[row] : -1;
+  const float token_logit = g.token_logit[row];  // (not written where there is no token)
   SoftSum a;
   for (int i = threadIdx.x & 63; i < g.parts; i += 4 * 64) {
     float4_t p[4];  // requested together
@@ -328,10 +326,10 @@ __global__ __launch_bounds__(256) void head_sums_kernel(HeadArgs g, TokenLogprob
     for (int q = 0; q < 4; ++q) p[q] = sums[min(i + q * 64, g.parts - 1)];
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-      if (i + q * 64 < g.parts) a.merge(SoftSum{p[q][0], p[q][1], p[q][2]});
+      if (i + q * 64 < g.parts) a.merge(SoftSum(p[q]));
   }
   a.merge_wave();
-  if ((threadIdx.x & 63) == 0) write_logprobs(a, out, row, g.N, g.token_logit + row);
+  if ((threadIdx.x & 63) == 0) write_logprobs(a, out, row, g.N, token, token_logit);
 }
 
 // The same with the alternatives, a block per row: they lie in the strips whose largest reaches the top_n-th largest of 64 or 256 groups
@@ -348,13 +346,14 @@ __global__ __launch_bounds__(256) void head_alternatives_kernel(HeadArgs g, Toke
   const float* strips = width == 64 ? g.strips + static_cast<int64_t>(row) * n_strips : reinterpret_cast<const float*>(sums);
   const int apart = width == 64 ? 1 : 4;
   const float* logits = g.logits + static_cast<int64_t>(row) * g.N;
+  const int token = g.tokens ? g.tokens[row] : -1;
+  const float token_logit = g.token_logit[row];  // (not written where there is no token)
   SoftSum a;
   for (int i = tid; i < g.parts; i += 256) {
-    const float4_t p = sums[i];
-    a.merge(SoftSum{p[0], p[1], p[2]});
+    a.merge(SoftSum(sums[i]));
   }
   a.merge_wave();
-  if ((tid & 63) == 0) waves[tid >> 6] = float4_t{a.m, a.s, a.u, 0.0f};
+  if ((tid & 63) == 0) waves[tid >> 6] = a.stored();
   if (tid == 0) {
     cand.n = 0;
     n_chosen = 0;
@@ -363,12 +362,9 @@ __global__ __launch_bounds__(256) void head_alternatives_kernel(HeadArgs g, Toke
   for (int i = tid; i < n_strips; i += 256) most = fmaxf(most, strips[i * apart]);
   // (not below the bound that the tiles went by: what lies below that has not been written)
   const float bound = fmaxf(first_bound(cand, top_n, most), g.bound ? g.bound[row] : -INFINITY);
-  a = SoftSum{};
+  a = SoftSum();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float4_t w = waves[i];
-    a.merge(SoftSum{w[0], w[1], w[2]});
-  }
+  for (int i = 0; i < 4; ++i) a.merge(SoftSum(waves[i]));
   key_t least = bound == -INFINITY ? 0 : key_of(bound, 0x7fffffff);  // what a candidate has to be ahead of
   int list = 0;
   const int at_once = width < 256 ? width : 256;  // columns of a strip
@@ -415,11 +411,11 @@ __global__ __launch_bounds__(256) void head_alternatives_kernel(HeadArgs g, Toke
     __syncthreads();
   }
   const int n = cand.n;
-  const float log_s = logf(a.s);
+  const float log_s = a.log_sum();
   thin_out(cand, list, n, top_n);
   __syncthreads();
   if (tid < top_n) write_alternative(out, row, tid, tid < n ? cand.list[list ^ 1][tid] : 0, a.m, log_s);
-  if (tid == 0) write_logprobs(a, out, row, g.N, g.token_logit + row);
+  if (tid == 0) write_logprobs(a, out, row, g.N, token, token_logit);
 }
 
 // ---- what a call takes ------------------------------------------------------------------------------------------------

@@ -25,7 +25,9 @@ struct LogprobArgs {
   TokenLogprobs out;
   // rows in several parts: what each leaves
   int parts, part_len;
-  float4_t* sums;  // [rows][parts]: m, S, U and the entries ahead of the token
+  float4_t* sums;  // [rows][parts]
+  int* ahead;      // [rows][parts]: entries ahead of the token
+  float* token_logit;  // [rows]
   key_t* keys;     // [rows][parts][top_n] in order, 0 past the last
 };
 
@@ -35,7 +37,7 @@ __device__ __forceinline__ float next_above(float v) {  // the smallest float ab
 }
 
 // One block per row, or per part of one, which it reads once: 64 bytes per thread at a time, the next 64 requested before they are
-// looked at.  A thread keeps m, S and U of its entries and raises m when a batch exceeds it.  The rank is a count against the token's
+// looked at.  A thread keeps the sums of its entries against the largest that its wavefront has seen, which few batches raise.  The rank is a count against the token's
 // logit, which is read first.  Alternatives: what is not below the bound that the first batch gives goes to a list in LDS, which is
 // thinned out to the first top_n - with the last one as the new bound - whenever it has grown to four times as many.  A list that
 // overflows (a row that rises, or is of one value) is given up: the alternatives are then found one after the other in top_n walks.
@@ -47,6 +49,7 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobArgs a)
   typedef T vec_t __attribute__((ext_vector_type(VE)));
   __shared__ __align__(16) Candidates<NT> cand;
   __shared__ float4_t waves[NT / 64];
+  __shared__ int waves_ahead[NT / 64];
   const int tid = threadIdx.x;
   const int top_n = a.out.top_n;
   const T* row = static_cast<const T*>(a.logits) + blockIdx.x * a.ld;
@@ -137,48 +140,52 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobArgs a)
         for (int e = 0; e < VE; ++e) ahead += x[q * VE + e] >= least;
       }
     }
-    if (most > sum.m) sum.raise(most);
+    if (__any(most >= sum.m)) {  // (m is the wavefront's: one decision, and few batches come here)
+      sum.raise(fmaxf(sum.m, wave_reduce_dpp(most, [](float v, float w) { return fmaxf(v, w); })));
 #pragma unroll
-    for (int e = 0; e < VB * VE; ++e) {
-      const float d = x[e] - sum.m;
-      const float p = __builtin_amdgcn_exp2f(d * kLog2e);
-      sum.s += p;
-      sum.u = fmaf(fmaxf(d, kGone), p, sum.u);
+      for (int e = 0; e < VB * VE; ++e) sum.add(x[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VB * VE; ++e) sum.add_smaller(x[e]);
     }
   }
-  {
-    if (stray_z > sum.m) sum.raise(stray_z);
-    const float d = stray_z - sum.m;
-    const float p = __builtin_amdgcn_exp2f(d * kLog2e);
-    sum.s += p;
-    sum.u = fmaf(fmaxf(d, kGone), p, sum.u);
+  if (head > 0 || tail < V) {
+    const float to = wave_reduce_dpp(stray_z, [](float v, float w) { return fmaxf(v, w); });
+    sum.raise(fmaxf(sum.m, to));
+    sum.add(stray_z);
     if (count) ahead += stray < V && (stray_z > zt || (stray_z == zt && stray < t));
-    // equal entries of the token's own vector in front of it
-    if (count && tid == 0 && t >= head && t < tail)
-      for (int i = t - (t - head) % VE; i < t; ++i) ahead += static_cast<float>(z[i]) == zt;
   }
+  // equal entries of the token's own vector in front of it
+  if (count && tid == 0 && t >= head && t < tail)
+    for (int i = t - (t - head) % VE; i < t; ++i) ahead += static_cast<float>(z[i]) == zt;
 
   // the block's sums
   sum.merge_wave();
   ahead = wave_reduce_dpp(ahead, [](int x, int y) { return x + y; });
-  if ((tid & 63) == 0) waves[tid >> 6] = float4_t{sum.m, sum.s, sum.u, as_float(ahead)};
+  if ((tid & 63) == 0) {
+    waves[tid >> 6] = sum.stored();
+    waves_ahead[tid >> 6] = ahead;
+  }
   __syncthreads();
-  sum = SoftSum{};
+  sum = SoftSum();
   ahead = 0;
 #pragma unroll
   for (int i = 0; i < NT / 64; ++i) {
-    const float4_t w = waves[i];
-    sum.merge(SoftSum{w[0], w[1], w[2]});
-    ahead += as_int(w[3]);
+    sum.merge(SoftSum(waves[i]));
+    ahead += waves_ahead[i];
   }
   const int64_t at = static_cast<int64_t>(blockIdx.x) * a.parts + blockIdx.y;
   float log_s = 0.0f;
   if constexpr (PART) {
-    if (tid == 0) a.sums[at] = float4_t{sum.m, sum.s, sum.u, as_float(ahead)};
-  } else if (tid < 64) {
-    log_s = logf(sum.s);
     if (tid == 0) {
-      write_logprobs(sum, a.out, blockIdx.x, V, &zt);
+      a.sums[at] = sum.stored();
+      a.ahead[at] = ahead;
+      if (blockIdx.y == 0) a.token_logit[blockIdx.x] = zt;
+    }
+  } else if (tid < 64) {
+    log_s = sum.log_sum();
+    if (tid == 0) {
+      write_logprobs(sum, a.out, blockIdx.x, V, token, zt);
       if (a.out.rank) a.out.rank[blockIdx.x] = !has_token || zt != zt ? -1 : ahead;
     }
   }
@@ -222,58 +229,58 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobArgs a)
 // A block per row over what its parts have left.  Of many keys a bound is made first, as of the entries of a row: at most top_n groups of
 // four threads, or of one, reach it, with as many keys each as a thread holds.
 constexpr int kMaxParts = 256;
-__global__ __launch_bounds__(kThreads) void token_logprobs_join_kernel(LogprobArgs a, int io) {
+__global__ __launch_bounds__(kThreads) void token_logprobs_join_kernel(LogprobArgs a) {
   __shared__ __align__(16) Candidates<kThreads> cand;
   __shared__ float4_t waves[kThreads / 64];
+  __shared__ int waves_ahead[kThreads / 64];
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x;
   const int top_n = a.out.top_n;
+  const int total = a.parts * top_n;
+  const key_t* keys = a.keys + row * total;
+  // everything that most calls need, requested at once
+  const key_t own = tid < total ? keys[tid] : 0;
+  const int token = a.out.tokens ? a.out.tokens[row] : -1;
+  const float zt = a.token_logit[row];
   SoftSum sum;
   int ahead = 0;
   if (tid < a.parts) {
-    const float4_t p = a.sums[row * a.parts + tid];
-    sum = SoftSum{p[0], p[1], p[2]};
-    ahead = as_int(p[3]);
+    sum = SoftSum(a.sums[row * a.parts + tid]);
+    ahead = a.ahead[row * a.parts + tid];
   }
   sum.merge_wave();
   ahead = wave_reduce_dpp(ahead, [](int x, int y) { return x + y; });
-  if ((tid & 63) == 0) waves[tid >> 6] = float4_t{sum.m, sum.s, sum.u, as_float(ahead)};
+  if ((tid & 63) == 0) {
+    waves[tid >> 6] = sum.stored();
+    waves_ahead[tid >> 6] = ahead;
+  }
   if (tid == 0) cand.n = 0;
   __syncthreads();
-  sum = SoftSum{};
+  sum = SoftSum();
   ahead = 0;
 #pragma unroll
   for (int i = 0; i < kThreads / 64; ++i) {
-    const float4_t w = waves[i];
-    sum.merge(SoftSum{w[0], w[1], w[2]});
-    ahead += as_int(w[3]);
-  }
-  const int token = a.out.tokens ? a.out.tokens[row] : -1;
-  const bool has_token = token >= 0 && token < a.V;
-  float zt = 0.0f;
-  if (has_token) {
-    const int64_t at = row * a.ld + token;
-    zt = io == RWKV_IO_F16 ? h2f(static_cast<const half_t*>(a.logits)[at]) : static_cast<const float*>(a.logits)[at];
+    sum.merge(SoftSum(waves[i]));
+    ahead += waves_ahead[i];
   }
   if (tid == 0) {
-    write_logprobs(sum, a.out, row, a.V, &zt);
-    if (a.out.rank) a.out.rank[row] = !has_token || zt != zt ? -1 : ahead;
+    write_logprobs(sum, a.out, row, a.V, token, zt);
+    if (a.out.rank) a.out.rank[row] = token < 0 || token >= a.V || zt != zt ? -1 : ahead;
   }
   if (top_n == 0) return;
-  const int total = a.parts * top_n;
-  const key_t* keys = a.keys + row * total;
   float bound = -INFINITY;
   if (total > 32) {
-    float most = -INFINITY;
-    for (int k = tid; k < total; k += kThreads)
+    float most = own ? key_value(own) : -INFINITY;
+    for (int k = tid + kThreads; k < total; k += kThreads)
       if (keys[k]) most = fmaxf(most, key_value(keys[k]));
     bound = first_bound(cand, top_n, most);
   }
-  for (int k = tid; k < total; k += kThreads)
+  if (own && key_value(own) >= bound) offer(cand, 0, own);
+  for (int k = tid + kThreads; k < total; k += kThreads)
     if (keys[k] && key_value(keys[k]) >= bound) offer(cand, 0, keys[k]);
   __syncthreads();
   const int n = cand.n;
-  const float log_s = logf(sum.s);
+  const float log_s = sum.log_sum();
   if (n <= kCandidates) {
     thin_out(cand, 0, n, top_n);
     __syncthreads();
@@ -307,15 +314,23 @@ int parts_of(int rows, int V, int io) {
   const int parts = std::min({4 * device_cu_count() / rows, ceil_div(V, batch), kMaxParts});
   return parts < 3 ? 1 : parts;
 }
-size_t sums_bytes(int rows, int parts) { return static_cast<size_t>(rows) * parts * sizeof(float4_t); }
+struct PartBytes {  // of the workspace, in this order
+  size_t sums, ahead, token_logit, keys;
+  size_t all() const { return sums + ahead + token_logit + keys; }
+};
+PartBytes part_bytes(int rows, int parts, int top_n) {
+  const auto align = [](size_t n) { return (n + 15) / 16 * 16; };
+  const size_t all = static_cast<size_t>(rows) * parts;
+  return {all * sizeof(float4_t), align(all * sizeof(int)), align(rows * sizeof(float)), all * top_n * sizeof(key_t)};
+}
 
 template <typename T>
-void launch_rows(hipStream_t st, int rows, int io, const LogprobArgs& a) {
+void launch_rows(hipStream_t st, int rows, const LogprobArgs& a) {
   if (a.parts == 1) {
     hipLaunchKernelGGL((token_logprobs_kernel<T, false>), dim3(rows), dim3(kThreads), 0, st, a);
   } else {
     hipLaunchKernelGGL((token_logprobs_kernel<T, true>), dim3(rows, a.parts), dim3(kThreads), 0, st, a);
-    hipLaunchKernelGGL(token_logprobs_join_kernel, dim3(rows), dim3(kThreads), 0, st, a, io);
+    hipLaunchKernelGGL(token_logprobs_join_kernel, dim3(rows), dim3(kThreads), 0, st, a);
   }
 }
 
@@ -323,17 +338,20 @@ void launch_rows(hipStream_t st, int rows, int io, const LogprobArgs& a) {
 
 size_t token_logprobs_workspace_bytes(int rows, int V, int top_n) {
   const int parts = parts_of(rows, V, RWKV_IO_F32);  // (fp16 rows go in no more)
-  return parts == 1 ? 0 : sums_bytes(rows, parts) + static_cast<size_t>(rows) * parts * top_n * sizeof(key_t);
+  return parts == 1 ? 0 : part_bytes(rows, parts, top_n).all();
 }
 
 int token_logprobs_launch(hipStream_t st, int rows, int V, int io, const void* logits, int64_t ld, const TokenLogprobs& out, void* workspace) {
   const int parts = parts_of(rows, V, io);
   // (a multiple of a vector, so that the parts of an aligned row are aligned)
-  LogprobArgs a = {logits, ld, V, out, parts, ceil_div(ceil_div(V, parts), 64) * 64, static_cast<float4_t*>(workspace),
-                   reinterpret_cast<key_t*>(static_cast<char*>(workspace) + sums_bytes(rows, parts))};
+  const PartBytes p = part_bytes(rows, parts, out.top_n);
+  char* ws = static_cast<char*>(workspace);
+  LogprobArgs a = {logits, ld, V, out, parts, ceil_div(ceil_div(V, parts), 64) * 64, reinterpret_cast<float4_t*>(ws),
+                   reinterpret_cast<int*>(ws + p.sums), reinterpret_cast<float*>(ws + p.sums + p.ahead),
+                   reinterpret_cast<key_t*>(ws + p.sums + p.ahead + p.token_logit)};
   a.parts = ceil_div(V, a.part_len);  // (rounding up may leave the last one without entries)
-  if (io == RWKV_IO_F16) launch_rows<half_t>(st, rows, io, a);
-  else launch_rows<float>(st, rows, io, a);
+  if (io == RWKV_IO_F16) launch_rows<half_t>(st, rows, a);
+  else launch_rows<float>(st, rows, a);
   RWKV_LAUNCH_CHECK();
   return RWKV_OK;
 }

@@ -18,16 +18,38 @@ __device__ __forceinline__ float lane_xor_f(float v) {
   return as_float(lane_xor_dpp<D>(as_int(v)));
 }
 
-// m = max z, S = sum e^(z - m), U = sum (z - m) e^(z - m) of the entries seen so far.  m starts at the lowest finite value, not at
-// -infinity: differences with it are no NaN, and S stays 0 as long as every entry is -infinity.  A NaN or +infinity among the entries
-// makes S a NaN that stays.
+// m = max z, S = sum e^(z - m), U = sum (z - m) e^(z - m) of the entries seen so far.  S is kept as n + s: n entries that are the
+// largest, a 1 each, and the others, so that the logarithm of a row that is nearly sure of one entry does not lose the others beside
+// the 1.  m starts at the lowest finite value, not at -infinity: differences with it are no NaN, and S stays 0 as long as every entry is
+// -infinity.  A NaN or +infinity among the entries makes s a NaN that stays.
 struct SoftSum {
-  float m = kLowest, s = 0.0f, u = 0.0f;
+  float m = kLowest, s = 0.0f, u = 0.0f, n = 0.0f;
+  __device__ __forceinline__ SoftSum() {}
+  __device__ __forceinline__ explicit SoftSum(const float4_t& v) : m(v[0]), s(v[1]), u(v[2]), n(v[3]) {}
+  __device__ __forceinline__ float4_t stored() const { return float4_t{m, s, u, n}; }
+  // an entry that is at most m
+  __device__ __forceinline__ void add(float z) {
+    const float d = z - m;
+    const float p = __builtin_amdgcn_exp2f(d * kLog2e);
+    s += d == 0.0f ? 0.0f : p;
+    n += d == 0.0f ? 1.0f : 0.0f;
+    u = fmaf(fmaxf(d, kGone), p, u);
+  }
+  // one that is less than m
+  __device__ __forceinline__ void add_smaller(float z) {
+    const float d = z - m;
+    const float p = __builtin_amdgcn_exp2f(d * kLog2e);
+    s += p;
+    u = fmaf(fmaxf(d, kGone), p, u);
+  }
+  // an m that is as large or larger
   __device__ __forceinline__ void raise(float to) {
+    const bool same = m == to;
     const float t = fmaxf(m - to, kGone);
     const float f = __builtin_amdgcn_exp2f(t * kLog2e);
-    u = f * fmaf(t, s, u);
-    s *= f;
+    u = f * fmaf(t, s + n, u);
+    s = same ? s : f * (s + n);
+    n = same ? n : 0.0f;
     m = to;
   }
   __device__ __forceinline__ void merge(SoftSum o) {
@@ -36,30 +58,40 @@ struct SoftSum {
     o.raise(to);
     s += o.s;
     u += o.u;
+    n += o.n;
   }
   // with what the lane of the other value of bit D has: both end with the same bits
   template <int D>
   __device__ __forceinline__ void merge_lanes() {
-    merge(SoftSum{lane_xor_f<D>(m), lane_xor_f<D>(s), lane_xor_f<D>(u)});
+    SoftSum o;
+    o.m = lane_xor_f<D>(m);
+    o.s = lane_xor_f<D>(s);
+    o.u = lane_xor_f<D>(u);
+    o.n = lane_xor_f<D>(n);
+    merge(o);
   }
   __device__ __forceinline__ void merge_wave() {  // the largest first: one exponential instead of twelve in a row
-    raise(wave_reduce_dpp(m, [](float x, float y) { return fmaxf(x, y); }));
+    const float to = wave_reduce_dpp(m, [](float x, float y) { return fmaxf(x, y); });
+    raise(to);
     s = wave_sum_dpp(s);
     u = wave_sum_dpp(u);
+    n = wave_sum_dpp(n);
+  }
+  __device__ __forceinline__ bool empty() const { return n + s == 0.0f; }
+  // ln(n + s); with n = 1 what the sum has lost of s is made good: ln(1 + s) = ln(w) s / (w - 1) for the rounded w = 1 + s
+  __device__ __forceinline__ float log_sum() const {
+    const float w = n + s;
+    const float l = logf(w);
+    return n != 1.0f ? l : w == 1.0f ? s : w < 2.0f ? l * (s / (w - 1.0f)) : l;
   }
 };
 
 // log probability and entropy of a row: ln S - U / S is a sum of two terms that are not negative, nothing cancels.  token_logit is
-// that of the row's token, read only where it is an entry.  Returns ln S.
-__device__ __forceinline__ float write_logprobs(const SoftSum& a, const TokenLogprobs& out, int64_t row, int V, const float* token_logit) {
-  const bool nothing = a.s == 0.0f;
-  const float log_s = logf(a.s);
-  if (out.logprob) {
-    const int t = out.tokens[row];
-    out.logprob[row] = t < 0 ? 0.0f : t >= V ? __builtin_nanf("") : nothing ? -INFINITY : *token_logit - a.m - log_s;
-  }
-  if (out.entropy) out.entropy[row] = nothing ? 0.0f : log_s - a.u / a.s;
-  return log_s;
+// that of the row's token, looked at only where it is an entry.
+__device__ __forceinline__ void write_logprobs(const SoftSum& a, const TokenLogprobs& out, int64_t row, int V, int token, float token_logit) {
+  const float log_s = a.log_sum();
+  if (out.logprob) out.logprob[row] = token < 0 ? 0.0f : token >= V ? __builtin_nanf("") : a.empty() ? -INFINITY : token_logit - a.m - log_s;
+  if (out.entropy) out.entropy[row] = a.empty() ? 0.0f : log_s - a.u / (a.n + a.s);
 }
 
 // The order "larger first, equal ones by index" as that of whole numbers: the value's bits made to rise with it above the index's

@@ -241,6 +241,26 @@ def test_logprobs_of_rows_anywhere(gpu, dtype, lead, extra, V, rows):
     check_logprobs(run_logprobs(gpu, z, tokens, 7, ld=V + extra, lead=lead), ref_logprobs(z, tokens, 7), V)
 
 
+@pytest.mark.parametrize("rows,V,dtype", [(3, 100, np.float32), (2, 65536, np.float32), (400, 5000, np.float32), (2, 50277, np.float16)])
+def test_rows_that_are_nearly_sure_keep_what_is_left(gpu, rows, V, dtype):
+    """Log probability and entropy near 0 are right relative to themselves: what remains beside the largest entry's 1 is not lost in it."""
+    rng = np.random.default_rng(37)
+    z = rng.standard_normal((rows, V)).astype(dtype)
+    at = rng.integers(0, V, rows)
+    z[np.arange(rows), at] = 30.0
+    got, ref = run_logprobs(gpu, z, at, 0), ref_logprobs(z, at, 0)
+    exact = z.astype(np.float64) - 30.0
+    exact[np.arange(rows), at] = -np.inf
+    rest = np.exp(exact).sum(axis=1)                  # beside the 1: some 1e-13 V
+    # 35 in the exponent, rounded three times, and the sum's chain; the entropy's terms carry d as a factor
+    tol = (3 * 36 + 4 + V / 256 + 64) * STEP
+    assert np.all(np.abs(got["logprob"] + np.log1p(rest)) <= tol * rest)
+    exact[np.arange(rows), at] = 0.0
+    entropy = np.log1p(rest) - (exact * np.exp(exact)).sum(axis=1) / (1 + rest)
+    assert np.all(np.abs(got["entropy"] - entropy) <= 2 * tol * entropy)
+    assert np.all(got["rank"] == ref["rank"])
+
+
 def test_a_row_does_not_depend_on_the_other_rows_and_calls_repeat(gpu):
     rng = np.random.default_rng(23)
     z = logits_of("plain", rng, 12, 65536, np.float32)
