@@ -3,6 +3,7 @@
 // scale per row and int8 weights (products in whole numbers, exact in 32 bits up to K = 133152: 127 * 127 K < 2^31).
 // Reference: the head product alone (src/rwkv7_fast_v4.cu:1325-1341).
 #include <algorithm>
+#include <utility>
 
 #include "gemm_tile.h"
 #include "softsum.h"
@@ -437,10 +438,17 @@ Plan plan_of(int fmt, bool x_int8, int M, int N, int K, int top_n) {
   Plan p = {};
   p.few = takes_few(M, K, x_int8 ? 1 : 2);
   p.rows = p.few ? M : std::min(M, top_n > 0 ? std::max(kLogits / N / 256, 1) * 256 : kSumRows);
-  // (us, 65536 x 4096 int8, 2048 rows: tiles of 128 rows 527, of 256 508, fp16 970 and 956, int8 weights under fp16 1033 and 890; 333 rows
-  // of 2048: 114 and 141, 116 and 141, 110 and 118 - a few rows of padding are worth more than the tile)
-  const int per_row = fmt == RWKV_FMT_W8 && !x_int8 ? 122 : 106;
-  p.tile = ceil_div(p.rows, 128) * 128 * per_row < ceil_div(p.rows, 256) * 256 * 100 ? 128 : 256;
+  // The tile whose rows, padding among them, cost least; a row of a lower tile costs more (us, 65536 columns, tiles of 128 / 192 / 256
+  // rows: 768 rows of 2048 fp16 226 / 233 / 220, int8 weights under them 210 / 187 / 182, of 4096 int8 224 / 230 / 216; 333 rows 111 / 118 /
+  // 136, 105 / 95 / 116, 113 / 120 / 137; 190 rows 77 / 67 / 75, 70 / 53 / 63, 80 / 68 / 78).
+  const bool w8 = fmt == RWKV_FMT_W8 && !x_int8;
+  int64_t least = INT64_MAX;
+  for (const auto& [rows, cost] : {std::pair<int, int>{256, 100}, {192, w8 ? 104 : 112}, {128, w8 ? 122 : 106}}) {
+    const int64_t all = static_cast<int64_t>(ceil_div(p.rows, rows)) * rows * cost;
+    if (all >= least) continue;
+    least = all;
+    p.tile = rows;
+  }
 
   p.parts = p.few ? ceil_div(N / 32, kFewThreads / 64 * few_bands(N)) : ceil_div(N, kTileCols);
   p.every = 1;
@@ -477,8 +485,10 @@ int launch_tiles(hipStream_t st, HeadArgs& g, int tile, int every, bool rest) {
   g.rest = rest;
   g.col_blocks = rest ? g.parts - ceil_div(g.parts, every) : ceil_div(g.parts, every);
   const dim3 grid(g.row_tiles * ceil_div(g.col_blocks, 8) * 8);
-  const auto kernel = tile == 256 ? (g.row_tiles == 1 ? head_tile_kernel<TYPES, 4, LOGITS, true> : head_tile_kernel<TYPES, 4, LOGITS, false>)
-                                  : (g.row_tiles == 1 ? head_tile_kernel<TYPES, 2, LOGITS, true> : head_tile_kernel<TYPES, 2, LOGITS, false>);
+  const bool one = g.row_tiles == 1;
+  const auto kernel = tile == 256 ? (one ? head_tile_kernel<TYPES, 4, LOGITS, true> : head_tile_kernel<TYPES, 4, LOGITS, false>)
+                    : tile == 192 ? (one ? head_tile_kernel<TYPES, 3, LOGITS, true> : head_tile_kernel<TYPES, 3, LOGITS, false>)
+                                  : (one ? head_tile_kernel<TYPES, 2, LOGITS, true> : head_tile_kernel<TYPES, 2, LOGITS, false>);
   hipLaunchKernelGGL(kernel, grid, dim3(64 * kTileWaves), 0, st, g);
   RWKV_LAUNCH_CHECK();
   return RWKV_OK;

@@ -28,8 +28,12 @@ struct LogprobArgs {
   float4_t* sums;  // [rows][parts]
   int* ahead;      // [rows][parts]: entries ahead of the token
   float* token_logit;  // [rows]
-  key_t* keys;     // [rows][parts][top_n] in order, 0 past the last
+  key_t* keys;     // [rows][parts][part_keys(top_n)] in any order, 0 past the last
 };
+
+// Candidates that a part hands on as they are, without sorting out its first top_n
+__host__ __device__ constexpr int part_keys(int top_n) { return top_n > 0 ? 2 * top_n + 8 : 0; }
+static_assert(part_keys(kMaxAlternatives) <= 256, "written by one thread each");
 
 __device__ __forceinline__ float next_above(float v) {  // the smallest float above v; NaN above +infinity
   const uint32_t b = __builtin_bit_cast(uint32_t, v);
@@ -191,12 +195,18 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobArgs a)
   }
   if (top_n == 0) return;
   static_assert(kMaxAlternatives <= 64, "one wavefront writes them");
+  const int slots = part_keys(top_n);
   auto write = [&](int place, key_t key) {
-    if constexpr (PART) a.keys[at * top_n + place] = key;
+    if constexpr (PART) a.keys[at * slots + place] = key;
     else write_alternative(a.out, blockIdx.x, place, key, sum.m, log_s);
   };
 
   const int n = cand.n;
+  if (PART && n <= slots) {
+    if (tid < slots) write(tid, tid < n ? cand.list[list][tid] : 0);
+    return;
+  }
+  if (PART && tid >= top_n && tid < slots) write(tid, 0);
   if (n <= kCandidates) {
     thin_out(cand, list, n, top_n);
     __syncthreads();
@@ -226,8 +236,7 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobArgs a)
   }
 }
 
-// A block per row over what its parts have left.  Of many keys a bound is made first, as of the entries of a row: at most top_n groups of
-// four threads, or of one, reach it, with as many keys each as a thread holds.
+// A block per row over what its parts have left.  Of many keys a bound is made first, as of the entries of a row.
 constexpr int kMaxParts = 256;
 __global__ __launch_bounds__(kThreads) void token_logprobs_join_kernel(LogprobArgs a) {
   __shared__ __align__(16) Candidates<kThreads> cand;
@@ -236,7 +245,7 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_join_kernel(LogprobAr
   const int tid = threadIdx.x;
   const int64_t row = blockIdx.x;
   const int top_n = a.out.top_n;
-  const int total = a.parts * top_n;
+  const int total = a.parts * part_keys(top_n);
   const key_t* keys = a.keys + row * total;
   // everything that most calls need, requested at once
   const key_t own = tid < total ? keys[tid] : 0;
@@ -321,7 +330,7 @@ struct PartBytes {  // of the workspace, in this order
 PartBytes part_bytes(int rows, int parts, int top_n) {
   const auto align = [](size_t n) { return (n + 15) / 16 * 16; };
   const size_t all = static_cast<size_t>(rows) * parts;
-  return {all * sizeof(float4_t), align(all * sizeof(int)), align(rows * sizeof(float)), all * top_n * sizeof(key_t)};
+  return {all * sizeof(float4_t), align(all * sizeof(int)), align(rows * sizeof(float)), all * part_keys(top_n) * sizeof(key_t)};
 }
 
 template <typename T>
