@@ -30,6 +30,7 @@ struct HeadArgs {
   const int* tokens;     // may be NULL
   float4_t* sums;        // [M][parts]: m, S, U of a part's columns (few rows: a block's, tiles: 256)
   float* token_logit;    // [M], written where the token is a column
+  int* firsts;           // one alternative from tiles: [M][parts], the first column of a part's largest logit; else NULL
   // alternatives only
   float* logits;         // [M,N], written where it may hold one
   float* strips;         // [M][4 parts]: largest of each 64 columns (tiles)
@@ -39,6 +40,9 @@ struct HeadArgs {
   int col_blocks, every;
   bool rest;
 };
+
+// of two places the one with the larger value, the lower of equal ones
+__device__ __forceinline__ int first_of(float m, int i, float o, int k) { return o > m ? k : o == m ? min(i, k) : i; }
 
 // ---- few rows: the weights are streamed once, which is what bounds it ------------------------------------------------
 // A wavefront takes whole bands of 32 columns, one after the other in memory, 8 KiB of them requested ahead of the 8 KiB that it
@@ -81,7 +85,7 @@ __global__ __launch_bounds__(kFewThreads) void head_few_kernel(HeadArgs g, int l
     w += kChunk * 64;
   };
   if (chunks > 0) request();
-  // x: 16-byte piece n of row r holds k = n * 16 / kXBytes ..; its place is [n / 2 (int8) or n / 4 and n % 2][h][row]
+  // x: 16-byte piece n of row r (int8: of k = 16 n, the lanes' h is n % 2; fp16: of k = 8 n, h is the second bit of n, i the first)
   {
     const int row_pieces = g.K * T::kXBytes / 16;
     const int R = 1 << log_rows;
@@ -179,7 +183,11 @@ __global__ __launch_bounds__(kFewThreads) void head_few_kernel(HeadArgs g, int l
 // ---- many rows: the tiles of the packed product -----------------------------------------------------------------------
 // A tile leaves m, S and U of its 256 columns for every row (16 bytes for 1 KiB of logits).  A lane has 32 columns of a row in
 // registers: they are reduced there, with the other half's 32 by a swap of rows, with the other three wavefronts' 64 each through LDS.
-// LOGITS: also the largest of each 64 columns, and the logits of those 64 where that is not below the row's bound.
+// LOGITS: also the largest of each 64 columns, and the logits of those 64 where that is not below the row's bound.  ONE: one tile of
+// rows, whose weights no other block reads.
+// What bounds it: the chip's power, as the packed product (matrix core busy 51 % of the time at 1.95 GHz); the sums take about a tenth.
+// 2048 rows of 4096 int8, 65536 columns: 495 us, 2.2 P operations/s (a plain product of 8192 x 8192 x 8192 reaches 2.08 on this card); fp16
+// 955 us, 1.15 PFLOP/s.  Through blocks of 256 rows of logits in memory the int8 case with 5 alternatives took 798 us, so 550.
 template <int TYPES, int MT, bool LOGITS, bool ONE>
 __global__ __launch_bounds__(64 * kTileWaves, 2) void head_tile_kernel(HeadArgs g) {
   typedef Types<TYPES> T;
@@ -208,7 +216,8 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void head_tile_kernel(HeadArgs 
       sc[nb][q] = half4_t{1, 1, 1, 1};
       if (TYPES != kF16F16) sc[nb][q] = *reinterpret_cast<const half4_t*>(g.scale + min(col0 + nb * 32, g.N - 32) + 8 * q + 4 * h);
     }
-  float4_t* merge = reinterpret_cast<float4_t*>(lds);  // [4][BM]
+  float4_t* merge = reinterpret_cast<float4_t*>(lds);          // [4][BM]
+  int* merge_first = reinterpret_cast<int*>(merge + 4 * W::BM);  // [4][BM]
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     const int r = (wm * MT + mt) * 32 + j;
@@ -261,6 +270,18 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void head_tile_kernel(HeadArgs 
       a.s -= 1.0f;
       a.n = 1.0f;
     }
+    int first = g.N;
+    if (!LOGITS && g.firsts) {
+#pragma unroll
+      for (int nb = 1; nb >= 0; --nb)
+        if (col0 + nb * 32 < g.N) {
+#pragma unroll
+          for (int v = 15; v >= 0; --v)
+            if ((TYPES == kI8W8 ? mul_f32(z[nb][v], xs) : z[nb][v]) == a.m) first = col0 + 4 * h + nb * 32 + 8 * (v >> 2) + (v & 3);
+        }
+      first = first_of(a.m, first, lane_xor_f<32>(a.m), lane_xor_dpp<32>(first));
+      if (h == 0) merge_first[wn * W::BM + r] = first;
+    }
     a.merge_lanes<32>();
     if (h == 0) merge[wn * W::BM + r] = a.stored();
     if constexpr (LOGITS) {
@@ -286,15 +307,18 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void head_tile_kernel(HeadArgs 
   if (r < W::BM && m0 + r < g.M) {
     SoftSum a;
     float4_t most;
+    int first = g.N;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float4_t o = merge[i * W::BM + r];
       most[i] = o[0];
+      if (!LOGITS && g.firsts) first = first_of(a.m, first, o[0], merge_first[i * W::BM + r]);
       a.merge(SoftSum(o));
     }
     const int64_t at = static_cast<int64_t>(m0 + r) * g.parts + col_block;
     g.sums[at] = a.stored();
     if constexpr (LOGITS) *reinterpret_cast<float4_t*>(g.strips + at * 4) = most;
+    else if (g.firsts) g.firsts[at] = first;
   }
 }
 
@@ -315,27 +339,40 @@ __global__ __launch_bounds__(256) void head_bound_kernel(HeadArgs g, int top_n, 
   if (lane == 0) bound[row] = found;
 }
 
-// Log probability and entropy from the parts' sums: a wavefront per row.
+// Log probability and entropy from the parts' sums, and the one alternative that they name: a wavefront per row.
 __global__ __launch_bounds__(256) void head_sums_kernel(HeadArgs g, TokenLogprobs out) {
   const int row = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= g.M) return;
-  const float4_t* sums = g.sums + static_cast<int64_t>(row) * g.parts;
+  const int64_t at = static_cast<int64_t>(row) * g.parts;
   const int token = g.tokens ? g.tokens[row] : -1;
   const float token_logit = g.token_logit[row];  // (not written where there is no token)
   SoftSum a;
+  int first = g.N;
   for (int i = threadIdx.x & 63; i < g.parts; i += 4 * 64) {
     float4_t p[4];  // requested together
+    int f[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) p[q] = sums[min(i + q * 64, g.parts - 1)];
+    for (int q = 0; q < 4; ++q) {
+      const int k = min(i + q * 64, g.parts - 1);
+      p[q] = g.sums[at + k];
+      f[q] = g.firsts ? g.firsts[at + k] : g.N;
+    }
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-      if (i + q * 64 < g.parts) a.merge(SoftSum(p[q]));
+      if (i + q * 64 < g.parts) {
+        first = first_of(a.m, first, p[q][0], f[q]);
+        a.merge(SoftSum(p[q]));
+      }
   }
+  const float mine = a.m;
   a.merge_wave();
-  if ((threadIdx.x & 63) == 0) write_logprobs(a, out, row, g.N, token, token_logit);
+  first = wave_reduce_dpp(mine == a.m ? first : g.N, [](int x, int y) { return min(x, y); });
+  if ((threadIdx.x & 63) != 0) return;
+  write_logprobs(a, out, row, g.N, token, token_logit);
+  if (out.top_n == 1) write_alternative(out, row, 0, a.m > kLowest && first < g.N ? key_of(a.m, first) : 0, a.m, a.log_sum());
 }
 
-// The same with the alternatives, a block per row: they lie in the strips whose largest reaches the top_n-th largest of 64 or 256 groups
+// The same with the alternatives, a block per row (2048 rows with 5: 14 us): they lie in the strips whose largest reaches the top_n-th largest of 64 or 256 groups
 // of strips - few more than top_n of them - whose logits are there.  768 columns at a time; the list never overflows, it is thinned out
 // first.  Strips of `width` columns: 64 with their largest in `strips` (tiles), or a part's with it in `sums` (few rows).
 __global__ __launch_bounds__(256) void head_alternatives_kernel(HeadArgs g, TokenLogprobs out, int width) {
@@ -428,8 +465,9 @@ struct Plan {
   int tile;        // rows of a tile
   int parts;       // of a row, with sums of their own
   int every;       // > 1: a first launch takes every so many blocks of columns and bounds the alternatives of the others
-  size_t sums, token_logit, logits, strips, bound;  // bytes
-  size_t bytes() const { return sums + token_logit + logits + strips + bound; }
+  bool lists;      // alternatives out of strips of logits, not the one that the sums name
+  size_t sums, token_logit, firsts, logits, strips, bound;  // bytes, in this order
+  size_t bytes() const { return sums + token_logit + firsts + logits + strips + bound; }
 };
 
 constexpr int kSumRows = 8192;    // rows at a time without alternatives: 32 MiB of sums at 65536 columns
@@ -439,7 +477,8 @@ constexpr int kFewestTurns = 6;   // turns of blocks on the chip from which on t
 Plan plan_of(int fmt, bool x_int8, int M, int N, int K, int top_n) {
   Plan p = {};
   p.few = takes_few(M, K, x_int8 ? 1 : 2);
-  p.rows = p.few ? M : std::min(M, top_n > 0 ? std::max(kLogits / N / 256, 1) * 256 : kSumRows);
+  p.lists = top_n > 1 || (top_n == 1 && p.few);
+  p.rows = p.few ? M : std::min(M, p.lists ? std::max(kLogits / N / 256, 1) * 256 : kSumRows);
   // The tile whose rows, padding among them, cost least; a row of a lower tile costs more (us, 65536 columns, tiles of 128 / 192 / 256
   // rows: 768 rows of 2048 fp16 226 / 233 / 220, int8 weights under them 210 / 187 / 182, of 4096 int8 224 / 230 / 216; 333 rows 111 / 118 /
   // 136, 105 / 95 / 116, 113 / 120 / 137; 190 rows 77 / 67 / 75, 70 / 53 / 63, 80 / 68 / 78).
@@ -453,7 +492,7 @@ Plan plan_of(int fmt, bool x_int8, int M, int N, int K, int top_n) {
   }
   p.parts = p.few ? ceil_div(N / 32, kFewThreads / 64 * few_bands(N)) : ceil_div(N, kTileCols);
   p.every = 1;
-  if (!p.few && top_n > 0) {
+  if (!p.few && p.lists) {
     const int64_t blocks = static_cast<int64_t>(ceil_div(p.rows, p.tile)) * p.parts, cus = device_cu_count();
     // (as many strips as groups of them are wanted, and no more than the bound's launch holds)
     if (blocks >= kFewestTurns * cus) p.every = std::min<int64_t>(ceil_div(blocks, cus), 4 * p.parts / std::max(2 * top_n, 128));
@@ -462,8 +501,9 @@ Plan plan_of(int fmt, bool x_int8, int M, int N, int K, int top_n) {
   const auto align = [](size_t n) { return (n + 255) / 256 * 256; };
   p.sums = align(static_cast<size_t>(p.rows) * p.parts * sizeof(float4_t));
   p.token_logit = align(static_cast<size_t>(p.rows) * 4);
-  if (top_n > 0) p.logits = align(static_cast<size_t>(p.rows) * N * 4);
-  if (top_n > 0 && !p.few) p.strips = p.sums;
+  if (top_n == 1 && !p.lists) p.firsts = align(static_cast<size_t>(p.rows) * p.parts * sizeof(int));
+  if (p.lists) p.logits = align(static_cast<size_t>(p.rows) * N * 4);
+  if (p.lists && !p.few) p.strips = p.sums;
   if (p.every > 1) p.bound = p.token_logit;
   return p;
 }
@@ -500,7 +540,7 @@ int launch_rows(hipStream_t st, const Plan& p, HeadArgs g, const TokenLogprobs& 
   int rc = RWKV_OK;
   if (p.few) {
     rc = launch_few<TYPES>(st, g);
-  } else if (out.top_n == 0) {
+  } else if (!p.lists) {
     rc = launch_tiles<TYPES, false>(st, g, p.tile, 1, false);
   } else {
     rc = launch_tiles<TYPES, true>(st, g, p.tile, p.every, false);
@@ -514,7 +554,7 @@ int launch_rows(hipStream_t st, const Plan& p, HeadArgs g, const TokenLogprobs& 
     }
   }
   if (rc != RWKV_OK) return rc;
-  if (out.top_n == 0) hipLaunchKernelGGL(head_sums_kernel, dim3(ceil_div(g.M, 4)), dim3(256), 0, st, g, out);
+  if (!p.lists) hipLaunchKernelGGL(head_sums_kernel, dim3(ceil_div(g.M, 4)), dim3(256), 0, st, g, out);
   else hipLaunchKernelGGL(head_alternatives_kernel, dim3(g.M), dim3(256), 0, st, g, out, p.few ? few_bands(g.N) * (kFewThreads / 64 * 32) : 64);
   RWKV_LAUNCH_CHECK();
   return RWKV_OK;
@@ -541,11 +581,18 @@ int linear_logprobs_launch(hipStream_t st, int fmt, int M, int N, int K, const v
     g.K = K;
     g.tokens = rows.logprob ? rows.tokens : nullptr;
     g.parts = p.parts;
-    g.sums = reinterpret_cast<float4_t*>(ws);
-    g.token_logit = reinterpret_cast<float*>(ws + p.sums);
-    g.logits = p.logits ? reinterpret_cast<float*>(ws + p.sums + p.token_logit) : nullptr;
-    g.strips = reinterpret_cast<float*>(ws + p.sums + p.token_logit + p.logits);
-    float* bound = reinterpret_cast<float*>(ws + p.sums + p.token_logit + p.logits + p.strips);
+    unsigned char* at = ws;
+    const auto take = [&at](size_t bytes) {
+      void* p = bytes ? at : nullptr;
+      at += bytes;
+      return p;
+    };
+    g.sums = static_cast<float4_t*>(take(p.sums));
+    g.token_logit = static_cast<float*>(take(p.token_logit));
+    g.firsts = static_cast<int*>(take(p.firsts));
+    g.logits = static_cast<float*>(take(p.logits));
+    g.strips = static_cast<float*>(take(p.strips));
+    float* bound = static_cast<float*>(take(p.bound));
     const int rc = x_scale ? launch_rows<kI8W8>(st, p, g, rows, bound)
                            : (fmt == RWKV_FMT_W8 ? launch_rows<kF16W8>(st, p, g, rows, bound) : launch_rows<kF16F16>(st, p, g, rows, bound));
     if (rc != RWKV_OK) return rc;

@@ -6,6 +6,9 @@
 //   scale = max|y| / 127;  q = rint(y / scale), ties to even;  scale = 0 and q = 0 where max|y| = 0
 //   a row whose y is not finite somewhere: scale = NaN and q = 0, so that whatever reads it is NaN too
 //
+// Bound by memory: 7 bytes a value, 2048 rows of 4096 (58.7 MB) 12.5 us = 4.7 TB/s, where a large copy moves 4.9; few rows by the launch
+// (one row of 768 2.4 us) and three block-wide reductions behind one trip to memory.
+//
 // y stays in fp32 from the sum to the code: an fp16 y in between would add half a step of 2^-11 of the value, an eighth of the
 // code's own rounding at the largest values.
 #include "ops.h"

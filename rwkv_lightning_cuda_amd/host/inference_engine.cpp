@@ -273,6 +273,7 @@ double InferenceEngine::TextScore::total() const { return std::accumulate(at.log
 // Rectangular calls of at most prefill_chunk_size_ positions over the texts that are not finished (a prefix, longest first); a text that
 // ends inside a chunk is filled up with token 0 and no target, and drops out of the state behind it.
 std::vector<InferenceEngine::TextScore> InferenceEngine::score(const std::vector<std::string>& texts, const ScoreOptions& options) const {
+  if (options.top_n < 0 || options.top_n > 64) throw std::runtime_error("top_n must lie in 0 .. 64");
   if (texts.empty()) return {};
   std::vector<size_t> original;
   const std::vector<std::vector<int64_t>> sorted = encode_prompts_sorted(texts, original);

@@ -168,6 +168,10 @@ HOST_TEST(engine_scores_texts_of_any_lengths) {
   }
   CHECK(engine.score({}, o).empty());
   CHECK_THROWS(engine.score({""}, o), "prompt is empty");
+  o.top_n = -1;
+  CHECK_THROWS(engine.score({base}, o), "top_n");
+  o.top_n = 65;
+  CHECK_THROWS(engine.score({base}, o), "top_n");
 }
 
 int main(int argc, char** argv) { return host_test::run_all(argc, argv, true); }

@@ -676,3 +676,40 @@ def test_outputs_that_are_not_asked_for(gpu):
         hip.token_logprobs(rows, V, d, None, ws, top_n=6, top_ids=ids, top_logprobs=tops)
         hip.device_sync()
         assert np.array_equal(ids.numpy(), whole["ids"]) and np.array_equal(tops.numpy(), whole["tops"])
+
+
+@pytest.mark.parametrize("types,M,top", [("i8", 3, 1), ("i8", 150, 1), ("f16", 150, 4), ("w8", 40, 1)])
+def test_head_outputs_that_are_not_asked_for(gpu, orc, types, M, top):
+    hip = gpu
+    N, K = 2080, 512
+    c = head_case(hip, orc, types, M, N, K, seed=71)
+    tokens = np.random.default_rng(2).integers(0, N, M)
+    whole = run_head(hip, c, tokens, top)
+    int8 = types == "i8"
+    dt = hip.DeviceArray.from_numpy(tokens.astype(np.int32))
+    ws = hip.DeviceArray((hip.linear_logprobs_workspace(c["fmt"], M, N, K, top, x_int8=int8),), np.uint8)
+    call = lambda t, **kw: hip.linear_logprobs(c["fmt"], M, N, K, c["x"], c["packed"], c["scale"], t, ws, x_scale=c["x_scale"], **kw)  # noqa: E731
+    one = hip.DeviceArray.zeros((M,), np.float32)
+    # (without alternatives a call may share its columns out otherwise: the last bits of the sums)
+    for name, t in (("logprob", dt), ("entropy", None)):
+        call(t, **{name: one})
+        hip.device_sync()
+        assert np.abs(one.numpy() - whole[name]).max() <= (N / 256 + 64) * 4 * STEP * 12
+    ids, tops = hip.DeviceArray.zeros((M, top), np.int32), hip.DeviceArray.zeros((M, top), np.float32)
+    call(None, top_n=top, top_ids=ids, top_logprobs=tops)
+    hip.device_sync()
+    assert np.array_equal(ids.numpy(), whole["ids"]) and np.array_equal(tops.numpy().view(np.uint32), whole["tops"].view(np.uint32))
+
+
+def test_norm_writes_the_sum_over_the_residual(gpu):
+    hip = gpu
+    rng = np.random.default_rng(3)
+    x, res = (rng.standard_normal((5, 768)).astype(np.float16) for _ in range(2))
+    w = np.ones(768, np.float16)
+    dx, dr, dw = (hip.DeviceArray.from_numpy(v) for v in (x, res, w))
+    q, scale = hip.DeviceArray((5, 768), np.int8), hip.DeviceArray((5,), np.float32)
+    hip.add_norm_q8(5, 768, dx, dr, dw, None, q, scale, x_out=dr)
+    hip.device_sync()
+    want = run_norm(hip, x, res, w, None, False)
+    assert np.array_equal(dr.numpy(), want[0]) and np.array_equal(q.numpy(), want[1]) and np.array_equal(scale.numpy(), want[2])
+    assert np.array_equal(dx.numpy(), x)
