@@ -45,10 +45,11 @@ __device__ __forceinline__ float next_above(float v) {  // the smallest float ab
 }
 
 // One block per row, or per part of one, which it reads once: 64 bytes per thread at a time, the next 64 requested before they are
-// looked at.  A thread keeps the sums of its entries against the largest that its wavefront has seen, which few batches raise.  The rank is a count against the token's
-// logit, which is read first.  Alternatives: what is not below the bound that the first batch gives goes to a list in LDS, which is
-// thinned out to the first top_n - with the last one as the new bound - whenever it has grown to four times as many.  A list that
-// overflows (a row that rises, or is of one value) is given up: the alternatives are then found one after the other in top_n walks.
+// looked at.  A thread keeps the sums of its entries against the largest that its wavefront has seen, which few batches raise.  The rank
+// is a count against the token's logit, which is read first.  Alternatives: what is not below the bound that the first batch gives goes to
+// a list in LDS, which is thinned out to the first top_n - with the last one as the new bound - whenever it has grown to four times as
+// many.  A list that overflows (a row that rises, or is of one value) is given up: the alternatives are then found one after the other in
+// top_n walks.
 template <typename T, bool PART>
 __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobArgs a) {
   constexpr int NT = kThreads;

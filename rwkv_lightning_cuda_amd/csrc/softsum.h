@@ -119,8 +119,8 @@ struct Candidates {
 };
 
 // A value that the top_n-th largest of the wavefront's N values per lane reaches: that value with its last 16 bits cut off (downwards: a
-// bound may be loose by 2^-7), found bit by bit from the first.  (16 counts of a ballot, 0.3 us; counting for each of 64 values how many
-// are larger took 3.2.)  -infinity where there are not as many; NaN counts as that.
+// bound may be loose by 2^-7), found bit by bit from the first.  (16 counts of a ballot: 0.7 us for a block's first bound; counting for each
+// of its values how many are larger took 3.2.)  -infinity where there are not as many; NaN counts as that.
 template <int N>
 __device__ __forceinline__ float wave_bound(const float (&v)[N], int top_n) {
   uint32_t r[N];

@@ -57,8 +57,8 @@ EXPORTS = [
 ]
 
 
-# Argument types of the entry points that a serving loop calls after every token: ctypes then converts plain ints itself (a call with
-# 17 arguments 3 us instead of 9).
+# Argument types of the entry points that a serving loop calls after every token: ctypes then converts plain ints itself (17 arguments:
+# 0.5 us less than an object made for each).
 _P, _N, _L, _S = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
 _ARGTYPES = {
     "rwkv_hip_add_norm_q8": [_P, _N, _N, _N, _P, _P, _P, _P, ctypes.c_float, _P, _P, _P],
