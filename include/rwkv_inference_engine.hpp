@@ -49,8 +49,8 @@ class InferenceEngine {
                                               const ControlCallback& should_stop = {}) const;
 
   // How probable a text is, token by token (no counterpart in the reference).  Row i of `at` belongs to tokens[i] given the tokens in
-  // front of it; row 0 has none: log probability and entropy 0, no alternatives.  Texts of any lengths in one call; each starts from
-  // an empty state.
+  // front of it; row 0 has none: log probability and entropy 0, no alternatives.  Texts of any lengths, and any number of them; each
+  // starts from an empty state.
   struct TextScore {
     std::vector<int64_t> tokens;
     TokenLogprobs at;

@@ -270,8 +270,15 @@ int InferenceEngine::prefill_prompt(const std::string& prompt, GenerationState& 
 
 double InferenceEngine::TextScore::total() const { return std::accumulate(at.logprob.begin(), at.logprob.end(), 0.0); }
 
-// Rectangular calls of at most prefill_chunk_size_ positions over the texts that are not finished (a prefix, longest first); a text that
-// ends inside a chunk is filled up with token 0 and no target, and drops out of the state behind it.
+namespace {
+// Positions and texts of one call: enough to fill the device, and what bounds the session's buffers and the states (7.2B: 34 MB a text)
+// however many texts there are.
+constexpr size_t kScorePositions = 8192, kScoreTexts = 256;
+}  // namespace
+
+// Groups of texts of like lengths (longest first), each in rectangular calls of at most prefill_chunk_size_ positions a text over those that
+// are not finished (a prefix of the group); a text that ends inside a chunk is filled up with token 0 and no target, and drops out of the
+// state behind it.
 std::vector<InferenceEngine::TextScore> InferenceEngine::score(const std::vector<std::string>& texts, const ScoreOptions& options) const {
   if (options.top_n < 0 || options.top_n > 64) throw std::runtime_error("top_n must lie in 0 .. 64");
   if (texts.empty()) return {};
@@ -288,35 +295,42 @@ std::vector<InferenceEngine::TextScore> InferenceEngine::score(const std::vector
     t.at.top_ids.assign(options.top_n, -1);
     t.at.top_logprobs.assign(options.top_n, -std::numeric_limits<float>::infinity());
   }
-  int width = 0;
-  GenerationState state;
-  for (size_t done = 0;; done += prefill_chunk_size_) {
-    int active = 0;
-    while (active < static_cast<int>(sorted.size()) && sorted[active].size() > done + 1) ++active;
-    if (active == 0) return out;
-    if (active != width) {
-      GenerationState next = model_->create_state(active);
-      if (done > 0) model_->copy_state_slice(state, 0, next, 0, active);
-      state = std::move(next);
-      width = active;
-    }
-    const size_t step = std::min(sorted[0].size() - 1 - done, static_cast<size_t>(prefill_chunk_size_));
-    std::vector<std::vector<int64_t>> tokens(active, std::vector<int64_t>(step, 0)), targets(active, std::vector<int64_t>(step, -1));
-    for (int b = 0; b < active; ++b)
-      for (size_t i = 0; i < step && done + i + 1 < sorted[b].size(); ++i) {
-        tokens[b][i] = sorted[b][done + i];
-        targets[b][i] = sorted[b][done + i + 1];
+  const size_t chunk = static_cast<size_t>(prefill_chunk_size_);
+  for (size_t first = 0, group = 0; first < sorted.size() && sorted[first].size() > 1; first += group) {
+    const size_t longest = sorted[first].size() - 1;
+    group = std::min({sorted.size() - first, kScoreTexts, std::max<size_t>(kScorePositions / std::min(longest, chunk), 1)});
+    size_t width = 0;
+    GenerationState state;
+    for (size_t done = 0; done < longest; done += chunk) {
+      size_t active = 0;
+      while (active < group && sorted[first + active].size() > done + 1) ++active;
+      if (active != width) {
+        GenerationState next = model_->create_state(static_cast<int>(active));
+        if (done > 0) model_->copy_state_slice(state, 0, next, 0, static_cast<int>(active));
+        state = std::move(next);
+        width = active;
       }
-    const TokenLogprobs part = model_->score(tokens, targets, state, options);
-    for (int b = 0; b < active; ++b) {
-      TokenLogprobs& at = out[original[b]].at;
-      const size_t n = std::min(step, sorted[b].size() - 1 - done), row = b * step, top = options.top_n;
-      at.logprob.insert(at.logprob.end(), part.logprob.begin() + row, part.logprob.begin() + row + n);
-      at.entropy.insert(at.entropy.end(), part.entropy.begin() + row, part.entropy.begin() + row + n);
-      at.top_ids.insert(at.top_ids.end(), part.top_ids.begin() + row * top, part.top_ids.begin() + (row + n) * top);
-      at.top_logprobs.insert(at.top_logprobs.end(), part.top_logprobs.begin() + row * top, part.top_logprobs.begin() + (row + n) * top);
+      const size_t step = std::min(longest - done, chunk);
+      std::vector<std::vector<int64_t>> tokens(active, std::vector<int64_t>(step, 0)), targets(active, std::vector<int64_t>(step, -1));
+      for (size_t b = 0; b < active; ++b) {
+        const std::vector<int64_t>& text = sorted[first + b];
+        for (size_t i = 0; i < step && done + i + 1 < text.size(); ++i) {
+          tokens[b][i] = text[done + i];
+          targets[b][i] = text[done + i + 1];
+        }
+      }
+      const TokenLogprobs part = model_->score(tokens, targets, state, options);
+      for (size_t b = 0; b < active; ++b) {
+        TokenLogprobs& at = out[original[first + b]].at;
+        const size_t n = std::min(step, sorted[first + b].size() - 1 - done), row = b * step, top = options.top_n;
+        at.logprob.insert(at.logprob.end(), part.logprob.begin() + row, part.logprob.begin() + row + n);
+        at.entropy.insert(at.entropy.end(), part.entropy.begin() + row, part.entropy.begin() + row + n);
+        at.top_ids.insert(at.top_ids.end(), part.top_ids.begin() + row * top, part.top_ids.begin() + (row + n) * top);
+        at.top_logprobs.insert(at.top_logprobs.end(), part.top_logprobs.begin() + row * top, part.top_logprobs.begin() + (row + n) * top);
+      }
     }
   }
+  return out;
 }
 
 // Single-row loop with an optional emitter.  The returned text is the concatenation of every generated
