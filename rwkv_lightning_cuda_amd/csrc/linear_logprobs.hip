@@ -372,13 +372,15 @@ __global__ __launch_bounds__(256) void head_sums_kernel(HeadArgs g, TokenLogprob
   if (out.top_n == 1) write_alternative(out, row, 0, a.m > kLowest && first < g.N ? key_of(a.m, first) : 0, a.m, a.log_sum());
 }
 
-// The same with the alternatives, a block per row (2048 rows with 5: 14 us): they lie in the strips whose largest reaches the top_n-th largest of 64 or 256 groups
-// of strips - few more than top_n of them - whose logits are there.  768 columns at a time; the list never overflows, it is thinned out
-// first.  Strips of `width` columns: 64 with their largest in `strips` (tiles), or a part's with it in `sums` (few rows).
+// The same with the alternatives, a block per row: they lie in the strips whose largest reaches the top_n-th largest of 64 or 256 groups
+// of strips - few more than top_n of them - whose logits are there.  1024 strips at a time (2048 rows of 1024 strips, 5 alternatives: 11 us; 256
+// strips at a time 14) and 768 columns; the list never overflows, it is thinned out first.  Strips of `width` columns: 64 with their largest in `strips` (tiles), or a part's with it in `sums` (few rows).
 __global__ __launch_bounds__(256) void head_alternatives_kernel(HeadArgs g, TokenLogprobs out, int width) {
   __shared__ __align__(16) Candidates<256> cand;
   __shared__ float4_t waves[4];
-  __shared__ int chosen[256];
+  constexpr int kStrips = 4;  // of a thread and turn
+  __shared__ uint16_t chosen[kStrips * 256];  // (eight such blocks have room on a CU)
+  static_assert(kMaxLogprobVocab / 64 <= 65536, "strips of 16 bits");
   __shared__ int n_chosen;
   const int tid = threadIdx.x, row = blockIdx.x, top_n = out.top_n;
   const float4_t* sums = g.sums + static_cast<int64_t>(row) * g.parts;
@@ -388,10 +390,17 @@ __global__ __launch_bounds__(256) void head_alternatives_kernel(HeadArgs g, Toke
   const float* logits = g.logits + static_cast<int64_t>(row) * g.N;
   const int token = g.tokens ? g.tokens[row] : -1;
   const float token_logit = g.token_logit[row];  // (not written where there is no token)
+  float strip[kStrips];
+  auto look = [&](int base) {
+#pragma unroll
+    for (int q = 0; q < kStrips; ++q) {
+      const int s = base + q * 256 + tid;
+      strip[q] = s < n_strips ? strips[s * apart] : -INFINITY;
+    }
+  };
+  look(0);
   SoftSum a;
-  for (int i = tid; i < g.parts; i += 256) {
-    a.merge(SoftSum(sums[i]));
-  }
+  for (int i = tid; i < g.parts; i += 256) a.merge(SoftSum(sums[i]));
   a.merge_wave();
   if ((tid & 63) == 0) waves[tid >> 6] = a.stored();
   if (tid == 0) {
@@ -399,7 +408,9 @@ __global__ __launch_bounds__(256) void head_alternatives_kernel(HeadArgs g, Toke
     n_chosen = 0;
   }
   float most = -INFINITY;
-  for (int i = tid; i < n_strips; i += 256) most = fmaxf(most, strips[i * apart]);
+#pragma unroll
+  for (int q = 0; q < kStrips; ++q) most = fmaxf(most, strip[q]);
+  for (int i = kStrips * 256 + tid; i < n_strips; i += 256) most = fmaxf(most, strips[i * apart]);
   // (not below the bound that the tiles went by: what lies below that has not been written)
   const float bound = fmaxf(first_bound(cand, top_n, most), g.bound ? g.bound[row] : -INFINITY);
   a = SoftSum();
@@ -411,12 +422,13 @@ __global__ __launch_bounds__(256) void head_alternatives_kernel(HeadArgs g, Toke
   const int pieces = width / at_once;
   constexpr int kAtOnce = 3;
   static_assert(kMaxAlternatives <= kCandidates - kAtOnce * 256, "a list that has been thinned out takes the next entries");
-  for (int base = 0; base < n_strips; base += 256) {
-    const int s = base + tid;
+  for (int base = 0; base < n_strips; base += kStrips * 256) {
+    if (base > 0) look(base);
     // (a strip whose largest ties with the last candidate and lies behind it has none)
-    if (s < n_strips) {
-      const float v = strips[s * apart];
-      if (v == v && key_of(v, s * width) > least) chosen[atomicAdd(&n_chosen, 1)] = s;
+#pragma unroll
+    for (int q = 0; q < kStrips; ++q) {
+      const int s = base + q * 256 + tid;
+      if (strip[q] > -INFINITY && key_of(strip[q], s * width) > least) chosen[atomicAdd(&n_chosen, 1)] = s;
     }
     __syncthreads();
     const int n = n_chosen * pieces;
