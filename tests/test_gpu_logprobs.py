@@ -444,6 +444,30 @@ def test_head_of_many_rows_finds_alternatives_wherever_they_lie(gpu, top, kind):
     check_logprobs({n: got[n][:1] for n in ("logprob", "entropy", "tops")}, ref, N, slack=3 * STEP * np.abs(c["z"][0]).max())
 
 
+@pytest.mark.parametrize("M,top", [(40, 5), (40, 64), (700, 20)])
+@pytest.mark.parametrize("kind", ["rising", "last only", "equal"])
+def test_head_of_a_wide_vocabulary_finds_alternatives_wherever_they_lie(gpu, M, top, kind):
+    """More strips of columns than the last launch looks at in one turn: each turn's better than the one before, all in the last strips, or
+    no entry better than another."""
+    hip = gpu
+    N, K = 200032, 256
+    codes = np.random.default_rng(4).integers(-3, 4, N)
+    if kind == "rising":
+        codes = codes + np.arange(N) // 2048
+    elif kind == "last only":
+        codes[-96:] += 50
+    else:
+        codes[:] = 2
+    c = crafted_head(hip, M, N, K, codes, top)
+    got = run_head(hip, c, np.full(M, N - 1), top, workspace=poisoned_workspace(hip, c, M, N, K, top))
+    want = np.lexsort((np.arange(N), -codes))[:top]
+    assert np.array_equal(got["ids"], np.tile(want.astype(np.int32), (M, 1)))
+    for name in ("logprob", "entropy", "tops"):
+        assert np.all(got[name] == got[name][0])
+    ref = ref_logprobs(c["z"][:1], [N - 1], top)
+    check_logprobs({n: got[n][:1] for n in ("logprob", "entropy", "tops")}, ref, N, slack=3 * STEP * np.abs(c["z"][0]).max())
+
+
 @pytest.mark.parametrize("types,M,top", [("i8", 2049, 5), ("f16", 1700, 2), ("w8", 2048, 20)])
 def test_head_of_many_rows_matches_the_formula(gpu, orc, types, M, top):
     """Two launches of tiles with a bound between them (and a second block of rows), some rows checked."""
