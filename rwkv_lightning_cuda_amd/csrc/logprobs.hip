@@ -11,15 +11,14 @@
 //
 // Entries of -infinity have probability 0 and are no alternatives; a row of nothing else gives log probability -infinity, entropy 0
 // and no alternative.
-#include <algorithm>
-
+#include "logprobs_parts.h"
 #include "softsum.h"
 
 namespace rwkv {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = kLogprobThreads;
 constexpr int kRefine = 4;  // batches between looks at whether the candidates can be thinned out
 
 struct LogprobArgs {
@@ -35,8 +34,7 @@ struct LogprobArgs {
   key_t* keys;     // [rows][parts][part_keys(top_n)] in any order, 0 past the last
 };
 
-// Candidates that a part hands on as they are, without sorting out its first top_n
-__host__ __device__ constexpr int part_keys(int top_n) { return top_n > 0 ? 2 * top_n + 8 : 0; }
+static_assert(sizeof(float4_t) == 16 && sizeof(key_t) == 8, "PartBytes");
 static_assert(part_keys(kMaxAlternatives) <= 256, "written by one thread each");
 
 __device__ __forceinline__ float next_above(float v) {  // the smallest float above v; NaN above +infinity
@@ -242,7 +240,6 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_kernel(LogprobArgs a)
 }
 
 // A block per row over what its parts have left.  Of many keys a bound is made first, as of the entries of a row.
-constexpr int kMaxParts = 256;
 __global__ __launch_bounds__(kThreads) void token_logprobs_join_kernel(LogprobArgs a) {
   __shared__ __align__(16) Candidates<kThreads> cand;
   __shared__ float4_t waves[kThreads / 64];
@@ -320,24 +317,6 @@ __global__ __launch_bounds__(kThreads) void token_logprobs_join_kernel(LogprobAr
   }
 }
 
-// Parts of a row: as many as bring the call to four blocks of 256 threads for every CU, each at least one batch long, and none where that
-// is fewer than three (us with the join, fp32, 65536 entries: 64 rows in 16 parts 12.6, in 4 18.3; 200 rows in 5 20.8, whole 24.9; 400
-// rows in 2 29.3, whole 27.9; 77 fp16 rows of 50277 in 7 12.3, in 13 13.6).
-int parts_of(int rows, int V, int io) {
-  const int batch = kThreads * (io == RWKV_IO_F16 ? 32 : 16);
-  const int parts = std::min({4 * device_cu_count() / rows, ceil_div(V, batch), kMaxParts});
-  return parts < 3 ? 1 : parts;
-}
-struct PartBytes {  // of the workspace, in this order
-  size_t sums, ahead, token_logit, keys;
-  size_t all() const { return sums + ahead + token_logit + keys; }
-};
-PartBytes part_bytes(int rows, int parts, int top_n) {
-  const auto align = [](size_t n) { return (n + 15) / 16 * 16; };
-  const size_t all = static_cast<size_t>(rows) * parts;
-  return {all * sizeof(float4_t), align(all * sizeof(int)), align(rows * sizeof(float)), all * part_keys(top_n) * sizeof(key_t)};
-}
-
 template <typename T>
 void launch_rows(hipStream_t st, int rows, const LogprobArgs& a) {
   if (a.parts == 1) {
@@ -350,13 +329,15 @@ void launch_rows(hipStream_t st, int rows, const LogprobArgs& a) {
 
 }  // namespace
 
-size_t token_logprobs_workspace_bytes(int rows, int V, int top_n) {
-  const int parts = parts_of(rows, V, RWKV_IO_F32);  // (fp16 rows go in no more)
-  return parts == 1 ? 0 : part_bytes(rows, parts, top_n).all();
-}
+size_t token_logprobs_workspace_bytes(int rows, int V, int top_n) { return logprob_bytes(rows, V, top_n, device_cu_count()); }
+size_t token_logprobs_block_workspace_bytes(int rows, int V, int top_n) { return most_logprob_bytes(rows, V, top_n, device_cu_count()); }
 
-int token_logprobs_launch(hipStream_t st, int rows, int V, int io, const void* logits, int64_t ld, const TokenLogprobs& out, void* workspace) {
-  const int parts = parts_of(rows, V, io);
+int token_logprobs_launch(hipStream_t st, int rows, int V, int io, const void* logits, int64_t ld, const TokenLogprobs& out, void* workspace,
+                          size_t workspace_bytes) {
+  const size_t need = token_logprobs_workspace_bytes(rows, V, out.top_n);
+  RWKV_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
+               "token_logprobs: workspace of %zu bytes (aligned to 16) needed, got %zu", need, workspace_bytes);
+  const int parts = logprob_parts(rows, V, io, device_cu_count());
   // (a multiple of a vector, so that the parts of an aligned row are aligned)
   const PartBytes p = part_bytes(rows, parts, out.top_n);
   char* ws = static_cast<char*>(workspace);
@@ -407,10 +388,7 @@ int rwkv_hip_token_logprobs(rwkv_stream_t s, int rows, int V, int io, const void
                              static_cast<int*>(rank), static_cast<int*>(top_ids), static_cast<float*>(top_logprobs)};
   const int rc = check_token_logprobs("token_logprobs", out);
   if (rc != RWKV_OK) return rc;
-  const size_t need = token_logprobs_workspace_bytes(rows, V, top_n);
-  RWKV_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
-               "token_logprobs: workspace of %zu bytes (aligned to 16) needed, got %zu", need, workspace_bytes);
-  return token_logprobs_launch(as_stream(s), rows, V, io, logits, ld, out, workspace);
+  return token_logprobs_launch(as_stream(s), rows, V, io, logits, ld, out, workspace, workspace_bytes);
 }
 
 }  // extern "C"

@@ -252,7 +252,9 @@ struct TokenLogprobs {
 };
 int check_token_logprobs(const char* who, const TokenLogprobs& out);
 size_t token_logprobs_workspace_bytes(int rows, int V, int top_n);
-int token_logprobs_launch(hipStream_t st, int rows, int V, int io, const void* logits, int64_t ld, const TokenLogprobs& out, void* workspace);
+size_t token_logprobs_block_workspace_bytes(int rows, int V, int top_n);  // of every call of up to `rows` rows (fewer may need more)
+int token_logprobs_launch(hipStream_t st, int rows, int V, int io, const void* logits, int64_t ld, const TokenLogprobs& out, void* workspace,
+                          size_t workspace_bytes);
 size_t linear_logprobs_workspace_bytes(int fmt, bool x_int8, int M, int N, int K, int top_n);
 // x_scale: x holds int8 codes
 int linear_logprobs_launch(hipStream_t st, int fmt, int M, int N, int K, const void* x, const float* x_scale, const void* packed,
