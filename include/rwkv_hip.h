@@ -303,7 +303,8 @@ int rwkv_hip_argmax(rwkv_stream_t s, int B, int V, const void* logits, void* out
  * -infinity gives log probability -infinity, entropy 0.  A row with a NaN or +infinity gives NaN for every log probability and the
  * entropy (NaN entries are no alternatives).  V <= 1048576.  Sums are held in fp32 in a fixed order: a call repeats bitwise, and a
  * row's results do not depend on the other rows' values (how a row is shared out goes by rows, V and top_n).  The workspace
- * (rwkv_hip_token_logprobs_workspace bytes, aligned to 16; NULL where 0) need not be cleared; calls that share one must not overlap. */
+ * (rwkv_hip_token_logprobs_workspace bytes, aligned to 16; NULL where 0) need not be cleared; calls that share one must not overlap.  What
+ * the query gives for some rows, V and top_n serves every call of that V and top_n with as many rows or fewer. */
 int rwkv_hip_token_logprobs_workspace(int rows, int V, int top_n, size_t* bytes);
 int rwkv_hip_token_logprobs(rwkv_stream_t s, int rows, int V, int io, const void* logits, int64_t ld, const void* tokens, int top_n,
                             void* logprob, void* entropy, void* rank, void* top_ids, void* top_logprobs, void* workspace,
@@ -312,8 +313,8 @@ int rwkv_hip_token_logprobs(rwkv_stream_t s, int rows, int V, int io, const void
  * text.  packed: rwkv_hip_pack_weights of fp16 weights (RWKV_FMT_F16) or int8 codes (RWKV_FMT_W8, scale f16 [N]).  x: f16 [M,K] with
  * x_scale NULL, or int8 [M,K] (RWKV_FMT_W8 only) with x_scale f32 [M] >= 0 as rwkv_hip_add_norm_q8 gives them, z = (whole-number
  * product) * scale * x_scale.  N % 32 == 0, K % 256 == 0, N <= 1048576, K <= 16384; x and packed aligned to 16 bytes, scale to 8.
- * Repeats bitwise.  Workspace as above (aligned to 16); with two alternatives or more it has a place for every logit of up to 2048 rows at
- * 65536 columns (0.54 GB, few of which are written), otherwise 45 MB at most. */
+ * Repeats bitwise.  Workspace as above (aligned to 16; for as many rows or fewer, the other sizes and types being the same); with two alternatives
+ * or more it has a place for every logit of up to 2048 rows at 65536 columns (0.54 GB, few of which are written), otherwise 45 MB at most. */
 int rwkv_hip_linear_logprobs_workspace(int fmt, int x_int8, int M, int N, int K, int top_n, size_t* bytes);
 int rwkv_hip_linear_logprobs(rwkv_stream_t s, int fmt, int M, int N, int K, const void* x, const void* x_scale, const void* packed,
                              const void* scale, const void* tokens, int top_n, void* logprob, void* entropy, void* top_ids,

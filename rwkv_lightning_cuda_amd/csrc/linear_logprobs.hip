@@ -516,8 +516,16 @@ Plan plan_of(int fmt, bool x_int8, int M, int N, int K, int top_n) {
   if (top_n == 1 && !p.lists) p.firsts = align(static_cast<size_t>(p.rows) * p.parts * sizeof(int));
   if (p.lists) p.logits = align(static_cast<size_t>(p.rows) * N * 4);
   if (p.lists && !p.few) p.strips = p.sums;
-  if (p.every > 1) p.bound = p.token_logit;
+  if (p.lists && !p.few) p.bound = p.token_logit;  // (whether or not this call bounds them: fewer rows may)
   return p;
+}
+
+// of every call of up to M rows: fewer may go without tiles and keep all logits
+size_t most_bytes(int fmt, bool x_int8, int M, int N, int K, int top_n) {
+  int few = std::min(M, kFewRows);
+  while (few > 0 && !takes_few(few, K, x_int8 ? 1 : 2)) --few;
+  const size_t tiles = plan_of(fmt, x_int8, M, N, K, top_n).bytes();
+  return few ? std::max(tiles, plan_of(fmt, x_int8, few, N, K, top_n).bytes()) : tiles;
 }
 
 template <int TYPES>
@@ -574,7 +582,7 @@ int launch_rows(hipStream_t st, const Plan& p, HeadArgs g, const TokenLogprobs& 
 
 }  // namespace
 
-size_t linear_logprobs_workspace_bytes(int fmt, bool x_int8, int M, int N, int K, int top_n) { return plan_of(fmt, x_int8, M, N, K, top_n).bytes(); }
+size_t linear_logprobs_workspace_bytes(int fmt, bool x_int8, int M, int N, int K, int top_n) { return most_bytes(fmt, x_int8, M, N, K, top_n); }
 
 int linear_logprobs_launch(hipStream_t st, int fmt, int M, int N, int K, const void* x, const float* x_scale, const void* packed,
                            const half_t* scale, const TokenLogprobs& out, void* workspace) {
@@ -653,7 +661,7 @@ int rwkv_hip_linear_logprobs(rwkv_stream_t s, int fmt, int M, int N, int K, cons
                              nullptr, static_cast<int*>(top_ids), static_cast<float*>(top_logprobs)};
   rc = check_token_logprobs("linear_logprobs", out);
   if (rc != RWKV_OK) return rc;
-  const size_t need = linear_logprobs_workspace_bytes(fmt, x_scale != nullptr, M, N, K, top_n);
+  const size_t need = plan_of(fmt, x_scale != nullptr, M, N, K, top_n).bytes();
   RWKV_REQUIRE(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
                "linear_logprobs: workspace of %zu bytes (aligned to 16) needed, got %zu", need, workspace_bytes);
   return linear_logprobs_launch(as_stream(s), fmt, M, N, K, x, static_cast<const float*>(x_scale), packed, static_cast<const half_t*>(scale), out,

@@ -329,12 +329,11 @@ void launch_rows(hipStream_t st, int rows, const LogprobArgs& a) {
 
 }  // namespace
 
-size_t token_logprobs_workspace_bytes(int rows, int V, int top_n) { return logprob_bytes(rows, V, top_n, device_cu_count()); }
-size_t token_logprobs_block_workspace_bytes(int rows, int V, int top_n) { return most_logprob_bytes(rows, V, top_n, device_cu_count()); }
+size_t token_logprobs_workspace_bytes(int rows, int V, int top_n) { return most_logprob_bytes(rows, V, top_n, device_cu_count()); }
 
 int token_logprobs_launch(hipStream_t st, int rows, int V, int io, const void* logits, int64_t ld, const TokenLogprobs& out, void* workspace,
                           size_t workspace_bytes) {
-  const size_t need = token_logprobs_workspace_bytes(rows, V, out.top_n);
+  const size_t need = logprob_bytes(rows, V, out.top_n, device_cu_count());
   RWKV_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
                "token_logprobs: workspace of %zu bytes (aligned to 16) needed, got %zu", need, workspace_bytes);
   const int parts = logprob_parts(rows, V, io, device_cu_count());

@@ -461,7 +461,7 @@ size_t score_rest_bytes(const rwkv_hip_model* m, bool act_int8, int rows, int to
     gemm = linear_packed_multi_workspace_bytes(block, m->C, 1, &p, RWKV_EPI_NONE, 1);
     if (rows % block) gemm = std::max(gemm, linear_packed_multi_workspace_bytes(rows % block, m->C, 1, &p, RWKV_EPI_NONE, 1));
   }
-  return align_up(static_cast<size_t>(block) * m->V * sizeof(float), 256) + align_up(token_logprobs_block_workspace_bytes(block, m->V, top_n), 256) + gemm;
+  return align_up(static_cast<size_t>(block) * m->V * sizeof(float), 256) + align_up(token_logprobs_workspace_bytes(block, m->V, top_n), 256) + gemm;
 }
 
 // The final norm of every row and the head's log probabilities; x1 + cm is the residual stream behind the last layer.
@@ -481,7 +481,7 @@ int enqueue_score(rwkv_hip_session* s, int rows, const ScoreArgs& a) {
   const int block = std::min(rows, kScoreLogitRows);
   float* logits = reinterpret_cast<float*>(a.rest);
   unsigned char* lp_ws = a.rest + align_up(static_cast<size_t>(block) * V * sizeof(float), 256);
-  const size_t lp_bytes = token_logprobs_block_workspace_bytes(block, V, a.out.top_n);  // (the last block may be a shorter one)
+  const size_t lp_bytes = token_logprobs_workspace_bytes(block, V, a.out.top_n);  // (the last block may be a shorter one)
   unsigned char* gemm_ws = lp_ws + align_up(lp_bytes, 256);
   for (int r = 0; r < rows; r += block) {
     const int n = std::min(block, rows - r);

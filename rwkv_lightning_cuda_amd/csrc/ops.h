@@ -251,8 +251,8 @@ struct TokenLogprobs {
   }
 };
 int check_token_logprobs(const char* who, const TokenLogprobs& out);
+// workspaces: of every call of up to so many rows (fewer may need more)
 size_t token_logprobs_workspace_bytes(int rows, int V, int top_n);
-size_t token_logprobs_block_workspace_bytes(int rows, int V, int top_n);  // of every call of up to `rows` rows (fewer may need more)
 int token_logprobs_launch(hipStream_t st, int rows, int V, int io, const void* logits, int64_t ld, const TokenLogprobs& out, void* workspace,
                           size_t workspace_bytes);
 size_t linear_logprobs_workspace_bytes(int fmt, bool x_int8, int M, int N, int K, int top_n);
