@@ -313,8 +313,10 @@ int rwkv_hip_token_logprobs(rwkv_stream_t s, int rows, int V, int io, const void
  * text.  packed: rwkv_hip_pack_weights of fp16 weights (RWKV_FMT_F16) or int8 codes (RWKV_FMT_W8, scale f16 [N]).  x: f16 [M,K] with
  * x_scale NULL, or int8 [M,K] (RWKV_FMT_W8 only) with x_scale f32 [M] >= 0 as rwkv_hip_add_norm_q8 gives them, z = (whole-number
  * product) * scale * x_scale.  N % 32 == 0, K % 256 == 0, N <= 1048576, K <= 16384; x and packed aligned to 16 bytes, scale to 8.
- * Repeats bitwise.  Workspace as above (aligned to 16; for as many rows or fewer, the other sizes and types being the same); with two alternatives
- * or more it has a place for every logit of up to 2048 rows at 65536 columns (0.54 GB, few of which are written), otherwise 45 MB at most. */
+ * Repeats bitwise.  Workspace as above (aligned to 16; for as many rows or fewer, the other sizes and types being the same): 45 MB at most without
+ * alternatives; with one the same, or 4 N bytes for each of up to 32 rows (134 MB at N = 1048576) where that is more; with two or more a
+ * place for every logit of as many rows as have 2^27 of them (2048 at N = 65536: 0.55 GB, few of which are written), never of fewer than
+ * 256 rows: 0.7 GB at most up to N = 524288 and 1.11 GB at N = 1048576. */
 int rwkv_hip_linear_logprobs_workspace(int fmt, int x_int8, int M, int N, int K, int top_n, size_t* bytes);
 int rwkv_hip_linear_logprobs(rwkv_stream_t s, int fmt, int M, int N, int K, const void* x, const void* x_scale, const void* packed,
                              const void* scale, const void* tokens, int top_n, void* logprob, void* entropy, void* top_ids,

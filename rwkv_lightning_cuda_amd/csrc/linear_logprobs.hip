@@ -482,7 +482,8 @@ struct Plan {
   size_t bytes() const { return sums + token_logit + firsts + logits + strips + bound; }
 };
 
-constexpr int kSumRows = 8192;    // rows at a time without alternatives: 32 MiB of sums at 65536 columns
+constexpr int kSumRows = 8192;    // rows at a time without lists of alternatives, and
+constexpr int kSums = 1 << 21;    // those times parts: 32 MiB of sums
 constexpr int kLogits = 1 << 27;  // and with them, rows times columns: 512 MiB of places for logits, few of which are written
 constexpr int kFewestTurns = 6;   // turns of blocks on the chip from which on two launches cost less than the logits they save
 
@@ -490,7 +491,8 @@ Plan plan_of(int fmt, bool x_int8, int M, int N, int K, int top_n) {
   Plan p = {};
   p.few = takes_few(M, K, x_int8 ? 1 : 2);
   p.lists = top_n > 1 || (top_n == 1 && p.few);
-  p.rows = p.few ? M : std::min(M, p.lists ? std::max(kLogits / N / 256, 1) * 256 : kSumRows);
+  p.parts = p.few ? ceil_div(N / 32, kFewThreads / 64 * few_bands(N)) : ceil_div(N, kTileCols);
+  p.rows = p.few ? M : p.lists ? std::min(M, std::max(kLogits / N / 256, 1) * 256) : std::min({M, kSumRows, std::max(kSums / p.parts / 256, 1) * 256});
   // The tile whose rows, padding among them, cost least; a row of a lower tile costs more (us, 65536 columns, tiles of 128 / 192 / 256
   // rows: 768 rows of 2048 fp16 226 / 233 / 220, int8 weights under them 210 / 187 / 182, of 4096 int8 224 / 230 / 216; 333 rows 111 / 118 /
   // 136, 105 / 95 / 116, 113 / 120 / 137; 190 rows 77 / 67 / 75, 70 / 53 / 63, 80 / 68 / 78).
@@ -502,7 +504,6 @@ Plan plan_of(int fmt, bool x_int8, int M, int N, int K, int top_n) {
     least = all;
     p.tile = rows;
   }
-  p.parts = p.few ? ceil_div(N / 32, kFewThreads / 64 * few_bands(N)) : ceil_div(N, kTileCols);
   p.every = 1;
   if (!p.few && p.lists) {
     const int64_t blocks = static_cast<int64_t>(ceil_div(p.rows, p.tile)) * p.parts, cus = device_cu_count();

@@ -55,3 +55,16 @@ def test_heads_of_fewer_rows_fit_the_workspace_of_more(hip, fmt, x_int8, N, top)
         needs = [head_needs(hip, fmt, M, N, K, top, x_int8) for M in rows]
         assert sizes == sorted(sizes), K
         assert all(need <= size for need, size in zip(needs, sizes)), K
+
+
+@pytest.mark.parametrize("fmt,x_int8", [(0, False), (1, True)])
+@pytest.mark.parametrize("N", [32, 2048, 65536, 200032, 262144, 524288, 1048576])
+def test_head_workspaces_keep_within_what_is_documented(hip, fmt, x_int8, N):
+    size = lambda M, K, top: hip.linear_logprobs_workspace(fmt, M, N, K, top, x_int8=x_int8)  # noqa: E731
+    for K in (256, 4096, 16384):
+        for M in (1, 32, 33, 600, 8192, 8193, 1 << 20):
+            assert size(M, K, 0) <= 45e6
+            few = min(M, 32) * N * 4 + 3e6      # (their logits, and the sums of at most 256 parts)
+            assert size(M, K, 1) <= max(45e6, few)
+            for top in (2, 64):
+                assert size(M, K, top) <= (0.7e9 if N <= 524288 else 1.11e9)
