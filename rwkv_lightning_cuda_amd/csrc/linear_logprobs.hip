@@ -241,6 +241,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void head_tile_kernel(HeadArgs 
         for (int v = 0; v < 16; ++v) a.m = fmaxf(a.m, z[nb][v]);
       }
     const float to_log2 = xs * kLog2e;
+    float all = 0.0f;
 #pragma unroll
     for (int nb = 0; nb < 2; ++nb)
       if (col0 + nb * 32 < g.N) {
@@ -248,10 +249,23 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void head_tile_kernel(HeadArgs 
         for (int v = 0; v < 16; ++v) {
           const float d = z[nb][v] - a.m;
           const float p = __builtin_amdgcn_exp2f(d * to_log2);
-          a.s += p;
-          a.u = fmaf(fmaxf(d, kLowest), p, a.u);
+          all += p;
+          a.s += __builtin_amdgcn_fractf(p);  // (p, but for the largest ones' 1: as add() keeps them apart)
+          a.u = fmaf(d, p, a.u);
         }
       }
+    if (__any(a.u != a.u && all == all)) {  // a d of -infinity, whose p is 0
+      a.u = 0.0f;
+#pragma unroll
+      for (int nb = 0; nb < 2; ++nb)
+        if (col0 + nb * 32 < g.N) {
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const float d = z[nb][v] - a.m;
+            a.u = fmaf(fmaxf(d, kLowest), __builtin_amdgcn_exp2f(d * to_log2), a.u);
+          }
+        }
+    }
     const int t = g.tokens && live ? g.tokens[row] - col0 : -1;
     if (t >= 0 && t < 64 && ((t >> 2) & 1) == h && col0 + t < g.N) {
       float zt = 0.0f;
@@ -266,10 +280,7 @@ __global__ __launch_bounds__(64 * kTileWaves, 2) void head_tile_kernel(HeadArgs 
       a.m *= xs;
       a.u *= xs;
     }
-    if (a.s >= 1.0f) {  // (the largest's own 1)
-      a.s -= 1.0f;
-      a.n = 1.0f;
-    }
+    a.n = rintf(all - a.s);
     int first = g.N;
     if (!LOGITS && g.firsts) {
 #pragma unroll
