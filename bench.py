@@ -75,6 +75,8 @@ def parse_args():
                          "rocprofv3 --pmc FETCH_SIZE / WRITE_SIZE readings are scaled by")
     ap.add_argument("--wkv7-op-only", action="store_true", help="only run the WKV7 op at the long-context configuration "
                     "(B 16, T 16384, 64 heads; two calls) and exit: the target of rocprofv3 counter runs")
+    ap.add_argument("--score-only", action="store_true", help="only time a scored pass (16 texts x 128 tokens of --preset, --fmt: "
+                    "forward, scored, with five alternatives, with the head's input in 8 bits) and exit")
     ap.add_argument("--no-cpu-baseline", action="store_true")
     ap.add_argument("--no-roofline", action="store_true")
     ap.add_argument("--fused-ln", type=int, default=-1, help="tuning hook: 1 / 0 force LayerNorm inside / outside the linear "
@@ -305,6 +307,46 @@ def wkv7_op_long_context(hip, H, reps=3):
     return res["wkv7_op"]
 
 
+def scored_pass(hip, model, dims, B=16, T=128, reps=10):
+    """Session.score against Session.forward on B texts of T tokens, one call each, ms: the median of `reps`, each kind of pass in turn.  int8
+    heads: also with the head's input in 8 bits, and how far its log probabilities are off."""
+    from rwkv_lightning_cuda_amd.model import Session, State
+
+    rng = np.random.default_rng(0)
+    tokens, targets = rng.integers(0, dims.V, (B, T)), rng.integers(0, dims.V, (B, T))
+    logits = hip.DeviceArray((B, dims.V), np.float32)
+    logprob, entropy = hip.DeviceArray((B * T,), np.float32), hip.DeviceArray((B * T,), np.float32)
+    ids, tops = hip.DeviceArray((B * T, 5), np.int32), hip.DeviceArray((B * T, 5), np.float32)
+    sess = Session(model)
+
+    def score(state, top=0, int8=False):
+        sess.score(tokens, targets, state, logprob, entropy, top, ids if top else None, tops if top else None, act_int8=int8)
+
+    passes = {"forward": lambda s: sess.forward(tokens, s, logits), "scored": score, "scored_top5": lambda s: score(s, 5)}
+    if model.mats[-1, hip.M_HEAD].fmt == hip.FMT_W8:
+        passes["scored_int8_head"] = lambda s: score(s, 0, True)
+        passes["scored_int8_head_top5"] = lambda s: score(s, 5, True)
+    times = {name: [] for name in passes}
+    values = {}
+    for rep in range(reps + 2):
+        for name, run in passes.items():
+            state = State(dims, B)
+            hip.device_sync()
+            t = time.perf_counter()
+            run(state)
+            t = time.perf_counter() - t
+            if rep >= 2:
+                times[name].append(t * 1e3)
+            values[name] = logprob.numpy().copy()
+    ms = {name: float(np.median(t)) for name, t in times.items()}
+    res = {"workload": "%d texts x %d tokens, one call from an empty state" % (B, T), "ms": ms, "scored_tok_s": B * T / (ms["scored"] * 1e-3)}
+    if "scored_int8_head" in values:
+        off = values["scored_int8_head"] - values["scored"]
+        res["int8_head_logprobs_off"] = {"rms": float(np.sqrt(np.mean(off * off))), "max": float(np.abs(off).max())}
+    sess.close()
+    return res
+
+
 def secondary_measurements(hip, model, dims, rng):
     """Batch-1, -2, -4, -8, -16 and -64 decode of the same model (128-token prefill per row, 64 timed steps) and the WKV7
     op alone."""
@@ -498,6 +540,9 @@ def main():
     B = args.batch
 
     model = HipModel.random_on_device(dims, fmt, seed=1)
+    if args.score_only:
+        print(json.dumps({"scored_pass": dict(scored_pass(hip, model, dims), preset=args.preset, fmt=args.fmt)}))
+        return
     sess = Session(model)
     if args.no_graph:
         sess.set_graph(False)
