@@ -1,6 +1,6 @@
 // The vocabulary's product with the log probabilities of its logits: z[M,N] = x[M,K] . W[N,K]^T in fp32 (not rounded to fp16 as the
 // logits of a forward pass are), then what logprobs.hip makes of the rows.  x fp16 with fp16 or int8 weights, or int8 codes with a
-// scale per row and int8 weights (products in whole numbers, exact in 32 bits up to K = 133152: 127 * 127 K < 2^31).
+// scale per row and int8 weights (products in whole numbers, exact in 32 bits: 128 * 128 K < 2^31 up to K = 131071).
 // Reference: the head product alone (src/rwkv7_fast_v4.cu:1325-1341).
 #include <algorithm>
 #include <utility>
@@ -186,8 +186,8 @@ __global__ __launch_bounds__(kFewThreads) void head_few_kernel(HeadArgs g, int l
 // LOGITS: also the largest of each 64 columns, and the logits of those 64 where that is not below the row's bound.  ONE: one tile of
 // rows, whose weights no other block reads.
 // What bounds it: the chip's power, as the packed product (matrix core busy 51 % of the time at 1.95 GHz); the sums take about a tenth.
-// 2048 rows of 4096 int8, 65536 columns: 495 us, 2.2 P operations/s (a plain product of 8192 x 8192 x 8192 reaches 2.08 on this card); fp16
-// 955 us, 1.15 PFLOP/s.  Through blocks of 256 rows of logits in memory the int8 case with 5 alternatives took 798 us, so 550.
+// 2048 rows of 4096 int8, 65536 columns: 499 to 522 us on several cards, 2.1 to 2.2 P operations/s (a plain product of 8192 x 8192 x 8192
+// reaches 2.08); fp16 979 us, 1.12 PFLOP/s.  Through blocks of 256 rows of logits in memory the int8 case with 5 alternatives took 798 us, so 550.
 template <int TYPES, int MT, bool LOGITS, bool ONE>
 __global__ __launch_bounds__(64 * kTileWaves, 2) void head_tile_kernel(HeadArgs g) {
   typedef Types<TYPES> T;

@@ -424,6 +424,7 @@ def add_norm_q8(rows, C, x, res, w, b, q, scale, x_out=None, norm=NORM_LAYER, ep
 
 
 def token_logprobs_workspace(rows, V, top_n=0):
+    """Bytes that serve every call of up to `rows` rows."""
     n = ctypes.c_size_t(0)
     check(load().rwkv_hip_token_logprobs_workspace(_i(rows), _i(V), _i(top_n), ctypes.byref(n)))
     return n.value
@@ -438,6 +439,7 @@ def token_logprobs(rows, V, logits, tokens, workspace=None, logprob=None, entrop
 
 
 def linear_logprobs_workspace(fmt, M, N, K, top_n=0, x_int8=False):
+    """Bytes that serve every call of up to M rows."""
     n = ctypes.c_size_t(0)
     check(load().rwkv_hip_linear_logprobs_workspace(_i(fmt), _i(1 if x_int8 else 0), _i(M), _i(N), _i(K), _i(top_n), ctypes.byref(n)))
     return n.value
