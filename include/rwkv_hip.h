@@ -91,6 +91,18 @@ int rwkv_hip_stream_wait_event(rwkv_stream_t s, void* ev);
  * at batch 1 is such a chain (8 launches per layer); this is the part of its time that no kernel can remove. */
 int rwkv_hip_measure_launch_chain(int links, int blocks, int threads, int use_graph, int reps, float* us_per_link);
 
+/* Rows of up to 8 tensors copied, forked, exchanged and cleared in one launch: what a cache of generation states needs when sequences
+ * branch, end and make room (ModelBackend::copy_state_slice, src/rwkv7_fast_v4.cu:1421-1504, moves a run of rows with a copy for every
+ * layer and tensor).  Tensor t is [planes_host[t], rows, row_bytes_host[t]] without gaps, from src_host[t] with src_rows rows to
+ * dst_host[t] with dst_rows; shift f16 [L,2,B,C] is 2 L planes of rows of 2 C bytes, wkv L planes, elapsed and penalties one.  The n
+ * (0 .. 512) moves are the same in every plane: row to_host[i] becomes what row from_host[i] was before the call (of several destinations
+ * each), or zeros where that is -1.  Other rows stay as they are.  All lists are host arrays and are read before the call returns.
+ * In place: dst_host[t] == src_host[t] for every t and dst_rows == src_rows; any moves are allowed, also onto one another's sources.
+ * Otherwise no destination may overlap a source or another destination.  A row may be a destination once.  Up to 65534 rows; any
+ * sizes and alignment (multiples of 16 bytes are fastest).  A captured call keeps its rows. */
+int rwkv_hip_copy_rows(rwkv_stream_t s, int tensors, void* const* dst_host, const void* const* src_host, const int64_t* planes_host,
+                       const int64_t* row_bytes_host, int dst_rows, int src_rows, int n, const int32_t* to_host, const int32_t* from_host);
+
 /* ---- WKV7 time-mix recurrence.  Replaces rwkv7_wkv_fp32io16_launch
  * (cuda/rwkv7_fast_v4_kernels.cuh:49-52, cuda/rwkv7_wkv_fp32_v2.cu:237-294).
  * state f32 [B,H,64,64] in/out; r,w,k,v,a,b,y [B,T,C], C == H*64.
@@ -290,6 +302,32 @@ int rwkv_hip_sample(rwkv_stream_t s, int B, int V, const void* logits, void* pen
                     double top_p, uint64_t seed, uint64_t step);
 /* lm_head -> argmax without the sampler: out i32 [B] = lowest index of the row maximum */
 int rwkv_hip_argmax(rwkv_stream_t s, int B, int V, const void* logits, void* out);
+
+/* One token per row, drawn with a given random number under filters of the row's own (no counterpart in the reference, whose sampler has
+ * one set of options for a batch and a generator of its own).  logits [logit_rows,V] of type io, rows ld >= V entries apart, any alignment
+ * of their type; row i draws from row source[i] (i32 [rows]; NULL: from row i), so several may draw from one.  Each of the following
+ * is a device tensor [rows] or NULL, which is the value in brackets:
+ *   temperature f32 (1)   0: the largest entry, the first of equal ones; +infinity: all entries alike
+ *   top_k i32 (0)         <= 0 or >= V: off
+ *   top_p f32 (1)         >= 1: off;  <= 0: the first entry
+ *   min_p f32 (0)         <= 0: off;  >= 1: the entries that equal the largest
+ * uniform f32 [rows] in 0 .. 1.  With z = logit - penalty in fp32, m = max z, e_i = exp((z_i - m) / temperature) (0 where that is below
+ * 2^-1000) and the order "larger z first, equal ones by index", the kept entries are the first min(top_k, the least number whose e sum
+ * to top_p of all, the number with e_i >= min_p), at least one.  token i32 [rows] is the first kept entry, by index, up to which the kept
+ * ones' sum is above uniform times their whole sum (1: the last one); logprob f32 [rows] (may be NULL) its log probability among
+ * the kept ones.  Powers and sums are in 64 bits in a fixed order: a call repeats bitwise, and a row's results depend neither on
+ * the other rows nor on its place among them.  Entries of -infinity are never drawn.  A row without a distribution - nothing but -infinity, a
+ * NaN or +infinity among its entries, a parameter that is NaN or negative (temperature, uniform), uniform above 1, a source outside
+ * 0 .. logit_rows - 1 - gets the token -1 and logprob 0.
+ * penalties f32 [rows,V] (NULL: none) are subtracted; penalties_out (NULL: not wanted; may be penalties) receives p * decay, plus, at the
+ * token, presence where p was 0 and frequency elsewhere (f32 [rows] each, NULL: 1, 0, 0): rwkv_hip_sample's rule.
+ * V <= 1048576.  The workspace (rwkv_hip_draw_tokens_workspace bytes, aligned to 16) need not be cleared; calls that share one must not
+ * overlap; one for some rows serves every call of that V with as many rows or fewer. */
+int rwkv_hip_draw_tokens_workspace(int rows, int V, size_t* bytes);
+int rwkv_hip_draw_tokens(rwkv_stream_t s, int rows, int V, int io, const void* logits, int64_t ld, int logit_rows, const void* source,
+                         const void* temperature, const void* top_k, const void* top_p, const void* min_p, const void* uniform,
+                         const void* penalties, const void* presence, const void* frequency, const void* decay, void* penalties_out,
+                         void* token, void* logprob, void* workspace, size_t workspace_bytes);
 
 /* Log probabilities of given tokens (no counterpart in the reference; what `logprobs` and `echo` of a server and the scoring of a text
  * ask for).  logits [rows,V] of type io (RWKV_IO_F32 / RWKV_IO_F16), rows ld >= V entries apart, any alignment of their type;

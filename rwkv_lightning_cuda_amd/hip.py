@@ -48,6 +48,7 @@ EXPORTS = [
     "rwkv_hip_add_layer_norm_cmix_mix", "rwkv_hip_add_layer_norm_tmix_mix6", "rwkv_hip_kk_a_gate",
     "rwkv_hip_lnx_rkvres_xg", "rwkv_hip_relu_square", "rwkv_hip_add_vec", "rwkv_hip_f16_to_f32",
     "rwkv_hip_advance_i32", "rwkv_hip_sample", "rwkv_hip_argmax", "rwkv_hip_add_norm_q8",
+    "rwkv_hip_draw_tokens_workspace", "rwkv_hip_draw_tokens", "rwkv_hip_copy_rows",
     "rwkv_hip_token_logprobs_workspace", "rwkv_hip_token_logprobs", "rwkv_hip_linear_logprobs_workspace", "rwkv_hip_linear_logprobs",
     "rwkv_hip_model_create", "rwkv_hip_model_destroy",
     "rwkv_hip_model_set_tensor", "rwkv_hip_model_set_matrix", "rwkv_hip_model_weight_bytes",
@@ -62,6 +63,8 @@ EXPORTS = [
 _P, _N, _L, _S = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
 _ARGTYPES = {
     "rwkv_hip_add_norm_q8": [_P, _N, _N, _N, _P, _P, _P, _P, ctypes.c_float, _P, _P, _P],
+    "rwkv_hip_draw_tokens": [_P, _N, _N, _N, _P, _L, _N] + [_P] * 14 + [_S],
+    "rwkv_hip_copy_rows": [_P, _N, _P, _P, _P, _P, _N, _N, _N, _P, _P],
     "rwkv_hip_token_logprobs": [_P, _N, _N, _N, _P, _L, _P, _N, _P, _P, _P, _P, _P, _P, _S],
     "rwkv_hip_linear_logprobs": [_P, _N, _N, _N, _N, _P, _P, _P, _P, _P, _N, _P, _P, _P, _P, _P, _S],
 }
@@ -421,6 +424,37 @@ def argmax(B, V, logits, out, stream=None):
 def add_norm_q8(rows, C, x, res, w, b, q, scale, x_out=None, norm=NORM_LAYER, eps=1e-5, stream=None):
     """Residual addition (res None: none), norm and int8 codes with a scale per row; x_out receives the sum."""
     check(load().rwkv_hip_add_norm_q8(_a(stream), int(rows), int(C), int(norm), _a(x), _a(res), _a(w), _a(b), eps, _a(x_out), _a(q), _a(scale)))
+
+
+def draw_tokens_workspace(rows, V):
+    """Bytes that serve every call of up to `rows` rows."""
+    n = ctypes.c_size_t(0)
+    check(load().rwkv_hip_draw_tokens_workspace(_i(rows), _i(V), ctypes.byref(n)))
+    return n.value
+
+
+def draw_tokens(rows, V, logits, uniform, token, workspace, logprob=None, temperature=None, top_k=None, top_p=None, min_p=None, source=None,
+                logit_rows=None, penalties=None, presence=None, frequency=None, decay=None, penalties_out=None, io=IO_F32, ld=None, stream=None):
+    """A token per row by uniform f32 [rows] under the row's own temperature, top_k, top_p and min_p (device tensors [rows], None: 1, off);
+    row i draws from logits row source[i] of logit_rows (None: its own); penalties_out receives the penalties after the token."""
+    check(load().rwkv_hip_draw_tokens(_a(stream), int(rows), int(V), int(io), _a(logits), int(V if ld is None else ld),
+                                      int(rows if logit_rows is None else logit_rows), _a(source), _a(temperature), _a(top_k), _a(top_p), _a(min_p),
+                                      _a(uniform), _a(penalties), _a(presence), _a(frequency), _a(decay), _a(penalties_out), _a(token),
+                                      _a(logprob), _a(workspace), workspace.nbytes if workspace is not None else 0))
+
+
+def copy_rows(tensors, dst_rows, src_rows, to, rows, stream=None):
+    """Row to[i] of every tensor becomes its row rows[i] (-1: zeros).  tensors: (destination, source, planes, bytes of a row) each, laid out
+    [planes, rows, bytes]; destination and source the same: in place."""
+    k, n = len(tensors), len(to)
+    if len(rows) != n:
+        raise ValueError("as many sources as destinations")
+    pointers = ctypes.c_void_p * k
+    sizes = ctypes.c_int64 * k
+    numbers = ctypes.c_int32 * n
+    check(load().rwkv_hip_copy_rows(_a(stream), k, pointers(*[_a(t[0]) for t in tensors]), pointers(*[_a(t[1]) for t in tensors]),
+                                    sizes(*[int(t[2]) for t in tensors]), sizes(*[int(t[3]) for t in tensors]), int(dst_rows), int(src_rows), n,
+                                    numbers(*[int(d) for d in to]), numbers(*[int(r) for r in rows])))
 
 
 def token_logprobs_workspace(rows, V, top_n=0):
