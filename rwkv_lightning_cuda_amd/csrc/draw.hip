@@ -27,7 +27,7 @@ namespace rwkv {
 namespace {
 
 constexpr int kSlot = 64;
-constexpr int kStatsThreads = 256;
+constexpr int kPart = 4096;      // entries of a block of draw_stats_kernel
 constexpr int kPickThreads = 1024;
 constexpr int kWideThreads = 1024;
 constexpr int kPickList = 4096;  // entries
@@ -36,18 +36,18 @@ constexpr int kBuckets = 256;    // of a histogram
 constexpr int kLast = 64;        // entries that one wavefront puts in order
 constexpr int kWaveSlots = 256;  // slots of a wavefront that reach the bound
 constexpr int kHeld = 8;         // of these, those whose entries it keeps in registers
-constexpr int kMost = 256;       // of a block: a list of more slots takes longer to make than the search for a window
-constexpr int kChunk = 64;       // slots of a wavefront in find_window: one entry of each a lane
-constexpr int kWindow = kWideList * 3 / 4;  // entries that find_window narrows a row down to
+constexpr int kMost = 256;       // of a block: with more of them the histograms say more than a list of their entries
+constexpr int kGrid = 4;         // buckets of the parts' histograms in an octave
+constexpr int kListed = 256;     // a top_k up to which a row needs no histograms
+constexpr double kOne = 2251799813685248.0;  // 2^51: a part holds 2^12 powers of at most 1
 constexpr double kLog2eD = 1.44269504088896340736;
 constexpr double kLowestPower = -1000.0;  // octaves
 constexpr double kWidest = 64.0;          // octaves that the first histogram covers
 
 // What draw_pick_kernel hands on of a row with more candidates than its list holds
 struct WideRow {
-  double mass;            // what top_p holds; +infinity: no top_p
+  double mass;  // what top_p holds; +infinity: no top_p
   float m;
-  float lowest, highest;  // powers: no candidate lies below, and the cut not above
   int waits;
 };
 
@@ -64,9 +64,15 @@ struct DrawArgs {
   const float* penalties;  // [rows,V]
   int* token;
   float* logprob;
-  double* slot_sum;  // [rows,slots]
-  float* slot_max;   // [rows,slots]
-  WideRow* wide;     // [rows]
+  // what draw_stats_kernel leaves: the largest entry of every slot and part, the sum of a slot's powers against its part's largest, and
+  // for some rows the parts' histograms: powers (times kOne) and numbers of the entries
+  int parts;
+  double* slot_sum;                // [rows,slots]
+  unsigned long long* part_mass;   // [rows,parts,kBuckets]
+  WideRow* wide;                   // [rows]
+  float* slot_max;                 // [rows,slots]
+  float* part_max;                 // [rows,parts]
+  unsigned* part_count;            // [rows,parts,kBuckets]
 };
 
 // a value that every lane holds, in scalar registers
@@ -87,6 +93,8 @@ struct Wish {
   __device__ __forceinline__ bool free() const { return top_k == INT_MAX && top_p >= 1.0 && min_p <= 0.0; }
   __device__ __forceinline__ bool likely(double e) const { return !(min_p > 0.0) || e >= min_p; }
   __device__ __forceinline__ bool needs_sum() const { return !greedy && (top_p < 1.0 || free()); }
+  // (a list of top_k entries, and of the rest of their slots, is short)
+  __device__ __forceinline__ bool needs_histogram() const { return !greedy && !free() && top_k > kListed; }
 };
 __device__ __forceinline__ Wish wish_of(const DrawArgs& a, int row) {
   Wish w;
@@ -228,20 +236,28 @@ __device__ __forceinline__ void each_entry(const Row<T>& r, int first_slot, int 
   }
 }
 
-// A block takes kStatsThreads * 4 * NV entries of a row, 16 lanes a slot.  VEC: four entries are one aligned load.
-template <typename T, bool VEC, int NV>
-__global__ __launch_bounds__(kStatsThreads) void draw_stats_kernel(DrawArgs a) {
+// The buckets of the parts' histograms: places on one grid of kGrid to an octave, counted down from the largest entry's, so that those of
+// different parts fit together; the last one holds whatever lies lower.
+__device__ __forceinline__ double grid_place(float z, double octaves) { return floor(static_cast<double>(z) * (octaves * kGrid)); }
+
+// A block takes a part of a row in NT threads, 16 lanes a slot.  VEC: four entries are one aligned load.
+template <typename T, bool VEC, int NT>
+__global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
+  constexpr int NV = kPart / 4 / NT;
   typedef T vec_t __attribute__((ext_vector_type(4)));
-  const int row = blockIdx.x;
+  __shared__ float most[NT / 64];
+  __shared__ unsigned long long mass[kBuckets];
+  __shared__ unsigned count[kBuckets];
+  const int row = blockIdx.x, part = blockIdx.y;
   const Wish w = wish_of(a, row);
   if (!w.valid) return;
   const Row<T> r = row_of<T>(a, row, w.source);
-  const bool sums = w.needs_sum();
-  const int first = (blockIdx.y * kStatsThreads * NV + threadIdx.x) * 4;
+  const bool sums = w.needs_sum(), histogram = w.needs_histogram(), counts = w.top_k != INT_MAX;
+  const int first = part * kPart + threadIdx.x * 4;
   float z[NV][4];
 #pragma unroll
   for (int q = 0; q < NV; ++q) {
-    const int i = first + q * kStatsThreads * 4;
+    const int i = first + q * NT * 4;
     if (VEC && i + 4 <= a.V) {
       const vec_t l = *reinterpret_cast<const vec_t*>(r.logits + i);
 #pragma unroll
@@ -253,29 +269,70 @@ __global__ __launch_bounds__(kStatsThreads) void draw_stats_kernel(DrawArgs a) {
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) z[q][j] = r.at(i + j);
+      for (int j = 0; j < 4; ++j) z[q][j] = r.logit(min(i + j, a.V - 1));
+      if (r.penalties) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) z[q][j] -= r.penalty(min(i + j, a.V - 1));
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) z[q][j] = i + j < a.V ? z[q][j] : -INFINITY;
     }
   }
+  if (histogram) {
+    for (int b = threadIdx.x; b < kBuckets; b += NT) {
+      mass[b] = 0;
+      count[b] = 0;
+    }
+  }
+  float m = -INFINITY;
 #pragma unroll
   for (int q = 0; q < NV; ++q) {
-    const int slot = (first + q * kStatsThreads * 4) / kSlot;
-    float m = -INFINITY;
+    const int slot = (first + q * NT * 4) / kSlot;
+    float mq = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) m = fmaxf(m, z[q][j] < INFINITY ? z[q][j] : INFINITY);  // (a NaN counts as +infinity: no distribution)
-    m = fmaxf(m, __builtin_bit_cast(float, lane_xor_dpp<8>(__builtin_bit_cast(int, m))));
-    m = fmaxf(m, __builtin_bit_cast(float, lane_xor_dpp<4>(__builtin_bit_cast(int, m))));
-    m = fmaxf(m, __builtin_bit_cast(float, lane_xor_dpp<2>(__builtin_bit_cast(int, m))));
-    m = fmaxf(m, __builtin_bit_cast(float, lane_xor_dpp<1>(__builtin_bit_cast(int, m))));
+    for (int j = 0; j < 4; ++j) mq = fmaxf(mq, z[q][j] < INFINITY ? z[q][j] : INFINITY);  // (a NaN counts as +infinity: no distribution)
+    mq = fmaxf(mq, __builtin_bit_cast(float, lane_xor_dpp<8>(__builtin_bit_cast(int, mq))));
+    mq = fmaxf(mq, __builtin_bit_cast(float, lane_xor_dpp<4>(__builtin_bit_cast(int, mq))));
+    mq = fmaxf(mq, __builtin_bit_cast(float, lane_xor_dpp<2>(__builtin_bit_cast(int, mq))));
+    mq = fmaxf(mq, __builtin_bit_cast(float, lane_xor_dpp<1>(__builtin_bit_cast(int, mq))));
+    if ((threadIdx.x & 15) == 0 && slot < a.slots) a.slot_max[static_cast<int64_t>(row) * a.slots + slot] = mq;
+    m = fmaxf(m, mq);
+  }
+  if (!sums && !histogram) return;
+  m = wave_reduce_dpp(m, [](float x, float y) { return fmaxf(x, y); });
+  if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NT / 64; ++i) m = fmaxf(m, most[i]);
+  m = scalar(m);
+  const int64_t at = static_cast<int64_t>(row) * a.parts + part;
+  if (threadIdx.x == 0) a.part_max[at] = m;
+  const double top = scalar(grid_place(m, w.octaves));
+#pragma unroll
+  for (int q = 0; q < NV; ++q) {
+    const int slot = (first + q * NT * 4) / kSlot;
     double sum = 0.0;
-    if (sums) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum += weight(z[q][j], m, w.octaves);
-      sum = row16_sum_d(sum);
+    for (int j = 0; j < 4; ++j) {
+      const double e = weight(z[q][j], m, w.octaves);
+      sum += e;
+      if (histogram && z[q][j] > -INFINITY && m < INFINITY) {
+        const int b = static_cast<int>(fmin(top - grid_place(z[q][j], w.octaves), static_cast<double>(kBuckets - 1)));
+        // (2^52 + e 2^51, rounded: its last 52 bits)
+        atomicAdd(&mass[b], __builtin_bit_cast(unsigned long long, fma(e, kOne, 2.0 * kOne)) - 0x4330000000000000ull);
+        if (counts) atomicAdd(&count[b], 1u);
+      }
     }
-    if ((threadIdx.x & 15) == 0 && slot < a.slots) {
-      const int64_t at = static_cast<int64_t>(row) * a.slots + slot;
-      a.slot_max[at] = m;
-      if (sums) a.slot_sum[at] = sum;
+    if (sums) {
+      sum = row16_sum_d(sum);
+      if ((threadIdx.x & 15) == 0 && slot < a.slots) a.slot_sum[static_cast<int64_t>(row) * a.slots + slot] = sum;
+    }
+  }
+  if (histogram) {
+    __syncthreads();
+    for (int b = threadIdx.x; b < kBuckets; b += NT) {
+      a.part_mass[at * kBuckets + b] = mass[b];
+      if (counts) a.part_count[at * kBuckets + b] = count[b];
     }
   }
 }
@@ -286,15 +343,14 @@ struct Shared {
   static constexpr int kWaves = NW, kList = LIST;
   double d[NW], d2[NW], total[NW], chunk[NW];
   float f[NW], f2[NW], most[NW], least[NW];
-  int i[NW], reach[NW], entries[NW], counted[2][NW];
-  float summed[2][NW];
+  int i[NW], reach[NW], entries[NW];
   unsigned count[kBuckets];
   unsigned long long mass[kBuckets];
   float last_z[kLast];
   int last_i[kLast];
   alignas(8) float list_z[LIST];  // entries in order of their indexes
   int list_i[LIST];
-  int bucket, missed, bucket_count, at, slot;
+  int bucket, bucket_count, at, slot;
   double above_mass, before;
   float cut_z;
   int cut_i;
@@ -709,7 +765,8 @@ __global__ __launch_bounds__(kPickThreads) void draw_pick_kernel(DrawArgs a) {
     return;
   }
 
-  const auto slot_share = [&](int s) { return slot_sum[s] * weight(slot_max[s], m, w.octaves); };
+  const float* part_max = a.part_max + static_cast<int64_t>(row) * a.parts;
+  const auto slot_share = [&](int s) { return slot_sum[s] * weight(part_max[s / (kPart / kSlot)], m, w.octaves); };
   double mine = 0.0;
 
   if (w.free()) {
@@ -773,8 +830,7 @@ __global__ __launch_bounds__(kPickThreads) void draw_pick_kernel(DrawArgs a) {
   if (wave == 0) {
     // Bucket b bounds the kept entries if, of the entries up to it, there are top_k (as many slots reach it), or top_p (what is in other
     // slots, and what their own entries below the bucket can hold at most, or all entries of the row, is less than the rest), or all that
-    // min_p keeps.  It lies above
-    // the cut if all entries of the slots that reach it are too few, and hold too little.
+    // min_p keeps.
     constexpr int kPer = kBuckets / 64;
     const double spare = (1.0 - w.top_p) * total - 1e-8 * total;
     const double unlikely = w.min_p > 0.0 ? 1e-3 - __builtin_amdgcn_logf(static_cast<float>(w.min_p)) : INFINITY;
@@ -789,7 +845,7 @@ __global__ __launch_bounds__(kPickThreads) void draw_pick_kernel(DrawArgs a) {
     const double held_upto = wave_upto(held);
     int at = upto - slots;
     double at_held = held_upto - held;
-    int bound = kBuckets - 1, missed = -1;
+    int bound = kBuckets - 1;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const int b = lane * kPer + j;
@@ -798,14 +854,9 @@ __global__ __launch_bounds__(kPickThreads) void draw_pick_kernel(DrawArgs a) {
       bool enough = at >= w.top_k || (b + 1) * width > unlikely;
       if (summed) enough |= fmin(total - at_held + static_cast<double>(at) * kSlot * edge(b) * 1.001, a.V * 1.001 * edge(b)) <= spare;
       if (enough) bound = min(bound, b);
-      if (at < w.top_k / kSlot && (!summed || at_held < 0.999 * cut.mass)) missed = b;
     }
     bound = wave_reduce_dpp(bound, [](int x, int y) { return min(x, y); });
-    missed = wave_reduce_dpp(missed, [](int x, int y) { return max(x, y); });
-    if (lane == 0) {
-      sh.bucket = bound;
-      sh.missed = missed;
-    }
+    if (lane == 0) sh.bucket = bound;
   }
   __syncthreads();
   const int bound = scalar(sh.bucket);
@@ -857,8 +908,7 @@ __global__ __launch_bounds__(kPickThreads) void draw_pick_kernel(DrawArgs a) {
   }
   n = scalar(n);
   if (!fits || n > kPickList) {
-    if (tid == 0)
-      a.wide[row] = {cut.mass, m, bound < kBuckets - 1 ? edge(bound) * 0.999f : 0.0f, sh.missed >= 0 ? edge(sh.missed) * 1.001f : 1.0001f, 1};
+    if (tid == 0) a.wide[row] = {cut.mass, m, 1};
     return;
   }
   const auto put = [&](float z, int slot) {
@@ -890,233 +940,185 @@ __global__ __launch_bounds__(kPickThreads) void draw_pick_kernel(DrawArgs a) {
 
 // ---- rows with more candidates than a list holds -----------------------------------------------------------------------
 constexpr int kWideWaves = kWideThreads / 64;
+constexpr int kMaxParts = kMaxLogprobVocab / kPart;
 struct WideShared : Shared<kWideWaves, kWideList> {
-  float queue[kWideWaves][128];
+  double part_scale[kMaxParts];  // a part's largest power, by kOne
+  double part_above[kMaxParts];  // and what the buckets in front of the window hold of it
+  int part_shift[kMaxParts];     // the part's first bucket, among the row's
+  double held[kBuckets];
+  int first, last;               // buckets of the window
 };
 static_assert(kMaxLogprobVocab / kSlot / kWideWaves <= kWideList / 2, "the sums of a chunk's slots lie where the list was");
 
-struct WindowOut {
-  Span span;
-  int n;              // entries in the list
-  int mine, mine_at;  // of them, this wavefront's
-  double kept_above;  // and its kept entries above them, by lanes
-};
+// The smallest float whose place on the grid is at least `place`; false: not found next to where it should be
+__device__ __forceinline__ bool grid_edge(double place, double octaves, float& z) {
+  z = octaves > 0.0 ? static_cast<float>(fmin(fmax(place / (octaves * kGrid), -static_cast<double>(FLT_MAX)), static_cast<double>(FLT_MAX))) : -FLT_MAX;
+  int left = 16;
+  while (grid_place(z, octaves) >= place && z > -FLT_MAX && left > 0) {
+    z = nextafterf(z, -INFINITY);
+    --left;
+  }
+  while (grid_place(z, octaves) < place && z < FLT_MAX && left > 0) {
+    z = nextafterf(z, INFINITY);
+    --left;
+  }
+  return left > 0;
+}
 
-enum class Window { kNone, kAll, kFound };
-
-// For rows with many candidates: a window of values about the cut that fits the list.  Every thread keeps fp32 powers of its entries
-// in registers, and the block halves the range of powers from `lowest` to `highest` by counting and summing, as long as fp32 tells on which
-// side the cut lies.  What lies above the window is then counted and summed in 64 bits, and the window's entries go to the list, in order.
-// (The caller finds out whether the cut lies inside.)  kAll: no candidate lies behind the cut.  kNone: nothing is found.
-// Halving takes 4 to 7 steps between the bounds that the slots give, a straight line through the sums two more.
+// A window of the row's values about the cut, from the parts' histograms: its entries go to the list, in order; what lies above it is known
+// from the histograms, for the row and for every wavefront's chunk of it.  False where they do not tell: nothing is changed but the list.
 template <typename T>
-__device__ __forceinline__ Window find_window(WideShared& sh, const Row<T>& r, int c0, int c1, const Wish& w, const Cut& cut, const WideRow& wide,
-                                              WindowOut& out) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const float m = wide.m;
-  const float octaves = fminf(static_cast<float>(w.octaves), 1e30f);
-  const float mass = static_cast<float>(cut.mass);
-  constexpr float kUnsure = 2e-5f;  // of a sum: the powers are good to 3e-6 down to 2^-64, and as many additions to as much
-  const auto reached = [&](int n, float held) { return n >= cut.top_k || held >= mass * (1.0f + kUnsure); };
-  const auto missed = [&](int n, float held) { return n < cut.top_k && held < mass * (1.0f - kUnsure); };
-  uint32_t lo = __builtin_bit_cast(uint32_t, fmaxf(wide.lowest, 0x1p-120f)), hi = __builtin_bit_cast(uint32_t, wide.highest);
-  if (lo >= hi) return Window::kAll;
-  float x[kChunk];
-  const int first = c0 * kSlot + lane, end = min(c1 * kSlot, r.V);
-  constexpr int kAhead = 16;  // (more loads at once, and their addresses need the registers of the entries)
-#pragma unroll
-  for (int g = 0; g < kChunk; g += kAhead) {
-    r.template load<kAhead>(first + g * kSlot, x, g);
-#pragma unroll
-    for (int k = g; k < g + kAhead; ++k) x[k] = first + k * kSlot < end ? __builtin_amdgcn_exp2f((x[k] - m) * octaves) : 0.0f;
-    __builtin_amdgcn_sched_barrier(0);
+__device__ __forceinline__ bool find_window(const DrawArgs& a, WideShared& sh, const Row<T>& r, int row, int c0, int c1, const Wish& w, const Cut& cut,
+                                            float m, Span& span, int& n, double& kept_above) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const double top = grid_place(m, w.octaves);
+  const float* part_max = a.part_max + static_cast<int64_t>(row) * a.parts;
+  const unsigned long long* part_mass = a.part_mass + static_cast<int64_t>(row) * a.parts * kBuckets;
+  const unsigned* part_count = a.part_count + static_cast<int64_t>(row) * a.parts * kBuckets;
+  const bool counts = w.top_k != INT_MAX;
+  for (int p = tid; p < a.parts; p += kWideThreads) {
+    const float mp = part_max[p];
+    sh.part_scale[p] = weight(mp, m, w.octaves) / kOne;
+    sh.part_shift[p] = mp > -INFINITY ? static_cast<int>(fmin(top - grid_place(mp, w.octaves), static_cast<double>(kBuckets))) : kBuckets;
   }
-  // (one place in the code that counts, whatever for: unrolled over 64 registers it is 2 KB, and instructions that are executed once cost
-  // their way from memory)
-  const bool by_mass = cut.mass < INFINITY, by_count = cut.top_k != INT_MAX;
-  enum { kLow, kHalve, kBelow, kAbove } state = kLow;
-  constexpr uint32_t kNear = 1u << 15;  // 2^-8 of a value
-  uint32_t at = lo, mid = 0, d = 0;
-  int n_lo = 0, n_hi = 0, turn = 0;
-  float held_lo = 0.0f, held_hi = 0.0f;
-  // how many entries there can be between the two ends: none weighs less than the lower one
-  const auto between = [&] {
-    const float most = by_mass ? (held_lo - held_hi) / __builtin_bit_cast(float, lo) : INFINITY;
-    return by_count ? fminf(most, static_cast<float>(n_lo - n_hi)) : most;
-  };
-  for (;;) {
-    const float least = __builtin_bit_cast(float, at);
-    int n = 0;
-    float held = 0.0f;
-    if (by_mass) {
-#pragma unroll
-      for (int k = 0; k < kChunk; ++k) held += x[k] >= least ? x[k] : 0.0f;
+  if (tid < kBuckets) {
+    sh.count[tid] = 0;
+    sh.held[tid] = 0.0;
+  }
+  __syncthreads();
+  // the row's histogram: bucket b of a part is its bucket b + shift; the part's last one says nothing but "lower"
+  if (tid < kBuckets - 1) {
+    double held = 0.0;
+    unsigned number = 0;
+#pragma unroll 8
+    for (int p = 0; p < a.parts; ++p) {
+      const int b = tid - sh.part_shift[p];
+      if (b >= 0) {
+        held += static_cast<double>(part_mass[p * kBuckets + b]) * sh.part_scale[p];
+        if (counts) number += part_count[p * kBuckets + b];
+      }
     }
-    if (by_count) {
+    sh.held[tid] = held;
+    sh.count[tid] = number;
+  }
+  __syncthreads();
+  if (wave == 0) {
+    // the bucket of the cut, and of the least entry that min_p keeps (rounding: one more on either side)
+    constexpr int kPer = kBuckets / 64;
+    int number = 0;
+    double held = 0.0;
 #pragma unroll
-      for (int k = 0; k < kChunk; ++k) n += x[k] >= least;
+    for (int j = 0; j < kPer; ++j) {
+      number += sh.count[lane * kPer + j];
+      held += sh.held[lane * kPer + j];
     }
-    held = wave_reduce_dpp(held, [](float x, float y) { return x + y; });
-    n = wave_reduce_dpp(n, [](int x, int y) { return x + y; });
-    // (two places in turn: a wavefront that writes one again has been past the barrier behind which the other was read)
-    turn ^= 1;
+    int at = wave_upto(number) - number;
+    const double held_upto = wave_upto(held);
+    double at_held = __shfl_up(held_upto, 1, 64);
+    if (lane == 0) at_held = 0.0;
+    int cut_at = kBuckets;
+#pragma unroll
+    for (int j = kPer - 1; j >= 0; --j) {
+      int upto = at;
+      double upto_held = at_held;
+#pragma unroll
+      for (int k = 0; k <= j; ++k) {
+        upto += sh.count[lane * kPer + k];
+        upto_held += sh.held[lane * kPer + k];
+      }
+      if (cut.reached(upto, upto_held)) cut_at = lane * kPer + j;
+    }
+    cut_at = wave_reduce_dpp(cut_at, [](int x, int y) { return min(x, y); });
+    int likely_at = kBuckets;
+    if (w.min_p > 0.0) {
+      const double z = m + log2(w.min_p) / w.octaves;
+      likely_at = static_cast<int>(fmin(fmax(top - floor(z * (w.octaves * kGrid)), 0.0), static_cast<double>(kBuckets)));
+    }
     if (lane == 0) {
-      sh.counted[turn][wave] = n;
-      sh.summed[turn][wave] = held;
+      sh.first = min(cut_at, max(likely_at - 1, 0));
+      sh.last = min(cut_at, likely_at + 1);
     }
-    __syncthreads();
-    n = 0;
-    held = 0.0f;
+  }
+  __syncthreads();
+  const int first = scalar(sh.first), last = scalar(sh.last);
+  float low, high;
+  bool told = last < kBuckets - 1 && grid_edge(top - last, w.octaves, low);
+  if (first > 0) told = told && grid_edge(top - first + 1.0, w.octaves, high);
+  else high = INFINITY;
+  if (!told) return false;
+  // in front of the window: of the row, of every part
+  int above = 0;
+  double above_mass = 0.0;
+  for (int b = 0; b < first; ++b) {
+    above += sh.count[b];
+    above_mass += sh.held[b];
+  }
+  for (int p = wave; p < a.parts; p += kWideWaves) {
+    double held = 0.0;
+    for (int b = lane; b < first - sh.part_shift[p]; b += 64) held += static_cast<double>(part_mass[p * kBuckets + b]);
+    held = wave_sum_d(held);
+    if (lane == 0) sh.part_above[p] = held * sh.part_scale[p];
+  }
+  // the window's entries, from the slots that reach it: each wavefront's to a part of the list of its own
+  constexpr int kShare = kWideList / kWideWaves;
+  const float* slot_max = a.slot_max + static_cast<int64_t>(row) * a.slots;
+  int inside = 0;
+  for (int s = c0; s < c1; s += 64) {
+    uint64_t left = __ballot(s + lane < c1 && slot_max[min(s + lane, c1 - 1)] >= low);
+    while (left != 0) {
+      constexpr int kAhead = 8;
+      float z[kAhead];
+      int slot[kAhead];
 #pragma unroll
-    for (int i = 0; i < kWideWaves; ++i) {
-      n += sh.counted[turn][i];
-      held += sh.summed[turn][i];
-    }
-    n = scalar(n);
-    held = scalar(held);
-    const bool is_reached = reached(n, held), is_missed = missed(n, held);
-    if (state == kLow) {
-      if (is_missed) return Window::kAll;
-      if (!is_reached) return Window::kNone;
-      n_lo = n;
-      held_lo = held;
-      state = kHalve;
-    } else if (state == kHalve) {
-      if (is_reached) {
-        lo = at;
-        n_lo = n;
-        held_lo = held;
-      } else if (is_missed) {
-        hi = at;
-        n_hi = n;
-        held_hi = held;
-      } else {  // next to the cut: as close to it as fp32 can tell
-        mid = at;
-        d = kNear;
-        state = kBelow;
+      for (int k = 0; k < kAhead; ++k) {
+        slot[k] = left != 0 ? s + __ffsll(static_cast<unsigned long long>(left)) - 1 : -1;
+        left &= left - 1;
+        z[k] = slot[k] >= 0 ? r.at(slot[k] * kSlot + lane) : -INFINITY;
       }
-    } else if (state == kBelow) {
-      if (is_reached) lo = at;
-      d *= 4;
-    } else {
-      if (is_missed) hi = at;
-      d *= 4;
-    }
-    if (state == kHalve) {
-      if (between() <= kWindow || hi - lo <= 1) break;
-      at = lo + (hi - lo) / 2;
-    }
-    if (state == kBelow) {
-      if (mid - lo > d) {
-        at = mid - d;
-      } else {
-        state = kAbove;
-        d = kNear;
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const uint64_t hit = __ballot(z[k] >= low && z[k] < high);
+        const int to = inside + __popcll(hit & ((1ull << lane) - 1));
+        if ((hit >> lane & 1) && to < kShare) {
+          sh.list_z[wave * kShare + to] = z[k];
+          sh.list_i[wave * kShare + to] = slot[k] * kSlot + lane;
+        }
+        inside += __popcll(hit);
       }
-    }
-    if (state == kAbove) {
-      if (hi - mid <= d) break;
-      at = mid + d;
     }
   }
-  // the window's ends as logits, further apart than fp32 powers are off
-  constexpr float kApart = 1e-4f;  // octaves
-  const float top = static_cast<float>(m + (__builtin_amdgcn_logf(__builtin_bit_cast(float, hi)) + kApart) / w.octaves);
-  const float bottom = static_cast<float>(m + (__builtin_amdgcn_logf(__builtin_bit_cast(float, lo)) - kApart) / w.octaves);
-  // What lies above the window is a fifth of a flat row's entries at a top_p of 0.95, spread evenly: it queues up until there is one for every
-  // lane (a power takes as long for one lane as for 64).  The window's entries go to the list, each wavefront's to a part of its own.
-  constexpr int kPart = kWideList / kWideWaves;
-  double sum = 0.0, kept = 0.0;
-  int higher = 0, inside = 0, waiting = 0;
-  float least = INFINITY, most = -INFINITY;
-  const bool picky = w.min_p > 0.0;
-  const uint64_t in_front = (1ull << lane) - 1;
-  float* queue = sh.queue[wave];
-  const auto add = [&](float z) {
-    const double v = weight(z, m, w.octaves);
-    sum += v;
-    if (picky) kept += v >= w.min_p ? v : 0.0;
-  };
-  each_entry(r, c0, c1, [&](float z, int i) {
-    const uint64_t over = __ballot(z > top), in = __ballot(z >= bottom && z <= top && z > -INFINITY);
-    if (over != 0) {
-      if (over >> lane & 1) queue[waiting + __popcll(over & in_front)] = z;
-      waiting += __popcll(over);
-      if (waiting >= 64) {
-        higher += 64;
-        waiting -= 64;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        add(queue[lane]);
-        const float next = queue[64 + lane];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        queue[lane] = next;
-      }
-    }
-    if (in != 0) {
-      const int to = inside + __popcll(in & in_front);
-      if ((in >> lane & 1) && to < kPart) {
-        sh.list_z[wave * kPart + to] = z;
-        sh.list_i[wave * kPart + to] = i;
-        least = fminf(least, z);
-        most = fmaxf(most, z);
-      }
-      inside += __popcll(in);
-    }
-  });
-  higher += waiting;
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  add(lane < waiting ? queue[lane] : -INFINITY);
-  const double sum_mine = sum;
-  sum = wave_sum_d(sum);
-  least = wave_reduce_dpp(least, [](float x, float y) { return fminf(x, y); });
-  most = wave_reduce_dpp(most, [](float x, float y) { return fmaxf(x, y); });
+  if (lane == 0) sh.entries[wave] = inside;
   __syncthreads();
-  if (lane == 0) {
-    sh.d[wave] = sum;
-    sh.i[wave] = higher;
-    sh.entries[wave] = inside;
-    sh.f[wave] = least;
-    sh.f2[wave] = most;
-  }
-  __syncthreads();
-  int all = 0, place = 0, n = 0, widest = 0;
-  sum = 0.0;
+  int all = 0, place = 0, widest = 0;
 #pragma unroll
   for (int i = 0; i < kWideWaves; ++i) {
     if (i == wave) place = all;
     all += sh.entries[i];
     widest = max(widest, sh.entries[i]);
-    n += sh.i[i];
-    sum += sh.d[i];
-    least = fminf(least, sh.f[i]);
-    most = fmaxf(most, sh.f2[i]);
   }
-  if (all == 0 || all > kWideList || widest > kPart || cut.reached(n, sum)) return Window::kNone;
-  // the parts move together
-  float z[kPart / 64];
-  int i[kPart / 64];
+  if (widest > kShare) return false;
+  // the shares move together
+  float z[kShare / 64];
+  int i[kShare / 64];
 #pragma unroll
-  for (int k = 0; k < kPart / 64; ++k) {
-    z[k] = sh.list_z[wave * kPart + k * 64 + lane];
-    i[k] = sh.list_i[wave * kPart + k * 64 + lane];
+  for (int k = 0; k < kShare / 64; ++k) {
+    z[k] = sh.list_z[wave * kShare + k * 64 + lane];
+    i[k] = sh.list_i[wave * kShare + k * 64 + lane];
   }
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < kPart / 64; ++k)
+  for (int k = 0; k < kShare / 64; ++k)
     if (k * 64 + lane < inside) {
       sh.list_z[place + k * 64 + lane] = z[k];
       sh.list_i[place + k * 64 + lane] = i[k];
     }
-  out.span = {n, scalar(sum), scalar(least), scalar(most)};
-  out.n = all;
-  out.mine = inside;
-  out.mine_at = place;
-  out.kept_above = picky ? kept : sum_mine;
+  sh.reach[wave] = place;
+  span = {scalar(above), scalar(above_mass), low, high};
+  n = scalar(all);
+  kept_above = 0.0;
+  for (int s = c0; s < c1; s += kPart / kSlot) kept_above += sh.part_above[s / (kPart / kSlot)];
   __syncthreads();
-  return Window::kFound;
+  return true;
 }
 
 template <typename T>
@@ -1134,21 +1136,22 @@ __global__ __launch_bounds__(kWideThreads) void draw_wide_kernel(DrawArgs a) {
     a.token[row] = token;
     if (a.logprob) a.logprob[row] = logprob;
   };
-  const int chunk = (a.slots + kWideWaves - 1) / kWideWaves;  // slots of a wavefront
+  // slots of a wavefront: whole parts
+  const int chunk = (a.parts + kWideWaves - 1) / kWideWaves * (kPart / kSlot);
   const int c0 = min(wave * chunk, a.slots), c1 = min(c0 + chunk, a.slots);
 
   Found found = {-INFINITY, INT_MAX};
-  WindowOut out;
-  Window window = cut.open() ? Window::kAll : Window::kNone;
-  if (!cut.open() && chunk <= kChunk && cut.mass > 0.0) {
-    window = find_window(sh, r, c0, c1, w, cut, wide, out);
-    if (window == Window::kFound &&
-        !find_cut(sh, static_cast<const Row<T>*>(nullptr), 0, 0, out.n, cut, m, w.octaves, a.V, out.span,
-                  buckets_of(out.span.high, static_cast<double>(out.span.high) - static_cast<double>(out.span.low)), false, found))
-      window = Window::kNone;  // (beside the cut)
-  }
-  if (window == Window::kNone)
+  Span span;
+  int n = 0;
+  double kept_above = 0.0;
+  const bool windowed = w.needs_histogram() && find_window(a, sh, r, row, c0, c1, w, cut, m, span, n, kept_above);
+  if (windowed) {
+    if (!cut.open() && n > 0)
+      find_cut(sh, static_cast<const Row<T>*>(nullptr), 0, 0, n, cut, m, w.octaves, a.V, span,
+               buckets_of(span.high < INFINITY ? span.high : m, (span.high < INFINITY ? span.high : m) - static_cast<double>(span.low)), false, found);
+  } else if (!cut.open()) {
     find_cut(sh, &r, c0, c1, 0, cut, m, w.octaves, a.V, {0, 0.0, -FLT_MAX, FLT_MAX}, buckets_of(m, kWidest / w.octaves), false, found);
+  }
 
   // the kept entries' sums by wavefronts, of the entry's wavefront by slots, of its slot by entries
   const auto kept_weight = [&](float z, int i) {
@@ -1156,10 +1159,11 @@ __global__ __launch_bounds__(kWideThreads) void draw_wide_kernel(DrawArgs a) {
     return found.keeps(z, i) && w.likely(e) ? e : 0.0;
   };
   double share = 0.0;
-  if (window == Window::kFound) {
+  if (windowed) {
     // (a list in order: this wavefront's part of it is what lies in its chunk)
-    share = out.kept_above;
-    for (int k = lane; k < out.mine; k += 64) share += kept_weight(sh.list_z[out.mine_at + k], sh.list_i[out.mine_at + k]);
+    share = lane == 0 ? kept_above : 0.0;
+    const int end = wave + 1 < kWideWaves ? sh.reach[wave + 1] : n;
+    for (int k = sh.reach[wave] + lane; k < end; k += 64) share += kept_weight(sh.list_z[k], sh.list_i[k]);
   } else {
     each_entry(r, c0, c1, [&](float z, int i) { share += kept_weight(z, i); });
   }
@@ -1239,22 +1243,39 @@ __global__ __launch_bounds__(256) void draw_penalties_kernel(int V, const float*
 
 template <typename T>
 void launch_draw(hipStream_t st, int rows, const DrawArgs& a, bool vec) {
-  const auto stats = [&](auto aligned, auto vectors) {
+  const auto stats = [&](auto aligned, auto threads) {
     constexpr bool kVec = decltype(aligned)::value;
-    constexpr int kNv = decltype(vectors)::value;
-    hipLaunchKernelGGL((draw_stats_kernel<T, kVec, kNv>), dim3(rows, ceil_div(a.V, kStatsThreads * 4 * kNv)), dim3(kStatsThreads), 0, st, a);
+    constexpr int kThreads = decltype(threads)::value;
+    hipLaunchKernelGGL((draw_stats_kernel<T, kVec, kThreads>), dim3(rows, a.parts), dim3(kThreads), 0, st, a);
   };
-  const bool few = static_cast<int64_t>(rows) * ceil_div(a.V, 4096) < 1024;
-  if (vec && few) stats(std::true_type{}, std::integral_constant<int, 1>{});
-  else if (vec) stats(std::true_type{}, std::integral_constant<int, 4>{});
-  else stats(std::false_type{}, std::integral_constant<int, 1>{});
+  // few parts: each by as many wavefronts as a block has
+  const bool few = static_cast<int64_t>(rows) * a.parts < 1024;
+  if (vec && few) stats(std::true_type{}, std::integral_constant<int, 1024>{});
+  else if (vec) stats(std::true_type{}, std::integral_constant<int, 256>{});
+  else if (few) stats(std::false_type{}, std::integral_constant<int, 1024>{});
+  else stats(std::false_type{}, std::integral_constant<int, 256>{});
   hipLaunchKernelGGL((draw_pick_kernel<T>), dim3(rows), dim3(kPickThreads), 0, st, a);
   if (a.top_k || a.top_p || a.min_p) hipLaunchKernelGGL((draw_wide_kernel<T>), dim3(rows), dim3(kWideThreads), 0, st, a);
 }
 
-size_t draw_bytes(int rows, int V) {
-  const size_t slots = static_cast<size_t>(rows) * ceil_div(V, kSlot);
-  return (slots * 12 + rows * sizeof(WideRow) + 15) / 16 * 16;
+// The arrays of a workspace, one after the other, those of 8 bytes first
+DrawArgs lay_out(DrawArgs a, int rows, void* workspace, size_t* bytes) {
+  a.slots = ceil_div(a.V, kSlot);
+  a.parts = ceil_div(a.V, kPart);
+  char* at = static_cast<char*>(workspace);
+  const auto take = [&](auto*& p, size_t n) {
+    p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(at);
+    at += n * sizeof(*p);
+  };
+  const size_t slots = static_cast<size_t>(rows) * a.slots, parts = static_cast<size_t>(rows) * a.parts;
+  take(a.slot_sum, slots);
+  take(a.part_mass, parts * kBuckets);
+  take(a.wide, rows);
+  take(a.slot_max, slots);
+  take(a.part_max, parts);
+  take(a.part_count, parts * kBuckets);
+  *bytes = (static_cast<size_t>(at - static_cast<char*>(workspace)) + 15) / 16 * 16;
+  return a;
 }
 
 }  // namespace
@@ -1267,7 +1288,9 @@ extern "C" {
 
 int rwkv_hip_draw_tokens_workspace(int rows, int V, size_t* bytes) {
   RWKV_REQUIRE(bytes && rows > 0 && V > 0 && V <= kMaxLogprobVocab, "draw_tokens_workspace: bad arguments");
-  *bytes = draw_bytes(rows, V);
+  DrawArgs a = {};
+  a.V = V;
+  lay_out(a, rows, nullptr, bytes);
   return RWKV_OK;
 }
 
@@ -1287,16 +1310,24 @@ int rwkv_hip_draw_tokens(rwkv_stream_t s, int rows, int V, int io, const void* l
     RWKV_REQUIRE((reinterpret_cast<uintptr_t>(p) & 3) == 0, "draw_tokens: 32-bit tensors must be aligned to 4 bytes");
   RWKV_REQUIRE(penalties || !(penalties_out || presence || frequency || decay), "draw_tokens: what becomes of penalties without any");
   RWKV_REQUIRE(penalties_out || !(presence || frequency || decay), "draw_tokens: presence, frequency and decay without penalties_out");
-  const size_t need = draw_bytes(rows, V);
+  DrawArgs a = {};
+  a.logits = logits;
+  a.ld = ld;
+  a.V = V;
+  a.logit_rows = logit_rows;
+  a.source = static_cast<const int*>(source);
+  a.temperature = static_cast<const float*>(temperature);
+  a.top_k = static_cast<const int*>(top_k);
+  a.top_p = static_cast<const float*>(top_p);
+  a.min_p = static_cast<const float*>(min_p);
+  a.uniform = static_cast<const float*>(uniform);
+  a.penalties = static_cast<const float*>(penalties);
+  a.token = static_cast<int*>(token);
+  a.logprob = static_cast<float*>(logprob);
+  size_t need = 0;
+  a = lay_out(a, rows, workspace, &need);
   RWKV_REQUIRE(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
                "draw_tokens: workspace of %zu bytes (aligned to 16) needed, got %zu", need, workspace_bytes);
-  const int slots = ceil_div(V, kSlot);
-  double* sums = static_cast<double*>(workspace);
-  WideRow* wide = reinterpret_cast<WideRow*>(sums + static_cast<size_t>(rows) * slots);
-  const DrawArgs a = {logits, ld, V, slots, logit_rows, static_cast<const int*>(source), static_cast<const float*>(temperature),
-                      static_cast<const int*>(top_k), static_cast<const float*>(top_p), static_cast<const float*>(min_p),
-                      static_cast<const float*>(uniform), static_cast<const float*>(penalties), static_cast<int*>(token), static_cast<float*>(logprob),
-                      sums, reinterpret_cast<float*>(wide + rows), wide};
   const uintptr_t misaligned = io == RWKV_IO_F16 ? 7 : 15;
   const bool vec = (reinterpret_cast<uintptr_t>(logits) & misaligned) == 0 && (ld % 4 == 0 || logit_rows == 1) &&
                    (!penalties || ((reinterpret_cast<uintptr_t>(penalties) & 15) == 0 && (V % 4 == 0 || rows == 1)));
