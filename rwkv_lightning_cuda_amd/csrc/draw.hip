@@ -11,11 +11,12 @@
 // of a row with many candidates would come out next to the one that the definition gives.  (The fp64 vector rate of this chip is that
 // of fp32; an entry costs some twenty operations.)
 //
-// Three launches.  draw_stats_kernel reads the rows with the whole chip: per 64 entries (a slot) the largest z and, where the
-// sum over the whole row is asked for, the sum of the slot's powers.  draw_pick_kernel has a block per row: the slots bound how small a kept
-// entry can be, the slots that reach the bound are read again, and the entries above it go to a list in LDS, in order.  Lists are
-// short for the filters that servers use; a row without filters needs none: its slots' sums give the token's slot.  draw_wide_kernel takes the
-// rows whose list would overflow (flat rows with top-p alone, a large top-k, many equal logits), a block each with the whole row in registers.
+// Two launches.  draw_stats_kernel reads the rows with the whole chip: per 64 entries (a slot) the largest z; per 4096 (a part), where the
+// row asks for it, sums of powers and a histogram of them.  draw_pick_kernel has a block per row, which finds out how small a kept entry can be,
+// reads the slots that reach that far again and puts their entries that do in a list in LDS, in order.  Lists are short for the filters that
+// servers use.  Where the list would overflow (flat rows with top-p alone, a large top-k) it holds the entries about the cut only, the histograms
+// say what lies above them, and a third look at one wavefront's share of the row finds the token.  Rows without filters need no list: the sums of
+// their slots give the token's.
 #include <cfloat>
 #include <climits>
 #include <type_traits>
@@ -28,28 +29,19 @@ namespace {
 
 constexpr int kSlot = 64;
 constexpr int kPart = 4096;      // entries of a block of draw_stats_kernel
-constexpr int kPickThreads = 1024;
-constexpr int kWideThreads = 1024;
-constexpr int kPickList = 4096;  // entries
-constexpr int kWideList = 8192;
+constexpr int kPickThreads = 512;
+constexpr int kList = 6144;      // entries
 constexpr int kBuckets = 256;    // of a histogram
 constexpr int kLast = 64;        // entries that one wavefront puts in order
 constexpr int kWaveSlots = 256;  // slots of a wavefront that reach the bound
 constexpr int kHeld = 8;         // of these, those whose entries it keeps in registers
 constexpr int kMost = 256;       // of a block: with more of them the histograms say more than a list of their entries
-constexpr int kGrid = 4;         // buckets of the parts' histograms in an octave
+constexpr int kGrid = 8;         // buckets of the parts' histograms in an octave
 constexpr int kListed = 256;     // a top_k up to which a row needs no histograms
 constexpr double kOne = 2251799813685248.0;  // 2^51: a part holds 2^12 powers of at most 1
 constexpr double kLog2eD = 1.44269504088896340736;
 constexpr double kLowestPower = -1000.0;  // octaves
 constexpr double kWidest = 64.0;          // octaves that the first histogram covers
-
-// What draw_pick_kernel hands on of a row with more candidates than its list holds
-struct WideRow {
-  double mass;  // what top_p holds; +infinity: no top_p
-  float m;
-  int waits;
-};
 
 struct DrawArgs {
   const void* logits;
@@ -64,15 +56,15 @@ struct DrawArgs {
   const float* penalties;  // [rows,V]
   int* token;
   float* logprob;
-  // what draw_stats_kernel leaves: the largest entry of every slot and part, the sum of a slot's powers against its part's largest, and
-  // for some rows the parts' histograms: powers (times kOne) and numbers of the entries
+  // What draw_stats_kernel leaves: the largest entry of every slot and part; for rows that need them the sums of the slots' or of the
+  // parts' powers, against the part's largest entry, and the parts' histograms: powers (times kOne) and numbers of the entries
   int parts;
-  double* slot_sum;                // [rows,slots]
-  unsigned long long* part_mass;   // [rows,parts,kBuckets]
-  WideRow* wide;                   // [rows]
-  float* slot_max;                 // [rows,slots]
-  float* part_max;                 // [rows,parts]
-  unsigned* part_count;            // [rows,parts,kBuckets]
+  double* slot_sum;               // [rows,slots]
+  double* part_sum;               // [rows,parts]
+  unsigned long long* part_mass;  // [rows,parts,kBuckets]
+  float* slot_max;                // [rows,slots]
+  float* part_max;                // [rows,parts]
+  unsigned* part_count;           // [rows,parts,kBuckets]
 };
 
 // a value that every lane holds, in scalar registers
@@ -92,9 +84,9 @@ struct Wish {
   bool valid, greedy;
   __device__ __forceinline__ bool free() const { return top_k == INT_MAX && top_p >= 1.0 && min_p <= 0.0; }
   __device__ __forceinline__ bool likely(double e) const { return !(min_p > 0.0) || e >= min_p; }
-  __device__ __forceinline__ bool needs_sum() const { return !greedy && (top_p < 1.0 || free()); }
   // (a list of top_k entries, and of the rest of their slots, is short)
   __device__ __forceinline__ bool needs_histogram() const { return !greedy && !free() && top_k > kListed; }
+  __device__ __forceinline__ bool needs_sums() const { return !greedy && (free() || (top_p < 1.0 && !needs_histogram())); }
 };
 __device__ __forceinline__ Wish wish_of(const DrawArgs& a, int row) {
   Wish w;
@@ -201,6 +193,16 @@ struct Row {
     const float z = logit(i);
     return penalties ? z - penalty(i) : z;
   }
+  // the lane's entries of several slots: the row's last one in place of those behind it
+  template <int N>
+  __device__ __forceinline__ void gather(const int (&slot)[N], int lane, float (&z)[N]) const {
+#pragma unroll
+    for (int k = 0; k < N; ++k) z[k] = logit(min(slot[k] * kSlot + lane, V - 1));
+    if (penalties) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) z[k] -= penalty(min(slot[k] * kSlot + lane, V - 1));
+    }
+  }
   // entries i, i + kSlot, ... to z[at], z[at + 1], ...: the row's last one in place of those behind it
   template <int N, int M>
   __device__ __forceinline__ void load(int i, float (&z)[M], int at) const {
@@ -246,13 +248,14 @@ __global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
   constexpr int NV = kPart / 4 / NT;
   typedef T vec_t __attribute__((ext_vector_type(4)));
   __shared__ float most[NT / 64];
+  __shared__ double wave_sum[NT / 64];
   __shared__ unsigned long long mass[kBuckets];
   __shared__ unsigned count[kBuckets];
   const int row = blockIdx.x, part = blockIdx.y;
   const Wish w = wish_of(a, row);
   if (!w.valid) return;
   const Row<T> r = row_of<T>(a, row, w.source);
-  const bool sums = w.needs_sum(), histogram = w.needs_histogram(), counts = w.top_k != INT_MAX;
+  const bool sums = w.needs_sums(), histogram = w.needs_histogram(), counts = w.top_k != INT_MAX;
   const int first = part * kPart + threadIdx.x * 4;
   float z[NV][4];
 #pragma unroll
@@ -308,6 +311,7 @@ __global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
   const int64_t at = static_cast<int64_t>(row) * a.parts + part;
   if (threadIdx.x == 0) a.part_max[at] = m;
   const double top = scalar(grid_place(m, w.octaves));
+  double all = 0.0;
 #pragma unroll
   for (int q = 0; q < NV; ++q) {
     const int slot = (first + q * NT * 4) / kSlot;
@@ -327,9 +331,17 @@ __global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
       sum = row16_sum_d(sum);
       if ((threadIdx.x & 15) == 0 && slot < a.slots) a.slot_sum[static_cast<int64_t>(row) * a.slots + slot] = sum;
     }
+    all += sum;
   }
   if (histogram) {
+    all = wave_sum_d(all);
+    if ((threadIdx.x & 63) == 0) wave_sum[threadIdx.x >> 6] = all;
     __syncthreads();
+    if (threadIdx.x == 0) {
+      all = 0.0;
+      for (int i = 0; i < NT / 64; ++i) all += wave_sum[i];
+      a.part_sum[at] = all;
+    }
     for (int b = threadIdx.x; b < kBuckets; b += NT) {
       a.part_mass[at * kBuckets + b] = mass[b];
       if (counts) a.part_count[at * kBuckets + b] = count[b];
@@ -700,12 +712,200 @@ __device__ __forceinline__ void draw_from_list(S& sh, int n, const Wish& w, cons
 }
 
 constexpr int kPickWaves = kPickThreads / 64;
-struct PickShared : Shared<kPickWaves, kPickList> {
+constexpr int kMaxParts = kMaxLogprobVocab / kPart;
+constexpr int kPartSlots = kPart / kSlot;
+struct PickShared : Shared<kPickWaves, kList> {
   uint16_t slots[kPickWaves][kWaveSlots];
+  double part_scale[kMaxParts];  // a part's largest power, by kOne
+  double part_above[kMaxParts];  // and what the buckets in front of the window hold of it
+  int part_shift[kMaxParts];     // the part's first bucket, among the row's
+  double held[kPickThreads];
+  unsigned number[kPickThreads];
+  double mass_at;
+  int first, last;               // buckets of the window
 };
+static_assert(kMaxLogprobVocab / kSlot / kPickWaves * sizeof(double) <= kList * sizeof(float), "the sums of a chunk's slots lie where the list was");
+static_assert(kPickThreads % kBuckets == 0, "so many threads for a bucket");
+
+// The smallest float whose place on the grid is at least `place`; false: not found next to where it should be
+__device__ __forceinline__ bool grid_edge(double place, double octaves, float& z) {
+  z = octaves > 0.0 ? static_cast<float>(fmin(fmax(place / (octaves * kGrid), -static_cast<double>(FLT_MAX)), static_cast<double>(FLT_MAX))) : -FLT_MAX;
+  int left = 16;
+  while (grid_place(z, octaves) >= place && z > -FLT_MAX && left > 0) {
+    z = nextafterf(z, -INFINITY);
+    --left;
+  }
+  while (grid_place(z, octaves) < place && z < FLT_MAX && left > 0) {
+    z = nextafterf(z, INFINITY);
+    --left;
+  }
+  return left > 0;
+}
+
+// The row's histogram out of its parts': the cut's sum, and the bucket in which the cut lies, or that of the least entry that min_p keeps
+template <typename W>
+__device__ __forceinline__ void place_window(const DrawArgs& a, PickShared& sh, int row, const W& w, float m, double top) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const float* part_max = a.part_max + static_cast<int64_t>(row) * a.parts;
+  const double* part_sum = a.part_sum + static_cast<int64_t>(row) * a.parts;
+  const unsigned long long* part_mass = a.part_mass + static_cast<int64_t>(row) * a.parts * kBuckets;
+  const unsigned* part_count = a.part_count + static_cast<int64_t>(row) * a.parts * kBuckets;
+  const bool counts = w.top_k != INT_MAX;
+  double mine = 0.0;
+  for (int p = tid; p < a.parts; p += kPickThreads) {
+    const float mp = part_max[p];
+    const double scale = weight(mp, m, w.octaves);
+    mine += part_sum[p] * scale;
+    sh.part_scale[p] = scale / kOne;
+    sh.part_shift[p] = mp > -INFINITY ? static_cast<int>(fmin(top - grid_place(mp, w.octaves), static_cast<double>(kBuckets))) : kBuckets;
+  }
+  mine = wave_sum_d(mine);
+  if (lane == 0) sh.total[wave] = mine;
+  __syncthreads();
+  // bucket b of a part is the row's bucket b + shift; a part's last one says nothing but "lower"
+  constexpr int kGroups = kPickThreads / kBuckets;
+  const int j = tid % kBuckets;
+  double held = 0.0;
+  unsigned number = 0;
+  if (j < kBuckets - 1) {
+#pragma unroll 8
+    for (int p = tid / kBuckets; p < a.parts; p += kGroups) {
+      const int b = j - sh.part_shift[p];
+      if (b >= 0) {
+        held += static_cast<double>(part_mass[p * kBuckets + b]) * sh.part_scale[p];
+        if (counts) number += part_count[p * kBuckets + b];
+      }
+    }
+  }
+  sh.held[tid] = held;
+  sh.number[tid] = number;
+  __syncthreads();
+  if (wave == 0) {
+    constexpr int kPer = kBuckets / 64;
+    double total = 0.0;
+#pragma unroll
+    for (int i = 0; i < kPickWaves; ++i) total += sh.total[i];
+    const Cut cut = {w.top_k, w.top_p < 1.0 ? w.top_p * total : INFINITY};
+    int numbers[kPer], all = 0;
+    double sums[kPer], all_held = 0.0;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      numbers[k] = 0;
+      sums[k] = 0.0;
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) {
+        numbers[k] += sh.number[g * kBuckets + lane * kPer + k];
+        sums[k] += sh.held[g * kBuckets + lane * kPer + k];
+      }
+      all += numbers[k];
+      all_held += sums[k];
+    }
+    int at = wave_upto(all) - all;
+    const double upto = wave_upto(all_held);
+    double at_held = __shfl_up(upto, 1, 64);
+    if (lane == 0) at_held = 0.0;
+    int cut_at = kBuckets;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      sh.count[lane * kPer + k] = at;  // (in front of the bucket)
+      sh.held[lane * kPer + k] = at_held;
+      at += numbers[k];
+      at_held += sums[k];
+      if (cut_at == kBuckets && cut.reached(at, at_held)) cut_at = lane * kPer + k;
+    }
+    cut_at = wave_reduce_dpp(cut_at, [](int x, int y) { return min(x, y); });
+    int likely_at = kBuckets;
+    if (w.min_p > 0.0) {  // (rounding: one more on either side)
+      const double z = m + log2(w.min_p) / w.octaves;
+      likely_at = static_cast<int>(fmin(fmax(top - floor(z * (w.octaves * kGrid)), 0.0), static_cast<double>(kBuckets)));
+    }
+    if (lane == 0) {
+      sh.mass_at = cut.mass;
+      sh.first = min(cut_at, max(likely_at - 1, 0));
+      sh.last = min(cut_at, likely_at + 1);
+    }
+  }
+  __syncthreads();
+}
+
+// The entries from `low` up to `high`, from the slots that reach it, to the list, in order; what lies above them is known from the
+// histograms, for every wavefront's chunk of the row.  False: the list is too short.  sh.reach: where each wavefront's begin
+template <typename T>
+__device__ __forceinline__ bool list_window(const DrawArgs& a, PickShared& sh, const Row<T>& r, int row, int c0, int c1, int first, float low, float high,
+                                            int& n, double& kept_above) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const unsigned long long* part_mass = a.part_mass + static_cast<int64_t>(row) * a.parts * kBuckets;
+  kept_above = 0.0;
+  for (int s = c0; s < c1; s += kPartSlots) {
+    const int p = s / kPartSlots;
+    double held = 0.0;
+    for (int b = lane; b < first - sh.part_shift[p]; b += 64) held += static_cast<double>(part_mass[p * kBuckets + b]);
+    kept_above += wave_sum_d(held) * sh.part_scale[p];
+  }
+  // each wavefront's to a share of the list
+  constexpr int kShare = kList / kPickWaves;
+  const float* slot_max = a.slot_max + static_cast<int64_t>(row) * a.slots;
+  int inside = 0;
+  constexpr int kAhead = 16;  // slots at once
+  for (int s = c0; s < c1; s += 64) {
+    const uint64_t reach = __ballot(s + lane < c1 && slot_max[min(s + lane, c1 - 1)] >= low);
+#pragma unroll 1
+    for (int g = 0; g < 64; g += kAhead) {
+      if ((reach >> g & ((1ull << kAhead) - 1)) == 0) continue;
+      const int i0 = (s + g) * kSlot + lane;
+      float z[kAhead];
+      r.template load<kAhead>(i0, z, 0);
+      const int end = min(c1 * kSlot, a.V);
+      if ((s + g + kAhead) * kSlot > end) {
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) z[k] = i0 + k * kSlot < end ? z[k] : -INFINITY;
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const uint64_t hit = __ballot(z[k] >= low && z[k] < high);
+        if (hit == 0) continue;
+        const int to = inside + __popcll(hit & ((1ull << lane) - 1));
+        if ((hit >> lane & 1) && to < kShare) {
+          sh.list_z[wave * kShare + to] = z[k];
+          sh.list_i[wave * kShare + to] = i0 + k * kSlot;
+        }
+        inside += __popcll(hit);
+      }
+    }
+  }
+  if (lane == 0) sh.entries[wave] = inside;
+  __syncthreads();
+  int all = 0, place = 0, widest = 0;
+#pragma unroll
+  for (int i = 0; i < kPickWaves; ++i) {
+    if (i == wave) place = all;
+    all += sh.entries[i];
+    widest = max(widest, sh.entries[i]);
+  }
+  if (widest > kShare) return false;
+  // the shares move together
+  float z[kShare / 64];
+  int i[kShare / 64];
+#pragma unroll
+  for (int k = 0; k < kShare / 64; ++k) {
+    z[k] = sh.list_z[wave * kShare + k * 64 + lane];
+    i[k] = sh.list_i[wave * kShare + k * 64 + lane];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kShare / 64; ++k)
+    if (k * 64 + lane < inside) {
+      sh.list_z[place + k * 64 + lane] = z[k];
+      sh.list_i[place + k * 64 + lane] = i[k];
+    }
+  sh.reach[wave] = place;
+  n = scalar(all);
+  __syncthreads();
+  return true;
+}
 
 template <typename T>
-__global__ __launch_bounds__(kPickThreads) void draw_pick_kernel(DrawArgs a) {
+__global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) {  // (four wavefronts per SIMD: two blocks per CU)
   __shared__ PickShared sh;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int row = blockIdx.x;
@@ -716,7 +916,6 @@ __global__ __launch_bounds__(kPickThreads) void draw_pick_kernel(DrawArgs a) {
     a.token[row] = token;
     if (a.logprob) a.logprob[row] = logprob;
   };
-  if (tid == 0) a.wide[row].waits = 0;
   const float* slot_max = a.slot_max + static_cast<int64_t>(row) * a.slots;
   const double* slot_sum = a.slot_sum + static_cast<int64_t>(row) * a.slots;
   // a thread has neighbouring slots
@@ -800,67 +999,84 @@ __global__ __launch_bounds__(kPickThreads) void draw_pick_kernel(DrawArgs a) {
     return;
   }
 
-  // how far down a kept entry can lie, from the slots
-  const bool summed = w.needs_sum();
-  double range = scalar(static_cast<double>(m) - static_cast<double>(lowest));
-  if (range * w.octaves > kWidest) range = kWidest / w.octaves;
-  const Buckets rough = buckets_of(m, scalar(range));
-  constexpr double kUnit = 1.0 / (1ll << 40);  // (a row's sum is at most 2^20)
-  for (int s = s0; s < s1; ++s) {
-    const float v = slot_max[s];
-    if (!(v > -INFINITY)) continue;
-    const int b = rough.of(v);
-    atomicAdd(&sh.count[b], 1u);
-    if (summed) {
-      const double share = slot_share(s);
-      mine += share;
-      atomicAdd(&sh.mass[b], static_cast<unsigned long long>(share * (1.0 / kUnit)));
+  // How far down a kept entry can lie.  Rows with histograms: to the end of the window in which the last one is; others: as far as the
+  // slots say.
+  const bool histogram = w.needs_histogram();
+  Cut cut = {w.top_k, INFINITY};
+  float low = -FLT_MAX, high = INFINITY;
+  int first = 0;
+  bool told = false;  // the window is known
+  if (histogram) {
+    const double top = grid_place(m, w.octaves);
+    place_window(a, sh, row, w, m, top);
+    cut.mass = scalar(sh.mass_at);
+    first = scalar(sh.first);
+    const int last = scalar(sh.last);
+    told = last < kBuckets - 1 && grid_edge(top - last, w.octaves, low) && (first == 0 || grid_edge(top - first + 1.0, w.octaves, high));
+    if (!told) low = -FLT_MAX;
+  } else {
+    const bool summed = w.needs_sums();
+    double range = scalar(static_cast<double>(m) - static_cast<double>(lowest));
+    if (range * w.octaves > kWidest) range = kWidest / w.octaves;
+    const Buckets rough = buckets_of(m, scalar(range));
+    constexpr double kUnit = 1.0 / (1ll << 40);  // (a row's sum is at most 2^20)
+    for (int s = s0; s < s1; ++s) {
+      const float v = slot_max[s];
+      if (!(v > -INFINITY)) continue;
+      const int b = rough.of(v);
+      atomicAdd(&sh.count[b], 1u);
+      if (summed) {
+        const double share = slot_share(s);
+        mine += share;
+        atomicAdd(&sh.mass[b], static_cast<unsigned long long>(share * (1.0 / kUnit)));
+      }
     }
+    mine = wave_sum_d(mine);
+    if (lane == 0) sh.total[wave] = mine;
+    __syncthreads();
+    double total = 0.0;
+#pragma unroll
+    for (int i = 0; i < kPickWaves; ++i) total += sh.total[i];
+    total = scalar(total);
+    cut.mass = scalar(w.top_p < 1.0 ? w.top_p * total : INFINITY);
+    const double width = scalar(range * w.octaves / kBuckets);  // octaves of a bucket
+    const auto edge = [&](int b) { return __builtin_amdgcn_exp2f(static_cast<float>(-(b + 1) * width)); };  // the least power of a bucket
+    if (wave == 0) {
+      // Bucket b bounds the kept entries if, of the entries up to it, there are top_k (as many slots reach it), or top_p (what is in other
+      // slots, and what their own entries below the bucket can hold at most, or all entries of the row, is less than the rest), or all that
+      // min_p keeps.
+      constexpr int kPer = kBuckets / 64;
+      const double spare = (1.0 - w.top_p) * total - 1e-8 * total;
+      const double unlikely = w.min_p > 0.0 ? 1e-3 - __builtin_amdgcn_logf(static_cast<float>(w.min_p)) : INFINITY;
+      int slots = 0;
+      double held = 0.0;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        slots += sh.count[lane * kPer + j];
+        held += static_cast<double>(sh.mass[lane * kPer + j]) * kUnit;
+      }
+      const int upto = wave_upto(slots);
+      const double held_upto = wave_upto(held);
+      int at = upto - slots;
+      double at_held = held_upto - held;
+      int bound = kBuckets - 1;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int b = lane * kPer + j;
+        at += sh.count[b];
+        at_held += static_cast<double>(sh.mass[b]) * kUnit;
+        bool enough = at >= w.top_k || (b + 1) * width > unlikely;
+        if (summed) enough |= fmin(total - at_held + static_cast<double>(at) * kSlot * edge(b) * 1.001, a.V * 1.001 * edge(b)) <= spare;
+        if (enough) bound = min(bound, b);
+      }
+      bound = wave_reduce_dpp(bound, [](int x, int y) { return min(x, y); });
+      if (lane == 0) sh.bucket = bound;
+    }
+    __syncthreads();
+    const int bound = scalar(sh.bucket);
+    if (bound < kBuckets - 1) low = nextafterf(static_cast<float>(m - (bound + 1) * range / kBuckets), -INFINITY);
   }
-  mine = wave_sum_d(mine);
-  if (lane == 0) sh.total[wave] = mine;
-  __syncthreads();
-  double total = 0.0;
-#pragma unroll
-  for (int i = 0; i < kPickWaves; ++i) total += sh.total[i];
-  total = scalar(total);
-  const Cut cut = {w.top_k, scalar(w.top_p < 1.0 ? w.top_p * total : INFINITY)};
-  const double width = scalar(range * w.octaves / kBuckets);  // octaves of a bucket
-  const auto edge = [&](int b) { return __builtin_amdgcn_exp2f(static_cast<float>(-(b + 1) * width)); };  // the least power of a bucket
-  if (wave == 0) {
-    // Bucket b bounds the kept entries if, of the entries up to it, there are top_k (as many slots reach it), or top_p (what is in other
-    // slots, and what their own entries below the bucket can hold at most, or all entries of the row, is less than the rest), or all that
-    // min_p keeps.
-    constexpr int kPer = kBuckets / 64;
-    const double spare = (1.0 - w.top_p) * total - 1e-8 * total;
-    const double unlikely = w.min_p > 0.0 ? 1e-3 - __builtin_amdgcn_logf(static_cast<float>(w.min_p)) : INFINITY;
-    int slots = 0;
-    double held = 0.0;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      slots += sh.count[lane * kPer + j];
-      held += static_cast<double>(sh.mass[lane * kPer + j]) * kUnit;
-    }
-    const int upto = wave_upto(slots);
-    const double held_upto = wave_upto(held);
-    int at = upto - slots;
-    double at_held = held_upto - held;
-    int bound = kBuckets - 1;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int b = lane * kPer + j;
-      at += sh.count[b];
-      at_held += static_cast<double>(sh.mass[b]) * kUnit;
-      bool enough = at >= w.top_k || (b + 1) * width > unlikely;
-      if (summed) enough |= fmin(total - at_held + static_cast<double>(at) * kSlot * edge(b) * 1.001, a.V * 1.001 * edge(b)) <= spare;
-      if (enough) bound = min(bound, b);
-    }
-    bound = wave_reduce_dpp(bound, [](int x, int y) { return min(x, y); });
-    if (lane == 0) sh.bucket = bound;
-  }
-  __syncthreads();
-  const int bound = scalar(sh.bucket);
-  const auto candidate = [&](float z) { return z > -INFINITY && rough.of(z) <= bound; };
+  const auto candidate = [&](float z) { return z >= low; };
 
   // the slots that reach the bound, each wavefront its own, in order; the entries of the first ones are requested at once
   int reach = 0;
@@ -907,250 +1123,50 @@ __global__ __launch_bounds__(kPickThreads) void draw_pick_kernel(DrawArgs a) {
     }
   }
   n = scalar(n);
-  if (!fits || n > kPickList) {
-    if (tid == 0) a.wide[row] = {cut.mass, m, 1};
+  if (fits && n <= kList) {
+    const auto put = [&](float z, int slot) {
+      const uint64_t hit = __ballot(candidate(z));
+      if (hit >> lane & 1) {
+        const int to = place + __popcll(hit & ((1ull << lane) - 1));
+        sh.list_z[to] = z;
+        sh.list_i[to] = slot * kSlot + lane;
+      }
+      place += __popcll(hit);
+    };
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k)
+      if (k < mine_reach) put(held[k], own[k]);
+    for (int k = kHeld; k < mine_reach; ++k) put(r.at(own[k] * kSlot + lane), own[k]);
+    __syncthreads();
+    if (n <= 64) {
+      if (wave == 0) draw_from_few(sh, n, w, cut, m, answer);
+      return;
+    }
+    Found found = {-INFINITY, INT_MAX};
+    if (!cut.open())
+      find_cut(sh, static_cast<const Row<T>*>(nullptr), 0, 0, n, cut, m, w.octaves, a.V, {0, 0.0, -FLT_MAX, FLT_MAX},
+               buckets_of(m, fmin(static_cast<double>(m) - low, kWidest / w.octaves)), false, found);
+    draw_from_list(sh, n, w, found, m, answer);
     return;
   }
-  const auto put = [&](float z, int slot) {
-    const uint64_t hit = __ballot(candidate(z));
-    if (hit >> lane & 1) {
-      const int to = place + __popcll(hit & ((1ull << lane) - 1));
-      sh.list_z[to] = z;
-      sh.list_i[to] = slot * kSlot + lane;
-    }
-    place += __popcll(hit);
-  };
-#pragma unroll
-  for (int k = 0; k < kHeld; ++k)
-    if (k < mine_reach) put(held[k], own[k]);
-  for (int k = kHeld; k < mine_reach; ++k) put(r.at(own[k] * kSlot + lane), own[k]);
-  __syncthreads();
-  if (n <= 64) {
-    if (wave == 0) draw_from_few(sh, n, w, cut, m, answer);
-    return;
-  }
-  Found found = {-INFINITY, INT_MAX};
-  if (!cut.open()) {
-    Buckets fine = rough;
-    fine.per_unit *= kBuckets / (bound + 1.0);
-    find_cut(sh, static_cast<const Row<T>*>(nullptr), 0, 0, n, cut, m, w.octaves, a.V, {0, 0.0, -FLT_MAX, FLT_MAX}, fine, false, found);
-  }
-  draw_from_list(sh, n, w, found, m, answer);
-}
 
-// ---- rows with more candidates than a list holds -----------------------------------------------------------------------
-constexpr int kWideWaves = kWideThreads / 64;
-constexpr int kMaxParts = kMaxLogprobVocab / kPart;
-struct WideShared : Shared<kWideWaves, kWideList> {
-  double part_scale[kMaxParts];  // a part's largest power, by kOne
-  double part_above[kMaxParts];  // and what the buckets in front of the window hold of it
-  int part_shift[kMaxParts];     // the part's first bucket, among the row's
-  double held[kBuckets];
-  int first, last;               // buckets of the window
-};
-static_assert(kMaxLogprobVocab / kSlot / kWideWaves <= kWideList / 2, "the sums of a chunk's slots lie where the list was");
-
-// The smallest float whose place on the grid is at least `place`; false: not found next to where it should be
-__device__ __forceinline__ bool grid_edge(double place, double octaves, float& z) {
-  z = octaves > 0.0 ? static_cast<float>(fmin(fmax(place / (octaves * kGrid), -static_cast<double>(FLT_MAX)), static_cast<double>(FLT_MAX))) : -FLT_MAX;
-  int left = 16;
-  while (grid_place(z, octaves) >= place && z > -FLT_MAX && left > 0) {
-    z = nextafterf(z, -INFINITY);
-    --left;
-  }
-  while (grid_place(z, octaves) < place && z < FLT_MAX && left > 0) {
-    z = nextafterf(z, INFINITY);
-    --left;
-  }
-  return left > 0;
-}
-
-// A window of the row's values about the cut, from the parts' histograms: its entries go to the list, in order; what lies above it is known
-// from the histograms, for the row and for every wavefront's chunk of it.  False where they do not tell: nothing is changed but the list.
-template <typename T>
-__device__ __forceinline__ bool find_window(const DrawArgs& a, WideShared& sh, const Row<T>& r, int row, int c0, int c1, const Wish& w, const Cut& cut,
-                                            float m, Span& span, int& n, double& kept_above) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const double top = grid_place(m, w.octaves);
-  const float* part_max = a.part_max + static_cast<int64_t>(row) * a.parts;
-  const unsigned long long* part_mass = a.part_mass + static_cast<int64_t>(row) * a.parts * kBuckets;
-  const unsigned* part_count = a.part_count + static_cast<int64_t>(row) * a.parts * kBuckets;
-  const bool counts = w.top_k != INT_MAX;
-  for (int p = tid; p < a.parts; p += kWideThreads) {
-    const float mp = part_max[p];
-    sh.part_scale[p] = weight(mp, m, w.octaves) / kOne;
-    sh.part_shift[p] = mp > -INFINITY ? static_cast<int>(fmin(top - grid_place(mp, w.octaves), static_cast<double>(kBuckets))) : kBuckets;
-  }
-  if (tid < kBuckets) {
-    sh.count[tid] = 0;
-    sh.held[tid] = 0.0;
-  }
-  __syncthreads();
-  // the row's histogram: bucket b of a part is its bucket b + shift; the part's last one says nothing but "lower"
-  if (tid < kBuckets - 1) {
-    double held = 0.0;
-    unsigned number = 0;
-#pragma unroll 8
-    for (int p = 0; p < a.parts; ++p) {
-      const int b = tid - sh.part_shift[p];
-      if (b >= 0) {
-        held += static_cast<double>(part_mass[p * kBuckets + b]) * sh.part_scale[p];
-        if (counts) number += part_count[p * kBuckets + b];
-      }
-    }
-    sh.held[tid] = held;
-    sh.count[tid] = number;
-  }
-  __syncthreads();
-  if (wave == 0) {
-    // the bucket of the cut, and of the least entry that min_p keeps (rounding: one more on either side)
-    constexpr int kPer = kBuckets / 64;
-    int number = 0;
-    double held = 0.0;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      number += sh.count[lane * kPer + j];
-      held += sh.held[lane * kPer + j];
-    }
-    int at = wave_upto(number) - number;
-    const double held_upto = wave_upto(held);
-    double at_held = __shfl_up(held_upto, 1, 64);
-    if (lane == 0) at_held = 0.0;
-    int cut_at = kBuckets;
-#pragma unroll
-    for (int j = kPer - 1; j >= 0; --j) {
-      int upto = at;
-      double upto_held = at_held;
-#pragma unroll
-      for (int k = 0; k <= j; ++k) {
-        upto += sh.count[lane * kPer + k];
-        upto_held += sh.held[lane * kPer + k];
-      }
-      if (cut.reached(upto, upto_held)) cut_at = lane * kPer + j;
-    }
-    cut_at = wave_reduce_dpp(cut_at, [](int x, int y) { return min(x, y); });
-    int likely_at = kBuckets;
-    if (w.min_p > 0.0) {
-      const double z = m + log2(w.min_p) / w.octaves;
-      likely_at = static_cast<int>(fmin(fmax(top - floor(z * (w.octaves * kGrid)), 0.0), static_cast<double>(kBuckets)));
-    }
-    if (lane == 0) {
-      sh.first = min(cut_at, max(likely_at - 1, 0));
-      sh.last = min(cut_at, likely_at + 1);
-    }
-  }
-  __syncthreads();
-  const int first = scalar(sh.first), last = scalar(sh.last);
-  float low, high;
-  bool told = last < kBuckets - 1 && grid_edge(top - last, w.octaves, low);
-  if (first > 0) told = told && grid_edge(top - first + 1.0, w.octaves, high);
-  else high = INFINITY;
-  if (!told) return false;
-  // in front of the window: of the row, of every part
-  int above = 0;
-  double above_mass = 0.0;
-  for (int b = 0; b < first; ++b) {
-    above += sh.count[b];
-    above_mass += sh.held[b];
-  }
-  for (int p = wave; p < a.parts; p += kWideWaves) {
-    double held = 0.0;
-    for (int b = lane; b < first - sh.part_shift[p]; b += 64) held += static_cast<double>(part_mass[p * kBuckets + b]);
-    held = wave_sum_d(held);
-    if (lane == 0) sh.part_above[p] = held * sh.part_scale[p];
-  }
-  // the window's entries, from the slots that reach it: each wavefront's to a part of the list of its own
-  constexpr int kShare = kWideList / kWideWaves;
-  const float* slot_max = a.slot_max + static_cast<int64_t>(row) * a.slots;
-  int inside = 0;
-  for (int s = c0; s < c1; s += 64) {
-    uint64_t left = __ballot(s + lane < c1 && slot_max[min(s + lane, c1 - 1)] >= low);
-    while (left != 0) {
-      constexpr int kAhead = 8;
-      float z[kAhead];
-      int slot[kAhead];
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        slot[k] = left != 0 ? s + __ffsll(static_cast<unsigned long long>(left)) - 1 : -1;
-        left &= left - 1;
-        z[k] = slot[k] >= 0 ? r.at(slot[k] * kSlot + lane) : -INFINITY;
-      }
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const uint64_t hit = __ballot(z[k] >= low && z[k] < high);
-        const int to = inside + __popcll(hit & ((1ull << lane) - 1));
-        if ((hit >> lane & 1) && to < kShare) {
-          sh.list_z[wave * kShare + to] = z[k];
-          sh.list_i[wave * kShare + to] = slot[k] * kSlot + lane;
-        }
-        inside += __popcll(hit);
-      }
-    }
-  }
-  if (lane == 0) sh.entries[wave] = inside;
-  __syncthreads();
-  int all = 0, place = 0, widest = 0;
-#pragma unroll
-  for (int i = 0; i < kWideWaves; ++i) {
-    if (i == wave) place = all;
-    all += sh.entries[i];
-    widest = max(widest, sh.entries[i]);
-  }
-  if (widest > kShare) return false;
-  // the shares move together
-  float z[kShare / 64];
-  int i[kShare / 64];
-#pragma unroll
-  for (int k = 0; k < kShare / 64; ++k) {
-    z[k] = sh.list_z[wave * kShare + k * 64 + lane];
-    i[k] = sh.list_i[wave * kShare + k * 64 + lane];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int k = 0; k < kShare / 64; ++k)
-    if (k * 64 + lane < inside) {
-      sh.list_z[place + k * 64 + lane] = z[k];
-      sh.list_i[place + k * 64 + lane] = i[k];
-    }
-  sh.reach[wave] = place;
-  span = {scalar(above), scalar(above_mass), low, high};
-  n = scalar(all);
-  kept_above = 0.0;
-  for (int s = c0; s < c1; s += kPart / kSlot) kept_above += sh.part_above[s / (kPart / kSlot)];
-  __syncthreads();
-  return true;
-}
-
-template <typename T>
-__global__ __launch_bounds__(kWideThreads) void draw_wide_kernel(DrawArgs a) {
-  __shared__ WideShared sh;
-  const int row = blockIdx.x;
-  const WideRow wide = a.wide[row];
-  if (!wide.waits) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const Wish w = wish_of(a, row);
-  const float m = wide.m;
-  const Cut cut = {w.top_k, wide.mass};
-  const Row<T> r = row_of<T>(a, row, w.source);
-  const auto answer = [&](int token, float logprob) {
-    a.token[row] = token;
-    if (a.logprob) a.logprob[row] = logprob;
-  };
-  // slots of a wavefront: whole parts
-  const int chunk = (a.parts + kWideWaves - 1) / kWideWaves * (kPart / kSlot);
+  // Many candidates.  The cut is looked for in the window alone; where that is wider than the list, or not known, in memory.
+  const int chunk = (a.parts + kPickWaves - 1) / kPickWaves * kPartSlots;  // slots of a wavefront: whole parts
   const int c0 = min(wave * chunk, a.slots), c1 = min(c0 + chunk, a.slots);
-
   Found found = {-INFINITY, INT_MAX};
-  Span span;
-  int n = 0;
+  Span span = {0, 0.0, low, FLT_MAX};
   double kept_above = 0.0;
-  const bool windowed = w.needs_histogram() && find_window(a, sh, r, row, c0, c1, w, cut, m, span, n, kept_above);
-  if (windowed) {
-    if (!cut.open() && n > 0)
-      find_cut(sh, static_cast<const Row<T>*>(nullptr), 0, 0, n, cut, m, w.octaves, a.V, span,
-               buckets_of(span.high < INFINITY ? span.high : m, (span.high < INFINITY ? span.high : m) - static_cast<double>(span.low)), false, found);
-  } else if (!cut.open()) {
-    find_cut(sh, &r, c0, c1, 0, cut, m, w.octaves, a.V, {0, 0.0, -FLT_MAX, FLT_MAX}, buckets_of(m, kWidest / w.octaves), false, found);
+  bool windowed = false;
+  if (told) {
+    if (high < INFINITY) span.high = nextafterf(high, -INFINITY);
+    span.above = scalar(static_cast<int>(sh.count[first]));
+    span.above_mass = scalar(sh.held[first]);
+    windowed = list_window(a, sh, r, row, c0, c1, first, low, high, n, kept_above);
+  }
+  if (!cut.open()) {
+    const double from = fmin(span.high, m);
+    find_cut(sh, windowed ? nullptr : &r, c0, c1, windowed ? n : 0, cut, m, w.octaves, a.V, span,
+             buckets_of(from, fmin(from - span.low, kWidest / w.octaves)), false, found);
   }
 
   // the kept entries' sums by wavefronts, of the entry's wavefront by slots, of its slot by entries
@@ -1162,10 +1178,13 @@ __global__ __launch_bounds__(kWideThreads) void draw_wide_kernel(DrawArgs a) {
   if (windowed) {
     // (a list in order: this wavefront's part of it is what lies in its chunk)
     share = lane == 0 ? kept_above : 0.0;
-    const int end = wave + 1 < kWideWaves ? sh.reach[wave + 1] : n;
+    const int end = wave + 1 < kPickWaves ? sh.reach[wave + 1] : n;
     for (int k = sh.reach[wave] + lane; k < end; k += 64) share += kept_weight(sh.list_z[k], sh.list_i[k]);
   } else {
-    each_entry(r, c0, c1, [&](float z, int i) { share += kept_weight(z, i); });
+    share = lane == 0 ? kept_above : 0.0;
+    each_entry(r, c0, c1, [&](float z, int i) {
+      if (z >= span.low && z <= span.high) share += kept_weight(z, i);
+    });
   }
   share = wave_sum_d(share);
   __syncthreads();
@@ -1173,13 +1192,13 @@ __global__ __launch_bounds__(kWideThreads) void draw_wide_kernel(DrawArgs a) {
   __syncthreads();
   double kept = 0.0;
 #pragma unroll
-  for (int i = 0; i < kWideWaves; ++i) kept += sh.chunk[i];
+  for (int i = 0; i < kPickWaves; ++i) kept += sh.chunk[i];
   const double target = w.u * kept;
   double upto = 0.0, before = 0.0, others = 0.0;
   int owner = -1;
   bool sure = false;
 #pragma unroll
-  for (int i = 0; i < kWideWaves; ++i) {
+  for (int i = 0; i < kPickWaves; ++i) {
     const double v = sh.chunk[i];
     if (v > 0.0 && !sure) {
       owner = i;
@@ -1189,17 +1208,21 @@ __global__ __launch_bounds__(kWideThreads) void draw_wide_kernel(DrawArgs a) {
     upto += v;
   }
 #pragma unroll
-  for (int i = 0; i < kWideWaves; ++i) others += i == owner ? 0.0 : sh.chunk[i];
+  for (int i = 0; i < kPickWaves; ++i) others += i == owner ? 0.0 : sh.chunk[i];
   const int o0 = owner * chunk, slots = min(o0 + chunk, a.slots) - o0;
   double* sums = reinterpret_cast<double*>(sh.list_z);
-  for (int s = wave; s < slots; s += 4 * kWideWaves) {
-    float z[4];
+  constexpr int kAhead = 8;
+  for (int s = wave; s < slots; s += kAhead * kPickWaves) {
+    float z[kAhead];
+    int slot[kAhead];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) z[k] = s + k * kWideWaves < slots ? r.at((o0 + s + k * kWideWaves) * kSlot + lane) : -INFINITY;
+    for (int k = 0; k < kAhead; ++k) slot[k] = o0 + min(s + k * kPickWaves, slots - 1);
+    r.gather(slot, lane, z);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const double sum = wave_sum_d(kept_weight(z[k], (o0 + s + k * kWideWaves) * kSlot + lane));
-      if (lane == 0 && s + k * kWideWaves < slots) sums[s + k * kWideWaves] = sum;
+    for (int k = 0; k < kAhead; ++k) {
+      const int i = slot[k] * kSlot + lane;
+      const double sum = wave_sum_d(i < a.V ? kept_weight(z[k], i) : 0.0);
+      if (lane == 0) sums[slot[k] - o0] = sum;
     }
   }
   __syncthreads();
@@ -1255,7 +1278,6 @@ void launch_draw(hipStream_t st, int rows, const DrawArgs& a, bool vec) {
   else if (few) stats(std::false_type{}, std::integral_constant<int, 1024>{});
   else stats(std::false_type{}, std::integral_constant<int, 256>{});
   hipLaunchKernelGGL((draw_pick_kernel<T>), dim3(rows), dim3(kPickThreads), 0, st, a);
-  if (a.top_k || a.top_p || a.min_p) hipLaunchKernelGGL((draw_wide_kernel<T>), dim3(rows), dim3(kWideThreads), 0, st, a);
 }
 
 // The arrays of a workspace, one after the other, those of 8 bytes first
@@ -1269,8 +1291,8 @@ DrawArgs lay_out(DrawArgs a, int rows, void* workspace, size_t* bytes) {
   };
   const size_t slots = static_cast<size_t>(rows) * a.slots, parts = static_cast<size_t>(rows) * a.parts;
   take(a.slot_sum, slots);
+  take(a.part_sum, parts);
   take(a.part_mass, parts * kBuckets);
-  take(a.wide, rows);
   take(a.slot_max, slots);
   take(a.part_max, parts);
   take(a.part_count, parts * kBuckets);
