@@ -17,6 +17,7 @@
 // servers use.  Where the list would overflow (flat rows with top-p alone, a large top-k) it holds the entries about the cut only, the histograms
 // say what lies above them, and a third look at one wavefront's share of the row finds the token.  Rows without filters need no list: the sums of
 // their slots give the token's.
+#include <algorithm>
 #include <cfloat>
 #include <climits>
 #include <type_traits>
@@ -116,11 +117,12 @@ __device__ __forceinline__ double fma_scalar(double a, double b, double c) {
 }
 // e of an entry z <= m; 0 for -infinity.  2^f for |f| <= 1/2 is 1 + f q(f), exact at 0, with the polynomial through (2^f - 1) / f at the nine
 // Chebyshev nodes of that range: 3.7e-14 off at most.
-__device__ __forceinline__ double weight(float z, float m, double octaves) {
+constexpr double kNinth = 1.0203121063391729e-07;  // the highest coefficient
+__device__ __forceinline__ double weight(float z, float m, double octaves, double ninth = kNinth) {
   const double y = (static_cast<double>(z) - static_cast<double>(m)) * octaves;
   const double n = rint(y);
   const double f = y - n;
-  double q = fma_scalar(f, 1.0203121063391729e-07, 1.3255224878668817e-06);
+  double q = fma_scalar(f, ninth, 1.3255224878668817e-06);
   q = fma_scalar(q, f, 1.525268684626772e-05);
   q = fma_scalar(q, f, 0.00015403455852453838);
   q = fma_scalar(q, f, 0.0013333558179043112);
@@ -130,6 +132,11 @@ __device__ __forceinline__ double weight(float z, float m, double octaves) {
   q = fma_scalar(q, f, 0.6931471805599453);
   const double v = ldexp(fma(q, f, 1.0), static_cast<int>(n));
   return y >= kLowestPower ? v : 0.0;  // (infinity times no octaves at all is a NaN, and none either)
+}
+// a constant that stays in vector registers (and is not made anew for every use)
+__device__ __forceinline__ double held_constant(double c) {
+  asm volatile("" : "+v"(c));
+  return c;
 }
 
 template <int D>
@@ -312,18 +319,19 @@ __global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
   if (threadIdx.x == 0) a.part_max[at] = m;
   const double top = scalar(grid_place(m, w.octaves));
   double all = 0.0;
+  const double ninth = held_constant(kNinth), one = held_constant(kOne), two = held_constant(2.0 * kOne);
 #pragma unroll
   for (int q = 0; q < NV; ++q) {
     const int slot = (first + q * NT * 4) / kSlot;
     double sum = 0.0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const double e = weight(z[q][j], m, w.octaves);
+      const double e = weight(z[q][j], m, w.octaves, ninth);
       sum += e;
-      if (histogram && z[q][j] > -INFINITY && m < INFINITY) {
+      if (histogram) {  // (-infinity, and whatever a row without a distribution holds: the last bucket, with nothing)
         const int b = static_cast<int>(fmin(top - grid_place(z[q][j], w.octaves), static_cast<double>(kBuckets - 1)));
         // (2^52 + e 2^51, rounded: its last 52 bits)
-        atomicAdd(&mass[b], __builtin_bit_cast(unsigned long long, fma(e, kOne, 2.0 * kOne)) - 0x4330000000000000ull);
+        atomicAdd(&mass[b], __builtin_bit_cast(unsigned long long, fma(e, one, two)) - 0x4330000000000000ull);
         if (counts) atomicAdd(&count[b], 1u);
       }
     }
@@ -1211,19 +1219,17 @@ __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) 
   for (int i = 0; i < kPickWaves; ++i) others += i == owner ? 0.0 : sh.chunk[i];
   const int o0 = owner * chunk, slots = min(o0 + chunk, a.slots) - o0;
   double* sums = reinterpret_cast<double*>(sh.list_z);
-  constexpr int kAhead = 8;
-  for (int s = wave; s < slots; s += kAhead * kPickWaves) {
-    float z[kAhead];
-    int slot[kAhead];
+  // (16 lanes a slot: four entries each, then four steps to their sum)
+  for (int s = wave * 4; s < slots; s += 4 * kPickWaves) {
+    const int own = o0 + min(s + lane / 16, slots - 1);
+    double sum = 0.0;
+    float z[4];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) slot[k] = o0 + min(s + k * kPickWaves, slots - 1);
-    r.gather(slot, lane, z);
+    for (int k = 0; k < 4; ++k) z[k] = r.at(own * kSlot + k * 16 + lane % 16);
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int i = slot[k] * kSlot + lane;
-      const double sum = wave_sum_d(i < a.V ? kept_weight(z[k], i) : 0.0);
-      if (lane == 0) sums[slot[k] - o0] = sum;
-    }
+    for (int k = 0; k < 4; ++k) sum += kept_weight(z[k], own * kSlot + k * 16 + lane % 16);
+    sum = row16_sum_d(sum);
+    if (lane % 16 == 0) sums[own - o0] = sum;
   }
   __syncthreads();
   if (wave != 0) return;
@@ -1266,13 +1272,13 @@ __global__ __launch_bounds__(256) void draw_penalties_kernel(int V, const float*
 
 template <typename T>
 void launch_draw(hipStream_t st, int rows, const DrawArgs& a, bool vec) {
+  // few parts: each by as many wavefronts as a block has.  (Several parts to a block, the next one requested ahead, took 10 % longer.)
+  const bool few = static_cast<int64_t>(rows) * a.parts < 4 * device_cu_count();
   const auto stats = [&](auto aligned, auto threads) {
     constexpr bool kVec = decltype(aligned)::value;
     constexpr int kThreads = decltype(threads)::value;
     hipLaunchKernelGGL((draw_stats_kernel<T, kVec, kThreads>), dim3(rows, a.parts), dim3(kThreads), 0, st, a);
   };
-  // few parts: each by as many wavefronts as a block has
-  const bool few = static_cast<int64_t>(rows) * a.parts < 1024;
   if (vec && few) stats(std::true_type{}, std::integral_constant<int, 1024>{});
   else if (vec) stats(std::true_type{}, std::integral_constant<int, 256>{});
   else if (few) stats(std::false_type{}, std::integral_constant<int, 1024>{});
