@@ -238,11 +238,16 @@ int copy_rows_launch(hipStream_t st, int tensors, void* const* dst, const void* 
     std::copy(moves.begin(), moves.end(), a.moves);
     std::copy(first.begin(), first.end(), a.first);
     a.tensors = t;
-    constexpr int kPer = 4;
+    // us with 1 / 2 / 4 / 8 units a thread: a fp16 state of the 7.2B shape to fifteen rows 57 / 58 / 63 / 67, half of 64 fp32 ones to a
+    // narrower batch 438 / 417 / 439 / 668.  Past the caches where more is moved than the last of them holds: nine of 48 such states to
+    // other places and as many cleared (0.93 GB) 168 instead of 189; three states of the 1.5B shape to eleven (0.14 GB) 28 instead of 26.
+    constexpr int kPer = 2;
     const int64_t blocks = lay_out_blocks(a.tensors, planes, kPer);
     RWKV_REQUIRE(blocks > 0, "copy_rows: too large for one call");
     const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(first.size() - 1));
-    hipLaunchKernelGGL((copy_rows_kernel<kPer, false>), grid, dim3(kThreads), 0, st, a);
+    const bool past = (moves.size() + first.size() - 1) * static_cast<double>(plane_bytes) >= 256.0 * (1 << 20);
+    if (past) hipLaunchKernelGGL((copy_rows_kernel<kPer, true>), grid, dim3(kThreads), 0, st, a);
+    else hipLaunchKernelGGL((copy_rows_kernel<kPer, false>), grid, dim3(kThreads), 0, st, a);
   }
   RWKV_LAUNCH_CHECK();
   return RWKV_OK;
