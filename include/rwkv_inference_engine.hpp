@@ -58,6 +58,23 @@ class InferenceEngine {
   };
   std::vector<TextScore> score(const std::vector<std::string>& texts, const ScoreOptions& options = {}) const;
 
+  // Several continuations of one prompt (no counterpart in the reference).  The prompt is run once; its state goes on in n places, each with
+  // random numbers of its own: continuation i of a seed is the same whatever n is, up to the rounding differences between the kernels of
+  // different batch widths.  Rows that have ended make room once at most half of the batch is left.
+  struct BranchOptions {
+    int max_tokens = 256;
+    std::vector<int64_t> stop_tokens{0, 261, 24281};
+    DrawOptions draw;
+    std::uint64_t seed = 0;
+  };
+  struct Branch {
+    std::string text;
+    std::vector<int> tokens;      // without the stop token
+    std::vector<float> logprobs;  // of these tokens, among those that the filters kept
+    bool stopped = false;         // by a stop token (whose log probability is not among them)
+  };
+  std::vector<Branch> branch_generate(const std::string& prompt, int n, const BranchOptions& options) const;
+
   std::string format_openai_prompt(const std::string& system,
                                    const std::vector<std::pair<std::string, std::string>>& messages,
                                    ThinkType think_type) const;

@@ -96,6 +96,12 @@ class IModelBackend {
                                  int count) const = 0;
   virtual PrefillCapacity query_prefill_capacity(int prefill_chunk_size) const = 0;
 
+  // Row to[i] of dst becomes row rows[i] of src (-1: an empty state): a sequence goes on in several places, or moves to another batch.  src and
+  // dst may be the same state; every row is then taken as it was before the call.  A row may be a destination once.  No counterpart in the
+  // reference.  Backends that do not override it copy runs of neighbouring rows with copy_state_slice, and refuse empty states and the same
+  // state on both sides.
+  virtual void copy_state_rows(const GenerationState& src, const std::vector<int>& rows, GenerationState& dst, const std::vector<int>& to) const;
+
   // forward_prefill without logits, with the log probability of target_batches (same shape; -1: none) at every position, rows of a
   // batch one after the other.  Backends that do not score refuse.
   virtual TokenLogprobs score(const std::vector<std::vector<int64_t>>& token_batches, const std::vector<std::vector<int64_t>>& target_batches,
@@ -131,6 +137,7 @@ class ModelBackend final : public IModelBackend {
   void copy_logits_slice(const DeviceLogits& src, int src_offset, DeviceLogits& dst, int dst_offset,
                          int count) const override;
   PrefillCapacity query_prefill_capacity(int prefill_chunk_size) const override;
+  void copy_state_rows(const GenerationState& src, const std::vector<int>& rows, GenerationState& dst, const std::vector<int>& to) const override;
   TokenLogprobs score(const std::vector<std::vector<int64_t>>& token_batches, const std::vector<std::vector<int64_t>>& target_batches,
                       GenerationState& state, const ScoreOptions& options) const override;
 

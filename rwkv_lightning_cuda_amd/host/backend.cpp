@@ -16,6 +16,7 @@
 #include <cstdlib>
 #include <limits>
 #include <mutex>
+#include <numeric>
 #include <sstream>
 #include <stdexcept>
 #include <thread>
@@ -730,27 +731,58 @@ void ModelBackend::copy_state_slice(const GenerationState& src, int src_offset, 
   if (src_offset + count > src.batch_size || dst_offset + count > dst.batch_size)
     throw std::runtime_error("state slice range exceeds batch size");
 
-  const ModelDims& d = impl_->spec.dims;
-  const std::size_t C = static_cast<std::size_t>(d.channels);
-  const std::size_t lane = static_cast<std::size_t>(d.heads) * d.head_size * d.head_size;
-  for (int layer = 0; layer < d.layers; ++layer) {
-    for (int which = 0; which < 2; ++which) {
-      const half* s = src.shift.p + (static_cast<std::size_t>(layer) * 2 + which) * src.batch_size * C + src_offset * C;
-      half* t = dst.shift.p + (static_cast<std::size_t>(layer) * 2 + which) * dst.batch_size * C + dst_offset * C;
-      check_hip(rwkv_hip_memcpy_d2d(t, s, count * C * sizeof(half)), "copy backend state slice shift");
-    }
-    if (impl_->use_wkv32) {
-      const float* s = src.wkv_state32.p + (static_cast<std::size_t>(layer) * src.batch_size + src_offset) * lane;
-      float* t = dst.wkv_state32.p + (static_cast<std::size_t>(layer) * dst.batch_size + dst_offset) * lane;
-      check_hip(rwkv_hip_memcpy_d2d(t, s, count * lane * sizeof(float)), "copy backend state slice wkv32");
-    } else {
-      const half* s = src.wkv_state.p + (static_cast<std::size_t>(layer) * src.batch_size + src_offset) * lane;
-      half* t = dst.wkv_state.p + (static_cast<std::size_t>(layer) * dst.batch_size + dst_offset) * lane;
-      check_hip(rwkv_hip_memcpy_d2d(t, s, count * lane * sizeof(half)), "copy backend state slice wkv");
-    }
+  // (a run that moves up inside its own state goes last part first)
+  constexpr int kRun = 512;
+  const bool up = &src == &dst && dst_offset > src_offset;
+  for (int done = 0; done < count; done += kRun) {
+    const int n = std::min(kRun, count - done), first = up ? count - done - n : done;
+    std::vector<int> rows(n), to(n);
+    std::iota(rows.begin(), rows.end(), src_offset + first);
+    std::iota(to.begin(), to.end(), dst_offset + first);
+    copy_state_rows(src, rows, dst, to);
   }
-  check_hip(rwkv_hip_memcpy_d2d(dst.elapsed.p + dst_offset, src.elapsed.p + src_offset, count * sizeof(int)),
-            "copy backend state slice elapsed");
+}
+
+void IModelBackend::copy_state_rows(const GenerationState& src, const std::vector<int>& rows, GenerationState& dst, const std::vector<int>& to) const {
+  if (rows.size() != to.size()) throw std::runtime_error("as many state rows as places for them");
+  if (&src == &dst) throw std::runtime_error("this backend does not move rows inside a state");
+  for (const int row : rows)
+    if (row < 0) throw std::runtime_error("this backend does not clear state rows");
+  for (std::size_t i = 0; i < rows.size();) {
+    std::size_t run = 1;
+    while (i + run < rows.size() && rows[i + run] == rows[i] + static_cast<int>(run) && to[i + run] == to[i] + static_cast<int>(run)) ++run;
+    copy_state_slice(src, rows[i], dst, to[i], static_cast<int>(run));
+    i += run;
+  }
+}
+
+// One launch for all layers and rows (the reference's copy_state_slice makes 3 L + 1 copies, src/rwkv7_fast_v4.cu:1421-1504).  On the NULL stream,
+// and waited for: the sessions' streams do not wait for it.
+void ModelBackend::copy_state_rows(const GenerationState& src, const std::vector<int>& rows, GenerationState& dst, const std::vector<int>& to) const {
+  if (rows.size() != to.size()) throw std::runtime_error("as many state rows as places for them");
+  if (src.batch_size <= 0 || dst.batch_size <= 0) throw std::runtime_error("state rows require non-empty source and destination");
+  if (src.wkv32 != dst.wkv32 || src.wkv32 != impl_->use_wkv32) throw std::runtime_error("state rows wkv precision mismatch");
+  const ModelDims& d = impl_->spec.dims;
+  const std::int64_t lane = static_cast<std::int64_t>(d.heads) * d.head_size * d.head_size;
+  const std::int64_t planes[3] = {2 * static_cast<std::int64_t>(d.layers), d.layers, 1};
+  const std::int64_t row_bytes[3] = {d.channels * static_cast<std::int64_t>(sizeof(half)),
+                                     lane * static_cast<std::int64_t>(src.wkv32 ? sizeof(float) : sizeof(half)), sizeof(int)};
+  const void* from_tensors[3] = {src.shift.p, src.wkv32 ? static_cast<const void*>(src.wkv_state32.p) : src.wkv_state.p, src.elapsed.p};
+  void* to_tensors[3] = {dst.shift.p, dst.wkv32 ? static_cast<void*>(dst.wkv_state32.p) : dst.wkv_state.p, dst.elapsed.p};
+  constexpr std::size_t kMoves = 512;  // of a call
+  if (&src == &dst && rows.size() > kMoves) throw std::runtime_error("more than 512 rows inside a state");
+  std::vector<char> taken(dst.batch_size, 0);
+  for (std::size_t i = 0; i < rows.size(); ++i) {  // (over all calls, ahead of the first)
+    if (rows[i] < -1 || rows[i] >= src.batch_size || to[i] < 0 || to[i] >= dst.batch_size) throw std::runtime_error("state row out of range");
+    if (taken[to[i]]) throw std::runtime_error("two state rows for one place");
+    taken[to[i]] = 1;
+  }
+  for (std::size_t i = 0; i < rows.size(); i += kMoves) {
+    const int n = static_cast<int>(std::min(kMoves, rows.size() - i));
+    check_hip(rwkv_hip_copy_rows(nullptr, 3, to_tensors, from_tensors, planes, row_bytes, dst.batch_size, src.batch_size, n, to.data() + i, rows.data() + i),
+              "copy backend state rows");
+  }
+  check_hip(rwkv_hip_stream_sync(nullptr), "copy backend state rows");
 }
 
 void ModelBackend::copy_logits_slice(const DeviceLogits& src, int src_offset, DeviceLogits& dst, int dst_offset,

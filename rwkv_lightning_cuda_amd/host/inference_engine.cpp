@@ -363,30 +363,32 @@ std::string InferenceEngine::generate_one(const std::string& prompt, GenerationS
 namespace {
 
 // Gathers the slots listed in `keep` (ascending) to the front of a state, a sampler state and a feed vector of
-// width keep.size(); `rows` maps a slot to its prompt.  Runs of neighbouring slots move with one slice copy.
+// width keep.size(); `rows` maps a slot to its prompt.
 void gather_live_slots(const IModelBackend& model, const std::vector<int>& keep, GenerationState& state,
                        SamplerPenaltyState& penalties, std::vector<size_t>& rows, std::vector<int64_t>& feed) {
   const int width = static_cast<int>(keep.size());
   GenerationState narrow = model.create_state(width);
   SamplerPenaltyState narrow_penalties = make_sampler_penalties(penalties.vocab_size, width, penalties.seed);
   narrow_penalties.step = penalties.step;
+  std::vector<int> to(width);
+  std::iota(to.begin(), to.end(), 0);
+  model.copy_state_rows(state, keep, narrow, to);
   const std::size_t row_bytes = static_cast<std::size_t>(penalties.vocab_size) * sizeof(float);
-  for (int to = 0; to < width;) {
+  for (int i = 0; i < width;) {
     int run = 1;
-    while (to + run < width && keep[to + run] == keep[to] + run) ++run;
-    model.copy_state_slice(state, keep[to], narrow, to, run);
+    while (i + run < width && keep[i + run] == keep[i] + run) ++run;
     rwkv7_fast_v4::check_hip(
-        rwkv_hip_memcpy_d2d(narrow_penalties.penalties.p + static_cast<std::size_t>(to) * penalties.vocab_size,
-                            penalties.penalties.p + static_cast<std::size_t>(keep[to]) * penalties.vocab_size,
+        rwkv_hip_memcpy_d2d(narrow_penalties.penalties.p + static_cast<std::size_t>(i) * penalties.vocab_size,
+                            penalties.penalties.p + static_cast<std::size_t>(keep[i]) * penalties.vocab_size,
                             run * row_bytes),
         "gather sampler penalties");
-    to += run;
+    i += run;
   }
   std::vector<size_t> new_rows(width);
   std::vector<int64_t> new_feed(width);
-  for (int to = 0; to < width; ++to) {
-    new_rows[to] = rows[keep[to]];
-    new_feed[to] = feed[keep[to]];
+  for (int i = 0; i < width; ++i) {
+    new_rows[i] = rows[keep[i]];
+    new_feed[i] = feed[keep[i]];
   }
   state = std::move(narrow);
   penalties = std::move(narrow_penalties);
@@ -572,6 +574,69 @@ InferenceEngine::GenerationStats InferenceEngine::generate_from_logits_stream(
   if (!tail.empty() && !emit(0, tail)) stats.stopped = true;
   stats.decode_seconds = seconds_since(decode_t0);
   return stats;
+}
+
+// The first token of all continuations is drawn from the prompt's one row of logits; those that go on get copies of its state.
+std::vector<InferenceEngine::Branch> InferenceEngine::branch_generate(const std::string& prompt, int n, const BranchOptions& options) const {
+  if (n <= 0) throw std::runtime_error("number of continuations must be positive");
+  std::vector<Branch> out(n);
+  GenerationState state = model_->create_state(1);
+  DeviceLogits logits;
+  prefill_prompt(prompt, state, logits);
+
+  const bool penalised = options.draw.alpha_presence != 0.0 || options.draw.alpha_frequency != 0.0;
+  DrawState draws = make_draw_state(model_->vocab_size(), n, penalised);
+  std::vector<int> live(n);  // row of the batch -> continuation, or -1
+  std::iota(live.begin(), live.end(), 0);
+  std::vector<int> source(n, 0);  // first step: everybody's logits are row 0
+  const int64_t filler = options.stop_tokens.empty() ? 0 : options.stop_tokens.front();
+  std::vector<float> uniform;
+  for (int step = 0; step < options.max_tokens; ++step) {
+    uniform.clear();
+    for (const int i : live) uniform.push_back(i < 0 ? 0.0f : uniform_of(options.seed, static_cast<std::uint64_t>(i), static_cast<std::uint64_t>(step)));
+    const DrawnTokens drawn = draw_tokens(logits, std::vector<DrawOptions>(live.size(), options.draw), uniform, draws, source);
+    std::vector<int> keep;
+    for (size_t row = 0; row < live.size(); ++row) {
+      if (live[row] < 0) continue;
+      Branch& b = out[live[row]];
+      const int token = drawn.tokens[row];
+      if (token < 0) throw std::runtime_error("logits without a distribution");
+      if (std::find(options.stop_tokens.begin(), options.stop_tokens.end(), token) != options.stop_tokens.end()) {
+        b.stopped = true;
+        live[row] = -1;
+        continue;
+      }
+      b.tokens.push_back(token);
+      b.logprobs.push_back(drawn.logprobs[row]);
+      keep.push_back(static_cast<int>(row));
+    }
+    if (keep.empty() || step + 1 == options.max_tokens) break;
+    if (step == 0 || 2 * keep.size() <= live.size()) {
+      const int width = static_cast<int>(keep.size());
+      std::vector<int> to(width), from(keep);
+      std::iota(to.begin(), to.end(), 0);
+      if (step == 0) std::fill(from.begin(), from.end(), 0);
+      if (step > 0 || n > 1) {
+        GenerationState next = model_->create_state(width);
+        model_->copy_state_rows(state, from, next, to);
+        state = std::move(next);
+      }
+      if (width < draws.batch_size) {
+        DrawState narrow = make_draw_state(model_->vocab_size(), width, penalised);
+        copy_draw_rows(draws, keep, narrow, to);
+        draws = std::move(narrow);
+      }
+      std::vector<int> next_live(width);
+      for (int i = 0; i < width; ++i) next_live[i] = live[keep[i]];
+      live.swap(next_live);
+      source.clear();
+    }
+    std::vector<int64_t> feed;
+    for (const int i : live) feed.push_back(i < 0 ? filler : out[i].tokens.back());
+    model_->forward_decode(feed, state, logits);
+  }
+  for (Branch& b : out) b.text = tokenizer_->decode(b.tokens);
+  return out;
 }
 
 std::string InferenceEngine::format_openai_prompt(const std::string& system,

@@ -229,6 +229,15 @@ class State:
         self.wkv = hip.DeviceArray.zeros((dims.L, B, dims.H, 64, 64), np.float16 if wkv_fp16 else np.float32)
         self.elapsed = hip.DeviceArray.zeros((B,), np.int32)
 
+    def copy_rows(self, to, rows, source=None, stream=None):
+        """Row to[i] becomes row rows[i] of `source` (default: this state, each row as it was before the call), or empty where that is -1."""
+        source = self if source is None else source
+        if source.wkv_fp16 != self.wkv_fp16 or source.shift.shape[::3] != self.shift.shape[::3]:
+            raise ValueError("states of two kinds")
+        L, _, _, C = self.shift.shape
+        hip.copy_rows([(self.shift, source.shift, 2 * L, 2 * C), (self.wkv, source.wkv, L, self.wkv.nbytes // (L * self.B)),
+                       (self.elapsed, source.elapsed, 1, 4)], self.B, source.B, to, rows, stream=stream)
+
 
 class Session:
     def __init__(self, model):

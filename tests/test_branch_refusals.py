@@ -16,6 +16,11 @@ def test_moves_in_order():
     assert "ok   any_moves_keep_what_the_rows_held" in out and "ok   the_largest_call_fits_whatever_the_cycles" in out
 
 
+def test_host_side_of_branches():
+    out = _run("branch_cpu_test")
+    assert "ok   numbers_depend_on_their_place_alone" in out and "ok   backends_with_slices_move_runs_of_rows" in out
+
+
 A = 1 << 20  # addresses that are never followed
 
 
