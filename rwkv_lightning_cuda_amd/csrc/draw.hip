@@ -8,8 +8,8 @@
 //   its log probability = -ln(1 + (K - e_token) / e_token), the difference summed without the token: nothing cancels
 //
 // Powers and sums are in 64 bits: which token is drawn goes by a comparison of two sums, and with fp32's 1e-7 one draw in some hundred
-// of a row with many candidates would come out next to the one that the definition gives.  (The fp64 vector rate of this chip is that
-// of fp32; an entry costs some twenty operations.)
+// of a row with many candidates would come out next to the one that the definition gives.  (An instruction on fp64 takes twice as long
+// as one on fp32 here; an entry costs some thirty of both.)
 //
 // Two launches.  draw_stats_kernel reads the rows with the whole chip: per 64 entries (a slot) the largest z; per 4096 (a part), where the
 // row asks for it, sums of powers and a histogram of them.  draw_pick_kernel has a block per row, which finds out how small a kept entry can be,
@@ -33,6 +33,7 @@ constexpr int kPart = 4096;      // entries of a block of draw_stats_kernel
 constexpr int kPickThreads = 512;
 constexpr int kList = 6144;      // entries
 constexpr int kBuckets = 256;    // of a histogram
+constexpr int kSums = kBuckets / 64;
 constexpr int kLast = 64;        // entries that one wavefront puts in order
 constexpr int kWaveSlots = 256;  // slots of a wavefront that reach the bound
 constexpr int kHeld = 8;         // of these, those whose entries it keeps in registers
@@ -57,11 +58,11 @@ struct DrawArgs {
   const float* penalties;  // [rows,V]
   int* token;
   float* logprob;
-  // What draw_stats_kernel leaves: the largest entry of every slot and part; for rows that need them the sums of the slots' or of the
-  // parts' powers, against the part's largest entry, and the parts' histograms: powers (times kOne) and numbers of the entries
+  // What draw_stats_kernel leaves: the largest entry of every slot and part; for rows that need them the sums of the slots' powers, against
+  // the part's largest entry, or the parts' histograms: powers (times kOne) and numbers of the entries, and the powers' sums over 64 buckets
   int parts;
   double* slot_sum;               // [rows,slots]
-  double* part_sum;               // [rows,parts]
+  double* part_sum;               // [rows,parts,kSums]
   unsigned long long* part_mass;  // [rows,parts,kBuckets]
   float* slot_max;                // [rows,slots]
   float* part_max;                // [rows,parts]
@@ -255,7 +256,6 @@ __global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
   constexpr int NV = kPart / 4 / NT;
   typedef T vec_t __attribute__((ext_vector_type(4)));
   __shared__ float most[NT / 64];
-  __shared__ double wave_sum[NT / 64];
   __shared__ unsigned long long mass[kBuckets];
   __shared__ unsigned count[kBuckets];
   const int row = blockIdx.x, part = blockIdx.y;
@@ -288,11 +288,10 @@ __global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
       for (int j = 0; j < 4; ++j) z[q][j] = i + j < a.V ? z[q][j] : -INFINITY;
     }
   }
-  if (histogram) {
-    for (int b = threadIdx.x; b < kBuckets; b += NT) {
-      mass[b] = 0;
-      count[b] = 0;
-    }
+  static_assert(NT >= kBuckets && NT % 64 == 0, "a thread for every bucket");
+  if (histogram && threadIdx.x < kBuckets) {
+    mass[threadIdx.x] = 0;
+    count[threadIdx.x] = 0;
   }
   float m = -INFINITY;
 #pragma unroll
@@ -318,7 +317,6 @@ __global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
   const int64_t at = static_cast<int64_t>(row) * a.parts + part;
   if (threadIdx.x == 0) a.part_max[at] = m;
   const double top = scalar(grid_place(m, w.octaves));
-  double all = 0.0;
   const double ninth = held_constant(kNinth), one = held_constant(kOne), two = held_constant(2.0 * kOne);
 #pragma unroll
   for (int q = 0; q < NV; ++q) {
@@ -327,7 +325,7 @@ __global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const double e = weight(z[q][j], m, w.octaves, ninth);
-      sum += e;
+      if (sums) sum += e;
       if (histogram) {  // (-infinity, and whatever a row without a distribution holds: the last bucket, with nothing)
         const int b = static_cast<int>(fmin(top - grid_place(z[q][j], w.octaves), static_cast<double>(kBuckets - 1)));
         // (2^52 + e 2^51, rounded: its last 52 bits)
@@ -339,22 +337,17 @@ __global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
       sum = row16_sum_d(sum);
       if ((threadIdx.x & 15) == 0 && slot < a.slots) a.slot_sum[static_cast<int64_t>(row) * a.slots + slot] = sum;
     }
-    all += sum;
   }
-  if (histogram) {
-    all = wave_sum_d(all);
-    if ((threadIdx.x & 63) == 0) wave_sum[threadIdx.x >> 6] = all;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      all = 0.0;
-      for (int i = 0; i < NT / 64; ++i) all += wave_sum[i];
-      a.part_sum[at] = all;
-    }
-    for (int b = threadIdx.x; b < kBuckets; b += NT) {
-      a.part_mass[at * kBuckets + b] = mass[b];
-      if (counts) a.part_count[at * kBuckets + b] = count[b];
-    }
-  }
+  if (!histogram) return;
+  // (sums of what the buckets hold: the same however many threads there were)
+  __syncthreads();
+  const int b = threadIdx.x;
+  if (b >= kBuckets) return;
+  const unsigned long long held = mass[b];
+  a.part_mass[at * kBuckets + b] = held;
+  if (counts) a.part_count[at * kBuckets + b] = count[b];
+  const double sum = wave_sum_d(static_cast<double>(held));
+  if ((b & 63) == 0) a.part_sum[at * kSums + b / 64] = sum;
 }
 
 // What one wavefront or thread finds for its block, and what wavefronts exchange: by the block functions, and at places of their own
@@ -755,7 +748,7 @@ template <typename W>
 __device__ __forceinline__ void place_window(const DrawArgs& a, PickShared& sh, int row, const W& w, float m, double top) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float* part_max = a.part_max + static_cast<int64_t>(row) * a.parts;
-  const double* part_sum = a.part_sum + static_cast<int64_t>(row) * a.parts;
+  const double* part_sum = a.part_sum + static_cast<int64_t>(row) * a.parts * kSums;
   const unsigned long long* part_mass = a.part_mass + static_cast<int64_t>(row) * a.parts * kBuckets;
   const unsigned* part_count = a.part_count + static_cast<int64_t>(row) * a.parts * kBuckets;
   const bool counts = w.top_k != INT_MAX;
@@ -763,8 +756,11 @@ __device__ __forceinline__ void place_window(const DrawArgs& a, PickShared& sh, 
   for (int p = tid; p < a.parts; p += kPickThreads) {
     const float mp = part_max[p];
     const double scale = weight(mp, m, w.octaves);
-    mine += part_sum[p] * scale;
+    double sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < kSums; ++k) sum += part_sum[p * kSums + k];
     sh.part_scale[p] = scale / kOne;
+    mine += sum * sh.part_scale[p];
     sh.part_shift[p] = mp > -INFINITY ? static_cast<int>(fmin(top - grid_place(mp, w.octaves), static_cast<double>(kBuckets))) : kBuckets;
   }
   mine = wave_sum_d(mine);
@@ -1297,7 +1293,7 @@ DrawArgs lay_out(DrawArgs a, int rows, void* workspace, size_t* bytes) {
   };
   const size_t slots = static_cast<size_t>(rows) * a.slots, parts = static_cast<size_t>(rows) * a.parts;
   take(a.slot_sum, slots);
-  take(a.part_sum, parts);
+  take(a.part_sum, parts * kSums);
   take(a.part_mass, parts * kBuckets);
   take(a.slot_max, slots);
   take(a.part_max, parts);
