@@ -840,11 +840,19 @@ __device__ __forceinline__ bool list_window(const DrawArgs& a, PickShared& sh, c
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const unsigned long long* part_mass = a.part_mass + static_cast<int64_t>(row) * a.parts * kBuckets;
   kept_above = 0.0;
-  for (int s = c0; s < c1; s += kPartSlots) {
-    const int p = s / kPartSlots;
-    double held = 0.0;
-    for (int b = lane; b < first - sh.part_shift[p]; b += 64) held += static_cast<double>(part_mass[p * kBuckets + b]);
-    kept_above += wave_sum_d(held) * sh.part_scale[p];
+  if (first > 0) {
+#pragma unroll 2
+    for (int s = c0; s < c1; s += kPartSlots) {
+      const int p = s / kPartSlots, end = first - sh.part_shift[p];
+      unsigned long long held[kSums];
+#pragma unroll
+      for (int k = 0; k < kSums; ++k) held[k] = part_mass[p * kBuckets + k * 64 + lane];
+      double sum = 0.0;
+#pragma unroll
+      for (int k = 0; k < kSums; ++k) sum += k * 64 + lane < end ? static_cast<double>(held[k]) : 0.0;
+      kept_above += sum * sh.part_scale[p];
+    }
+    kept_above = wave_sum_d(kept_above);
   }
   // each wavefront's to a share of the list
   constexpr int kShare = kList / kPickWaves;
