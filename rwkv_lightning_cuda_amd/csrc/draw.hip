@@ -37,9 +37,13 @@ constexpr int kSums = kBuckets / 64;
 constexpr int kLast = 64;        // entries that one wavefront puts in order
 constexpr int kWaveSlots = 256;  // slots of a wavefront that reach the bound
 constexpr int kHeld = 8;         // of these, those whose entries it keeps in registers
-constexpr int kMost = 256;       // of a block: with more of them the histograms say more than a list of their entries
+// Slots of a block that reach the bound: with more of them the histograms of a row that has some lead to the cut sooner than a list of the
+// entries.  V = 65536, list / window, us: 128 slots 25 / 32 at 8 rows and 55 / 60 at 256, 256 slots 32 / 33 and 64 / 61, 512 42 / 33 and 82 / 63.
+constexpr int kMost = 256;
 constexpr int kGrid = 8;         // buckets of the parts' histograms in an octave
-constexpr int kListed = 256;     // a top_k up to which a row needs no histograms
+// A top_k up to which a row does without histograms.  V = 65536, without / with them, us: 64 18 / 23 at 8 rows and 31 / 50 at 256, 256 30 / 33
+// and 48 / 64, 384 38 / 33 and 60 / 63.
+constexpr int kListed = 256;
 constexpr double kOne = 2251799813685248.0;  // 2^51: a part holds 2^12 powers of at most 1
 constexpr double kLog2eD = 1.44269504088896340736;
 constexpr double kLowestPower = -1000.0;  // octaves
@@ -1122,7 +1126,7 @@ __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) 
     if (i == wave) place = n;
     n += sh.i[i];
   }
-  bool fits = widest <= kWaveSlots && all <= kMost;
+  const bool fits = widest <= kWaveSlots && (!told || all <= kMost);
   if (fits && widest > kHeld) {
     for (int k = kHeld; k < mine_reach; ++k) entries += __popcll(__ballot(candidate(r.at(own[k] * kSlot + lane))));
     if (lane == 0) sh.entries[wave] = entries;
@@ -1276,8 +1280,9 @@ __global__ __launch_bounds__(256) void draw_penalties_kernel(int V, const float*
 
 template <typename T>
 void launch_draw(hipStream_t st, int rows, const DrawArgs& a, bool vec) {
-  // few parts: each by as many wavefronts as a block has.  (Several parts to a block, the next one requested ahead, took 10 % longer.)
-  const bool few = static_cast<int64_t>(rows) * a.parts < 4 * device_cu_count();
+  // Few parts: each by as many wavefronts as a block has.  V = 65536 without filters, 1024 threads / 256, us: 16 rows 10.5 / 11.0,
+  // 32 rows 12.3 / 11.8, 256 rows 39 / 30.  (Several parts to a block, the next one requested ahead, took 10 % longer.)
+  const bool few = static_cast<int64_t>(rows) * a.parts < 2 * device_cu_count();
   const auto stats = [&](auto aligned, auto threads) {
     constexpr bool kVec = decltype(aligned)::value;
     constexpr int kThreads = decltype(threads)::value;

@@ -148,6 +148,19 @@ def test_rows_of_any_shape(gpu, kind, V, dtype):
     check(run(gpu, z, *args, u), ref(z.astype(np.float32), *args, u))
 
 
+@pytest.mark.parametrize("V", [20000, 65536, 400000])
+@pytest.mark.parametrize("kind", ["peaked", "flat", "few values"])
+def test_every_top_k(gpu, kind, V):
+    """Where the lists end and the histograms begin, and candidates in more slots than either holds"""
+    rng = np.random.default_rng(21)
+    k = np.array([63, 64, 65, 192, 255, 256, 257, 258, 600, 2000, 7000])
+    rows = len(k)
+    z = logits_of(rng, rows, V, kind)
+    args = np.ones(rows), k, np.where(np.arange(rows) % 2, 0.98, 1.0), np.zeros(rows)
+    u = rng.random(rows).astype(np.float32)
+    check(run(gpu, z, *args, u), ref(z, *args, u))
+
+
 def test_the_largest_vocabulary(gpu):
     rng = np.random.default_rng(8)
     z = logits_of(rng, 6, 1048576, "flat")
