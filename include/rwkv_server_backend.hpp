@@ -97,7 +97,7 @@ class IModelBackend {
   virtual PrefillCapacity query_prefill_capacity(int prefill_chunk_size) const = 0;
 
   // Row to[i] of dst becomes row rows[i] of src (-1: an empty state): a sequence goes on in several places, or moves to another batch.  src and
-  // dst may be the same state; every row is then taken as it was before the call.  A row may be a destination once.  No counterpart in the
+  // dst may be the same state (up to 512 rows then); every row is taken as it was before the call.  A row may be a destination once.  No counterpart in the
   // reference.  Backends that do not override it copy runs of neighbouring rows with copy_state_slice, and refuse empty states and the same
   // state on both sides.
   virtual void copy_state_rows(const GenerationState& src, const std::vector<int>& rows, GenerationState& dst, const std::vector<int>& to) const;

@@ -185,6 +185,15 @@ HOST_TEST(a_greedy_branch_is_what_the_engine_generates) {
   for (const float p : one[0].logprobs) CHECK_EQ(p, 0.0f);
   const auto five = engine.branch_generate(prompt, 5, branch);
   for (const auto& b : five) CHECK(b.tokens == five[0].tokens);
+  // no step, and a first step that is the last
+  branch.max_tokens = 0;
+  for (const auto& b : engine.branch_generate(prompt, 3, branch)) CHECK(b.tokens.empty() && b.text.empty() && !b.stopped);
+  branch.max_tokens = 1;
+  branch.stop_tokens.clear();
+  for (const auto& b : engine.branch_generate(prompt, 3, branch)) CHECK(b.tokens == std::vector<int>(five[0].tokens.begin(), five[0].tokens.begin() + 1));
+  branch.stop_tokens = {five[0].tokens[0]};
+  branch.max_tokens = 9;
+  for (const auto& b : engine.branch_generate(prompt, 3, branch)) CHECK(b.tokens.empty() && b.stopped);
 }
 
 // Every token of every branch, given the tokens in front of it, against a pass of its own at width 1: a state or penalty row that went to the
