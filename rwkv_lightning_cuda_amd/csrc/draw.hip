@@ -45,7 +45,7 @@ constexpr int kGrid = 8;         // buckets of the parts' histograms in an octav
 // and 48 / 64, 384 38 / 33 and 60 / 63.
 constexpr int kListed = 256;
 constexpr double kOne = 2251799813685248.0;  // 2^51: a part holds 2^12 powers of at most 1
-constexpr double kLog2eD = 1.44269504088896340736;
+constexpr double kLog2eD = 1.44269504088896340736, kLn2D = 0.69314718055994530942;
 constexpr double kLowestPower = -1000.0;  // octaves
 constexpr double kWidest = 64.0;          // octaves that the first histogram covers
 
@@ -82,9 +82,15 @@ __device__ __forceinline__ double scalar(double v) {
   return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
 
+// What makes powers of differences: log2(e) / temperature, the difference that 2^kLowestPower belongs to, and buckets of the grid to a unit
+struct Power {
+  double octaves, lowest;
+  float grid;
+};
+
 // What a row asks for.  Filters that are off: top_k = INT_MAX, top_p >= 1, min_p <= 0.
 struct Wish {
-  double octaves;  // log2(e) / temperature
+  Power power;
   double top_p, min_p, u;
   int top_k, source;
   bool valid, greedy;
@@ -106,7 +112,9 @@ __device__ __forceinline__ Wish wish_of(const DrawArgs& a, int row) {
   w.u = a.uniform[row];
   w.valid = w.source >= 0 && w.source < a.logit_rows && t >= 0.0f && w.top_p == w.top_p && min_p == min_p && w.u >= 0.0 && w.u <= 1.0;
   w.greedy = t == 0.0f;
-  w.octaves = scalar(w.greedy ? 0.0 : kLog2eD / static_cast<double>(t));
+  w.power.octaves = scalar(w.greedy ? 0.0 : kLog2eD / static_cast<double>(t));
+  w.power.lowest = scalar(fmax(kLowestPower * kLn2D * static_cast<double>(t), -1e300));  // (above -infinity at any temperature)
+  w.power.grid = scalar(static_cast<float>(w.power.octaves * kGrid));
   w.top_p = scalar(w.top_p);
   w.min_p = scalar(w.min_p);
   w.u = scalar(w.u);
@@ -120,13 +128,16 @@ __device__ __forceinline__ double fma_scalar(double a, double b, double c) {
   asm("v_fma_f64 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "s"(c));
   return r;
 }
-// e of an entry z <= m; 0 for -infinity.  2^f for |f| <= 1/2 is 1 + f q(f), exact at 0, with the polynomial through (2^f - 1) / f at the nine
-// Chebyshev nodes of that range: 3.7e-14 off at most.
+// e of an entry z <= m; 0 for -infinity.  The difference's octaves are rounded by the addition of a number whose last bit is 1, and the integer
+// is what its low bits then hold.  2^f for |f| <= 1/2 is 1 + f q(f), exact at 0, with the polynomial through (2^f - 1) / f at the nine Chebyshev
+// nodes of that range: 3.7e-14 off at most.
 constexpr double kNinth = 1.0203121063391729e-07;  // the highest coefficient
-__device__ __forceinline__ double weight(float z, float m, double octaves, double ninth = kNinth) {
-  const double y = (static_cast<double>(z) - static_cast<double>(m)) * octaves;
-  const double n = rint(y);
-  const double f = y - n;
+constexpr double kRound = 6755399441055744.0;      // 1.5 2^52
+__device__ __forceinline__ double weight(float z, float m, const Power& p, double ninth = kNinth, double round = kRound) {
+  const double d = static_cast<double>(z) - static_cast<double>(m);
+  const double y = fma(d, p.octaves, round);
+  const int n = static_cast<int>(static_cast<uint32_t>(__builtin_bit_cast(uint64_t, y)));
+  const double f = fma(d, p.octaves, round - y);
   double q = fma_scalar(f, ninth, 1.3255224878668817e-06);
   q = fma_scalar(q, f, 1.525268684626772e-05);
   q = fma_scalar(q, f, 0.00015403455852453838);
@@ -135,8 +146,8 @@ __device__ __forceinline__ double weight(float z, float m, double octaves, doubl
   q = fma_scalar(q, f, 0.055504108664760424);
   q = fma_scalar(q, f, 0.2402265069581299);
   q = fma_scalar(q, f, 0.6931471805599453);
-  const double v = ldexp(fma(q, f, 1.0), static_cast<int>(n));
-  return y >= kLowestPower ? v : 0.0;  // (infinity times no octaves at all is a NaN, and none either)
+  const double v = ldexp(fma(q, f, 1.0), n);
+  return d >= p.lowest ? v : 0.0;  // (not where d is -infinity or, with an m of -infinity, a NaN)
 }
 // a constant that stays in vector registers (and is not made anew for every use)
 __device__ __forceinline__ double held_constant(double c) {
@@ -151,12 +162,43 @@ __device__ __forceinline__ double lane_xor_d(double v) {
   const uint32_t hi = static_cast<uint32_t>(lane_xor_dpp<D>(static_cast<int>(b >> 32)));
   return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
+// the value of the lane N places on, around a row of 16 (a lane that is always there: no register is cleared for those that are not)
+template <int N>
+__device__ __forceinline__ int row16_turn(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, 0x120 + N, 0xf, 0xf, true);
+}
+template <int N>
+__device__ __forceinline__ double row16_turn(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = static_cast<uint32_t>(row16_turn<N>(static_cast<int>(b)));
+  const uint32_t hi = static_cast<uint32_t>(row16_turn<N>(static_cast<int>(b >> 32)));
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
 __device__ __forceinline__ double row16_sum_d(double v) {
-  v += lane_xor_d<8>(v);
-  v += lane_xor_d<4>(v);
-  v += lane_xor_d<2>(v);
-  v += lane_xor_d<1>(v);
+  v += row16_turn<8>(v);
+  v += row16_turn<4>(v);
+  v += row16_turn<2>(v);
+  v += row16_turn<1>(v);
   return v;
+}
+__device__ __forceinline__ int row16_max(int v) {
+  v = max(v, row16_turn<8>(v));
+  v = max(v, row16_turn<4>(v));
+  v = max(v, row16_turn<2>(v));
+  return max(v, row16_turn<1>(v));
+}
+// floats as integers in the same order, and back (no NaN)
+__device__ __forceinline__ int in_order(float v) {
+  const int b = __builtin_bit_cast(int, v);
+  return b ^ (b >> 31 & INT_MAX);
+}
+__device__ __forceinline__ float from_order(int b) { return __builtin_bit_cast(float, b ^ (b >> 31 & INT_MAX)); }
+// The largest of four (the instruction itself: fmaxf would first quiet every operand); +infinity if one is a NaN
+__device__ __forceinline__ float max_of(const float (&z)[4]) {
+  float a, b;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(a) : "v"(z[0]), "v"(z[1]), "v"(z[2]));
+  asm("v_max_f32 %0, %1, %2" : "=v"(b) : "v"(a), "v"(z[3]));
+  return __builtin_isunordered(z[0], z[1]) || __builtin_isunordered(z[2], z[3]) ? INFINITY : b;
 }
 __device__ __forceinline__ double wave_sum_d(double v) {
   v += lane_xor_d<32>(v);
@@ -251,8 +293,9 @@ __device__ __forceinline__ void each_entry(const Row<T>& r, int first_slot, int 
 }
 
 // The buckets of the parts' histograms: places on one grid of kGrid to an octave, counted down from the largest entry's, so that those of
-// different parts fit together; the last one holds whatever lies lower.
-__device__ __forceinline__ double grid_place(float z, double octaves) { return floor(static_cast<double>(z) * (octaves * kGrid)); }
+// different parts fit together; the last one holds whatever lies lower.  In 32 bits: a smaller z never has a higher place, and a difference
+// of two places below kBuckets is exact (of whole numbers up to 2^24, or of two that lie within a factor of two); buckets need not be alike.
+__device__ __forceinline__ float grid_place(float z, const Power& p) { return floorf(z * p.grid); }
 
 // A block takes a part of a row in NT threads, 16 lanes a slot.  VEC: four entries are one aligned load.
 template <typename T, bool VEC, int NT>
@@ -301,13 +344,7 @@ __global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
 #pragma unroll
   for (int q = 0; q < NV; ++q) {
     const int slot = (first + q * NT * 4) / kSlot;
-    float mq = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) mq = fmaxf(mq, z[q][j] < INFINITY ? z[q][j] : INFINITY);  // (a NaN counts as +infinity: no distribution)
-    mq = fmaxf(mq, __builtin_bit_cast(float, lane_xor_dpp<8>(__builtin_bit_cast(int, mq))));
-    mq = fmaxf(mq, __builtin_bit_cast(float, lane_xor_dpp<4>(__builtin_bit_cast(int, mq))));
-    mq = fmaxf(mq, __builtin_bit_cast(float, lane_xor_dpp<2>(__builtin_bit_cast(int, mq))));
-    mq = fmaxf(mq, __builtin_bit_cast(float, lane_xor_dpp<1>(__builtin_bit_cast(int, mq))));
+    const float mq = from_order(row16_max(in_order(max_of(z[q]))));  // (a NaN counts as +infinity: no distribution)
     if ((threadIdx.x & 15) == 0 && slot < a.slots) a.slot_max[static_cast<int64_t>(row) * a.slots + slot] = mq;
     m = fmaxf(m, mq);
   }
@@ -320,18 +357,18 @@ __global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
   m = scalar(m);
   const int64_t at = static_cast<int64_t>(row) * a.parts + part;
   if (threadIdx.x == 0) a.part_max[at] = m;
-  const double top = scalar(grid_place(m, w.octaves));
-  const double ninth = held_constant(kNinth), one = held_constant(kOne), two = held_constant(2.0 * kOne);
+  const float top = scalar(grid_place(m, w.power));
+  const double ninth = held_constant(kNinth), one = held_constant(kOne), two = held_constant(2.0 * kOne), round = held_constant(kRound);
 #pragma unroll
   for (int q = 0; q < NV; ++q) {
     const int slot = (first + q * NT * 4) / kSlot;
     double sum = 0.0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const double e = weight(z[q][j], m, w.octaves, ninth);
+      const double e = weight(z[q][j], m, w.power, ninth, round);
       if (sums) sum += e;
       if (histogram) {  // (-infinity, and whatever a row without a distribution holds: the last bucket, with nothing)
-        const int b = static_cast<int>(fmin(top - grid_place(z[q][j], w.octaves), static_cast<double>(kBuckets - 1)));
+        const int b = static_cast<int>(fminf(top - grid_place(z[q][j], w.power), static_cast<float>(kBuckets - 1)));
         // (2^52 + e 2^51, rounded: its last 52 bits)
         atomicAdd(&mass[b], __builtin_bit_cast(unsigned long long, fma(e, one, two)) - 0x4330000000000000ull);
         if (counts) atomicAdd(&count[b], 1u);
@@ -504,7 +541,7 @@ __device__ __forceinline__ int equal_ones(const Cut& cut, int above, double abov
 // equal ones.  False: the cut lies behind the span (`inside`: it is known not to).  Sums in fixed point: any order of the additions gives
 // the same.
 template <typename S, typename R>
-__device__ __forceinline__ bool find_cut(S& sh, const R* row, int c0, int c1, int n, const Cut& cut, float m, double octaves, int V, Span span,
+__device__ __forceinline__ bool find_cut(S& sh, const R* row, int c0, int c1, int n, const Cut& cut, float m, const Power& power, int V, Span span,
                                          Buckets buckets, bool inside, Found& found) {
   constexpr int kThreads = S::kWaves * 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -533,7 +570,7 @@ __device__ __forceinline__ bool find_cut(S& sh, const R* row, int c0, int c1, in
     each([&](float z) {
       const int b = buckets.of(z);
       atomicAdd(&sh.count[b], 1u);
-      if (cut.mass < INFINITY) atomicAdd(&sh.mass[b], static_cast<unsigned long long>(fma(weight(z, m, octaves), per_unit, 0.5)));
+      if (cut.mass < INFINITY) atomicAdd(&sh.mass[b], static_cast<unsigned long long>(fma(weight(z, m, power), per_unit, 0.5)));
     });
     __syncthreads();
     if (wave == 0) find_bucket(sh, cut, span.above, span.above_mass, unit, inside);
@@ -568,7 +605,7 @@ __device__ __forceinline__ bool find_cut(S& sh, const R* row, int c0, int c1, in
     const bool equal = span.low == span.high, last = equal || count <= kLast;
     if (last || (!in_list && count <= S::kList)) {
       // in order of their indexes: equal ones are counted, a few go to one wavefront, and those of a row that fit it to the list
-      const int want = equal ? equal_ones(cut, span.above, span.above_mass, count, weight(span.low, m, octaves)) : 0;
+      const int want = equal ? equal_ones(cut, span.above, span.above_mass, count, weight(span.low, m, power)) : 0;
       const int q = (n + kThreads - 1) / kThreads, k0 = min(tid * q, n), k1 = min(k0 + q, n);
       int have = 0, sum;
       if (in_list) {
@@ -609,7 +646,7 @@ __device__ __forceinline__ bool find_cut(S& sh, const R* row, int c0, int c1, in
       if (last) {
         if (!equal && wave == 0) {
           const float z = lane < count ? sh.last_z[lane] : -INFINITY;
-          const double e = weight(z, m, octaves);
+          const double e = weight(z, m, power);
           int rank = 0;
           double ahead = 0.0;
           rank_of(z, e, count, rank, ahead);
@@ -650,7 +687,7 @@ __device__ __forceinline__ void draw_from_few(const S& sh, int n, const Wish& w,
   const int lane = threadIdx.x & 63;
   const float z = lane < n ? sh.list_z[lane] : -INFINITY;
   const int i = lane < n ? sh.list_i[lane] : 0;
-  const double e = weight(z, m, w.octaves);
+  const double e = weight(z, m, w.power);
   bool kept = lane < n;
   if (!cut.open()) {
     int rank = 0;
@@ -682,7 +719,7 @@ __device__ __forceinline__ void draw_from_list(S& sh, int n, const Wish& w, cons
     const int k = tid * q + j;
     if (j < q && k < n) {
       const float z = sh.list_z[k];
-      const double v = weight(z, m, w.octaves);
+      const double v = weight(z, m, w.power);
       if (found.keeps(z, sh.list_i[k]) && w.likely(v)) e[j] = v;
     }
     mine += e[j];
@@ -713,7 +750,7 @@ __device__ __forceinline__ void draw_from_list(S& sh, int n, const Wish& w, cons
   for (int j = 0; j < kMine; ++j)
     if (tid * q + j != at || j >= q) others += e[j];
   others = block_sum_d(others, sh.d2);
-  if (tid == 0) answer(sh.list_i[at], static_cast<float>(-log1p(others / weight(sh.list_z[at], m, w.octaves))));
+  if (tid == 0) answer(sh.list_i[at], static_cast<float>(-log1p(others / weight(sh.list_z[at], m, w.power))));
 }
 
 constexpr int kPickWaves = kPickThreads / 64;
@@ -733,14 +770,15 @@ static_assert(kMaxLogprobVocab / kSlot / kPickWaves * sizeof(double) <= kList * 
 static_assert(kPickThreads % kBuckets == 0, "so many threads for a bucket");
 
 // The smallest float whose place on the grid is at least `place`; false: not found next to where it should be
-__device__ __forceinline__ bool grid_edge(double place, double octaves, float& z) {
-  z = octaves > 0.0 ? static_cast<float>(fmin(fmax(place / (octaves * kGrid), -static_cast<double>(FLT_MAX)), static_cast<double>(FLT_MAX))) : -FLT_MAX;
+__device__ __forceinline__ bool grid_edge(double place, const Power& p, float& z) {
+  constexpr double kMax = FLT_MAX;
+  z = p.grid > 0.0f ? static_cast<float>(fmin(fmax(place / p.grid, -kMax), kMax)) : -FLT_MAX;
   int left = 16;
-  while (grid_place(z, octaves) >= place && z > -FLT_MAX && left > 0) {
+  while (grid_place(z, p) >= place && z > -FLT_MAX && left > 0) {
     z = nextafterf(z, -INFINITY);
     --left;
   }
-  while (grid_place(z, octaves) < place && z < FLT_MAX && left > 0) {
+  while (grid_place(z, p) < place && z < FLT_MAX && left > 0) {
     z = nextafterf(z, INFINITY);
     --left;
   }
@@ -749,7 +787,7 @@ __device__ __forceinline__ bool grid_edge(double place, double octaves, float& z
 
 // The row's histogram out of its parts': the cut's sum, and the bucket in which the cut lies, or that of the least entry that min_p keeps
 template <typename W>
-__device__ __forceinline__ void place_window(const DrawArgs& a, PickShared& sh, int row, const W& w, float m, double top) {
+__device__ __forceinline__ void place_window(const DrawArgs& a, PickShared& sh, int row, const W& w, float m, float top) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const float* part_max = a.part_max + static_cast<int64_t>(row) * a.parts;
   const double* part_sum = a.part_sum + static_cast<int64_t>(row) * a.parts * kSums;
@@ -759,13 +797,13 @@ __device__ __forceinline__ void place_window(const DrawArgs& a, PickShared& sh, 
   double mine = 0.0;
   for (int p = tid; p < a.parts; p += kPickThreads) {
     const float mp = part_max[p];
-    const double scale = weight(mp, m, w.octaves);
+    const double scale = weight(mp, m, w.power);
     double sum = 0.0;
 #pragma unroll
     for (int k = 0; k < kSums; ++k) sum += part_sum[p * kSums + k];
     sh.part_scale[p] = scale / kOne;
     mine += sum * sh.part_scale[p];
-    sh.part_shift[p] = mp > -INFINITY ? static_cast<int>(fmin(top - grid_place(mp, w.octaves), static_cast<double>(kBuckets))) : kBuckets;
+    sh.part_shift[p] = mp > -INFINITY ? static_cast<int>(fminf(top - grid_place(mp, w.power), static_cast<float>(kBuckets))) : kBuckets;
   }
   mine = wave_sum_d(mine);
   if (lane == 0) sh.total[wave] = mine;
@@ -822,15 +860,18 @@ __device__ __forceinline__ void place_window(const DrawArgs& a, PickShared& sh, 
       if (cut_at == kBuckets && cut.reached(at, at_held)) cut_at = lane * kPer + k;
     }
     cut_at = wave_reduce_dpp(cut_at, [](int x, int y) { return min(x, y); });
-    int likely_at = kBuckets;
-    if (w.min_p > 0.0) {  // (rounding: one more on either side)
-      const double z = m + log2(w.min_p) / w.octaves;
-      likely_at = static_cast<int>(fmin(fmax(top - floor(z * (w.octaves * kGrid)), 0.0), static_cast<double>(kBuckets)));
+    // and the buckets of an entry that min_p surely keeps and of one that it surely does not
+    int kept_at = kBuckets, dropped_at = kBuckets;
+    if (w.min_p > 0.0) {
+      const double edge = log2(w.min_p);
+      const auto bucket = [&](float z) { return static_cast<int>(fminf(fmaxf(top - grid_place(z, w.power), 0.0f), static_cast<float>(kBuckets))); };
+      kept_at = bucket(nextafterf(static_cast<float>(m + (edge + 1e-3) / w.power.octaves), INFINITY));
+      dropped_at = bucket(nextafterf(static_cast<float>(m + (edge - 1e-3) / w.power.octaves), -INFINITY));
     }
     if (lane == 0) {
       sh.mass_at = cut.mass;
-      sh.first = min(cut_at, max(likely_at - 1, 0));
-      sh.last = min(cut_at, likely_at + 1);
+      sh.first = min(cut_at, kept_at);
+      sh.last = min(cut_at, dropped_at);
     }
   }
   __syncthreads();
@@ -981,7 +1022,7 @@ __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) 
   }
 
   const float* part_max = a.part_max + static_cast<int64_t>(row) * a.parts;
-  const auto slot_share = [&](int s) { return slot_sum[s] * weight(part_max[s / (kPart / kSlot)], m, w.octaves); };
+  const auto slot_share = [&](int s) { return slot_sum[s] * weight(part_max[s / (kPart / kSlot)], m, w.power); };
   double mine = 0.0;
 
   if (w.free()) {
@@ -1011,7 +1052,7 @@ __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) 
     for (int s = s0; s < s1; ++s)
       if (s != slot) others += slot_share(s);
     others = block_sum_d(others, sh.d2);
-    if (wave == 0) draw_entry([&](float z, int) { return weight(z, m, w.octaves); }, r, slot, sh.before, target, others, answer);
+    if (wave == 0) draw_entry([&](float z, int) { return weight(z, m, w.power); }, r, slot, sh.before, target, others, answer);
     return;
   }
 
@@ -1023,17 +1064,18 @@ __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) 
   int first = 0;
   bool told = false;  // the window is known
   if (histogram) {
-    const double top = grid_place(m, w.octaves);
+    const float top = grid_place(m, w.power);
     place_window(a, sh, row, w, m, top);
     cut.mass = scalar(sh.mass_at);
     first = scalar(sh.first);
     const int last = scalar(sh.last);
-    told = last < kBuckets - 1 && grid_edge(top - last, w.octaves, low) && (first == 0 || grid_edge(top - first + 1.0, w.octaves, high));
+    const double from = top;
+    told = last < kBuckets - 1 && grid_edge(from - last, w.power, low) && (first == 0 || grid_edge(from - first + 1.0, w.power, high));
     if (!told) low = -FLT_MAX;
   } else {
     const bool summed = w.needs_sums();
     double range = scalar(static_cast<double>(m) - static_cast<double>(lowest));
-    if (range * w.octaves > kWidest) range = kWidest / w.octaves;
+    if (range * w.power.octaves > kWidest) range = kWidest / w.power.octaves;
     const Buckets rough = buckets_of(m, scalar(range));
     constexpr double kUnit = 1.0 / (1ll << 40);  // (a row's sum is at most 2^20)
     for (int s = s0; s < s1; ++s) {
@@ -1055,7 +1097,7 @@ __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) 
     for (int i = 0; i < kPickWaves; ++i) total += sh.total[i];
     total = scalar(total);
     cut.mass = scalar(w.top_p < 1.0 ? w.top_p * total : INFINITY);
-    const double width = scalar(range * w.octaves / kBuckets);  // octaves of a bucket
+    const double width = scalar(range * w.power.octaves / kBuckets);  // octaves of a bucket
     const auto edge = [&](int b) { return __builtin_amdgcn_exp2f(static_cast<float>(-(b + 1) * width)); };  // the least power of a bucket
     if (wave == 0) {
       // Bucket b bounds the kept entries if, of the entries up to it, there are top_k (as many slots reach it), or top_p (what is in other
@@ -1160,8 +1202,8 @@ __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) 
     }
     Found found = {-INFINITY, INT_MAX};
     if (!cut.open())
-      find_cut(sh, static_cast<const Row<T>*>(nullptr), 0, 0, n, cut, m, w.octaves, a.V, {0, 0.0, -FLT_MAX, FLT_MAX},
-               buckets_of(m, fmin(static_cast<double>(m) - low, kWidest / w.octaves)), false, found);
+      find_cut(sh, static_cast<const Row<T>*>(nullptr), 0, 0, n, cut, m, w.power, a.V, {0, 0.0, -FLT_MAX, FLT_MAX},
+               buckets_of(m, fmin(static_cast<double>(m) - low, kWidest / w.power.octaves)), false, found);
     draw_from_list(sh, n, w, found, m, answer);
     return;
   }
@@ -1181,13 +1223,13 @@ __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) 
   }
   if (!cut.open()) {
     const double from = fmin(span.high, m);
-    find_cut(sh, windowed ? nullptr : &r, c0, c1, windowed ? n : 0, cut, m, w.octaves, a.V, span,
-             buckets_of(from, fmin(from - span.low, kWidest / w.octaves)), false, found);
+    find_cut(sh, windowed ? nullptr : &r, c0, c1, windowed ? n : 0, cut, m, w.power, a.V, span,
+             buckets_of(from, fmin(from - span.low, kWidest / w.power.octaves)), false, found);
   }
 
   // the kept entries' sums by wavefronts, of the entry's wavefront by slots, of its slot by entries
   const auto kept_weight = [&](float z, int i) {
-    const double e = weight(z, m, w.octaves);
+    const double e = weight(z, m, w.power);
     return found.keeps(z, i) && w.likely(e) ? e : 0.0;
   };
   double share = 0.0;
