@@ -1132,69 +1132,75 @@ __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) 
     }
     __syncthreads();
     const int bound = scalar(sh.bucket);
-    if (bound < kBuckets - 1) low = nextafterf(static_cast<float>(m - (bound + 1) * range / kBuckets), -INFINITY);
+    if (bound < kBuckets - 1) low = fmaxf(nextafterf(static_cast<float>(m - (bound + 1) * range / kBuckets), -INFINITY), -FLT_MAX);
   }
   const auto candidate = [&](float z) { return z >= low; };
 
-  // the slots that reach the bound, each wavefront its own, in order; the entries of the first ones are requested at once
-  int reach = 0;
+  // the slots that reach the bound, each wavefront its own
+  int reach = 0, n = 0;
   for (int s = s0; s < s1; ++s) reach += candidate(slot_max[s]);
   const int reach_upto = wave_upto(reach);
   const int mine_reach = __builtin_amdgcn_readlane(reach_upto, 63);
-  uint16_t* own = sh.slots[wave];
-  for (int s = s0, to = reach_upto - reach; s < s1; ++s)
-    if (candidate(slot_max[s])) {
-      if (to < kWaveSlots) own[to] = static_cast<uint16_t>(s);
-      ++to;
-    }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  float held[kHeld];
-#pragma unroll
-  for (int k = 0; k < kHeld; ++k) held[k] = k < mine_reach ? r.at(own[k] * kSlot + lane) : -INFINITY;
-  int entries = 0;
-#pragma unroll
-  for (int k = 0; k < kHeld; ++k) entries += __popcll(__ballot(candidate(held[k])));
-  if (lane == 0) {
-    sh.reach[wave] = mine_reach;
-    sh.i[wave] = entries;
-  }
+  if (lane == 0) sh.reach[wave] = mine_reach;
   __syncthreads();
-  int all = 0, widest = 0, n = 0, place = 0;
+  int all = 0, widest = 0;
 #pragma unroll
   for (int i = 0; i < kPickWaves; ++i) {
     all += sh.reach[i];
     widest = max(widest, sh.reach[i]);
-    if (i == wave) place = n;
-    n += sh.i[i];
   }
-  const bool fits = widest <= kWaveSlots && (!told || all <= kMost);
-  if (fits && widest > kHeld) {
-    for (int k = kHeld; k < mine_reach; ++k) entries += __popcll(__ballot(candidate(r.at(own[k] * kSlot + lane))));
-    if (lane == 0) sh.entries[wave] = entries;
+  all = scalar(all);
+  widest = scalar(widest);
+  bool fits = widest <= kWaveSlots && (!told || all <= kMost);
+  if (fits) {
+    // in order; their entries kHeld slots at a time, the first of which stay in registers
+    uint16_t* own = sh.slots[wave];
+    for (int s = s0, to = reach_upto - reach; s < s1; ++s)
+      if (candidate(slot_max[s])) own[to++] = static_cast<uint16_t>(s);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const auto load = [&](int k0, int (&slot)[kHeld], float (&z)[kHeld]) {
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k) slot[k] = own[min(k0 + k, mine_reach - 1)];
+      r.gather(slot, lane, z);
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k) z[k] = k0 + k < mine_reach && slot[k] * kSlot + lane < a.V ? z[k] : -INFINITY;
+    };
+    int slot[kHeld], place = 0, entries = 0;
+    float held[kHeld];
+    if (mine_reach > 0) load(0, slot, held);
+    for (int k0 = 0; k0 < mine_reach;) {
+      if (k0 > 0) load(k0, slot, held);
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k) entries += __popcll(__ballot(candidate(held[k])));
+      k0 += kHeld;
+    }
+    if (lane == 0) sh.i[wave] = entries;
     __syncthreads();
-    n = 0;
 #pragma unroll
     for (int i = 0; i < kPickWaves; ++i) {
       if (i == wave) place = n;
-      n += sh.entries[i];
+      n += sh.i[i];
+    }
+    n = scalar(n);
+    fits = n <= kList;
+    if (fits) {
+      for (int k0 = 0; k0 < mine_reach; k0 += kHeld) {
+        if (mine_reach > kHeld) load(k0, slot, held);
+#pragma unroll
+        for (int k = 0; k < kHeld; ++k) {
+          const uint64_t hit = __ballot(candidate(held[k]));
+          if (hit >> lane & 1) {
+            const int to = place + __popcll(hit & ((1ull << lane) - 1));
+            sh.list_z[to] = held[k];
+            sh.list_i[to] = slot[k] * kSlot + lane;
+          }
+          place += __popcll(hit);
+        }
+      }
     }
   }
-  n = scalar(n);
-  if (fits && n <= kList) {
-    const auto put = [&](float z, int slot) {
-      const uint64_t hit = __ballot(candidate(z));
-      if (hit >> lane & 1) {
-        const int to = place + __popcll(hit & ((1ull << lane) - 1));
-        sh.list_z[to] = z;
-        sh.list_i[to] = slot * kSlot + lane;
-      }
-      place += __popcll(hit);
-    };
-#pragma unroll
-    for (int k = 0; k < kHeld; ++k)
-      if (k < mine_reach) put(held[k], own[k]);
-    for (int k = kHeld; k < mine_reach; ++k) put(r.at(own[k] * kSlot + lane), own[k]);
+  if (fits) {
     __syncthreads();
     if (n <= 64) {
       if (wave == 0) draw_from_few(sh, n, w, cut, m, answer);
