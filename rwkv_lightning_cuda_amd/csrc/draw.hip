@@ -38,12 +38,14 @@ constexpr int kLast = 64;        // entries that one wavefront puts in order
 constexpr int kWaveSlots = 256;  // slots of a wavefront that reach the bound
 constexpr int kHeld = 8;         // of these, those whose entries it keeps in registers
 // Slots of a block that reach the bound: with more of them the histograms of a row that has some lead to the cut sooner than a list of the
-// entries.  V = 65536, list / window, us: 128 slots 25 / 32 at 8 rows and 55 / 60 at 256, 256 slots 32 / 33 and 64 / 61, 512 42 / 33 and 82 / 63.
-constexpr int kMost = 256;
+// entries.  V = 65536, list / window, us: 225 slots 26 / 31 at 8 rows and 49 / 55 at 256, 400 slots 31 / 31 and 55 / 56, 640 39 / 31 and 64 / 56.
+constexpr int kMost = 384;
+// A top_k up to which a row does without histograms, and the most slots to a place of it (the slots' maxima bound the kept entries the worse the
+// fewer they are).  Without / with histograms, us: 8 rows of 65536, top_k 128 19 / 23, 512 30 / 31, 640 34 / 31; 128 rows 23 / 36, 34 / 43, 47 / 43;
+// 8 rows of 16384 (256 slots), top_k 128 20 / 22, 192 24 / 24, 256 56 / 26; of 4096 (64 slots), 32 19 / 19, 64 29 / 23.
+constexpr int kListed = 512;
+constexpr int kSlotsListed = 2;
 constexpr int kGrid = 8;         // buckets of the parts' histograms in an octave
-// A top_k up to which a row does without histograms.  V = 65536, without / with them, us: 64 18 / 23 at 8 rows and 31 / 50 at 256, 256 30 / 33
-// and 48 / 64, 384 38 / 33 and 60 / 63.
-constexpr int kListed = 256;
 constexpr double kOne = 2251799813685248.0;  // 2^51: a part holds 2^12 powers of at most 1
 constexpr double kLog2eD = 1.44269504088896340736, kLn2D = 0.69314718055994530942;
 constexpr double kLowestPower = -1000.0;  // octaves
@@ -92,12 +94,12 @@ struct Power {
 struct Wish {
   Power power;
   double top_p, min_p, u;
-  int top_k, source;
+  int top_k, listed, source;
   bool valid, greedy;
   __device__ __forceinline__ bool free() const { return top_k == INT_MAX && top_p >= 1.0 && min_p <= 0.0; }
   __device__ __forceinline__ bool likely(double e) const { return !(min_p > 0.0) || e >= min_p; }
   // (a list of top_k entries, and of the rest of their slots, is short)
-  __device__ __forceinline__ bool needs_histogram() const { return !greedy && !free() && top_k > kListed; }
+  __device__ __forceinline__ bool needs_histogram() const { return !greedy && !free() && top_k > listed; }
   __device__ __forceinline__ bool needs_sums() const { return !greedy && (free() || (top_p < 1.0 && !needs_histogram())); }
 };
 __device__ __forceinline__ Wish wish_of(const DrawArgs& a, int row) {
@@ -106,6 +108,7 @@ __device__ __forceinline__ Wish wish_of(const DrawArgs& a, int row) {
   w.source = a.source ? a.source[row] : row;
   w.top_k = a.top_k ? a.top_k[row] : 0;
   if (w.top_k <= 0 || w.top_k >= a.V) w.top_k = INT_MAX;
+  w.listed = min(kListed, a.slots / kSlotsListed);
   w.top_p = a.top_p ? a.top_p[row] : 1.0f;
   w.min_p = a.min_p ? fminf(a.min_p[row], 1.0f) : 0.0f;
   const float min_p = a.min_p ? a.min_p[row] : 0.0f;

@@ -153,7 +153,7 @@ def test_rows_of_any_shape(gpu, kind, V, dtype):
 def test_every_top_k(gpu, kind, V):
     """Where the lists end and the histograms begin, and candidates in more slots than either holds"""
     rng = np.random.default_rng(21)
-    k = np.array([63, 64, 65, 192, 255, 256, 257, 258, 600, 2000, 7000])
+    k = np.array([63, 64, 65, 192, 255, 256, 257, 258, 600, 2000, 7000, 384, 500, 511, 512, 513, V // 128 - 1, V // 128, V // 128 + 1])
     rows = len(k)
     z = logits_of(rng, rows, V, kind)
     args = np.ones(rows), k, np.where(np.arange(rows) % 2, 0.98, 1.0), np.zeros(rows)
