@@ -165,30 +165,34 @@ __device__ __forceinline__ double lane_xor_d(double v) {
   const uint32_t hi = static_cast<uint32_t>(lane_xor_dpp<D>(static_cast<int>(b >> 32)));
   return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
-// the value of the lane N places on, around a row of 16 (a lane that is always there: no register is cleared for those that are not)
-template <int N>
-__device__ __forceinline__ int row16_turn(int v) {
-  return __builtin_amdgcn_update_dpp(0, v, 0x120 + N, 0xf, 0xf, true);
+// The value of a lane with which this one shares a step of a sum over 2, 4, 8 or 16 lanes (where the steps before it have made equal what
+// lies closer).  It is always there: no register is cleared for lanes that are not.
+template <int STEP>
+__device__ __forceinline__ int partner(int v) {
+  constexpr int kCtrl = STEP == 1 ? 0xB1 : STEP == 2 ? 0x4E : STEP == 4 ? 0x141 : 0x128;  // lane ^ 1, ^ 2, 7 - lane of 8, 8 places on
+  return __builtin_amdgcn_update_dpp(0, v, kCtrl, 0xf, 0xf, true);
 }
-template <int N>
-__device__ __forceinline__ double row16_turn(double v) {
+template <int STEP>
+__device__ __forceinline__ double partner(double v) {
   const uint64_t b = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = static_cast<uint32_t>(row16_turn<N>(static_cast<int>(b)));
-  const uint32_t hi = static_cast<uint32_t>(row16_turn<N>(static_cast<int>(b >> 32)));
+  const uint32_t lo = static_cast<uint32_t>(partner<STEP>(static_cast<int>(b)));
+  const uint32_t hi = static_cast<uint32_t>(partner<STEP>(static_cast<int>(b >> 32)));
   return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
+template <int LANES = 16>
 __device__ __forceinline__ double row16_sum_d(double v) {
-  v += row16_turn<8>(v);
-  v += row16_turn<4>(v);
-  v += row16_turn<2>(v);
-  v += row16_turn<1>(v);
+  v += partner<1>(v);
+  v += partner<2>(v);
+  v += partner<4>(v);
+  if constexpr (LANES == 16) v += partner<8>(v);
   return v;
 }
+template <int LANES>
 __device__ __forceinline__ int row16_max(int v) {
-  v = max(v, row16_turn<8>(v));
-  v = max(v, row16_turn<4>(v));
-  v = max(v, row16_turn<2>(v));
-  return max(v, row16_turn<1>(v));
+  v = max(v, partner<1>(v));
+  v = max(v, partner<2>(v));
+  v = max(v, partner<4>(v));
+  return LANES == 16 ? max(v, partner<8>(v)) : v;
 }
 // floats as integers in the same order, and back (no NaN)
 __device__ __forceinline__ int in_order(float v) {
@@ -196,12 +200,17 @@ __device__ __forceinline__ int in_order(float v) {
   return b ^ (b >> 31 & INT_MAX);
 }
 __device__ __forceinline__ float from_order(int b) { return __builtin_bit_cast(float, b ^ (b >> 31 & INT_MAX)); }
-// The largest of four (the instruction itself: fmaxf would first quiet every operand); +infinity if one is a NaN
-__device__ __forceinline__ float max_of(const float (&z)[4]) {
-  float a, b;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(a) : "v"(z[0]), "v"(z[1]), "v"(z[2]));
-  asm("v_max_f32 %0, %1, %2" : "=v"(b) : "v"(a), "v"(z[3]));
-  return __builtin_isunordered(z[0], z[1]) || __builtin_isunordered(z[2], z[3]) ? INFINITY : b;
+// The largest of N (the instruction itself: fmaxf would first quiet every operand); +infinity if one is a NaN
+template <int N>
+__device__ __forceinline__ float max_of(const float (&z)[N]) {
+  float m = z[0];
+  bool nan = false;
+#pragma unroll
+  for (int j = 0; j < N; j += 2) {
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(m) : "v"(m), "v"(z[j]), "v"(z[j + 1]));
+    nan |= __builtin_isunordered(z[j], z[j + 1]);
+  }
+  return nan ? INFINITY : m;
 }
 __device__ __forceinline__ double wave_sum_d(double v) {
   v += lane_xor_d<32>(v);
@@ -300,10 +309,14 @@ __device__ __forceinline__ void each_entry(const Row<T>& r, int first_slot, int 
 // of two places below kBuckets is exact (of whole numbers up to 2^24, or of two that lie within a factor of two); buckets need not be alike.
 __device__ __forceinline__ float grid_place(float z, const Power& p) { return floorf(z * p.grid); }
 
-// A block takes a part of a row in NT threads, 16 lanes a slot.  VEC: four entries are one aligned load.
-template <typename T, bool VEC, int NT>
+// A block takes a part of a row in NT threads, each E entries at a time: so many neighbours add up as E / 4 sums of four, then those, then the
+// slot's threads, in the same order whatever E is.  VEC: four entries are one aligned load.  What bounds it: the loads and what is computed, one
+// after the other in a block and only in part beside one another (512 rows of 65536, us: loads and maxima alone 26, that is 5.1 TB/s; sums of the
+// entries themselves 30; of their powers 40; histograms 45).
+template <typename T, bool VEC, int NT, int E>
 __global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
-  constexpr int NV = kPart / 4 / NT;
+  constexpr int NV = kPart / E / NT, kLanes = kSlot / E;
+  static_assert(E == 4 || E == 8, "a slot is 16 or 8 lanes");
   typedef T vec_t __attribute__((ext_vector_type(4)));
   __shared__ float most[NT / 64];
   __shared__ unsigned long long mass[kBuckets];
@@ -313,29 +326,35 @@ __global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
   if (!w.valid) return;
   const Row<T> r = row_of<T>(a, row, w.source);
   const bool sums = w.needs_sums(), histogram = w.needs_histogram(), counts = w.top_k != INT_MAX;
-  const int first = part * kPart + threadIdx.x * 4;
-  float z[NV][4];
+  const int first = part * kPart + threadIdx.x * E;
+  float z[NV][E];
 #pragma unroll
   for (int q = 0; q < NV; ++q) {
-    const int i = first + q * NT * 4;
-    if (VEC && i + 4 <= a.V) {
-      const vec_t l = *reinterpret_cast<const vec_t*>(r.logits + i);
+    const int i = first + q * NT * E;
+    if (VEC && i + E <= a.V) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) z[q][j] = static_cast<float>(l[j]);
+      for (int k = 0; k < E; k += 4) {
+        const vec_t l = *reinterpret_cast<const vec_t*>(r.logits + i + k);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) z[q][k + j] = static_cast<float>(l[j]);
+      }
       if (r.penalties) {
-        const float4_t p = *reinterpret_cast<const float4_t*>(r.penalties + i);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) z[q][j] -= p[j];
+        for (int k = 0; k < E; k += 4) {
+          const float4_t p = *reinterpret_cast<const float4_t*>(r.penalties + i + k);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) z[q][k + j] -= p[j];
+        }
       }
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) z[q][j] = r.logit(min(i + j, a.V - 1));
+      for (int j = 0; j < E; ++j) z[q][j] = r.logit(min(i + j, a.V - 1));
       if (r.penalties) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) z[q][j] -= r.penalty(min(i + j, a.V - 1));
+        for (int j = 0; j < E; ++j) z[q][j] -= r.penalty(min(i + j, a.V - 1));
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) z[q][j] = i + j < a.V ? z[q][j] : -INFINITY;
+      for (int j = 0; j < E; ++j) z[q][j] = i + j < a.V ? z[q][j] : -INFINITY;
     }
   }
   static_assert(NT >= kBuckets && NT % 64 == 0, "a thread for every bucket");
@@ -346,9 +365,9 @@ __global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
   float m = -INFINITY;
 #pragma unroll
   for (int q = 0; q < NV; ++q) {
-    const int slot = (first + q * NT * 4) / kSlot;
-    const float mq = from_order(row16_max(in_order(max_of(z[q]))));  // (a NaN counts as +infinity: no distribution)
-    if ((threadIdx.x & 15) == 0 && slot < a.slots) a.slot_max[static_cast<int64_t>(row) * a.slots + slot] = mq;
+    const int slot = (first + q * NT * E) / kSlot;
+    const float mq = from_order(row16_max<kLanes>(in_order(max_of(z[q]))));  // (a NaN counts as +infinity: no distribution)
+    if (threadIdx.x % kLanes == 0 && slot < a.slots) a.slot_max[static_cast<int64_t>(row) * a.slots + slot] = mq;
     m = fmaxf(m, mq);
   }
   if (!sums && !histogram) return;
@@ -364,12 +383,18 @@ __global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
   const double ninth = held_constant(kNinth), one = held_constant(kOne), two = held_constant(2.0 * kOne), round = held_constant(kRound);
 #pragma unroll
   for (int q = 0; q < NV; ++q) {
-    const int slot = (first + q * NT * 4) / kSlot;
-    double sum = 0.0;
+    const int slot = (first + q * NT * E) / kSlot;
+    double sum = 0.0, four = 0.0;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < E; ++j) {
       const double e = weight(z[q][j], m, w.power, ninth, round);
-      if (sums) sum += e;
+      if (sums) {
+        four += e;
+        if (j % 4 == 3) {
+          sum += four;
+          four = 0.0;
+        }
+      }
       if (histogram) {  // (-infinity, and whatever a row without a distribution holds: the last bucket, with nothing)
         const int b = static_cast<int>(fminf(top - grid_place(z[q][j], w.power), static_cast<float>(kBuckets - 1)));
         // (2^52 + e 2^51, rounded: its last 52 bits)
@@ -378,8 +403,8 @@ __global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
       }
     }
     if (sums) {
-      sum = row16_sum_d(sum);
-      if ((threadIdx.x & 15) == 0 && slot < a.slots) a.slot_sum[static_cast<int64_t>(row) * a.slots + slot] = sum;
+      sum = row16_sum_d<kLanes>(sum);
+      if (threadIdx.x % kLanes == 0 && slot < a.slots) a.slot_sum[static_cast<int64_t>(row) * a.slots + slot] = sum;
     }
   }
   if (!histogram) return;
@@ -1334,10 +1359,12 @@ void launch_draw(hipStream_t st, int rows, const DrawArgs& a, bool vec) {
   // Few parts: each by as many wavefronts as a block has.  V = 65536 without filters, 1024 threads / 256, us: 16 rows 10.5 / 11.0,
   // 32 rows 12.3 / 11.8, 256 rows 39 / 30.  (Several parts to a block, the next one requested ahead, took 10 % longer.)
   const bool few = static_cast<int64_t>(rows) * a.parts < 2 * device_cu_count();
+  // Eight neighbours to a thread take fewer steps to a slot's sum (256 rows without filters 31.2 -> 29.9), but single loads reach over twice the
+  // distance (77 rows of 50277 fp16 47.9 -> 48.2).
   const auto stats = [&](auto aligned, auto threads) {
     constexpr bool kVec = decltype(aligned)::value;
     constexpr int kThreads = decltype(threads)::value;
-    hipLaunchKernelGGL((draw_stats_kernel<T, kVec, kThreads>), dim3(rows, a.parts), dim3(kThreads), 0, st, a);
+    hipLaunchKernelGGL((draw_stats_kernel<T, kVec, kThreads, kVec && kThreads == 256 ? 8 : 4>), dim3(rows, a.parts), dim3(kThreads), 0, st, a);
   };
   if (vec && few) stats(std::true_type{}, std::integral_constant<int, 1024>{});
   else if (vec) stats(std::true_type{}, std::integral_constant<int, 256>{});
