@@ -1339,6 +1339,9 @@ __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) 
 }
 
 // What the penalties are after the token: all decayed, the token's own raised by `presence` where it had none, else by `frequency`.
+// Bound by memory (64 rows of 65536: 6 us, 5.6 TB/s); all of a thread's entries are requested ahead of its first store.  (Entries behind the row's
+// end are read as its last one, which another thread may have written already where out is penalties: what they hold is not used.)
+constexpr int kEach = 8;  // entries of a thread
 __global__ __launch_bounds__(256) void draw_penalties_kernel(int V, const float* penalties, float* out, const int* token, const float* presence,
                                                              const float* frequency, const float* decay) {
   const int row = blockIdx.x;
@@ -1346,11 +1349,14 @@ __global__ __launch_bounds__(256) void draw_penalties_kernel(int V, const float*
   const float keep = decay ? decay[row] : 1.0f;
   const float once = presence ? presence[row] : 0.0f, again = frequency ? frequency[row] : 0.0f;
   const int64_t base = static_cast<int64_t>(row) * V;
-  for (int k = 0; k < 16; ++k) {
-    const int i = (blockIdx.y * 16 + k) * 256 + threadIdx.x;
-    if (i >= V) break;
-    const float p = penalties[base + i];
-    out[base + i] = fmaf(p, keep, i != pick ? 0.0f : p == 0.0f ? once : again);
+  const int first = blockIdx.y * kEach * 256 + threadIdx.x;
+  float p[kEach];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) p[k] = penalties[base + min(first + k * 256, V - 1)];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int i = first + k * 256;
+    if (i < V) out[base + i] = fmaf(p[k], keep, i != pick ? 0.0f : p[k] == 0.0f ? once : again);
   }
 }
 
@@ -1449,7 +1455,7 @@ int rwkv_hip_draw_tokens(rwkv_stream_t s, int rows, int V, int io, const void* l
   if (io == RWKV_IO_F16) launch_draw<half_t>(as_stream(s), rows, a, vec);
   else launch_draw<float>(as_stream(s), rows, a, vec);
   if (penalties_out)
-    hipLaunchKernelGGL(draw_penalties_kernel, dim3(rows, ceil_div(V, 4096)), dim3(256), 0, as_stream(s), V, static_cast<const float*>(penalties),
+    hipLaunchKernelGGL(draw_penalties_kernel, dim3(rows, ceil_div(V, kEach * 256)), dim3(256), 0, as_stream(s), V, static_cast<const float*>(penalties),
                        static_cast<float*>(penalties_out), static_cast<const int*>(token), static_cast<const float*>(presence),
                        static_cast<const float*>(frequency), static_cast<const float*>(decay));
   RWKV_LAUNCH_CHECK();
