@@ -310,14 +310,15 @@ __device__ __forceinline__ void each_entry(const Row<T>& r, int first_slot, int 
 __device__ __forceinline__ float grid_place(float z, const Power& p) { return floorf(z * p.grid); }
 
 // A block takes a part of a row in NT threads, each E entries at a time: so many neighbours add up as E / 4 sums of four, then those, then the
-// slot's threads, in the same order whatever E is.  VEC: four entries are one aligned load.  What bounds it: the loads and what is computed, one
+// slot's threads, in the same order whatever E is.  Loads are as wide as they are apart, at any alignment.  What bounds it: the loads and what is computed, one
 // after the other in a block and only in part beside one another (512 rows of 65536, us: loads and maxima alone 26, that is 5.1 TB/s; sums of the
 // entries themselves 30; of their powers 40; histograms 45).
-template <typename T, bool VEC, int NT, int E>
+template <typename T, int NT, int E>
 __global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
   constexpr int NV = kPart / E / NT, kLanes = kSlot / E;
   static_assert(E == 4 || E == 8, "a slot is 16 or 8 lanes");
-  typedef T vec_t __attribute__((ext_vector_type(4)));
+  typedef T vec_t __attribute__((ext_vector_type(4), aligned(sizeof(T))));  // (a load need not be aligned)
+  typedef float pen_t __attribute__((ext_vector_type(4), aligned(sizeof(float))));
   __shared__ float most[NT / 64];
   __shared__ unsigned long long mass[kBuckets];
   __shared__ unsigned count[kBuckets];
@@ -331,7 +332,7 @@ __global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
 #pragma unroll
   for (int q = 0; q < NV; ++q) {
     const int i = first + q * NT * E;
-    if (VEC && i + E <= a.V) {
+    if (i + E <= a.V) {
 #pragma unroll
       for (int k = 0; k < E; k += 4) {
         const vec_t l = *reinterpret_cast<const vec_t*>(r.logits + i + k);
@@ -341,7 +342,7 @@ __global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
       if (r.penalties) {
 #pragma unroll
         for (int k = 0; k < E; k += 4) {
-          const float4_t p = *reinterpret_cast<const float4_t*>(r.penalties + i + k);
+          const pen_t p = *reinterpret_cast<const pen_t*>(r.penalties + i + k);
 #pragma unroll
           for (int j = 0; j < 4; ++j) z[q][k + j] -= p[j];
         }
@@ -1361,21 +1362,13 @@ __global__ __launch_bounds__(256) void draw_penalties_kernel(int V, const float*
 }
 
 template <typename T>
-void launch_draw(hipStream_t st, int rows, const DrawArgs& a, bool vec) {
+void launch_draw(hipStream_t st, int rows, const DrawArgs& a) {
   // Few parts: each by as many wavefronts as a block has.  V = 65536 without filters, 1024 threads / 256, us: 16 rows 10.5 / 11.0,
-  // 32 rows 12.3 / 11.8, 256 rows 39 / 30.  (Several parts to a block, the next one requested ahead, took 10 % longer.)
+  // 32 rows 12.3 / 11.8, 256 rows 39 / 30.  (Several parts to a block, the next one requested ahead, took 10 % longer.)  Eight neighbours to
+  // one of 256 threads instead of four take fewer steps to a slot's sum: 256 rows without filters 31.2 -> 29.9.
   const bool few = static_cast<int64_t>(rows) * a.parts < 2 * device_cu_count();
-  // Eight neighbours to a thread take fewer steps to a slot's sum (256 rows without filters 31.2 -> 29.9), but single loads reach over twice the
-  // distance (77 rows of 50277 fp16 47.9 -> 48.2).
-  const auto stats = [&](auto aligned, auto threads) {
-    constexpr bool kVec = decltype(aligned)::value;
-    constexpr int kThreads = decltype(threads)::value;
-    hipLaunchKernelGGL((draw_stats_kernel<T, kVec, kThreads, kVec && kThreads == 256 ? 8 : 4>), dim3(rows, a.parts), dim3(kThreads), 0, st, a);
-  };
-  if (vec && few) stats(std::true_type{}, std::integral_constant<int, 1024>{});
-  else if (vec) stats(std::true_type{}, std::integral_constant<int, 256>{});
-  else if (few) stats(std::false_type{}, std::integral_constant<int, 1024>{});
-  else stats(std::false_type{}, std::integral_constant<int, 256>{});
+  if (few) hipLaunchKernelGGL((draw_stats_kernel<T, 1024, 4>), dim3(rows, a.parts), dim3(1024), 0, st, a);
+  else hipLaunchKernelGGL((draw_stats_kernel<T, 256, 8>), dim3(rows, a.parts), dim3(256), 0, st, a);
   hipLaunchKernelGGL((draw_pick_kernel<T>), dim3(rows), dim3(kPickThreads), 0, st, a);
 }
 
@@ -1449,11 +1442,8 @@ int rwkv_hip_draw_tokens(rwkv_stream_t s, int rows, int V, int io, const void* l
   a = lay_out(a, rows, workspace, &need);
   RWKV_REQUIRE(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
                "draw_tokens: workspace of %zu bytes (aligned to 16) needed, got %zu", need, workspace_bytes);
-  const uintptr_t misaligned = io == RWKV_IO_F16 ? 7 : 15;
-  const bool vec = (reinterpret_cast<uintptr_t>(logits) & misaligned) == 0 && (ld % 4 == 0 || logit_rows == 1) &&
-                   (!penalties || ((reinterpret_cast<uintptr_t>(penalties) & 15) == 0 && (V % 4 == 0 || rows == 1)));
-  if (io == RWKV_IO_F16) launch_draw<half_t>(as_stream(s), rows, a, vec);
-  else launch_draw<float>(as_stream(s), rows, a, vec);
+  if (io == RWKV_IO_F16) launch_draw<half_t>(as_stream(s), rows, a);
+  else launch_draw<float>(as_stream(s), rows, a);
   if (penalties_out)
     hipLaunchKernelGGL(draw_penalties_kernel, dim3(rows, ceil_div(V, kEach * 256)), dim3(256), 0, as_stream(s), V, static_cast<const float*>(penalties),
                        static_cast<float*>(penalties_out), static_cast<const int*>(token), static_cast<const float*>(presence),
