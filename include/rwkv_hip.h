@@ -310,7 +310,7 @@ int rwkv_hip_argmax(rwkv_stream_t s, int B, int V, const void* logits, void* out
  *   temperature f32 (1)   0: the largest entry, the first of equal ones; +infinity: all entries alike
  *   top_k i32 (0)         <= 0 or >= V: off
  *   top_p f32 (1)         >= 1: off;  <= 0: the first entry
- *   min_p f32 (0)         <= 0: off;  >= 1: the entries that equal the largest
+ *   min_p f32 (0)         <= 0: off;  >= 1: the entries as probable as the largest, to 64 bits
  * uniform f32 [rows] in 0 .. 1.  With z = logit - penalty in fp32, m = max z, e_i = exp((z_i - m) / temperature) (0 where that is below
  * 2^-1000) and the order "larger z first, equal ones by index", the kept entries are the first min(top_k, the least number whose e sum
  * to top_p of all, the number with e_i >= min_p), at least one.  token i32 [rows] is the first kept entry, by index, up to which the kept

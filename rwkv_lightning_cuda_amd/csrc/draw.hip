@@ -97,6 +97,8 @@ struct Wish {
   int top_k, listed, source;
   bool valid, greedy;
   __device__ __forceinline__ bool free() const { return top_k == INT_MAX && top_p >= 1.0 && min_p <= 0.0; }
+  // a kept entry is the token once the sum up to it passes this (1: none but the last one, whatever the sums are rounded to)
+  __device__ __forceinline__ double target(double kept) const { return u < 1.0 ? u * kept : INFINITY; }
   __device__ __forceinline__ bool likely(double e) const { return !(min_p > 0.0) || e >= min_p; }
   // (a list of top_k entries, and of the rest of their slots, is short)
   __device__ __forceinline__ bool needs_histogram() const { return !greedy && !free() && top_k > listed; }
@@ -728,7 +730,7 @@ __device__ __forceinline__ void draw_from_few(const S& sh, int n, const Wish& w,
   }
   const double share = kept && w.likely(e) ? e : 0.0;
   const double upto = wave_upto(share);
-  const double target = w.u * __shfl(upto, 63, 64);
+  const double target = w.target(__shfl(upto, 63, 64));
   const uint64_t has = __ballot(share > 0.0), hit = __ballot(share > 0.0 && upto > target);
   const int at = hit ? __ffsll(static_cast<unsigned long long>(hit)) - 1 : 63 - __clzll(static_cast<long long>(has));
   const double others = wave_sum_d(lane == at ? 0.0 : share);
@@ -755,7 +757,7 @@ __device__ __forceinline__ void draw_from_list(S& sh, int n, const Wish& w, cons
   }
   double kept;
   const double before = block_before(mine, sh.d, &kept);
-  const double target = w.u * kept;
+  const double target = w.target(kept);
   int owner = block_min(mine > 0.0 && before + mine > target ? tid : INT_MAX, sh.i);
   if (owner == INT_MAX) owner = -block_min(mine > 0.0 ? -tid : 0, sh.i);
   if (tid == owner) {
@@ -1055,7 +1057,11 @@ __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) 
   }
 
   const float* part_max = a.part_max + static_cast<int64_t>(row) * a.parts;
-  const auto slot_share = [&](int s) { return slot_sum[s] * weight(part_max[s / (kPart / kSlot)], m, w.power); };
+  // (0 for a slot whose entries all lie below every power, though its part's largest does not: none of them could be drawn)
+  const auto slot_share = [&](int s) {
+    const double share = slot_sum[s] * weight(part_max[s / (kPart / kSlot)], m, w.power);
+    return static_cast<double>(slot_max[s]) - m >= w.power.lowest ? share : 0.0;
+  };
   double mine = 0.0;
 
   if (w.free()) {
@@ -1063,7 +1069,7 @@ __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) 
     for (int s = s0; s < s1; ++s) mine += slot_share(s);
     double kept;
     const double before = block_before(mine, sh.d, &kept);
-    const double target = w.u * kept;
+    const double target = w.target(kept);
     int owner = block_min(mine > 0.0 && before + mine > target ? tid : INT_MAX, sh.i);
     if (owner == INT_MAX) owner = -block_min(mine > 0.0 ? -tid : 0, sh.i);
     if (tid == owner) {
@@ -1290,7 +1296,7 @@ __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) 
   double kept = 0.0;
 #pragma unroll
   for (int i = 0; i < kPickWaves; ++i) kept += sh.chunk[i];
-  const double target = w.u * kept;
+  const double target = w.target(kept);
   double upto = 0.0, before = 0.0, others = 0.0;
   int owner = -1;
   bool sure = false;
