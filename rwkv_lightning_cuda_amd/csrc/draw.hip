@@ -219,6 +219,10 @@ __device__ __forceinline__ double wave_sum_d(double v) {
   v += lane_xor_d<16>(v);
   return row16_sum_d(v);
 }
+// of a ballot, the bits of the lanes in front of this one
+__device__ __forceinline__ int lanes_before(uint64_t hit) {
+  return __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(hit >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(hit), 0));
+}
 template <typename T>
 __device__ __forceinline__ T wave_upto(T v) {  // sum over this lane and those in front of it
   const int lane = threadIdx.x & 63;
@@ -669,7 +673,7 @@ __device__ __forceinline__ bool find_cut(S& sh, const R* row, int c0, int c1, in
         place = scalar(place);
         each_entry(*row, c0, c1, [&](float z, int i) {
           const uint64_t hit = __ballot(span.has(z));
-          if (hit >> lane & 1) take(z, i, place + __popcll(hit & ((1ull << lane) - 1)));
+          if (__builtin_amdgcn_inverse_ballot_w64(hit)) take(z, i, place + lanes_before(hit));
           place += __popcll(hit);
         });
       }
@@ -933,6 +937,8 @@ __device__ __forceinline__ bool list_window(const DrawArgs& a, PickShared& sh, c
   // each wavefront's to a share of the list
   constexpr int kShare = kList / kPickWaves;
   const float* slot_max = a.slot_max + static_cast<int64_t>(row) * a.slots;
+  float* share_z = sh.list_z + wave * kShare;
+  int* share_i = sh.list_i + wave * kShare;
   int inside = 0;
   constexpr int kAhead = 16;  // slots at once
   for (int s = c0; s < c1; s += 64) {
@@ -950,12 +956,12 @@ __device__ __forceinline__ bool list_window(const DrawArgs& a, PickShared& sh, c
       }
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
-        const uint64_t hit = __ballot(z[k] >= low && z[k] < high);
-        if (hit == 0) continue;
-        const int to = inside + __popcll(hit & ((1ull << lane) - 1));
-        if ((hit >> lane & 1) && to < kShare) {
-          sh.list_z[wave * kShare + to] = z[k];
-          sh.list_i[wave * kShare + to] = i0 + k * kSlot;
+        // (those too many fall on the last place: then the share is too short anyhow)
+        const uint64_t hit = __ballot(z[k] >= low) & __ballot(z[k] < high);
+        const int to = min(inside + lanes_before(hit), kShare - 1);
+        if (__builtin_amdgcn_inverse_ballot_w64(hit)) {
+          share_z[to] = z[k];
+          share_i[to] = i0 + k * kSlot;
         }
         inside += __popcll(hit);
       }
@@ -1229,8 +1235,8 @@ __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) 
 #pragma unroll
         for (int k = 0; k < kHeld; ++k) {
           const uint64_t hit = __ballot(candidate(held[k]));
-          if (hit >> lane & 1) {
-            const int to = place + __popcll(hit & ((1ull << lane) - 1));
+          if (__builtin_amdgcn_inverse_ballot_w64(hit)) {
+            const int to = place + lanes_before(hit);
             sh.list_z[to] = held[k];
             sh.list_i[to] = slot[k] * kSlot + lane;
           }
