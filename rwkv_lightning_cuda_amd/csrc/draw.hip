@@ -1001,7 +1001,7 @@ __device__ __forceinline__ bool list_window(const DrawArgs& a, PickShared& sh, c
 // A block draws for a row.  What bounds it is the chain of its steps, each a trip to memory or a few hundred instructions between barriers: V =
 // 65536 with top_k 50 and top_p 9 us (maxima 1.6, bound 2.8, slots 0.8, list 2), with top-p over a flat row 28 (window 4, listing 10, cut 4, sums
 // 10).  512 threads whatever the batch is, so that sums split alike; two blocks to a CU: 512 rows at once, whose chains fill one another's
-// waits (47 us).
+// waits (44 us).
 template <typename T>
 __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) {  // (four wavefronts per SIMD: two blocks per CU)
   __shared__ PickShared sh;
