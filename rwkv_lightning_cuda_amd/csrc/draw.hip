@@ -1179,6 +1179,9 @@ __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) 
     const int bound = scalar(sh.bucket);
     if (bound < kBuckets - 1) low = fmaxf(nextafterf(static_cast<float>(m - (bound + 1) * range / kBuckets), -INFINITY), -FLT_MAX);
   }
+  // Entries below every power change neither the token nor a sum (masks of a finite value: 64 rows of 65536 with 30 entries that are not
+  // masked, top_k 50: 15 us instead of 143).
+  low = fmaxf(low, nextafterf(static_cast<float>(m + w.power.lowest), -INFINITY));
   const auto candidate = [&](float z) { return z >= low; };
 
   // the slots that reach the bound, each wavefront its own

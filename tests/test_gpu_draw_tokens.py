@@ -260,6 +260,23 @@ def test_the_last_entry_of_all(gpu, V):
         check(run(gpu, z, *args, u), ref(z, *args, u))
 
 
+@pytest.mark.parametrize("mask", [-65504.0, -3.4e38, -800.0, -600.0])
+@pytest.mark.parametrize("V,dtype", [(5000, np.float32), (65536, np.float32), (50277, np.float16)])
+def test_masks_of_a_finite_value(gpu, mask, V, dtype):
+    """Fewer entries that are not masked than the filters ask for; masks with a probability of nothing, and of a little"""
+    rng = np.random.default_rng(31)
+    rows = 12
+    z = np.full((rows, V), max(mask, float(np.finfo(dtype).min)), dtype)
+    for r in range(rows):
+        z[r, rng.integers(0, V, 1 + 5 * r)] = rng.standard_normal(1 + 5 * r) * 3.0
+    args = styles(rows)
+    for top_k in (args[1], np.full(rows, 50), np.full(rows, 700)):
+        args[1] = top_k
+        for u in (rng.random(rows), np.zeros(rows), np.ones(rows)):
+            u = u.astype(np.float32)
+            check(run(gpu, z, *args, u), ref(z.astype(np.float32), *args, u))
+
+
 @pytest.mark.parametrize("u", [0.0, 1.0])
 def test_entries_below_every_power(gpu, u):
     """Entries some 1000 octaves below the largest have no probability, whatever they are beside the largest of their own part"""
