@@ -36,7 +36,7 @@ constexpr int kBuckets = 256;    // of a histogram
 constexpr int kSums = kBuckets / 64;
 constexpr int kLast = 64;        // entries that one wavefront puts in order
 constexpr int kWaveSlots = 256;  // slots of a wavefront that reach the bound
-constexpr int kHeld = 8;         // of these, those whose entries it keeps in registers
+constexpr int kHeld = 8;         // of these, those that it reads at once
 // Slots of a block that reach the bound: with more of them the histograms of a row that has some lead to the cut sooner than a list of the
 // entries.  V = 65536, list / window, us: 225 slots 26 / 31 at 8 rows and 49 / 55 at 256, 400 slots 31 / 31 and 55 / 56, 640 39 / 31 and 64 / 56.
 constexpr int kMost = 384;
