@@ -1282,9 +1282,11 @@ __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) 
   }
 
   // the kept entries' sums by wavefronts, of the entry's wavefront by slots, of its slot by entries
+  // (nothing below the window, in which the histograms say the last one is: where sums that are rounded otherwise do not reach the cut there,
+  // it is the window's last entry)
   const auto kept_weight = [&](float z, int i) {
     const double e = weight(z, m, w.power);
-    return found.keeps(z, i) && w.likely(e) ? e : 0.0;
+    return z >= span.low && found.keeps(z, i) && w.likely(e) ? e : 0.0;
   };
   double share = 0.0;
   if (windowed) {

@@ -1,0 +1,111 @@
+"""draw_tokens where the cut lies among entries that are tens of octaves below the largest: how many of them are kept is a comparison of sums
+that agree in their first eight digits or more.  Rows of few values, so that the definition can be taken with fifty digits."""
+import math
+from decimal import Decimal, getcontext
+
+import numpy as np
+import pytest
+
+from test_gpu_draw_tokens import check, run
+
+pytestmark = pytest.mark.gpu
+
+getcontext().prec = 50
+BELOW_ONE = 1.0 - 2.0 ** -24  # the largest top_p that is on
+
+
+def ref_levels(z, t, k, p, u):
+    """(token, log probability) of a row of few values.  Powers and sums with fifty digits.  What decides is asserted to lie further from a border
+    than 64-bit sums can be off: sums of at most 2 with some 32 roundings of 2^-53, and powers beside the largest good to 4e-14."""
+    t, p, u = (Decimal(float(np.float32(v))) for v in (t, p, u))
+    values, which = np.unique(z, return_inverse=True)
+    m = Decimal(float(values[-1]))
+    e = [Decimal(0) if v == -np.inf else ((Decimal(float(v)) - m) / t).exp() for v in values]
+    have = np.bincount(which, minlength=len(values))
+    total = sum(int(n) * w for n, w in zip(have, e))
+    tail = total - int(have[-1])
+    slack = (1 + tail) * 32 * Decimal(2) ** -53 + tail * Decimal("1e-13")
+    # kept entries of every level, the largest first
+    keep = np.zeros(len(values), np.int64)
+    above, number = Decimal(0), 0
+    left = k if 0 < k < len(z) else len(z)
+    for level in range(len(values) - 1, -1, -1):
+        n = int(have[level])
+        if e[level] == 0:
+            break
+        want = n
+        if p < 1:
+            need = p * total - above
+            assert abs(need - n * e[level]) > slack, "the end of a level"
+            if need <= n * e[level]:
+                want = max(1, int((need / e[level]).to_integral_value("ROUND_CEILING")))
+                if need > 0:
+                    assert min(want * e[level] - need, need - (want - 1) * e[level]) > slack, "an entry's end"
+        keep[level] = min(want, left - number)
+        above += int(keep[level]) * e[level]
+        number += int(keep[level])
+        if want < n or number == left:
+            break
+        if p < 1 and above >= p * total:
+            break
+    # running sums by index: entries of each level so far that are kept
+    so_far = [np.minimum(np.cumsum(which == level), keep[level]) if e[level] > 0 else None for level in range(len(values))]
+    upto = lambda i: sum((int(c[i]) * w for c, w in zip(so_far, e) if c is not None), Decimal(0)) if i >= 0 else Decimal(0)  # noqa: E731
+    kept = upto(len(z) - 1)
+    if u == 1:
+        token = max(int(np.nonzero(np.diff(c, prepend=0))[0][-1]) for c, n in zip(so_far, keep) if n > 0)
+    else:
+        lo, hi = 0, len(z) - 1  # the first with a sum above u times the whole
+        while lo < hi:
+            mid = (lo + hi) // 2
+            lo, hi = (lo, mid) if upto(mid) > u * kept else (mid + 1, hi)
+        token = lo
+        assert upto(token) - u * kept > slack and (token == 0 or u * kept - upto(token - 1) > slack or upto(token - 1) == 0), "a token's end"
+    weight = e[which[token]]
+    return token, float(-((kept - weight) / weight + 1).ln())
+
+
+def check_levels(hip, rows, chunk=4):
+    """rows: (z, t, k, p, u), all of one length"""
+    for at in range(0, len(rows), chunk):
+        some = rows[at:at + chunk]
+        z = np.stack([r[0] for r in some])
+        t, k, p, u = (np.array([r[i] for r in some]) for i in range(1, 5))
+        want = [ref_levels(*r) for r in some]
+        got = run(hip, z, t, k, p, np.zeros(len(some)), u.astype(np.float32))
+        check(got, (np.array([w[0] for w in want], np.int32), np.array([w[1] for w in want])))
+
+
+def two_levels(V, seed, first, second, share):
+    """The largest entry alone in its part; behind it entries of two values in any order"""
+    rng = np.random.default_rng(seed)
+    z = np.full(V, -np.inf, np.float32)
+    z[0] = 0.0
+    rest = np.full(V - 4096, second, np.float32)
+    rest[rng.permutation(V - 4096)[:share]] = first
+    z[4096:] = rest
+    return z
+
+
+def level_end(z, first):
+    """The largest top_p with which the entries from `first` up are just enough"""
+    values, have = np.unique(z[z > -np.inf], return_counts=True)
+    w = [int(n) * Decimal(float(v)).exp() for v, n in zip(values, have)]
+    share = sum(x for x, v in zip(w, values) if v >= first) / sum(w)
+    p = np.float32(share)
+    return p if Decimal(float(p)) <= share else np.nextafter(p, np.float32(0))
+
+
+@pytest.mark.parametrize("V", [65536, 1048576])
+def test_what_lies_below_the_window_is_not_kept(gpu, V):
+    """The cut is the last entry of a level of many, in front of another: sums that are rounded otherwise than the histograms' miss it"""
+    if V == 65536:
+        z = two_levels(V, 1, -14.296875, -15.296875, 32768)
+        rows = [(z, 1.0, 0, 0.9936519861221313, u) for u in (0.99, 0.995, 1.0)]
+    else:
+        rows = []
+        for i, step in enumerate((1802, 1811, 1823, 1832, 1840, 1857)):
+            first = -step / 128
+            z = two_levels(V, 2 + i, first, first - 1.0, V // 2)
+            rows += [(z, 1.0, 0, level_end(z, first), u) for u in (0.8, 1.0)]
+    check_levels(gpu, rows)
