@@ -135,10 +135,10 @@ __device__ __forceinline__ double fma_scalar(double a, double b, double c) {
 }
 // e of an entry z <= m; 0 for -infinity.  The difference's octaves are rounded by the addition of a number whose last bit is 1, and the integer
 // is what its low bits then hold.  2^f for |f| <= 1/2 is 1 + f q(f), exact at 0, with the polynomial through (2^f - 1) / f at the nine Chebyshev
-// nodes of that range: 3.7e-14 off at most.
+// nodes of that range: 3.7e-14 off at most.  `raised`: octaves to multiply it by.
 constexpr double kNinth = 1.0203121063391729e-07;  // the highest coefficient
 constexpr double kRound = 6755399441055744.0;      // 1.5 2^52
-__device__ __forceinline__ double weight(float z, float m, const Power& p, double ninth = kNinth, double round = kRound) {
+__device__ __forceinline__ double weight(float z, float m, const Power& p, double ninth = kNinth, double round = kRound, int raised = 0) {
   const double d = static_cast<double>(z) - static_cast<double>(m);
   const double y = fma(d, p.octaves, round);
   const int n = static_cast<int>(static_cast<uint32_t>(__builtin_bit_cast(uint64_t, y)));
@@ -151,8 +151,12 @@ __device__ __forceinline__ double weight(float z, float m, const Power& p, doubl
   q = fma_scalar(q, f, 0.055504108664760424);
   q = fma_scalar(q, f, 0.2402265069581299);
   q = fma_scalar(q, f, 0.6931471805599453);
-  const double v = ldexp(fma(q, f, 1.0), n);
+  const double v = ldexp(fma(q, f, 1.0), n + raised);
   return d >= p.lowest ? v : 0.0;  // (not where d is -infinity or, with an m of -infinity, a NaN)
+}
+// A power of at most 1 (or a little more) in units of 1 / kOne: 2^52 + e 2^51, rounded, holds it in its last 52 bits.
+__device__ __forceinline__ unsigned long long in_units(double e, double one = kOne, double two = 2.0 * kOne) {
+  return __builtin_bit_cast(unsigned long long, fma(e, one, two)) - 0x4330000000000000ull;
 }
 // a constant that stays in vector registers (and is not made anew for every use)
 __device__ __forceinline__ double held_constant(double c) {
@@ -404,8 +408,7 @@ __global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
       }
       if (histogram) {  // (-infinity, and whatever a row without a distribution holds: the last bucket, with nothing)
         const int b = static_cast<int>(fminf(top - grid_place(z[q][j], w.power), static_cast<float>(kBuckets - 1)));
-        // (2^52 + e 2^51, rounded: its last 52 bits)
-        atomicAdd(&mass[b], __builtin_bit_cast(unsigned long long, fma(e, one, two)) - 0x4330000000000000ull);
+        atomicAdd(&mass[b], in_units(e, one, two));
         if (counts) atomicAdd(&count[b], 1u);
       }
     }
@@ -435,6 +438,8 @@ struct Shared {
   int i[NW], reach[NW], entries[NW];
   unsigned count[kBuckets];
   unsigned long long mass[kBuckets];
+  unsigned carry[kBuckets];  // 2^64 of the mass
+  int raised[kBuckets];      // octaves by which a bucket's powers are raised ahead of kOne
   float last_z[kLast];
   int last_i[kLast];
   alignas(8) float list_z[LIST];  // entries in order of their indexes
@@ -488,12 +493,18 @@ __device__ __forceinline__ T block_before(T v, T (&buf)[NW], T* total) {
 
 // Buckets of equal width in z, from `top` down: a smaller z is never in an earlier bucket.
 struct Buckets {
-  double top, per_unit;
+  double top, per_unit, width;
   __device__ __forceinline__ int of(float z) const {
     return static_cast<int>(fmin((top - static_cast<double>(z)) * per_unit, static_cast<double>(kBuckets - 1)));
   }
+  // octaves by which all of a bucket lies below m (up to the lowest power), rounded down
+  __device__ __forceinline__ int below(int b, float m, const Power& p) const {
+    return static_cast<int>(fmin(fmax((static_cast<double>(m) - top + b * width) * p.octaves, 0.0), -kLowestPower));
+  }
 };
-__device__ __forceinline__ Buckets buckets_of(double top, double range) { return {top, scalar(range > 0.0 ? kBuckets / range : 0.0)}; }
+__device__ __forceinline__ Buckets buckets_of(double top, double range) {
+  return {top, scalar(range > 0.0 ? kBuckets / range : 0.0), scalar(range > 0.0 ? range / kBuckets : 0.0)};
+}
 
 // What ends the kept entries, in the order: the first entry with which they are top_k or hold top_p
 struct Cut {
@@ -520,15 +531,18 @@ struct Span {
 // One wavefront over a histogram: the first bucket in which the cut lies, the entries and the mass in front of it.  Where the sums do not
 // reach the cut: kBuckets, or the last bucket that holds anything (`inside`: the cut is known to lie in this histogram, and rounding hides it).
 template <typename S>
-__device__ __forceinline__ void find_bucket(S& sh, const Cut& cut, int above, double above_mass, double unit, bool inside) {
+__device__ __forceinline__ void find_bucket(S& sh, const Cut& cut, int above, double above_mass, bool inside) {
   constexpr int kPer = kBuckets / 64;
   const int lane = threadIdx.x & 63;
+  const auto mass_of = [&](int b) {
+    return ldexp((static_cast<double>(sh.carry[b]) * 0x1p64 + static_cast<double>(sh.mass[b])) * (1.0 / kOne), -sh.raised[b]);
+  };
   int n = 0;
   double held = 0.0;
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
     n += sh.count[lane * kPer + j];
-    held += static_cast<double>(sh.mass[lane * kPer + j]) * unit;
+    held += mass_of(lane * kPer + j);
   }
   const int n_upto = wave_upto(n);
   const double held_upto = wave_upto(held);
@@ -553,7 +567,7 @@ __device__ __forceinline__ void find_bucket(S& sh, const Cut& cut, int above, do
     sh.at = at_n;
     sh.above_mass = at_held;
     at_n += count;
-    at_held += static_cast<double>(sh.mass[lane * kPer + j]) * unit;
+    at_held += mass_of(lane * kPer + j);
     found = cut.reached(at_n, at_held);
   }
 }
@@ -574,14 +588,14 @@ __device__ __forceinline__ int equal_ones(const Cut& cut, int above, double abov
 // The last entry that the cut leaves, among the entries of a span: the first `n` of the list, or, with a Row, all of a row until the list
 // holds what is left.  Histograms of the span, each over the bucket of the one before in which the cut lies, until it holds few entries or
 // equal ones.  False: the cut lies behind the span (`inside`: it is known not to).  Sums in fixed point: any order of the additions gives
-// the same.
+// the same.  Every bucket has a unit of its own, 2^-51 of the largest power that it can hold: of a row that is nearly sure the cut lies some forty
+// octaves down, where a unit for all would leave few bits or none.  (The list's powers stay below 2^64 units, a row's are carried.)
 template <typename S, typename R>
-__device__ __forceinline__ bool find_cut(S& sh, const R* row, int c0, int c1, int n, const Cut& cut, float m, const Power& power, int V, Span span,
+__device__ __forceinline__ bool find_cut(S& sh, const R* row, int c0, int c1, int n, const Cut& cut, float m, const Power& power, Span span,
                                          Buckets buckets, bool inside, Found& found) {
   constexpr int kThreads = S::kWaves * 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int scale = 62 - (32 - __clz(V));  // (V weights of at most 1 stay below 2^63)
-  const double unit = ldexp(1.0, -scale), per_unit = ldexp(1.0, scale);
+  static_assert(S::kList <= 8000, "the list's powers in units");
   bool in_list = row == nullptr;
   const auto each = [&](auto&& f) {
     if (in_list) {
@@ -600,15 +614,21 @@ __device__ __forceinline__ bool find_cut(S& sh, const R* row, int c0, int c1, in
     for (int b = tid; b < kBuckets; b += kThreads) {
       sh.count[b] = 0;
       sh.mass[b] = 0;
+      sh.carry[b] = 0;
+      sh.raised[b] = buckets.below(b, m, power);
     }
     __syncthreads();
     each([&](float z) {
       const int b = buckets.of(z);
       atomicAdd(&sh.count[b], 1u);
-      if (cut.mass < INFINITY) atomicAdd(&sh.mass[b], static_cast<unsigned long long>(fma(weight(z, m, power), per_unit, 0.5)));
+      if (cut.mass < INFINITY) {
+        const unsigned long long units = in_units(weight(z, m, power, kNinth, kRound, sh.raised[b]));
+        if (in_list) atomicAdd(&sh.mass[b], units);
+        else if (atomicAdd(&sh.mass[b], units) > ~units) atomicAdd(&sh.carry[b], 1u);
+      }
     });
     __syncthreads();
-    if (wave == 0) find_bucket(sh, cut, span.above, span.above_mass, unit, inside);
+    if (wave == 0) find_bucket(sh, cut, span.above, span.above_mass, inside);
     __syncthreads();
     const int b = scalar(sh.bucket);
     if (b == kBuckets) return false;
@@ -1256,7 +1276,7 @@ __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) 
     }
     Found found = {-INFINITY, INT_MAX};
     if (!cut.open())
-      find_cut(sh, static_cast<const Row<T>*>(nullptr), 0, 0, n, cut, m, w.power, a.V, {0, 0.0, -FLT_MAX, FLT_MAX},
+      find_cut(sh, static_cast<const Row<T>*>(nullptr), 0, 0, n, cut, m, w.power, {0, 0.0, -FLT_MAX, FLT_MAX},
                buckets_of(m, fmin(static_cast<double>(m) - low, kWidest / w.power.octaves)), false, found);
     draw_from_list(sh, n, w, found, m, answer);
     return;
@@ -1277,7 +1297,7 @@ __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) 
   }
   if (!cut.open()) {
     const double from = fmin(span.high, m);
-    find_cut(sh, windowed ? nullptr : &r, c0, c1, windowed ? n : 0, cut, m, w.power, a.V, span,
+    find_cut(sh, windowed ? nullptr : &r, c0, c1, windowed ? n : 0, cut, m, w.power, span,
              buckets_of(from, fmin(from - span.low, kWidest / w.power.octaves)), false, found);
   }
 

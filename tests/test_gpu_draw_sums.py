@@ -109,3 +109,43 @@ def test_what_lies_below_the_window_is_not_kept(gpu, V):
             z = two_levels(V, 2 + i, first, first - 1.0, V // 2)
             rows += [(z, 1.0, 0, level_end(z, first), u) for u in (0.8, 1.0)]
     check_levels(gpu, rows)
+
+
+def down(octaves):
+    """A value so many octaves below 0 or a little more, exact in 32 bits beside numbers of a few tens"""
+    return -math.ceil(octaves * math.log(2.0) * 64) / 64
+
+
+def floor_row(V, seed, levels, n=None, alone=True, top=0.0):
+    """One large entry and `n` (default: all) others of the values `levels` in turn, in any order; alone: the first part has only the large one"""
+    rng = np.random.default_rng(seed)
+    z = np.full(V, -np.inf, np.float32)
+    free = np.arange(4096 if alone else 0, V)
+    at = free if n is None else rng.permutation(free)[:n]
+    z[at] = rng.permutation(np.resize(np.asarray(levels) + top, len(at)))
+    z[0 if alone else int(rng.integers(0, V))] = top
+    return z
+
+
+# octaves of the others, how many, top_k, top_p: all of them to be searched in memory; a list; a list of a top_k's; a window in memory; a window's list
+CUTS = {
+    "row": [([33], None, 0, BELOW_ONE), ([36, 36.4], None, 0, BELOW_ONE), ([39], None, 0, BELOW_ONE)],
+    "list": [([33], 5000, 0, BELOW_ONE), ([35], 5000, 0, BELOW_ONE), ([30, 33.5], 3000, 0, 1.0 - 2.0 ** -20)],
+    "top_k": [([31.5], 400, 512, BELOW_ONE), ([30.25, 32], 500, 500, BELOW_ONE), ([30], 300, 512, 1.0 - 2.0 ** -23)],
+    "window": [([25], None, 0, 0.999), ([20.5, 24], None, 0, 0.98), ([12, 13, 14, 28], None, 0, 0.5)],
+    "window's list": [(np.arange(24, 28, 0.03), None, 0, 1.0 - 2.0 ** -12), (np.arange(14, 20, 0.05), None, 0, 0.9)],
+}
+
+
+@pytest.mark.parametrize("path", list(CUTS))
+@pytest.mark.parametrize("V", [65536, 300001])
+def test_cuts_far_below_the_largest(gpu, V, path):
+    rows = [(floor_row(V, 40 + i, [down(o) for o in octaves], n), 1.0, k, p, u) for i, (octaves, n, k, p) in enumerate(CUTS[path])
+            for u in (0.5, 0.9999995, 1.0)]
+    check_levels(gpu, rows)
+
+
+@pytest.mark.parametrize("octaves", [36, 39, 41.99, 42.6, 43.5])
+def test_cuts_of_the_largest_vocabulary(gpu, octaves):
+    z = floor_row(1048576, 7, [down(octaves)])
+    check_levels(gpu, [(z, 1.0, 0, BELOW_ONE, u) for u in (0.5, BELOW_ONE, 1.0)])
