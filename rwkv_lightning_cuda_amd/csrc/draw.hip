@@ -46,7 +46,8 @@ constexpr int kMost = 384;
 constexpr int kListed = 512;
 constexpr int kSlotsListed = 2;
 constexpr int kGrid = 8;         // buckets of the parts' histograms in an octave
-constexpr double kOne = 2251799813685248.0;  // 2^51: a part holds 2^12 powers of at most 1
+constexpr double kOne = 2251799813685248.0;  // 2^51: 2^12 powers of at most 1 stay below 2^64
+constexpr double kPartOne = kOne / 2.0;      // of the parts' histograms, where they are at most 2
 constexpr double kLog2eD = 1.44269504088896340736, kLn2D = 0.69314718055994530942;
 constexpr double kLowestPower = -1000.0;  // octaves
 constexpr double kWidest = 64.0;          // octaves that the first histogram covers
@@ -65,7 +66,8 @@ struct DrawArgs {
   int* token;
   float* logprob;
   // What draw_stats_kernel leaves: the largest entry of every slot and part; for rows that need them the sums of the slots' powers, against
-  // the part's largest entry, or the parts' histograms: powers (times kOne) and numbers of the entries, and the powers' sums over 64 buckets
+  // the part's largest entry, or the parts' histograms: powers (raised by part_raised, times kPartOne) and numbers of the entries, and the powers' sums
+  // over 64 buckets (times kPartOne)
   int parts;
   double* slot_sum;               // [rows,slots]
   double* part_sum;               // [rows,parts,kSums]
@@ -117,7 +119,7 @@ __device__ __forceinline__ Wish wish_of(const DrawArgs& a, int row) {
   w.u = a.uniform[row];
   w.valid = w.source >= 0 && w.source < a.logit_rows && t >= 0.0f && w.top_p == w.top_p && min_p == min_p && w.u >= 0.0 && w.u <= 1.0;
   w.greedy = t == 0.0f;
-  w.power.octaves = scalar(w.greedy ? 0.0 : kLog2eD / static_cast<double>(t));
+  w.power.octaves = scalar(w.greedy ? 0.0 : fmax(kLog2eD / static_cast<double>(t), kLowestPower / -1e300));  // (an infinite t: -1e300 is the lowest)
   w.power.lowest = scalar(fmax(kLowestPower * kLn2D * static_cast<double>(t), -1e300));  // (above -infinity at any temperature)
   w.power.grid = scalar(static_cast<float>(w.power.octaves * kGrid));
   w.top_p = scalar(w.top_p);
@@ -135,11 +137,14 @@ __device__ __forceinline__ double fma_scalar(double a, double b, double c) {
 }
 // e of an entry z <= m; 0 for -infinity.  The difference's octaves are rounded by the addition of a number whose last bit is 1, and the integer
 // is what its low bits then hold.  2^f for |f| <= 1/2 is 1 + f q(f), exact at 0, with the polynomial through (2^f - 1) / f at the nine Chebyshev
-// nodes of that range: 3.7e-14 off at most.  `raised`: octaves to multiply it by.
+// nodes of that range: 3.7e-14 off at most.  `raised`: octaves to multiply it by.  ALWAYS: 2^kLowestPower in place of 0 (for units in which that is
+// nothing).
 constexpr double kNinth = 1.0203121063391729e-07;  // the highest coefficient
 constexpr double kRound = 6755399441055744.0;      // 1.5 2^52
+template <bool ALWAYS = false>
 __device__ __forceinline__ double weight(float z, float m, const Power& p, double ninth = kNinth, double round = kRound, int raised = 0) {
-  const double d = static_cast<double>(z) - static_cast<double>(m);
+  double d = static_cast<double>(z) - static_cast<double>(m);
+  if constexpr (ALWAYS) d = fmax(d, p.lowest);
   const double y = fma(d, p.octaves, round);
   const int n = static_cast<int>(static_cast<uint32_t>(__builtin_bit_cast(uint64_t, y)));
   const double f = fma(d, p.octaves, round - y);
@@ -152,9 +157,10 @@ __device__ __forceinline__ double weight(float z, float m, const Power& p, doubl
   q = fma_scalar(q, f, 0.2402265069581299);
   q = fma_scalar(q, f, 0.6931471805599453);
   const double v = ldexp(fma(q, f, 1.0), n + raised);
+  if constexpr (ALWAYS) return v;
   return d >= p.lowest ? v : 0.0;  // (not where d is -infinity or, with an m of -infinity, a NaN)
 }
-// A power of at most 1 (or a little more) in units of 1 / kOne: 2^52 + e 2^51, rounded, holds it in its last 52 bits.
+// A power in units of 1 / `one`, up to 2^51 of them or a little more: 2^52 + e one, rounded, holds it in its last 52 bits.
 __device__ __forceinline__ unsigned long long in_units(double e, double one = kOne, double two = 2.0 * kOne) {
   return __builtin_bit_cast(unsigned long long, fma(e, one, two)) - 0x4330000000000000ull;
 }
@@ -318,6 +324,14 @@ __device__ __forceinline__ void each_entry(const Row<T>& r, int first_slot, int 
 // different parts fit together; the last one holds whatever lies lower.  In 32 bits: a smaller z never has a higher place, and a difference
 // of two places below kBuckets is exact (of whole numbers up to 2^24, or of two that lie within a factor of two); buckets need not be alike.
 __device__ __forceinline__ float grid_place(float z, const Power& p) { return floorf(z * p.grid); }
+// Octaves by which the powers of bucket b of a part are raised before they are rounded to units of 1 / kPartOne: beside a part's largest those far down,
+// in the last bucket above all, keep their digits so.  Raised powers are at most 2: bucket b is b places below the largest entry's, so its
+// entries are b - 1 or more below that entry, and less by what rounding makes of two places (2^-24 of either), which is less than seven as far
+// as kFarthest.
+__device__ __forceinline__ int part_raised(int b) { return static_cast<unsigned>(b) / kGrid; }
+// From this place on rounding is not a matter of a few places: a part's sum is taken from its entries, and the row's cut looked for among them.  (That is
+// where the temperature is some 10^-7 of the largest entry, and neighbouring numbers are octaves apart.)
+constexpr float kFarthest = 33554432.0f;  // 2^25
 
 // A block takes a part of a row in NT threads, each E entries at a time: so many neighbours add up as E / 4 sums of four, then those, then the
 // slot's threads, in the same order whatever E is.  Loads are as wide as they are apart, at any alignment.  What bounds it: the loads and what is computed, one
@@ -391,42 +405,59 @@ __global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
   const int64_t at = static_cast<int64_t>(row) * a.parts + part;
   if (threadIdx.x == 0) a.part_max[at] = m;
   const float top = scalar(grid_place(m, w.power));
-  const double ninth = held_constant(kNinth), one = held_constant(kOne), two = held_constant(2.0 * kOne), round = held_constant(kRound);
-#pragma unroll
-  for (int q = 0; q < NV; ++q) {
-    const int slot = (first + q * NT * E) / kSlot;
+  const double ninth = held_constant(kNinth), one = held_constant(kPartOne), two = held_constant(2.0 * kOne), round = held_constant(kRound);
+  const auto slot_sum = [&](int q) {
     double sum = 0.0, four = 0.0;
 #pragma unroll
     for (int j = 0; j < E; ++j) {
-      const double e = weight(z[q][j], m, w.power, ninth, round);
-      if (sums) {
-        four += e;
-        if (j % 4 == 3) {
-          sum += four;
-          four = 0.0;
-        }
-      }
-      if (histogram) {  // (-infinity, and whatever a row without a distribution holds: the last bucket, with nothing)
-        const int b = static_cast<int>(fminf(top - grid_place(z[q][j], w.power), static_cast<float>(kBuckets - 1)));
-        atomicAdd(&mass[b], in_units(e, one, two));
-        if (counts) atomicAdd(&count[b], 1u);
+      four += weight(z[q][j], m, w.power, ninth, round);
+      if (j % 4 == 3) {
+        sum += four;
+        four = 0.0;
       }
     }
-    if (sums) {
-      sum = row16_sum_d<kLanes>(sum);
+    return row16_sum_d<kLanes>(sum);
+  };
+  if (sums) {
+#pragma unroll
+    for (int q = 0; q < NV; ++q) {
+      const int slot = (first + q * NT * E) / kSlot;
+      const double sum = slot_sum(q);
       if (threadIdx.x % kLanes == 0 && slot < a.slots) a.slot_sum[static_cast<int64_t>(row) * a.slots + slot] = sum;
     }
+    return;
   }
-  if (!histogram) return;
+#pragma unroll
+  for (int q = 0; q < NV; ++q)
+#pragma unroll
+    for (int j = 0; j < E; ++j) {  // (-infinity, and whatever a row without a distribution holds: the last bucket, with nothing)
+      const int b = static_cast<int>(fminf(top - grid_place(z[q][j], w.power), static_cast<float>(kBuckets - 1)));
+      atomicAdd(&mass[b], in_units(weight<true>(z[q][j], m, w.power, ninth, round, part_raised(b)), one, two));
+      if (counts) atomicAdd(&count[b], 1u);
+    }
   // (sums of what the buckets hold: the same however many threads there were)
   __syncthreads();
   const int b = threadIdx.x;
-  if (b >= kBuckets) return;
-  const unsigned long long held = mass[b];
-  a.part_mass[at * kBuckets + b] = held;
-  if (counts) a.part_count[at * kBuckets + b] = count[b];
-  const double sum = wave_sum_d(static_cast<double>(held));
-  if ((b & 63) == 0) a.part_sum[at * kSums + b / 64] = sum;
+  const bool far = !(fabsf(top) < kFarthest);
+  if (b < kBuckets) {
+    const unsigned long long held = mass[b];
+    a.part_mass[at * kBuckets + b] = held;
+    if (counts) a.part_count[at * kBuckets + b] = count[b];
+    const double sum = wave_sum_d(ldexp(static_cast<double>(held), -part_raised(b)));
+    if ((b & 63) == 0 && !far) a.part_sum[at * kSums + b / 64] = sum;
+  }
+  if (!far) return;
+  double* slots = reinterpret_cast<double*>(mass);
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < NV; ++q) {
+    const double sum = slot_sum(q);
+    if (threadIdx.x % kLanes == 0) slots[(threadIdx.x + q * NT) / kLanes] = sum;
+  }
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  const double sum = wave_sum_d(slots[threadIdx.x]);
+  if (threadIdx.x < kSums) a.part_sum[at * kSums + threadIdx.x] = threadIdx.x == 0 ? sum * kPartOne : 0.0;
 }
 
 // What one wavefront or thread finds for its block, and what wavefronts exchange: by the block functions, and at places of their own
@@ -439,7 +470,6 @@ struct Shared {
   unsigned count[kBuckets];
   unsigned long long mass[kBuckets];
   unsigned carry[kBuckets];  // 2^64 of the mass
-  int raised[kBuckets];      // octaves by which a bucket's powers are raised ahead of kOne
   float last_z[kLast];
   int last_i[kLast];
   alignas(8) float list_z[LIST];  // entries in order of their indexes
@@ -493,17 +523,19 @@ __device__ __forceinline__ T block_before(T v, T (&buf)[NW], T* total) {
 
 // Buckets of equal width in z, from `top` down: a smaller z is never in an earlier bucket.
 struct Buckets {
-  double top, per_unit, width;
+  double top, per_unit;
+  float octaves, first;  // of a bucket, and from m to the first one (a little less)
   __device__ __forceinline__ int of(float z) const {
     return static_cast<int>(fmin((top - static_cast<double>(z)) * per_unit, static_cast<double>(kBuckets - 1)));
   }
-  // octaves by which all of a bucket lies below m (up to the lowest power), rounded down
-  __device__ __forceinline__ int below(int b, float m, const Power& p) const {
-    return static_cast<int>(fmin(fmax((static_cast<double>(m) - top + b * width) * p.octaves, 0.0), -kLowestPower));
-  }
+  // octaves by which all of a bucket lies below m, rounded down: by so many its powers are raised before they are rounded to units of 1 / kOne
+  __device__ __forceinline__ int raised(int b) const { return static_cast<int>(fmaxf(fmaf(static_cast<float>(b), octaves, first), 0.0f)); }
 };
-__device__ __forceinline__ Buckets buckets_of(double top, double range) {
-  return {top, scalar(range > 0.0 ? kBuckets / range : 0.0), scalar(range > 0.0 ? range / kBuckets : 0.0)};
+// (`range` is at most 1000 octaves: an error of 32 bits in either term stays below the hundredth)
+__device__ __forceinline__ Buckets buckets_of(double top, double range, float m, const Power& p) {
+  range = fmax(range, 0.0);
+  return {top, scalar(range > 0.0 ? kBuckets / range : 0.0), scalar(static_cast<float>(range * p.octaves / kBuckets)),
+          scalar(static_cast<float>((static_cast<double>(m) - top) * p.octaves) - 0.01f)};
 }
 
 // What ends the kept entries, in the order: the first entry with which they are top_k or hold top_p
@@ -531,18 +563,17 @@ struct Span {
 // One wavefront over a histogram: the first bucket in which the cut lies, the entries and the mass in front of it.  Where the sums do not
 // reach the cut: kBuckets, or the last bucket that holds anything (`inside`: the cut is known to lie in this histogram, and rounding hides it).
 template <typename S>
-__device__ __forceinline__ void find_bucket(S& sh, const Cut& cut, int above, double above_mass, bool inside) {
+__device__ __forceinline__ void find_bucket(S& sh, const Cut& cut, const Buckets& buckets, int above, double above_mass, bool inside) {
   constexpr int kPer = kBuckets / 64;
   const int lane = threadIdx.x & 63;
-  const auto mass_of = [&](int b) {
-    return ldexp((static_cast<double>(sh.carry[b]) * 0x1p64 + static_cast<double>(sh.mass[b])) * (1.0 / kOne), -sh.raised[b]);
-  };
   int n = 0;
-  double held = 0.0;
+  double masses[kPer], held = 0.0;
 #pragma unroll
   for (int j = 0; j < kPer; ++j) {
-    n += sh.count[lane * kPer + j];
-    held += mass_of(lane * kPer + j);
+    const int b = lane * kPer + j;
+    masses[j] = ldexp(fma(static_cast<double>(sh.carry[b]), 0x1p64, static_cast<double>(sh.mass[b])) * (1.0 / kOne), -buckets.raised(b));
+    n += sh.count[b];
+    held += masses[j];
   }
   const int n_upto = wave_upto(n);
   const double held_upto = wave_upto(held);
@@ -567,7 +598,7 @@ __device__ __forceinline__ void find_bucket(S& sh, const Cut& cut, int above, do
     sh.at = at_n;
     sh.above_mass = at_held;
     at_n += count;
-    at_held += mass_of(lane * kPer + j);
+    at_held += masses[j];
     found = cut.reached(at_n, at_held);
   }
 }
@@ -615,20 +646,19 @@ __device__ __forceinline__ bool find_cut(S& sh, const R* row, int c0, int c1, in
       sh.count[b] = 0;
       sh.mass[b] = 0;
       sh.carry[b] = 0;
-      sh.raised[b] = buckets.below(b, m, power);
     }
     __syncthreads();
     each([&](float z) {
       const int b = buckets.of(z);
       atomicAdd(&sh.count[b], 1u);
       if (cut.mass < INFINITY) {
-        const unsigned long long units = in_units(weight(z, m, power, kNinth, kRound, sh.raised[b]));
+        const unsigned long long units = in_units(weight(z, m, power, kNinth, kRound, buckets.raised(b)));
         if (in_list) atomicAdd(&sh.mass[b], units);
         else if (atomicAdd(&sh.mass[b], units) > ~units) atomicAdd(&sh.carry[b], 1u);
       }
     });
     __syncthreads();
-    if (wave == 0) find_bucket(sh, cut, span.above, span.above_mass, inside);
+    if (wave == 0) find_bucket(sh, cut, buckets, span.above, span.above_mass, inside);
     __syncthreads();
     const int b = scalar(sh.bucket);
     if (b == kBuckets) return false;
@@ -719,7 +749,7 @@ __device__ __forceinline__ bool find_cut(S& sh, const R* row, int c0, int c1, in
       in_list = true;
       n = count;
     }
-    buckets = buckets_of(span.high, static_cast<double>(span.high) - static_cast<double>(span.low));
+    buckets = buckets_of(span.high, static_cast<double>(span.high) - static_cast<double>(span.low), m, power);
   }
 }
 
@@ -813,8 +843,7 @@ constexpr int kMaxParts = kMaxLogprobVocab / kPart;
 constexpr int kPartSlots = kPart / kSlot;
 struct PickShared : Shared<kPickWaves, kList> {
   uint16_t slots[kPickWaves][kWaveSlots];
-  double part_scale[kMaxParts];  // a part's largest power, by kOne
-  double part_above[kMaxParts];  // and what the buckets in front of the window hold of it
+  double part_scale[kMaxParts];  // a part's largest power, by kPartOne
   int part_shift[kMaxParts];     // the part's first bucket, among the row's
   double held[kPickThreads];
   unsigned number[kPickThreads];
@@ -856,7 +885,7 @@ __device__ __forceinline__ void place_window(const DrawArgs& a, PickShared& sh, 
     double sum = 0.0;
 #pragma unroll
     for (int k = 0; k < kSums; ++k) sum += part_sum[p * kSums + k];
-    sh.part_scale[p] = scale / kOne;
+    sh.part_scale[p] = scale / kPartOne;
     mine += sum * sh.part_scale[p];
     sh.part_shift[p] = mp > -INFINITY ? static_cast<int>(fminf(top - grid_place(mp, w.power), static_cast<float>(kBuckets))) : kBuckets;
   }
@@ -873,7 +902,7 @@ __device__ __forceinline__ void place_window(const DrawArgs& a, PickShared& sh, 
     for (int p = tid / kBuckets; p < a.parts; p += kGroups) {
       const int b = j - sh.part_shift[p];
       if (b >= 0) {
-        held += static_cast<double>(part_mass[p * kBuckets + b]) * sh.part_scale[p];
+        held += ldexp(static_cast<double>(part_mass[p * kBuckets + b]) * sh.part_scale[p], -part_raised(b));
         if (counts) number += part_count[p * kBuckets + b];
       }
     }
@@ -949,7 +978,10 @@ __device__ __forceinline__ bool list_window(const DrawArgs& a, PickShared& sh, c
       for (int k = 0; k < kSums; ++k) held[k] = part_mass[p * kBuckets + k * 64 + lane];
       double sum = 0.0;
 #pragma unroll
-      for (int k = 0; k < kSums; ++k) sum += k * 64 + lane < end ? static_cast<double>(held[k]) : 0.0;
+      for (int k = 0; k < kSums; ++k) {
+        const int b = k * 64 + lane;
+        sum += b < end ? ldexp(static_cast<double>(held[k]), -part_raised(b)) : 0.0;
+      }
       kept_above += sum * sh.part_scale[p];
     }
     kept_above = wave_sum_d(kept_above);
@@ -1135,13 +1167,13 @@ __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) 
     first = scalar(sh.first);
     const int last = scalar(sh.last);
     const double from = top;
-    told = last < kBuckets - 1 && grid_edge(from - last, w.power, low) && (first == 0 || grid_edge(from - first + 1.0, w.power, high));
+    told = fabsf(top) < kFarthest && last < kBuckets - 1 && grid_edge(from - last, w.power, low) && (first == 0 || grid_edge(from - first + 1.0, w.power, high));
     if (!told) low = -FLT_MAX;
   } else {
     const bool summed = w.needs_sums();
     double range = scalar(static_cast<double>(m) - static_cast<double>(lowest));
     if (range * w.power.octaves > kWidest) range = kWidest / w.power.octaves;
-    const Buckets rough = buckets_of(m, scalar(range));
+    const Buckets rough = buckets_of(m, scalar(range), m, w.power);
     constexpr double kUnit = 1.0 / (1ll << 40);  // (a row's sum is at most 2^20)
     for (int s = s0; s < s1; ++s) {
       const float v = slot_max[s];
@@ -1277,7 +1309,7 @@ __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) 
     Found found = {-INFINITY, INT_MAX};
     if (!cut.open())
       find_cut(sh, static_cast<const Row<T>*>(nullptr), 0, 0, n, cut, m, w.power, {0, 0.0, -FLT_MAX, FLT_MAX},
-               buckets_of(m, fmin(static_cast<double>(m) - low, kWidest / w.power.octaves)), false, found);
+               buckets_of(m, fmin(static_cast<double>(m) - low, kWidest / w.power.octaves), m, w.power), false, found);
     draw_from_list(sh, n, w, found, m, answer);
     return;
   }
@@ -1298,7 +1330,7 @@ __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) 
   if (!cut.open()) {
     const double from = fmin(span.high, m);
     find_cut(sh, windowed ? nullptr : &r, c0, c1, windowed ? n : 0, cut, m, w.power, span,
-             buckets_of(from, fmin(from - span.low, kWidest / w.power.octaves)), false, found);
+             buckets_of(from, fmin(from - span.low, kWidest / w.power.octaves), m, w.power), false, found);
   }
 
   // the kept entries' sums by wavefronts, of the entry's wavefront by slots, of its slot by entries

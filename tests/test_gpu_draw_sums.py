@@ -149,3 +149,85 @@ def test_cuts_far_below_the_largest(gpu, V, path):
 def test_cuts_of_the_largest_vocabulary(gpu, octaves):
     z = floor_row(1048576, 7, [down(octaves)])
     check_levels(gpu, [(z, 1.0, 0, BELOW_ONE, u) for u in (0.5, BELOW_ONE, 1.0)])
+
+
+@pytest.mark.parametrize("path", list(CUTS))
+@pytest.mark.parametrize("V", [65536, 300001])
+def test_cuts_beside_the_largest_in_its_own_part(gpu, V, path):
+    """The others stand in the part of the largest, too, whose histogram has to hold both"""
+    rows = [(floor_row(V, 60 + i, [down(o) for o in octaves], n, alone=False), 1.0, k, p, u) for i, (octaves, n, k, p) in enumerate(CUTS[path])
+            for u in (0.5, 0.9999995, 1.0)]
+    check_levels(gpu, rows)
+
+
+@pytest.mark.parametrize("octaves", [36, 39, 41.99, 42.6, 43.5])
+def test_cuts_of_the_largest_vocabulary_anywhere(gpu, octaves):
+    z = floor_row(1048576, 8, [down(octaves)], alone=False)
+    check_levels(gpu, [(z, 1.0, 0, BELOW_ONE, u) for u in (0.5, BELOW_ONE, 1.0)])
+
+
+def test_few_parts_with_a_low_floor(gpu):
+    """One part or two: what the floor's powers lose beside the largest all falls on one sum"""
+    rows = [(floor_row(8000, 90 + i, [down(o)], alone=False), 1.0, 0, BELOW_ONE, u) for i, o in enumerate((33, 34, 35.5, 36.3)) for u in (0.5, 1.0)]
+    check_levels(gpu, rows)
+
+
+@pytest.mark.parametrize("t", [1e-4, 1e-5, 1e-6, 1e-7, 1e-20, 50.0, 1e10])
+def test_cuts_at_any_temperature(gpu, t):
+    """At low temperatures neighbours among the numbers lie octaves apart, and their places on the histograms' grid far behind 2^24"""
+    t = float(np.float32(t))
+    rows = []
+    for i, octaves in enumerate((20, 33.5, 36.7)):
+        for at, top in ((777, 0.0), (40000, 9.75), (65535, -30.0)):
+            z = np.full(65536, top - octaves * math.log(2.0) * t, np.float32)
+            z[at] = top
+            if z[0] == z[at]:
+                z[at] = np.nextafter(z[at], np.float32(np.inf))
+            rows += [(z, t, 0, p, u) for p, u in ((BELOW_ONE, 0.5), (BELOW_ONE, 1.0), (0.75, 1.0))]
+    check_levels(gpu, rows)
+
+
+def ref_spread(z, t, p, u):
+    """As ref_levels for rows of any values, with top_p alone: powers and sums of 64 bits behind the point (long double)"""
+    ld = np.longdouble
+    z, t, p, u = z.astype(ld), ld(np.float32(t)), ld(np.float32(p)), ld(np.float32(u))
+    y = (z - z.max()) / t
+    e = np.where(y < -1000 * math.log(2.0), ld(0), np.exp(np.maximum(y, ld(-1000))))
+    order = np.lexsort((np.arange(len(z)), -z))
+    upto = np.cumsum(e[order])
+    total = upto[-1]
+    tail = total - e[order[0]]
+    slack = (1 + tail) * 32 * ld(2) ** -53 + tail * ld(1e-13)
+    n = int(np.searchsorted(upto, p * total)) + 1
+    assert upto[n - 1] - p * total > slack and (n == 1 or p * total - upto[n - 2] > slack), "an entry's end"
+    kept = np.zeros(len(z), ld)
+    kept[order[:n]] = e[order[:n]]
+    upto = np.cumsum(kept)
+    if u == 1:
+        token = int(np.nonzero(kept)[0][-1])
+    else:
+        token = int(np.nonzero((upto > u * upto[-1]) & (kept > 0))[0][0])
+        assert upto[token] - u * upto[-1] > slack and (token == 0 or u * upto[-1] - upto[token - 1] > slack or upto[token - 1] == 0), "a token's end"
+    others = np.sort(np.delete(kept, token)).sum()
+    return token, float(-np.log1p(others / kept[token]))
+
+
+def check_spread(hip, rows):
+    z = np.stack([r[0] for r in rows])
+    t, p, u = (np.array([r[i] for r in rows], np.float32) for i in (1, 2, 3))
+    want = [ref_spread(*r) for r in rows]
+    got = run(hip, z, t, np.zeros(len(rows)), p, np.zeros(len(rows)), u)
+    check(got, (np.array([w[0] for w in want], np.int32), np.array([w[1] for w in want])))
+
+
+@pytest.mark.parametrize("V", [9000, 65536])
+@pytest.mark.parametrize("ends", [(36, 39), (20, 40), (5, 45)])
+def test_tails_that_are_spread(gpu, V, ends):
+    rng = np.random.default_rng([V, *ends])
+    rows = []
+    for i, p in enumerate((BELOW_ONE, 0.9999999, 0.9999998, 0.999999, 0.9999, 0.9)):
+        z = rng.uniform(-ends[1], -ends[0], V).astype(np.float32) * np.float32(math.log(2.0))
+        z[rng.integers(0, V)] = 0.0
+        t = (1.0, 0.7, 1.3)[i % 3]
+        rows += [(z * np.float32(t), t, p, u) for u in (float(rng.random()), 1.0)]
+    check_spread(gpu, rows)
