@@ -731,11 +731,11 @@ void ModelBackend::copy_state_slice(const GenerationState& src, int src_offset, 
   if (src_offset + count > src.batch_size || dst_offset + count > dst.batch_size)
     throw std::runtime_error("state slice range exceeds batch size");
 
-  // (a run that moves up inside its own state goes last part first)
-  constexpr int kRun = 512;
-  const bool up = &src == &dst && dst_offset > src_offset;
-  for (int done = 0; done < count; done += kRun) {
-    const int n = std::min(kRun, count - done), first = up ? count - done - n : done;
+  // (inside its own state a run goes in parts, one that moves up last part first)
+  const bool inside = &src == &dst, up = inside && dst_offset > src_offset;
+  const int run = inside ? 512 : count;
+  for (int done = 0; done < count; done += run) {
+    const int n = std::min(run, count - done), first = up ? count - done - n : done;
     std::vector<int> rows(n), to(n);
     std::iota(rows.begin(), rows.end(), src_offset + first);
     std::iota(to.begin(), to.end(), dst_offset + first);
@@ -757,7 +757,7 @@ void IModelBackend::copy_state_rows(const GenerationState& src, const std::vecto
 }
 
 // One launch for all layers and rows (the reference's copy_state_slice makes 3 L + 1 copies, src/rwkv7_fast_v4.cu:1421-1504).  On the NULL stream,
-// and waited for: the sessions' streams do not wait for it.
+// and waited for: the sessions' streams do not wait for it.  A launch numbers up to kLaunchRows rows; those of wider states are copied run by run.
 void ModelBackend::copy_state_rows(const GenerationState& src, const std::vector<int>& rows, GenerationState& dst, const std::vector<int>& to) const {
   if (rows.size() != to.size()) throw std::runtime_error("as many state rows as places for them");
   if (src.batch_size <= 0 || dst.batch_size <= 0) throw std::runtime_error("state rows require non-empty source and destination");
@@ -770,12 +770,45 @@ void ModelBackend::copy_state_rows(const GenerationState& src, const std::vector
   const void* from_tensors[3] = {src.shift.p, src.wkv32 ? static_cast<const void*>(src.wkv_state32.p) : src.wkv_state.p, src.elapsed.p};
   void* to_tensors[3] = {dst.shift.p, dst.wkv32 ? static_cast<void*>(dst.wkv_state32.p) : dst.wkv_state.p, dst.elapsed.p};
   constexpr std::size_t kMoves = 512;  // of a call
+  constexpr int kLaunchRows = 65534;
   if (&src == &dst && rows.size() > kMoves) throw std::runtime_error("more than 512 rows inside a state");
   std::vector<char> taken(dst.batch_size, 0);
   for (std::size_t i = 0; i < rows.size(); ++i) {  // (over all calls, ahead of the first)
     if (rows[i] < -1 || rows[i] >= src.batch_size || to[i] < 0 || to[i] >= dst.batch_size) throw std::runtime_error("state row out of range");
     if (taken[to[i]]) throw std::runtime_error("two state rows for one place");
     taken[to[i]] = 1;
+  }
+  if (std::max(src.batch_size, dst.batch_size) > kLaunchRows) {
+    if (&src == &dst) {  // by way of a state of their own
+      std::vector<int> live, places(rows.size()), live_places;
+      std::iota(places.begin(), places.end(), 0);
+      for (const int place : places)
+        if (rows[place] >= 0) {
+          live.push_back(rows[place]);
+          live_places.push_back(place);
+        }
+      if (rows.empty()) return;
+      GenerationState held = create_state(static_cast<int>(rows.size()));
+      copy_state_rows(src, live, held, live_places);
+      copy_state_rows(held, places, dst, to);
+      return;
+    }
+    for (std::size_t i = 0; i < rows.size();) {
+      std::size_t n = 1;
+      const int step = rows[i] < 0 ? 0 : 1;
+      while (i + n < rows.size() && rows[i + n] == rows[i] + step * static_cast<int>(n) && to[i + n] == to[i] + static_cast<int>(n)) ++n;
+      for (int t = 0; t < 3; ++t)
+        for (std::int64_t plane = 0; plane < planes[t]; ++plane) {
+          char* place = static_cast<char*>(to_tensors[t]) + (plane * dst.batch_size + to[i]) * row_bytes[t];
+          const char* tensor = static_cast<const char*>(from_tensors[t]);
+          check_hip(rows[i] < 0 ? rwkv_hip_memset(place, 0, n * row_bytes[t])
+                                : rwkv_hip_memcpy_d2d(place, tensor + (plane * src.batch_size + rows[i]) * row_bytes[t], n * row_bytes[t]),
+                    "copy backend state rows");
+        }
+      i += n;
+    }
+    check_hip(rwkv_hip_stream_sync(nullptr), "copy backend state rows");
+    return;
   }
   for (std::size_t i = 0; i < rows.size(); i += kMoves) {
     const int n = static_cast<int>(std::min(kMoves, rows.size() - i));
