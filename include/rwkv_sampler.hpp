@@ -76,7 +76,8 @@ DrawState make_draw_state(int vocab_size, int batch_size, bool with_penalties = 
 DrawnTokens draw_tokens(const DeviceLogits& logits, const std::vector<DrawOptions>& options, const std::vector<float>& uniform, DrawState& state,
                         const std::vector<int>& source = {});
 
-// The penalties of row rows[i] move to row to[i] (-1: none yet); as a sequence's state does with IModelBackend::copy_state_rows
+// The penalties of row rows[i] move to row to[i] (-1: none yet); as a sequence's state does with IModelBackend::copy_state_rows.  A row may be a
+// destination once; up to 65534 rows, and 512 moves inside a state.  What is refused moves nothing.
 void copy_draw_rows(const DrawState& src, const std::vector<int>& rows, DrawState& dst, const std::vector<int>& to);
 
 // A uniform number in [0, 1) that depends on the three arguments alone, 24 bits of it: the number that step `step` of sequence `sequence`

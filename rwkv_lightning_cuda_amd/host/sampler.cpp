@@ -173,6 +173,13 @@ void copy_draw_rows(const DrawState& src, const std::vector<int>& rows, DrawStat
     throw std::runtime_error("draw states do not match");
   if (rows.size() != to.size()) throw std::runtime_error("as many draw rows as places for them");
   if (&src == &dst && rows.size() > 512) throw std::runtime_error("more than 512 rows inside a draw state");
+  if (std::max(src.batch_size, dst.batch_size) > 65534) throw std::runtime_error("more than 65534 rows of a draw state");
+  std::vector<char> taken(dst.batch_size, 0);
+  for (std::size_t i = 0; i < rows.size(); ++i) {  // (over all launches, ahead of the first)
+    if (rows[i] < -1 || rows[i] >= src.batch_size || to[i] < 0 || to[i] >= dst.batch_size) throw std::runtime_error("draw row out of range");
+    if (taken[to[i]]) throw std::runtime_error("two draw rows for one place");
+    taken[to[i]] = 1;
+  }
   if (src.penalties.p == nullptr) return;
   const std::int64_t planes = 1, bytes = src.vocab_size * static_cast<std::int64_t>(sizeof(float));
   void* to_tensor = dst.penalties.p;
