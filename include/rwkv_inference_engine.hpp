@@ -60,7 +60,7 @@ class InferenceEngine {
 
   // Several continuations of one prompt (no counterpart in the reference).  The prompt is run once; its state goes on in n places, each with
   // random numbers of its own: continuation i of a seed is the same whatever n is, up to the rounding differences between the kernels of
-  // different batch widths.  Rows that have ended make room once at most half of the batch is left.
+  // different batch widths.  Rows that have ended make room once at most half of the batch is left.  n is at most 65534.
   struct BranchOptions {
     int max_tokens = 256;
     std::vector<int64_t> stop_tokens{0, 261, 24281};

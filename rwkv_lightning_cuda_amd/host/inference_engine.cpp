@@ -579,6 +579,7 @@ InferenceEngine::GenerationStats InferenceEngine::generate_from_logits_stream(
 // The first token of all continuations is drawn from the prompt's one row of logits; those that go on get copies of its state.
 std::vector<InferenceEngine::Branch> InferenceEngine::branch_generate(const std::string& prompt, int n, const BranchOptions& options) const {
   if (n <= 0) throw std::runtime_error("number of continuations must be positive");
+  if (n > 65534) throw std::runtime_error("number of continuations must be at most 65534");  // (rows of the draws' state)
   std::vector<Branch> out(n);
   GenerationState state = model_->create_state(1);
   DeviceLogits logits;

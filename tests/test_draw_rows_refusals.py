@@ -1,7 +1,7 @@
-"""Rows of draw states that the C++ host API refuses (no GPU)."""
+"""Rows of draw states and numbers of continuations that the C++ host API refuses (no GPU)."""
 from test_host_api import _run
 
 
 def test_draw_rows_that_are_refused():
     out = _run("draw_rows_cpu_test")
-    assert "ok   draw_rows_that_are_refused" in out
+    assert "ok   draw_rows_that_are_refused" in out and "ok   numbers_of_continuations_that_are_refused" in out
