@@ -590,7 +590,7 @@ std::vector<InferenceEngine::Branch> InferenceEngine::branch_generate(const std:
   std::vector<int> live(n);  // row of the batch -> continuation, or -1
   std::iota(live.begin(), live.end(), 0);
   std::vector<int> source(n, 0);  // first step: everybody's logits are row 0
-  const int64_t filler = options.stop_tokens.empty() ? 0 : options.stop_tokens.front();
+  constexpr int64_t kFiller = 0;  // fed to rows that have ended (a stop token need not be one of the model's)
   std::vector<float> uniform;
   for (int step = 0; step < options.max_tokens; ++step) {
     uniform.clear();
@@ -633,7 +633,7 @@ std::vector<InferenceEngine::Branch> InferenceEngine::branch_generate(const std:
       source.clear();
     }
     std::vector<int64_t> feed;
-    for (const int i : live) feed.push_back(i < 0 ? filler : out[i].tokens.back());
+    for (const int i : live) feed.push_back(i < 0 ? kFiller : out[i].tokens.back());
     model_->forward_decode(feed, state, logits);
   }
   for (Branch& b : out) b.text = tokenizer_->decode(b.tokens);

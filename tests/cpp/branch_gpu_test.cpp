@@ -262,4 +262,23 @@ HOST_TEST(a_branch_belongs_to_its_seed_and_place) {
   CHECK(same < 4);
 }
 
+// Stop tokens that the model does not have are never drawn, and no branch that has ended is fed one
+HOST_TEST(stop_tokens_outside_the_vocabulary) {
+  InferenceEngine engine(tiny(), tokenizer(), "tiny");
+  InferenceEngine::BranchOptions o;
+  o.max_tokens = 10;
+  o.seed = 3;
+  o.stop_tokens.clear();
+  for (int t = 0; t < kVocab; t += 9) o.stop_tokens.push_back(t);
+  const auto want = engine.branch_generate("User: hi", 9, o);
+  int stopped = 0;
+  for (const auto& b : want) stopped += b.stopped;
+  CHECK(stopped > 0 && stopped < 9);
+  for (const int64_t outside : {int64_t{kVocab}, int64_t{70000}, int64_t{-1}}) {
+    o.stop_tokens.insert(o.stop_tokens.begin(), outside);
+    const auto got = engine.branch_generate("User: hi", 9, o);
+    for (int i = 0; i < 9; ++i) CHECK(got[i].tokens == want[i].tokens && got[i].logprobs == want[i].logprobs && got[i].stopped == want[i].stopped);
+  }
+}
+
 int main(int argc, char** argv) { return host_test::run_all(argc, argv, true); }
