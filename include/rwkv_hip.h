@@ -6,7 +6,10 @@
  * `rwkv_stream_t` is an opaque stream handle (NULL = the default stream).
  *
  * Every function returns 0 on success or a negative RWKV_E_* code and never terminates the
- * process; rwkv_hip_last_error() returns the calling thread's last message.
+ * process; rwkv_hip_last_error() returns the calling thread's last message.  Several threads may call at once,
+ * each with a session of its own: a session that captures a decode graph waits for the other threads' allocations,
+ * copies and waits for the device, and holds up those that come (a device-wide HIP call that a program makes
+ * beside this library, hipDeviceSynchronize or hipFree, still spoils a capture: the step then returns an error).
  *
  * Each entry point names the reference interface it replaces (paths relative to the
  * reference repository root).  The reference's kernel ABI is the C++-linkage launcher list in

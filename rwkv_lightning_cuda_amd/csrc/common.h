@@ -16,6 +16,29 @@ void set_error(const char* fmt, ...);
 // Compute units of the current device (asked once per device; 256 if the query fails).
 int device_cu_count();
 
+// Calls that wait for the device or that the runtime sets in order with every stream (allocations, copies on the NULL stream, waits for the
+// device) spoil a capture that another thread has begun, whatever the capture's mode and stream.  So they keep apart: while a DeviceCall lives, no
+// thread captures a decode graph, and a Capture waits for those that live and holds up those that come.  A thread's second DeviceCall is part of
+// its first one.
+struct DeviceCall {
+  DeviceCall();
+  ~DeviceCall();
+  DeviceCall(const DeviceCall&) = delete;
+  DeviceCall& operator=(const DeviceCall&) = delete;
+};
+struct Capture {
+  Capture();
+  ~Capture();
+  Capture(const Capture&) = delete;
+  Capture& operator=(const Capture&) = delete;
+};
+hipError_t device_malloc(void** p, size_t bytes);
+hipError_t device_free(void* p);
+hipError_t pinned_malloc(void** p, size_t bytes);
+hipError_t pinned_free(void* p);
+hipError_t device_wait();
+hipError_t graph_exec_destroy(hipGraphExec_t exec);
+
 inline hipStream_t as_stream(rwkv_stream_t s) { return reinterpret_cast<hipStream_t>(s); }
 
 #define RWKV_HIP_TRY(expr)                                                              \

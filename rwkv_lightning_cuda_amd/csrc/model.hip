@@ -29,8 +29,8 @@ struct Matrix {
   half_t* scale_by_group = nullptr;  // int4, in the same block behind the codes: scale and zero point as [K/128][N]
   uint8_t* zp_by_group = nullptr;
   void free_copies() {
-    if (packed) (void)hipFree(packed);
-    if (sparse_t) (void)hipFree(sparse_t);
+    if (packed) (void)device_free(packed);
+    if (sparse_t) (void)device_free(sparse_t);
     packed = sparse_t = nullptr;
     scale_by_group = nullptr;
     zp_by_group = nullptr;
@@ -67,9 +67,9 @@ struct rwkv_hip_model {
     for (Layer& l : layers) {
       for (Matrix& mat : l.m) mat.free_copies();
       for (void* q : l.lora_in_packed)
-        if (q) (void)hipFree(q);
+        if (q) (void)device_free(q);
       for (half_t* q : l.lora_out_packed)
-        if (q) (void)hipFree(q);
+        if (q) (void)device_free(q);
     }
   }
 };
@@ -296,15 +296,15 @@ int ensure_arena(rwkv_hip_session* s, int B, int T) {
   if (need > s->arena.cap) {
     // a larger shape invalidates captured graphs (they hold arena addresses)
     for (auto& g : s->graphs) {
-      if (g.exec) (void)hipGraphExecDestroy(g.exec);
+      if (g.exec) (void)graph_exec_destroy(g.exec);
       if (g.graph) (void)hipGraphDestroy(g.graph);
     }
     s->graphs.clear();
     RWKV_HIP_TRY(hipStreamSynchronize(s->stream));
-    if (s->arena.base) RWKV_HIP_TRY(hipFree(s->arena.base));
+    if (s->arena.base) RWKV_HIP_TRY(device_free(s->arena.base));
     s->arena.base = nullptr;
     s->arena.cap = 0;
-    RWKV_HIP_TRY(hipMalloc(reinterpret_cast<void**>(&s->arena.base), need));
+    RWKV_HIP_TRY(device_malloc(reinterpret_cast<void**>(&s->arena.base), need));
     s->arena.cap = need;
     s->arena_B = 0;
     s->arena_T = 0;
@@ -339,38 +339,38 @@ int ensure_arena(rwkv_hip_session* s, int B, int T) {
     const size_t ws = packed_workspace_bytes(m, B, static_cast<int>(rows));
     if (ws > s->gemm_ws_bytes) {
       for (auto& g : s->graphs) {
-        if (g.exec) (void)hipGraphExecDestroy(g.exec);
+        if (g.exec) (void)graph_exec_destroy(g.exec);
         if (g.graph) (void)hipGraphDestroy(g.graph);
       }
       s->graphs.clear();
       RWKV_HIP_TRY(hipStreamSynchronize(s->stream));
-      if (s->gemm_ws) RWKV_HIP_TRY(hipFree(s->gemm_ws));
+      if (s->gemm_ws) RWKV_HIP_TRY(device_free(s->gemm_ws));
       s->gemm_ws = nullptr;
       s->gemm_ws_bytes = 0;
-      RWKV_HIP_TRY(hipMalloc(&s->gemm_ws, ws));
+      RWKV_HIP_TRY(device_malloc(&s->gemm_ws, ws));
       s->gemm_ws_bytes = ws;
     }
   }
   if (!s->sparse_ws && ffn_sparse_supported(RWKV_FMT_W8, m->C, m->F)) {
     const size_t bytes = ffn_sparse_workspace_bytes(kSparseMaxRows, m->C, m->F);
-    RWKV_HIP_TRY(hipMalloc(&s->sparse_ws, bytes));
+    RWKV_HIP_TRY(device_malloc(&s->sparse_ws, bytes));
     s->sparse_ws_bytes = bytes;
   }
   if (static_cast<int>(rows) > s->tokens_cap) {
     // captured decode graphs read their tokens from the old buffer (embedding gather, token feedback)
     for (auto& g : s->graphs) {
-      if (g.exec) (void)hipGraphExecDestroy(g.exec);
+      if (g.exec) (void)graph_exec_destroy(g.exec);
       if (g.graph) (void)hipGraphDestroy(g.graph);
     }
     s->graphs.clear();
     RWKV_HIP_TRY(hipStreamSynchronize(s->stream));
-    if (s->tokens_dev) RWKV_HIP_TRY(hipFree(s->tokens_dev));
-    if (s->tokens_pinned) RWKV_HIP_TRY(hipHostFree(s->tokens_pinned));
+    if (s->tokens_dev) RWKV_HIP_TRY(device_free(s->tokens_dev));
+    if (s->tokens_pinned) RWKV_HIP_TRY(pinned_free(s->tokens_pinned));
     s->tokens_dev = nullptr;
     s->tokens_pinned = nullptr;
     s->tokens_cap = 0;
-    RWKV_HIP_TRY(hipMalloc(reinterpret_cast<void**>(&s->tokens_dev), rows * sizeof(int64_t)));
-    RWKV_HIP_TRY(hipHostMalloc(reinterpret_cast<void**>(&s->tokens_pinned), rows * sizeof(int64_t), hipHostMallocDefault));
+    RWKV_HIP_TRY(device_malloc(reinterpret_cast<void**>(&s->tokens_dev), rows * sizeof(int64_t)));
+    RWKV_HIP_TRY(pinned_malloc(reinterpret_cast<void**>(&s->tokens_pinned), rows * sizeof(int64_t)));
     s->tokens_cap = static_cast<int>(rows);
   }
   return RWKV_OK;
@@ -954,16 +954,22 @@ int run_step(rwkv_hip_session* s, int B, half_t* shift, void* wkv, int* elapsed,
       auto victim = std::min_element(s->graphs.begin(), s->graphs.end(),
                                      [](const GraphEntry& x, const GraphEntry& y) { return x.last_use < y.last_use; });
       RWKV_HIP_TRY(hipStreamSynchronize(s->stream));
-      if (victim->exec) (void)hipGraphExecDestroy(victim->exec);
+      if (victim->exec) (void)graph_exec_destroy(victim->exec);
       if (victim->graph) (void)hipGraphDestroy(victim->graph);
       s->graphs.erase(victim);
     }
     GraphEntry e;
     e.B = B; e.shift = shift; e.wkv = wkv; e.elapsed = elapsed; e.logits = logits;
-    RWKV_HIP_TRY(hipStreamBeginCapture(s->stream, hipStreamCaptureModeThreadLocal));
-    const int rc = enqueue_forward(s, B, 1, shift, wkv, elapsed, logits);
     hipGraph_t graph = nullptr;
-    const hipError_t end = hipStreamEndCapture(s->stream, &graph);
+    int rc;
+    hipError_t end, made = hipSuccess;
+    {
+      Capture capture;
+      RWKV_HIP_TRY(hipStreamBeginCapture(s->stream, hipStreamCaptureModeThreadLocal));
+      rc = enqueue_forward(s, B, 1, shift, wkv, elapsed, logits);
+      end = hipStreamEndCapture(s->stream, &graph);
+      if (rc == RWKV_OK && end == hipSuccess) made = hipGraphInstantiate(&e.exec, graph, nullptr, nullptr, 0);
+    }
     if (rc != RWKV_OK) {
       if (graph) (void)hipGraphDestroy(graph);
       return rc;
@@ -972,8 +978,12 @@ int run_step(rwkv_hip_session* s, int B, half_t* shift, void* wkv, int* elapsed,
       set_error("hipStreamEndCapture failed: %s", hipGetErrorString(end));
       return RWKV_E_RUNTIME;
     }
+    if (made != hipSuccess) {
+      set_error("hipGraphInstantiate failed: %s", hipGetErrorString(made));
+      (void)hipGraphDestroy(graph);
+      return made == hipErrorOutOfMemory ? RWKV_E_NOMEM : RWKV_E_RUNTIME;
+    }
     e.graph = graph;
-    RWKV_HIP_TRY(hipGraphInstantiate(&e.exec, graph, nullptr, nullptr, 0));
     g_graph_captures.fetch_add(1, std::memory_order_relaxed);
     s->graphs.push_back(e);
     g = &s->graphs.back();
@@ -1045,12 +1055,12 @@ int rwkv_hip_model_set_tensor(rwkv_hip_model* m, int layer, int id, const void* 
     if (id != w1_ids[i]) continue;
     void*& slot = m->layers[layer].lora_in_packed[i];
     if (slot) {
-      RWKV_HIP_TRY(hipDeviceSynchronize());
-      RWKV_HIP_TRY(hipFree(slot));
+      RWKV_HIP_TRY(device_wait());
+      RWKV_HIP_TRY(device_free(slot));
       slot = nullptr;
     }
     if (linear_packed_supported(RWKV_FMT_F16, kPackedMinRows, ranks[i], m->C)) {
-      RWKV_HIP_TRY(hipMalloc(&slot, static_cast<size_t>(ranks[i]) * m->C * 2));
+      RWKV_HIP_TRY(device_malloc(&slot, static_cast<size_t>(ranks[i]) * m->C * 2));
       const int rc = pack_weights_launch(nullptr, RWKV_FMT_F16, ranks[i], m->C, data, slot);
       if (rc != RWKV_OK) return rc;
       RWKV_HIP_TRY(hipStreamSynchronize(nullptr));
@@ -1062,12 +1072,12 @@ int rwkv_hip_model_set_tensor(rwkv_hip_model* m, int layer, int id, const void* 
     if (id != w2_ids[i]) continue;
     half_t*& slot = m->layers[layer].lora_out_packed[i];
     if (slot) {
-      RWKV_HIP_TRY(hipDeviceSynchronize());
-      RWKV_HIP_TRY(hipFree(slot));
+      RWKV_HIP_TRY(device_wait());
+      RWKV_HIP_TRY(device_free(slot));
       slot = nullptr;
     }
     if (ranks[i] > 0 && ranks[i] % 8 == 0) {
-      RWKV_HIP_TRY(hipMalloc(reinterpret_cast<void**>(&slot), lora_pack_w2_halfs(m->C, ranks[i]) * sizeof(half_t)));
+      RWKV_HIP_TRY(device_malloc(reinterpret_cast<void**>(&slot), lora_pack_w2_halfs(m->C, ranks[i]) * sizeof(half_t)));
       const int rc = lora_pack_w2_launch(nullptr, m->C, ranks[i], p, slot);
       if (rc != RWKV_OK) return rc;
       RWKV_HIP_TRY(hipStreamSynchronize(nullptr));
@@ -1095,7 +1105,7 @@ int rwkv_hip_model_set_matrix(rwkv_hip_model* m, int layer, int id, int fmt, con
   }
   Matrix& slot = id == RWKV_M_HEAD ? m->head : m->layers[layer].m[id];
   if (slot.packed || slot.sparse_t) {
-    RWKV_HIP_TRY(hipDeviceSynchronize());
+    RWKV_HIP_TRY(device_wait());
     slot.free_copies();
   }
   if (linear_packed_supported(fmt, kPackedMinRows, N, K)) {
@@ -1103,7 +1113,7 @@ int rwkv_hip_model_set_matrix(rwkv_hip_model* m, int layer, int id, int fmt, con
     const size_t bytes = fmt == RWKV_FMT_F16 ? static_cast<size_t>(N) * K * 2
                                              : (fmt == RWKV_FMT_W8 ? static_cast<size_t>(N) * K : static_cast<size_t>(N) * K / 2);
     const size_t groups = fmt == RWKV_FMT_W4 ? static_cast<size_t>(N) * (K / 128) : 0;
-    RWKV_HIP_TRY(hipMalloc(&mat.packed, bytes + groups * 3));
+    RWKV_HIP_TRY(device_malloc(&mat.packed, bytes + groups * 3));
     int rc = pack_weights_launch(nullptr, fmt, N, K, data, mat.packed);
     if (rc == RWKV_OK && fmt == RWKV_FMT_W4) {
       mat.scale_by_group = reinterpret_cast<half_t*>(static_cast<unsigned char*>(mat.packed) + bytes);
@@ -1118,7 +1128,7 @@ int rwkv_hip_model_set_matrix(rwkv_hip_model* m, int layer, int id, int fmt, con
   }
   if (id == RWKV_M_FFN_VALUE && ffn_sparse_supported(fmt, N, K)) {
     // third copy: transposed, for decode steps of one sequence
-    RWKV_HIP_TRY(hipMalloc(&mat.sparse_t, ffn_sparse_packed_bytes(fmt, N, K)));
+    RWKV_HIP_TRY(device_malloc(&mat.sparse_t, ffn_sparse_packed_bytes(fmt, N, K)));
     const int rc = fmt == RWKV_FMT_W4 ? ffn_sparse_pack_w4_launch(nullptr, N, K, data, mat.scale, mat.zp, mat.sparse_t)
                                       : ffn_sparse_pack_launch(nullptr, fmt, N, K, data, mat.sparse_t);
     if (rc != RWKV_OK) {
@@ -1164,6 +1174,7 @@ int rwkv_hip_session_create(rwkv_hip_session** out, const rwkv_hip_model* m) {
   }
   s->model = m;
 
+  DeviceCall call;
   const hipError_t err = hipStreamCreateWithFlags(&s->stream, hipStreamNonBlocking);
   if (err != hipSuccess) {
     set_error("hipStreamCreateWithFlags failed: %s", hipGetErrorString(err));
@@ -1177,21 +1188,22 @@ int rwkv_hip_session_create(rwkv_hip_session** out, const rwkv_hip_model* m) {
 int rwkv_hip_session_destroy(rwkv_hip_session* s) {
   if (!s) return RWKV_OK;
   (void)hipStreamSynchronize(s->stream);
+  DeviceCall call;
   for (auto& g : s->graphs) {
-    if (g.exec) (void)hipGraphExecDestroy(g.exec);
+    if (g.exec) (void)graph_exec_destroy(g.exec);
     if (g.graph) (void)hipGraphDestroy(g.graph);
   }
-  if (s->arena.base) (void)hipFree(s->arena.base);
-  if (s->gemm_ws) (void)hipFree(s->gemm_ws);
-  if (s->score_ws) (void)hipFree(s->score_ws);
-  if (s->targets_pinned) (void)hipHostFree(s->targets_pinned);
-  if (s->sparse_ws) (void)hipFree(s->sparse_ws);
+  if (s->arena.base) (void)device_free(s->arena.base);
+  if (s->gemm_ws) (void)device_free(s->gemm_ws);
+  if (s->score_ws) (void)device_free(s->score_ws);
+  if (s->targets_pinned) (void)pinned_free(s->targets_pinned);
+  if (s->sparse_ws) (void)device_free(s->sparse_ws);
   for (float* p : s->widened)
-    if (p) (void)hipFree(p);
-  if (s->tokens_dev) (void)hipFree(s->tokens_dev);
-  if (s->tokens_pinned) (void)hipHostFree(s->tokens_pinned);
-  if (s->argmax_dev) (void)hipFree(s->argmax_dev);
-  if (s->history_dev) (void)hipFree(s->history_dev);
+    if (p) (void)device_free(p);
+  if (s->tokens_dev) (void)device_free(s->tokens_dev);
+  if (s->tokens_pinned) (void)pinned_free(s->tokens_pinned);
+  if (s->argmax_dev) (void)device_free(s->argmax_dev);
+  if (s->history_dev) (void)device_free(s->history_dev);
   (void)hipStreamDestroy(s->stream);
   delete s;
   return RWKV_OK;
@@ -1219,7 +1231,7 @@ int rwkv_hip_session_set_profile(rwkv_hip_session* s, int on) {
 static int drop_graphs(rwkv_hip_session* s) {
   RWKV_HIP_TRY(hipStreamSynchronize(s->stream));
   for (auto& g : s->graphs) {
-    if (g.exec) (void)hipGraphExecDestroy(g.exec);
+    if (g.exec) (void)graph_exec_destroy(g.exec);
     if (g.graph) (void)hipGraphDestroy(g.graph);
   }
   s->graphs.clear();
@@ -1333,10 +1345,10 @@ int rwkv_hip_session_debug_buffer(rwkv_hip_session* s, int id, void** ptr) {
   const int slot = id == kR32 ? 0 : 1 + id - kK32;
   RWKV_HIP_TRY(hipStreamSynchronize(s->stream));
   if (n > s->widened_cap[slot]) {
-    if (s->widened[slot]) RWKV_HIP_TRY(hipFree(s->widened[slot]));
+    if (s->widened[slot]) RWKV_HIP_TRY(device_free(s->widened[slot]));
     s->widened[slot] = nullptr;
     s->widened_cap[slot] = 0;
-    RWKV_HIP_TRY(hipMalloc(reinterpret_cast<void**>(&s->widened[slot]), n * sizeof(float)));
+    RWKV_HIP_TRY(device_malloc(reinterpret_cast<void**>(&s->widened[slot]), n * sizeof(float)));
     s->widened_cap[slot] = n;
   }
   TRY(rwkv_hip_f16_to_f32(s->stream, static_cast<int64_t>(n), id == kR32 ? b.r : table[id], s->widened[slot]));
@@ -1402,17 +1414,17 @@ int rwkv_hip_score(rwkv_hip_session* s, const int64_t* tokens_host, const int64_
   const size_t targets_bytes = align_up(static_cast<size_t>(rows) * sizeof(int), 256);
   const size_t need = 2 * targets_bytes + score_rest_bytes(m, a.act_int8, rows, top_n);
   if (need > s->score_ws_bytes) {
-    if (s->score_ws) RWKV_HIP_TRY(hipFree(s->score_ws));
+    if (s->score_ws) RWKV_HIP_TRY(device_free(s->score_ws));
     s->score_ws = nullptr;
     s->score_ws_bytes = 0;
-    RWKV_HIP_TRY(hipMalloc(&s->score_ws, need));
+    RWKV_HIP_TRY(device_malloc(&s->score_ws, need));
     s->score_ws_bytes = need;
   }
   if (rows > s->targets_cap) {
-    if (s->targets_pinned) RWKV_HIP_TRY(hipHostFree(s->targets_pinned));
+    if (s->targets_pinned) RWKV_HIP_TRY(pinned_free(s->targets_pinned));
     s->targets_pinned = nullptr;
     s->targets_cap = 0;
-    RWKV_HIP_TRY(hipHostMalloc(reinterpret_cast<void**>(&s->targets_pinned), rows * sizeof(int), hipHostMallocDefault));
+    RWKV_HIP_TRY(pinned_malloc(reinterpret_cast<void**>(&s->targets_pinned), rows * sizeof(int)));
     s->targets_cap = rows;
   }
   unsigned char* ws = static_cast<unsigned char*>(s->score_ws);
@@ -1439,18 +1451,18 @@ int rwkv_hip_decode_greedy(rwkv_hip_session* s, const int64_t* first_tokens_host
   TRY(ensure_arena(s, B, 1));
   RWKV_HIP_TRY(hipStreamSynchronize(s->stream));
   if (B > s->argmax_cap) {
-    if (s->argmax_dev) RWKV_HIP_TRY(hipFree(s->argmax_dev));
+    if (s->argmax_dev) RWKV_HIP_TRY(device_free(s->argmax_dev));
     s->argmax_dev = nullptr;
     s->argmax_cap = 0;
-    RWKV_HIP_TRY(hipMalloc(reinterpret_cast<void**>(&s->argmax_dev), sizeof(int) * B));
+    RWKV_HIP_TRY(device_malloc(reinterpret_cast<void**>(&s->argmax_dev), sizeof(int) * B));
     s->argmax_cap = B;
   }
   const size_t hist = static_cast<size_t>(steps) * B;
   if (hist > s->history_cap) {
-    if (s->history_dev) RWKV_HIP_TRY(hipFree(s->history_dev));
+    if (s->history_dev) RWKV_HIP_TRY(device_free(s->history_dev));
     s->history_dev = nullptr;
     s->history_cap = 0;
-    RWKV_HIP_TRY(hipMalloc(reinterpret_cast<void**>(&s->history_dev), sizeof(int) * hist));
+    RWKV_HIP_TRY(device_malloc(reinterpret_cast<void**>(&s->history_dev), sizeof(int) * hist));
     s->history_cap = hist;
   }
   std::copy(first_tokens_host, first_tokens_host + B, s->tokens_pinned);

@@ -3,6 +3,7 @@
 #include <cstring>
 #include <map>
 #include <mutex>
+#include <shared_mutex>
 #include <vector>
 
 #include "common.h"
@@ -35,6 +36,67 @@ int device_cu_count() {
     cached[dev] = n;
   }
   return cached[dev];
+}
+
+namespace {
+
+struct CaptureGate {
+  std::mutex turn;  // held by a capture that waits, so that calls that come do not pass it
+  std::shared_mutex inside;
+};
+CaptureGate& capture_gate() {
+  static CaptureGate* gate = new CaptureGate();  // never destroyed: threads may outlive static objects
+  return *gate;
+}
+thread_local int g_device_calls = 0;
+thread_local bool g_capturing = false;
+
+}  // namespace
+
+DeviceCall::DeviceCall() {
+  if (g_capturing || g_device_calls++ > 0) return;
+  CaptureGate& gate = capture_gate();
+  std::lock_guard<std::mutex> turn(gate.turn);
+  gate.inside.lock_shared();
+}
+DeviceCall::~DeviceCall() {
+  if (g_capturing || --g_device_calls > 0) return;
+  capture_gate().inside.unlock_shared();
+}
+Capture::Capture() {
+  CaptureGate& gate = capture_gate();
+  std::lock_guard<std::mutex> turn(gate.turn);
+  gate.inside.lock();
+  g_capturing = true;
+}
+Capture::~Capture() {
+  g_capturing = false;
+  capture_gate().inside.unlock();
+}
+
+hipError_t device_malloc(void** p, size_t bytes) {
+  DeviceCall call;
+  return hipMalloc(p, bytes);
+}
+hipError_t device_free(void* p) {
+  DeviceCall call;
+  return hipFree(p);
+}
+hipError_t pinned_malloc(void** p, size_t bytes) {
+  DeviceCall call;
+  return hipHostMalloc(p, bytes, hipHostMallocDefault);
+}
+hipError_t pinned_free(void* p) {
+  DeviceCall call;
+  return hipHostFree(p);
+}
+hipError_t graph_exec_destroy(hipGraphExec_t exec) {
+  DeviceCall call;
+  return hipGraphExecDestroy(exec);
+}
+hipError_t device_wait() {
+  DeviceCall call;
+  return hipDeviceSynchronize();
 }
 
 }  // namespace rwkv
@@ -80,10 +142,11 @@ int rwkv_hip_measure_launch_chain(int links, int blocks, int threads, int use_gr
   };
   do {
     if (fail(hipStreamCreateWithFlags(&st, hipStreamNonBlocking), "stream create")) break;
-    if (fail(hipMalloc(reinterpret_cast<void**>(&counter), 256), "malloc")) break;
+    if (fail(device_malloc(reinterpret_cast<void**>(&counter), 256), "malloc")) break;
     if (fail(hipMemsetAsync(counter, 0, 256, st), "memset")) break;
     if (fail(hipEventCreate(&e0), "event create") || fail(hipEventCreate(&e1), "event create")) break;
     if (use_graph) {
+      Capture capture;
       if (fail(hipStreamBeginCapture(st, hipStreamCaptureModeThreadLocal), "begin capture")) break;
       chain();
       if (fail(hipStreamEndCapture(st, &graph), "end capture")) break;
@@ -103,6 +166,7 @@ int rwkv_hip_measure_launch_chain(int links, int blocks, int threads, int use_gr
     float ms = 0.0f;
     if (fail(hipEventElapsedTime(&ms, e0, e1), "elapsed")) break;
     unsigned count = 0;
+    DeviceCall call;
     if (fail(hipMemcpy(&count, counter, sizeof(count), hipMemcpyDeviceToHost), "copy back")) break;
     if (count != static_cast<unsigned>(links) * (reps + 1)) {
       set_error("measure_launch_chain: the chain counted %u links instead of %u", count, static_cast<unsigned>(links) * (reps + 1));
@@ -111,11 +175,11 @@ int rwkv_hip_measure_launch_chain(int links, int blocks, int threads, int use_gr
     }
     *us_per_link = ms * 1e3f / (static_cast<float>(reps) * links);
   } while (false);
-  if (exec) (void)hipGraphExecDestroy(exec);
+  if (exec) (void)graph_exec_destroy(exec);
   if (graph) (void)hipGraphDestroy(graph);
   if (e0) (void)hipEventDestroy(e0);
   if (e1) (void)hipEventDestroy(e1);
-  if (counter) (void)hipFree(counter);
+  if (counter) (void)device_free(counter);
   if (st) (void)hipStreamDestroy(st);
   return rc;
 }
@@ -144,12 +208,12 @@ int rwkv_hip_malloc(void** ptr, size_t bytes) {
   RWKV_REQUIRE(ptr != nullptr, "ptr is NULL");
   *ptr = nullptr;
   if (bytes == 0) return RWKV_OK;
-  RWKV_HIP_TRY(hipMalloc(ptr, bytes));
+  RWKV_HIP_TRY(device_malloc(ptr, bytes));
   return RWKV_OK;
 }
 
 int rwkv_hip_free(void* ptr) {
-  if (ptr) RWKV_HIP_TRY(hipFree(ptr));
+  if (ptr) RWKV_HIP_TRY(device_free(ptr));
   return RWKV_OK;
 }
 
@@ -182,13 +246,14 @@ void recycle_trim_locked(RecycleBin& bin, size_t keep) {
         break;
       }
     }
-    (void)hipFree(entry.second);
+    (void)device_free(entry.second);
     bin.held -= entry.first.second;
   }
 }
 }  // namespace
 
 int rwkv_hip_malloc_recycled(void** ptr, size_t bytes) {
+  DeviceCall call;
   RWKV_REQUIRE(ptr != nullptr, "ptr is NULL");
   *ptr = nullptr;
   if (bytes == 0) return RWKV_OK;
@@ -212,22 +277,23 @@ int rwkv_hip_malloc_recycled(void** ptr, size_t bytes) {
       return RWKV_OK;
     }
   }
-  hipError_t err = hipMalloc(ptr, bytes);
+  hipError_t err = device_malloc(ptr, bytes);
   if (err == hipErrorOutOfMemory) {  // give the held blocks back and try once more
     (void)hipGetLastError();
     std::lock_guard<std::mutex> guard(bin.lock);
     recycle_trim_locked(bin, 0);
-    err = hipMalloc(ptr, bytes);
+    err = device_malloc(ptr, bytes);
   }
   RWKV_HIP_TRY(err);
   return RWKV_OK;
 }
 
 int rwkv_hip_free_recycled(void* ptr, size_t bytes) {
+  DeviceCall call;
   if (!ptr) return RWKV_OK;
   if (bytes == 0 || bytes > kRecycleMaxHeld) return rwkv_hip_free(ptr);
   // like hipFree, returns only when the device no longer uses the block
-  RWKV_HIP_TRY(hipDeviceSynchronize());
+  RWKV_HIP_TRY(device_wait());
   int dev = 0;
   RWKV_HIP_TRY(hipGetDevice(&dev));
   RecycleBin& bin = recycle_bin();
@@ -241,6 +307,7 @@ int rwkv_hip_free_recycled(void* ptr, size_t bytes) {
 }
 
 int rwkv_hip_recycle_trim(void) {
+  DeviceCall call;
   RecycleBin& bin = recycle_bin();
   std::lock_guard<std::mutex> guard(bin.lock);
   recycle_trim_locked(bin, 0);
@@ -251,24 +318,27 @@ int rwkv_hip_host_alloc(void** ptr_host, size_t bytes) {
   RWKV_REQUIRE(ptr_host != nullptr, "ptr is NULL");
   *ptr_host = nullptr;
   if (bytes == 0) return RWKV_OK;
-  RWKV_HIP_TRY(hipHostMalloc(ptr_host, bytes, hipHostMallocDefault));
+  RWKV_HIP_TRY(pinned_malloc(ptr_host, bytes));
   return RWKV_OK;
 }
 
 int rwkv_hip_host_free(void* ptr_host) {
-  if (ptr_host) RWKV_HIP_TRY(hipHostFree(ptr_host));
+  if (ptr_host) RWKV_HIP_TRY(pinned_free(ptr_host));
   return RWKV_OK;
 }
 
 int rwkv_hip_memcpy_h2d(void* dst, const void* src_host, size_t bytes) {
+  DeviceCall call;
   if (bytes) RWKV_HIP_TRY(hipMemcpy(dst, src_host, bytes, hipMemcpyHostToDevice));
   return RWKV_OK;
 }
 int rwkv_hip_memcpy_d2h(void* dst_host, const void* src, size_t bytes) {
+  DeviceCall call;
   if (bytes) RWKV_HIP_TRY(hipMemcpy(dst_host, src, bytes, hipMemcpyDeviceToHost));
   return RWKV_OK;
 }
 int rwkv_hip_memcpy_d2d(void* dst, const void* src, size_t bytes) {
+  DeviceCall call;
   if (bytes) RWKV_HIP_TRY(hipMemcpy(dst, src, bytes, hipMemcpyDeviceToDevice));
   return RWKV_OK;
 }
@@ -285,10 +355,12 @@ int rwkv_hip_memcpy_d2d_async(rwkv_stream_t s, void* dst, const void* src, size_
   return RWKV_OK;
 }
 int rwkv_hip_memset(void* ptr, int value, size_t bytes) {
+  DeviceCall call;
   if (bytes) RWKV_HIP_TRY(hipMemset(ptr, value, bytes));
   return RWKV_OK;
 }
 int rwkv_hip_mem_info(size_t* free_bytes, size_t* total_bytes) {
+  DeviceCall call;
   RWKV_REQUIRE(free_bytes && total_bytes, "NULL output");
   RWKV_HIP_TRY(hipMemGetInfo(free_bytes, total_bytes));
   {  // blocks held for recycling are free memory to the caller (an allocation that needs them gets them)
@@ -303,11 +375,13 @@ int rwkv_hip_stream_create(rwkv_stream_t* s) {
   RWKV_REQUIRE(s != nullptr, "stream out is NULL");
   hipStream_t st = nullptr;
   // default priority on purpose: every stream of this library runs at the same priority
+  DeviceCall call;
   RWKV_HIP_TRY(hipStreamCreateWithFlags(&st, hipStreamNonBlocking));
   *s = st;
   return RWKV_OK;
 }
 int rwkv_hip_stream_destroy(rwkv_stream_t s) {
+  DeviceCall call;
   if (s) RWKV_HIP_TRY(hipStreamDestroy(as_stream(s)));
   return RWKV_OK;
 }
@@ -316,7 +390,7 @@ int rwkv_hip_stream_sync(rwkv_stream_t s) {
   return RWKV_OK;
 }
 int rwkv_hip_device_sync(void) {
-  RWKV_HIP_TRY(hipDeviceSynchronize());
+  RWKV_HIP_TRY(device_wait());
   return RWKV_OK;
 }
 
