@@ -1391,7 +1391,7 @@ __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) 
   }
   __syncthreads();
   if (wave != 0) return;
-  // one wavefront over up to 1024 sums, 64 at a time
+  // one wavefront over a chunk's sums (up to kMaxLogprobVocab / kSlot / kPickWaves), 64 at a time
   int slot = 0;
   double slot_before = 0.0;
   sure = false;
