@@ -30,6 +30,7 @@ namespace {
 
 constexpr int kSlot = 64;
 constexpr int kPart = 4096;      // entries of a block of draw_stats_kernel
+constexpr int kStatsThreads = 256;
 constexpr int kPickThreads = 512;
 constexpr int kList = 6144;      // entries
 constexpr int kBuckets = 256;    // of a histogram
@@ -38,11 +39,11 @@ constexpr int kLast = 64;        // entries that one wavefront puts in order
 constexpr int kWaveSlots = 256;  // slots of a wavefront that reach the bound
 constexpr int kHeld = 8;         // of these, those that it reads at once
 // Slots of a block that reach the bound: with more of them the histograms of a row that has some lead to the cut sooner than a list of the
-// entries.  V = 65536, list / window, us: 225 slots 26 / 31 at 8 rows and 49 / 55 at 256, 400 slots 31 / 31 and 55 / 56, 640 39 / 31 and 64 / 56.
+// entries.  V = 65536, list / window, us: 236 slots 26 / 31 at 8 rows and 47 / 54 at 256, 371 slots 31 / 31 and 52 / 55, 659 38 / 31 and 62 / 55.
 constexpr int kMost = 384;
 // A top_k up to which a row does without histograms, and the most slots to a place of it (the slots' maxima bound the kept entries the worse the
-// fewer they are).  Without / with histograms, us: 8 rows of 65536, top_k 128 19 / 23, 512 30 / 31, 640 34 / 31; 128 rows 23 / 36, 34 / 43, 47 / 43;
-// 8 rows of 16384 (256 slots), top_k 128 20 / 22, 192 24 / 24, 256 56 / 26; of 4096 (64 slots), 32 19 / 19, 64 29 / 23.
+// fewer they are).  Without / with histograms, us: 8 rows of 65536, top_k 128 19 / 23, 512 29 / 31, 640 34 / 31; 256 rows 29 / 45, 42 / 55, 46 / 55;
+// 8 rows of 16384 (256 slots), top_k 128 20 / 23, 192 24 / 24, 256 55 / 26; of 4096 (64 slots), 32 19 / 20, 64 28 / 24.
 constexpr int kListed = 512;
 constexpr int kSlotsListed = 2;
 constexpr int kGrid = 8;         // buckets of the parts' histograms in an octave
@@ -333,14 +334,15 @@ __device__ __forceinline__ int part_raised(int b) { return static_cast<unsigned>
 // where the temperature is some 10^-7 of the largest entry, and neighbouring numbers are octaves apart.)
 constexpr float kFarthest = 33554432.0f;  // 2^25
 
-// A block takes a part of a row in NT threads, each E entries at a time: so many neighbours add up as E / 4 sums of four, then those, then the
-// slot's threads, in the same order whatever E is.  Loads are as wide as they are apart, at any alignment.  What bounds it: the loads and what is computed, one
-// after the other in a block and only in part beside one another (512 rows of 65536, us: loads and maxima alone 26, that is 5.1 TB/s; sums of the
-// entries themselves 30; of their powers 40; histograms 45).
-template <typename T, int NT, int E>
-__global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
-  constexpr int NV = kPart / E / NT, kLanes = kSlot / E;
-  static_assert(E == 4 || E == 8, "a slot is 16 or 8 lanes");
+// A block takes a part of a row in NT threads, each E neighbours at a time, which add up as sums of four, then those, then the slot's threads.
+// Loads are as wide as they are apart, at any alignment.  What bounds it: the loads and what is computed, one after the other in a block and only in
+// part beside one another (512 rows of 65536, us: loads and maxima alone 26, that is 5.1 TB/s; sums of the entries themselves 30; of their powers
+// 40; histograms 45).  Four neighbours to a thread take more steps to a slot's sum: 256 rows of 65536 without filters 27.7 a call instead of 25.7,
+// with top-p 56.5 instead of 54.7; 1024 threads for few parts gain nothing (1 to 16 rows 4.0 to 4.6 with either, 31 rows 6.6 instead of
+// 5.1); several parts to a block, the next one requested ahead, took 10 % longer.
+template <typename T>
+__global__ __launch_bounds__(kStatsThreads) void draw_stats_kernel(DrawArgs a) {
+  constexpr int NT = kStatsThreads, E = 8, NV = kPart / E / NT, kLanes = kSlot / E;
   typedef T vec_t __attribute__((ext_vector_type(4), aligned(sizeof(T))));  // (a load need not be aligned)
   typedef float pen_t __attribute__((ext_vector_type(4), aligned(sizeof(float))));
   __shared__ float most[NT / 64];
@@ -435,7 +437,7 @@ __global__ __launch_bounds__(NT) void draw_stats_kernel(DrawArgs a) {
       atomicAdd(&mass[b], in_units(weight<true>(z[q][j], m, w.power, ninth, round, part_raised(b)), one, two));
       if (counts) atomicAdd(&count[b], 1u);
     }
-  // (sums of what the buckets hold: the same however many threads there were)
+  // (sums of what the buckets hold: in one order, whatever order the entries came in)
   __syncthreads();
   const int b = threadIdx.x;
   const bool far = !(fabsf(top) < kFarthest);
@@ -1051,9 +1053,9 @@ __device__ __forceinline__ bool list_window(const DrawArgs& a, PickShared& sh, c
 }
 
 // A block draws for a row.  What bounds it is the chain of its steps, each a trip to memory or a few hundred instructions between barriers: V =
-// 65536 with top_k 50 and top_p 9 us (maxima 1.6, bound 2.8, slots 0.8, list 2), with top-p over a flat row 28 (window 4, listing 10, cut 4, sums
+// 65536 with top_k 20 and top_p 10 us (maxima 1.6, bound 2.8, slots 0.8, list 2), with top-p over a flat row 28 (window 4, listing 10, cut 4, sums
 // 10).  512 threads whatever the batch is, so that sums split alike; two blocks to a CU: 512 rows at once, whose chains fill one another's
-// waits (44 us).
+// waits (45 us).
 template <typename T>
 __global__ __launch_bounds__(kPickThreads, 4) void draw_pick_kernel(DrawArgs a) {  // (four wavefronts per SIMD: two blocks per CU)
   __shared__ PickShared sh;
@@ -1436,12 +1438,7 @@ __global__ __launch_bounds__(256) void draw_penalties_kernel(int V, const float*
 
 template <typename T>
 void launch_draw(hipStream_t st, int rows, const DrawArgs& a) {
-  // Few parts: each by as many wavefronts as a block has.  V = 65536 without filters, 1024 threads / 256, us: 16 rows 10.5 / 11.0,
-  // 32 rows 12.3 / 11.8, 256 rows 39 / 30.  (Several parts to a block, the next one requested ahead, took 10 % longer.)  Eight neighbours to
-  // one of 256 threads instead of four take fewer steps to a slot's sum: 256 rows without filters 31.2 -> 29.9.
-  const bool few = static_cast<int64_t>(rows) * a.parts < 2 * device_cu_count();
-  if (few) hipLaunchKernelGGL((draw_stats_kernel<T, 1024, 4>), dim3(rows, a.parts), dim3(1024), 0, st, a);
-  else hipLaunchKernelGGL((draw_stats_kernel<T, 256, 8>), dim3(rows, a.parts), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((draw_stats_kernel<T>), dim3(rows, a.parts), dim3(kStatsThreads), 0, st, a);
   hipLaunchKernelGGL((draw_pick_kernel<T>), dim3(rows), dim3(kPickThreads), 0, st, a);
 }
 
